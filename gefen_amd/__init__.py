@@ -2,9 +2,14 @@
 
 ``from gefen_amd import Gefen, GefenMuon`` replaces ``from gefen import Gefen, GefenMuon``
 (reference __init__.py:1-13); the optimizer classes are loaded lazily.
+
+Beside the optimizers, what a training step does around them: ``linear_cross_entropy``
+(the loss of an output matrix with its gradients, without the logits), ``gradient_norm``,
+``clip_gradients`` and ``clip_grad_norm_``.
 """
 
-__all__ = ["Gefen", "GefenMuon", "kernels"]
+__all__ = ["Gefen", "GefenMuon", "kernels", "linear_cross_entropy", "gradient_norm", "clip_gradients",
+           "clip_grad_norm_"]
 
 
 def __getattr__(name):
@@ -16,4 +21,12 @@ def __getattr__(name):
         from .gefen_muon import GefenMuon
 
         return GefenMuon
+    if name == "linear_cross_entropy":
+        from .kernels.linear_cross_entropy import linear_cross_entropy
+
+        return linear_cross_entropy
+    if name in ("gradient_norm", "clip_gradients", "clip_grad_norm_"):
+        from .kernels import gradient_norm as module
+
+        return getattr(module, name)
     raise AttributeError("module {!r} has no attribute {!r}".format(__name__, name))

@@ -77,6 +77,13 @@ SIGNATURES = {
     "gefen_gram_bf16_batched": (I32, [P, I64, I64, P, I64, I64, I32, I32, I32, DBL, P]),
     "gefen_gemm_bf16_nt_batched_apply": (I32, [P, I64, I64, P, I64, I64, P, I64, I64, I32, I32, I32, I32, DBL, DBL,
                                                P, P]),
+    "gefen_gradient_norm_workspace_size": (SZ, [P, I32]),
+    "gefen_gradient_norm": (I32, [P, I32, DBL, P, P, P]),
+    "gefen_clip_gradients": (I32, [P, I32, DBL, DBL, P, P, P]),
+    "gefen_scale_gradients": (I32, [P, I32, P, DBL, P]),
+    "gefen_linear_cross_entropy_workspace_size": (SZ, [P]),
+    "gefen_linear_cross_entropy": (I32, [P, P, SZ, P]),
+    "gefen_scale_by": (I32, [P, I64, P, I64, I32, P, P]),
 }
 
 # numpy mirror of struct gefen_step_task / gefen_muon_task (natural C alignment)
@@ -103,8 +110,26 @@ PERIOD_TASK = np.dtype([
 HISTOGRAM_TASK = np.dtype([
     ("grad", np.uint64), ("numel", np.int64), ("period", np.int64), ("dtype", np.int32), ("pad", np.int32),
 ])
+GRADIENT_TASK = np.dtype([
+    ("src", np.uint64), ("dst", np.uint64), ("numel", np.int64), ("src_dtype", np.int32), ("dst_dtype", np.int32),
+])
+
+
+class LinearCrossEntropyTask(ctypes.Structure):
+    """struct gefen_linear_cross_entropy_task"""
+
+    _fields_ = [(name, P) for name in ("hidden", "weight", "targets", "losses", "loss", "grad_hidden", "grad_weight",
+                                       "grad")]
+    _fields_ += [(name, I64) for name in ("n", "v", "d", "hidden_row_stride", "hidden_col_stride",
+                                          "weight_row_stride", "weight_col_stride", "ignore_index",
+                                          "workspace_limit")]
+    _fields_ += [("label_smoothing", DBL), ("dtype", I32), ("targets_int32", I32), ("reduction", I32), ("pad", I32)]
+
+
+REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2
 STEP_SUMMARY = np.dtype([("launches", np.int32), ("shared", np.int32), ("small", np.int32), ("tables", np.int32)])
 assert PERIOD_TASK.itemsize == 40 and HISTOGRAM_TASK.itemsize == 32
+assert GRADIENT_TASK.itemsize == 32 and ctypes.sizeof(LinearCrossEntropyTask) == 160
 assert STEP_TASK.itemsize == 128 and MUON_TASK.itemsize == 72 and MUON_APPLY_TASK.itemsize == 56
 
 _LIB = None

@@ -54,5 +54,7 @@ extern "C" size_t gefen_struct_size(int which) {
     return which == 0   ? sizeof(gefen_step_task)
            : which == 1 ? sizeof(gefen_muon_task)
            : which == 2 ? sizeof(gefen_muon_apply_task)
+           : which == 3 ? sizeof(gefen_gradient_task)
+           : which == 4 ? sizeof(gefen_linear_cross_entropy_task)
                         : 0;
 }

@@ -39,7 +39,8 @@ int gefen_abi_version(void);
  * diagnostic: gefen_step_tasks_noalloc leaves it unchanged. */
 int64_t gefen_device_allocations(void);
 /* sizeof(gefen_step_task) for which = 0, sizeof(gefen_muon_task) for which = 1,
- * sizeof(gefen_muon_apply_task) for which = 2:
+ * sizeof(gefen_muon_apply_task) for which = 2, sizeof(gefen_gradient_task) for which = 3,
+ * sizeof(gefen_linear_cross_entropy_task) for which = 4:
  * lets bindings check their mirror of the structs. */
 size_t gefen_struct_size(int which);
 
@@ -433,6 +434,78 @@ int gefen_gemm_bf16_nt_batched(const void* a, int64_t lda, int64_t stride_a, con
  * 64, k * ldxt * 2 < 2^31, rows 16-byte aligned (else ValueError). */
 int gefen_gram_bf16_batched(const void* xt, int64_t ldxt, int64_t stride_xt, void* c, int64_t ldc,
                             int64_t stride_c, int batch, int m, int k, double alpha, gefen_stream_t stream);
+
+/* ------------------------------------------------------------------ gradient norm and clipping
+ * The global norm of a set of gradients and its bound, as a training loop applies them
+ * between backward and step: t = (sum |g|^2)^(1/2) (norm_type 2), sum |g| (1) or max |g|
+ * (infinity) over every element of every task; dst = src * min(1, max_norm / (t + 1e-6)),
+ * rounded once to dst's dtype.  Sums are float64 and joined in a fixed order: a norm does
+ * not depend on scheduling.  A NaN anywhere gives a NaN norm, and NaN gradients. */
+typedef struct gefen_gradient_task {
+    const void* src;    /* numel contiguous elements */
+    void* dst;          /* where the scaled gradient goes: src itself, or memory apart from every
+                         * other task's (not read by gefen_gradient_norm) */
+    int64_t numel;      /* 0 is fine */
+    int32_t src_dtype;
+    int32_t dst_dtype;  /* equal to src_dtype in place */
+} gefen_gradient_task;
+
+/* Bytes that gefen_gradient_norm and gefen_clip_gradients need as workspace (8-byte aligned). */
+size_t gefen_gradient_norm_workspace_size(const gefen_gradient_task* tasks, int num_tasks);
+/* *norm (device) = the norm; 0 without elements. */
+int gefen_gradient_norm(const gefen_gradient_task* tasks, int num_tasks, double norm_type, float* norm,
+                        void* workspace, gefen_stream_t stream);
+/* The norm into *norm and the scaled gradients into dst.  Gradients scaled in place are
+ * not written when the norm is within the bound. */
+int gefen_clip_gradients(const gefen_gradient_task* tasks, int num_tasks, double norm_type, double max_norm,
+                         float* norm, void* workspace, gefen_stream_t stream);
+/* The scaling alone, by a norm that is known (device): one shard of a sharded model. */
+int gefen_scale_gradients(const gefen_gradient_task* tasks, int num_tasks, const float* norm, double max_norm,
+                          gefen_stream_t stream);
+
+/* ------------------------------------------------------------------ linear cross entropy
+ * Softmax cross entropy of logits l = hidden @ weight^T that are never kept, with the
+ * gradients of hidden and weight:
+ *   loss_n = lse_n - (1 - e) l[n, y_n] - (e / V) sum_v l[n, v],   lse_n = log sum_v exp l[n, v]
+ * with e = label_smoothing; rows whose target is ignore_index have no loss, and nothing
+ * they hold is read into a result.  A target outside [0, V) gives a NaN loss (and NaN
+ * gradients).  Products accumulate in float32; exp(l - max) is rounded once to 16 bits
+ * for the gradients' products (float32 operands keep 24 bits throughout). */
+enum { GEFEN_REDUCE_NONE = 0, GEFEN_REDUCE_MEAN = 1, GEFEN_REDUCE_SUM = 2 };
+/* workspace_limit = 0: what the values kept for the gradients may take */
+#define GEFEN_LCE_DEFAULT_LIMIT ((int64_t)4 << 30)
+
+typedef struct gefen_linear_cross_entropy_task {
+    const void* hidden;   /* [n, d], any strides (elements) */
+    const void* weight;   /* [v, d], any strides (elements); read in place when its rows are
+                           * contiguous, 16-byte aligned and d is a multiple of 64 (not float32) */
+    const void* targets;  /* [n] contiguous, int64 or int32 */
+    float* losses;        /* [n]: loss of each row, 0 where ignored; may be NULL */
+    float* loss;          /* the reduced loss; may be NULL (must be for GEFEN_REDUCE_NONE) */
+    void* grad_hidden;    /* [n, d] contiguous, of dtype; NULL: not wanted */
+    void* grad_weight;    /* [v, d] contiguous, of dtype; NULL: not wanted */
+    const float* grad;    /* gradient of the loss (device): one value, or one per row for
+                           * GEFEN_REDUCE_NONE; NULL: 1 */
+    int64_t n, v, d;
+    int64_t hidden_row_stride, hidden_col_stride, weight_row_stride, weight_col_stride;
+    int64_t ignore_index;
+    int64_t workspace_limit;  /* bytes of the values kept per piece of rows; 0: the default */
+    double label_smoothing;   /* in [0, 1] */
+    int32_t dtype;            /* of hidden, weight and their gradients */
+    int32_t targets_int32;    /* 1: targets are int32 */
+    int32_t reduction;        /* the mean is over the rows that have a loss */
+    int32_t pad;
+} gefen_linear_cross_entropy_task;
+
+/* Bytes of workspace that the call needs (0: invalid task, see gefen_last_error). */
+size_t gefen_linear_cross_entropy_workspace_size(const gefen_linear_cross_entropy_task* task);
+/* workspace: 16-byte aligned device memory.  No synchronisation, no allocation. */
+int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task* task, void* workspace,
+                               size_t workspace_bytes, gefen_stream_t stream);
+/* dst *= *factor (device) for one or two tensors, left untouched where the factor is 1:
+ * the gradients of a loss whose own gradient arrives later.  b may be NULL. */
+int gefen_scale_by(void* a, int64_t a_numel, void* b, int64_t b_numel, int dtype, const float* factor,
+                   gefen_stream_t stream);
 
 #ifdef __cplusplus
 }
