@@ -12,22 +12,27 @@
 // * Positions whose target is ignore_index take no part: the rows that count are
 //   gathered first (k_rows, k_pack), so a masked prompt costs nothing and whatever it
 //   holds (NaN included) reaches nothing.
-// * The logits' product keeps, for every row and slot of 32 WI columns, the slot's
+// * The logits' product keeps, for every row and slot of 64 columns, the slot's
 //   maximum m and sum of exp(l - m), both float32, and when gradients are wanted
-//   exp(l - m) itself in 16 bits.  That one rounding (2^-8 relative at most for bf16) is what
-//   the gradient's products take as their operand anyway.
+//   exp(l - m) itself in 16 bits: an unsigned format of its own with three significant
+//   bits more than bf16 (two more than half), so that G is in effect rounded once.
 // * One pass over those values turns them into G (k_gradient_rows): a row's lse comes
 //   from its slots, and exp(m - lse) scales each slot.  The target's entry is formed in
 //   float32 from its own logit, so that p - 1 of a confident row does not cancel in
-//   16 bits.
+//   16 bits.  Rounding G to the operands' type is the one rounding below float32 on the
+//   way to the gradients: its errors are independent between the many terms of each sum
+//   and stay below that of the gradients' own rounding.
+// * For few rows one term can be most of a sum, and the products wait for W or dW
+//   anyway: G is then two planes, twice the type's bits (kTwoPlaneRows).
 // * Rows are taken in pieces whose G fits a bounded workspace; the logits of a piece
 //   exist only as these 16-bit values, and never all of them at once when the
 //   positions do not fit.  dW is summed over the pieces in float32.
 //
 // A half-precision G is scaled by 2^15 (and its products by 2^-15), which keeps
-// probabilities down to 1e-9 out of half's subnormals.  float32 runs on three bf16
-// planes per operand and six plane products: 24 bits, at 2.6 times the rate of the
-// float32 matrix instructions.
+// probabilities down to 1e-9 out of half's subnormals.  float32 runs as two half planes
+// per operand and three products, each matrix scaled by the power of two that brings its
+// largest finite element to 2^14: elements keep 22 bits down to 2^-29 of the largest
+// one, at five times the rate of the float32 matrix instructions.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -40,6 +45,7 @@ namespace gefen {
 namespace lce {
 
 constexpr float kHalfScale = 32768.0f;  // of a half-precision G
+constexpr int kSlot = 64;               // columns that share a maximum
 constexpr int kRowAlign = 256;          // rows of a piece, columns of G
 constexpr int kMaxVocab = 4 << 20;      // 256 rows of G within 2^31 bytes
 constexpr int kMaxWidth = 1 << 20;
@@ -48,6 +54,7 @@ constexpr int kMaxWidth = 1 << 20;
 struct Meta {
     int32_t count;    // rows that take part
     float grad_max;   // largest |gradient| of a row (per-row gradients)
+    uint32_t top[2];  // float32: largest finite magnitude of hidden and weight, as bits
 };
 
 __device__ __forceinline__ int piece_rows(const Meta* m, int from, int most) {
@@ -100,26 +107,73 @@ __global__ __launch_bounds__(kRowsThreads) void k_rows(const void* __restrict__ 
         for (int w = 1; w < kRowsThreads / 64; ++w) gmax = nanmax(gmax, wave_max[w]);
         meta->count = base;
         meta->grad_max = gmax;
+        meta->top[0] = meta->top[1] = 0;
     }
 }
 
-__device__ __forceinline__ void split3(float x, uint16_t out[3]) {
+// x (scaled into half's range) as a half and what it leaves times kLowScale.
+__device__ __forceinline__ void split_half(float x, uint16_t* hi, uint16_t* lo) {
+    const f16_t h = from_f32<f16_t>(x);
+    *hi = h.bits;
+    // what is not finite has no remainder worth adding: inf - inf is NaN
+    *lo = (h.bits & 0x7c00) == 0x7c00 ? 0 : from_f32<f16_t>((x - to_f32(h)) * kLowScale).bits;
+}
+__device__ __forceinline__ void split_bf16(float x, uint16_t* hi, uint16_t* lo) {
     const bf16_t h = from_f32<bf16_t>(x);
-    const float r1 = x - to_f32(h);
-    const bf16_t m = from_f32<bf16_t>(r1);
-    const float r2 = r1 - to_f32(m);
-    out[0] = h.bits;
-    // an infinite or NaN x has no remainder worth adding: inf - inf is NaN
-    const bool fin = fabsf(to_f32(h)) < INFINITY;
-    out[1] = fin ? m.bits : 0;
-    out[2] = fin ? from_f32<bf16_t>(r2).bits : 0;
+    *hi = h.bits;
+    *lo = (h.bits & 0x7f80) == 0x7f80 ? 0 : from_f32<bf16_t>(x - to_f32(h)).bits;
+}
+
+// exp(l - m) in [0, 1] as 16 unsigned bits on its way to G: 4 exponent and 12 mantissa
+// bits for a half G, 6 and 10 for a bf16 one, with subnormals.  The float's own exponent
+// is brought down by a product with a power of two (subnormal results are rounded by the
+// hardware), and the mantissa is rounded to nearest.  Relative error 2^-13 down to 2^-14
+// (bf16: 2^-11 down to 2^-62), 2^-27 absolute below.
+template <bool F16>
+__device__ __forceinline__ uint16_t pack_exp(float e) {
+    constexpr int drop = F16 ? 11 : 13;
+    const uint32_t u = __float_as_uint(e * (F16 ? 0x1p-112f : 0x1p-64f));
+    return (uint16_t)((u + ((1u << (drop - 1)) - 1) + ((u >> drop) & 1u)) >> drop);
+}
+template <bool F16>
+__device__ __forceinline__ float unpack_exp(uint16_t x) {
+    return __uint_as_float((uint32_t)x << (F16 ? 11 : 13)) * (F16 ? 0x1p112f : 0x1p64f);
+}
+
+// Exponent that brings a matrix's largest finite magnitude (its bits in `top`) to 2^14.
+__device__ __forceinline__ int half_exponent(uint32_t top) {
+    return top == 0 ? 0 : 14 - max((int)(top >> 23) - 127, -112);
+}
+
+// meta->top[which] = the largest finite magnitude of a float32 matrix, as its bits; with
+// a map, of the rows that take part.  Maxima of integers: any order gives the same.
+struct Top {
+    const float* src;
+    int64_t row_stride, col_stride;
+    int32_t n, d;
+    const int32_t* map;
+    Meta* meta;
+    int32_t which;
+};
+__global__ __launch_bounds__(256) void k_top(const Top t) {
+    const int rows = t.map ? t.meta->count : t.n;
+    uint32_t top = 0;
+    for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+        const float* s = t.src + (int64_t)(t.map ? t.map[r] : r) * t.row_stride;
+        for (int c = threadIdx.x; c < t.d; c += 256) {
+            const uint32_t u = abs_key(s[(int64_t)c * t.col_stride]);
+            top = u < 0x7f800000u && u > top ? u : top;
+        }
+    }
+    top = wave_group_max_u32(top, 64);
+    if ((threadIdx.x & 63) == 0) atomicMax(&t.meta->top[t.which], top);
 }
 
 // Rows of a matrix of any strides as the products read them: dp = D rounded up to 64
-// columns, zero-padded, one plane or the four of a float32 operand.  With a map: row r is src row map[r]
+// columns, zero-padded, one plane or those of a float32 operand, scaled.  With a map: row r is src row map[r]
 // for r < meta->count and zero up to the next multiple of kRowAlign, and the rows that
 // take no part get a zero gradient and a zero loss.
-constexpr int kPackPlanes = 4;
+constexpr int kPackPlanes = 3;  // of a float32 operand: high, low, high where finite
 struct Pack {
     const void* src;
     int64_t row_stride, col_stride;
@@ -129,6 +183,7 @@ struct Pack {
     int64_t plane;
     const int32_t* map;
     const Meta* meta;
+    int32_t which;      // float32: whose largest magnitude in meta->top
     void* zero_rows;    // [n, d] gradient, rows of d elements of `size` bytes (may be null)
     float* zero_losses;  // [n] (may be null)
 };
@@ -154,19 +209,16 @@ __global__ __launch_bounds__(256) void k_pack(const Pack p) {
     }
     const int c0 = (int)(blockIdx.y * 256 + threadIdx.x) * 8;
     if (c0 >= p.dp) return;
-    uint16_t out[4][8] = {};
+    uint16_t out[kPackPlanes][8] = {};
     if (live) {
         if (p.f32) {
+            const int ex = half_exponent(p.meta->top[p.which]);
             const float* s = static_cast<const float*>(p.src) + row * p.row_stride;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (c0 + e < p.d) {
-                    uint16_t t[3];
-                    split3(s[(int64_t)(c0 + e) * p.col_stride], t);
-                    out[0][e] = t[0];
-                    out[1][e] = t[1];
-                    out[2][e] = t[2];
-                    out[3][e] = (t[0] & 0x7f80) == 0x7f80 ? 0 : t[0];
+                    split_half(ldexpf(s[(int64_t)(c0 + e) * p.col_stride], ex), &out[0][e], &out[1][e]);
+                    out[2][e] = (out[0][e] & 0x7c00) == 0x7c00 ? 0 : out[0][e];
                 }
         } else {
             const uint16_t* s = static_cast<const uint16_t*>(p.src) + row * p.row_stride;
@@ -200,9 +252,9 @@ struct Logits {
     float* target_logit;  // [row], over all pieces
     const int32_t* tgt;
     const Meta* meta;
-    uint16_t* g;        // [row][ldg] exp(l - slot maximum), `planes` of them (null: loss only)
+    uint16_t* g;        // [row][ldg] exp(l - slot maximum), packed or in two planes (null: loss only)
     int64_t ldg, g_plane;
-    int32_t planes;
+    int32_t planes, f32;
 };
 
 template <typename C>
@@ -214,50 +266,49 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
     const int live = tiles_n * a.tiles_m;
     if ((int)blockIdx.x >= live) return;
     int ti, tj;
-    tile_of(logical_block(blockIdx.x, live), a.tiles_m, tiles_n, &ti, &tj);
+    tile_of<C::GROUP_M>(logical_block(blockIdx.x, live), a.tiles_m, tiles_n, &ti, &tj);
     const int m0 = ti * C::TM, n0 = tj * C::TN;
-    f32x16 acc[WI][WJ];
+    f32x4 acc[WI][WJ];
     product_tile<C>(a.w, a.x, m0, n0, 0, a.steps, a.segs, smem, acc);
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = m0 + (wave / C::WAVES_N) * (32 * WI), wn = (wave % C::WAVES_N) * (32 * WJ);
-    const int slot = wm / (32 * WI);
-    const int hi = 4 * (lane >> 5);
-    const bool part = wm + 32 * WI > a.v;  // the last columns end inside this wave's
+    const int wm = m0 + (wave / C::WAVES_N) * C::WM, wn = n0 + (wave % C::WAVES_N) * C::WN;
+    const int hi = 4 * (lane >> 4);
+    const int slot = wm / kSlot;
+    static_assert(C::WM == kSlot, "a wave's columns are a slot");
     if (wm >= a.v && !a.g) return;
+    const int ex = a.f32 ? -half_exponent(a.meta->top[0]) - half_exponent(a.meta->top[1]) : 0;
+    const bool part = wm + C::WM > a.v;  // the last columns end inside this wave's
 #pragma unroll
     for (int j = 0; j < WJ; ++j) {
-        const int n = n0 + wn + j * 32 + (lane & 31);
+        const int n = wn + j * 16 + (lane & 15);
         float m = -INFINITY, sum = 0.0f;
-        if (part) {
-#pragma unroll
-            for (int i = 0; i < WI; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (wm + i * 32 + 8 * (r >> 2) + hi + (r & 3) >= a.v) acc[i][j][r] = -INFINITY;
-        }
 #pragma unroll
         for (int i = 0; i < WI; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) m = nanmax(m, acc[i][j][r]);
-        m = nanmax(m, __shfl_xor(m, 32, 64));
+            for (int r = 0; r < 4; ++r) {
+                if (a.f32) acc[i][j][r] = ldexpf(acc[i][j][r], ex);
+                if (part && wm + i * 16 + hi + r >= a.v) acc[i][j][r] = -INFINITY;
+                m = fmaxf(m, acc[i][j][r]);  // skips NaN, which the sum of exp keeps
+            }
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
         if (a.sums) {
 #pragma unroll
             for (int i = 0; i < WI; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    sum += (!part || wm + i * 32 + 8 * (r >> 2) + hi + (r & 3) < a.v) ? acc[i][j][r] : 0.0f;
+                for (int r = 0; r < 4; ++r) sum += !part || wm + i * 16 + hi + r < a.v ? acc[i][j][r] : 0.0f;
+            sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
         }
-        const int64_t at = n < rows ? (int64_t)n * a.slots + slot : 0;
         const int y = n < rows ? a.tgt[a.from + n] - wm : -1;
-        if (y >= 0 && y < 32 * WI && ((y >> 2) & 1) == (lane >> 5)) {
+        if (y >= 0 && y < C::WM && (y & 12) == hi) {
             float t = 0.0f;
 #pragma unroll
             for (int i = 0; i < WI; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (i * 32 + 8 * (r >> 2) + hi + (r & 3) == y) t = acc[i][j][r];
+                for (int r = 0; r < 4; ++r)
+                    if (i * 16 + hi + r == y) t = acc[i][j][r];
             a.target_logit[a.from + n] = t;
         }
         // a slot of no finite value: exp(-inf - 0) = 0
@@ -266,50 +317,36 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
 #pragma unroll
         for (int i = 0; i < WI; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
+            for (int r = 0; r < 4; ++r) {
                 const float x = acc[i][j][r] - ref;
-                const float e = a.planes == 3 ? expf(x) : __expf(x);
-                acc[i][j][r] = e;
-                s += e;
+                acc[i][j][r] = a.f32 ? expf(x) : __expf(x);
+                s += acc[i][j][r];
             }
+        s += __shfl_xor(s, 16, 64);
         s += __shfl_xor(s, 32, 64);
-        if (n < rows && lane < 32 && wm < a.v) {
+        if (n < rows && lane < 16 && wm < a.v) {
+            const int64_t at = (int64_t)n * a.slots + slot;
             a.stats[at] = make_float2(m, s);
             if (a.sums) a.sums[at] = sum;
         }
-    }
-    if (!a.g) return;
-    const float scale = C::F16 ? kHalfScale : 1.0f;
-#pragma unroll
-    for (int j = 0; j < WJ; ++j) {
+        if (!a.g) continue;
         // rows past the piece's end stay inside the workspace (it holds whole tiles)
-        uint16_t* row = a.g + (int64_t)(n0 + wn + j * 32 + (lane & 31)) * a.ldg + wm + hi;
+        uint16_t* row = a.g + (int64_t)n * a.ldg + wm + hi;
 #pragma unroll
-        for (int i = 0; i < WI; ++i)
+        for (int i = 0; i < WI; ++i) {
+            uint16_t o[2][4];
 #pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                uint16_t o[3][4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float e = acc[i][j][4 * r4 + r];
-                    if (a.planes == 3) {
-                        uint16_t t[3];
-                        split3(e, t);
-                        o[0][r] = t[0];
-                        o[1][r] = t[1];
-                        o[2][r] = t[2];
-                    } else if constexpr (C::F16) {
-                        o[0][r] = from_f32<f16_t>(e * scale).bits;
-                    } else {
-                        o[0][r] = from_f32<bf16_t>(e).bits;
-                    }
-                }
-                uint16_t* p = row + i * 32 + 8 * r4;
-                for (int k = 0; k < a.planes; ++k)
-                    *reinterpret_cast<uint2*>(p + k * a.g_plane) =
-                        make_uint2((uint32_t)o[k][0] | ((uint32_t)o[k][1] << 16),
-                                   (uint32_t)o[k][2] | ((uint32_t)o[k][3] << 16));
+            for (int r = 0; r < 4; ++r) {
+                const float e = acc[i][j][r];
+                if (a.planes == 1) o[0][r] = pack_exp<C::F16>(e);
+                else if constexpr (C::F16) split_half(e * kHalfScale, &o[0][r], &o[1][r]);
+                else split_bf16(e, &o[0][r], &o[1][r]);
             }
+            for (int k = 0; k < a.planes; ++k)
+                *reinterpret_cast<uint2*>(row + i * 16 + k * a.g_plane) =
+                    make_uint2((uint32_t)o[k][0] | ((uint32_t)o[k][1] << 16),
+                               (uint32_t)o[k][2] | ((uint32_t)o[k][3] << 16));
+        }
     }
 }
 
@@ -325,7 +362,7 @@ struct Rows {
     float* losses;          // [n], original order
     uint16_t* g;
     int64_t ldg, g_plane;
-    int32_t v, slots, slot_width, from, most, planes, f16;
+    int32_t v, slots, from, most, planes;
     float smoothing;
 };
 
@@ -336,6 +373,7 @@ __device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
 }
 
 constexpr int kGradThreads = 256;
+template <bool F16>
 __global__ __launch_bounds__(kGradThreads) void k_gradient_rows(const Rows a) {
     __shared__ float2 part[kGradThreads / 64];
     __shared__ float part_sum[kGradThreads / 64];
@@ -384,7 +422,7 @@ __global__ __launch_bounds__(kGradThreads) void k_gradient_rows(const Rows a) {
         a.losses[n] = loss;
     }
     if (!a.g) return;
-    float w = a.f16 ? kHalfScale : 1.0f;
+    float w = F16 ? kHalfScale : 1.0f;
     if (a.row_grad) {
         const float g = a.row_grad[n], top = a.meta->grad_max;
         w *= top == 0.0f ? 0.0f : g / top;
@@ -393,34 +431,28 @@ __global__ __launch_bounds__(kGradThreads) void k_gradient_rows(const Rows a) {
     if (y < 0) w = NAN;
     // the target's entry from its own logit: p - 1 without cancellation in 16 bits
     const float at_target = expm1f(tl - lse) + e - unit;
-    const float back = a.f16 ? 1.0f / kHalfScale : 1.0f;
+    const float back = F16 && a.planes == 2 ? 1.0f / kHalfScale : 1.0f;
     for (int c = blockIdx.y * kGradThreads + threadIdx.x; c < chunks; c += gridDim.y * kGradThreads) {
         const int v0 = c * 8;
         uint16_t* p = a.g + (int64_t)r * a.ldg + v0;
-        Vec<uint16_t, 8> x[3];
+        Vec<uint16_t, 8> x[2];
         if (v0 >= a.v) {
-            x[0] = x[1] = x[2] = Vec<uint16_t, 8>{};
+            x[0] = x[1] = Vec<uint16_t, 8>{};
         } else {
-            const float f = expf(stats[v0 / a.slot_width].x - lse) * back;
+            const float f = expf(stats[v0 / kSlot].x - lse) * back;
             for (int k = 0; k < a.planes; ++k) x[k] = vload<uint16_t, 8>(p + k * a.g_plane, 0);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 float q;
-                if (a.planes == 3) q = (to_f32(bf16_t{x[2].v[i]}) + to_f32(bf16_t{x[1].v[i]})) + to_f32(bf16_t{x[0].v[i]});
-                else if (a.f16) q = to_f32(f16_t{x[0].v[i]});
-                else q = to_f32(bf16_t{x[0].v[i]});
+                if (a.planes == 1) q = F16 ? unpack_exp<true>(x[0].v[i]) : unpack_exp<false>(x[0].v[i]);
+                else if (F16) q = to_f32(f16_t{x[0].v[i]}) + to_f32(f16_t{x[1].v[i]}) * (1.0f / kLowScale);
+                else q = to_f32(bf16_t{x[0].v[i]}) + to_f32(bf16_t{x[1].v[i]});
                 q = q * f - unit;
                 if (v0 + i == y) q = at_target;
                 q = v0 + i < a.v ? q * w : 0.0f;
-                if (a.planes == 3) {
-                    uint16_t t[3];
-                    split3(q, t);
-                    x[0].v[i] = t[0];
-                    x[1].v[i] = t[1];
-                    x[2].v[i] = t[2];
-                } else {
-                    x[0].v[i] = a.f16 ? from_f32<f16_t>(q).bits : from_f32<bf16_t>(q).bits;
-                }
+                if (a.planes == 1) x[0].v[i] = F16 ? from_f32<f16_t>(q).bits : from_f32<bf16_t>(q).bits;
+                else if (F16) split_half(q, &x[0].v[i], &x[1].v[i]);
+                else split_bf16(q, &x[0].v[i], &x[1].v[i]);
             }
         }
         for (int k = 0; k < a.planes; ++k) vstore(p + k * a.g_plane, 0, x[k]);
@@ -463,7 +495,8 @@ struct Grad {
 };
 
 __device__ __forceinline__ float grad_factor(const Grad& g) {
-    float f = g.dtype == GEFEN_F16 ? 1.0f / kHalfScale : 1.0f;
+    float f = g.dtype == GEFEN_BF16 ? 1.0f : 1.0f / kHalfScale;
+    if (g.dtype == GEFEN_F32) f = ldexpf(f, -half_exponent(g.meta->top[g.dh ? 1 : 0]));
     if (g.by_row) return f * g.meta->grad_max;
     if (g.grad) f *= *g.grad;
     if (g.mean) f = g.meta->count ? f / (float)g.meta->count : 0.0f;
@@ -508,36 +541,34 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_grad(const Grad g) {
     const int lb = logical_block(blockIdx.x, live);
     const int split = lb / (tiles_n * g.tiles_m);
     int ti, tj;
-    tile_of(lb - split * tiles_n * g.tiles_m, g.tiles_m, tiles_n, &ti, &tj);
+    tile_of<C::GROUP_M>(lb - split * tiles_n * g.tiles_m, g.tiles_m, tiles_n, &ti, &tj);
     const int m0 = ti * C::TM, n0 = tj * C::TN;
     const int steps = g.dh ? g.steps : (rows + C::BK - 1) / C::BK;
     const int k0 = (int)((int64_t)steps * split / g.splits), k1 = (int)((int64_t)steps * (split + 1) / g.splits);
-    f32x16 acc[WI][WJ];
+    f32x4 acc[WI][WJ];
     product_tile<C>(g.a, g.b, m0, n0, k0, k1, g.segs, smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = m0 + (wave / C::WAVES_N) * (32 * WI), wn = n0 + (wave % C::WAVES_N) * (32 * WJ);
+    const int wm = m0 + (wave / C::WAVES_N) * C::WM, wn = n0 + (wave % C::WAVES_N) * C::WN;
     const float factor = grad_factor(g);
 #pragma unroll
     for (int j = 0; j < WJ; ++j) {
-        const int n = wn + j * 32 + (lane & 31);
+        const int n = wn + j * 16 + (lane & 15);
         if (n >= n_all) continue;
         const int64_t row = g.dh ? g.map[g.from + n] : n;
 #pragma unroll
-        for (int i = 0; i < WI; ++i)
+        for (int i = 0; i < WI; ++i) {
+            const int m = wm + i * 16 + 4 * (lane >> 4);
+            if (m >= g.d) continue;
+            float v[4];
 #pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                const int m = wm + i * 32 + 8 * r4 + 4 * (lane >> 5);
-                if (m >= g.d) continue;
-                float v[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = acc[i][j][4 * r4 + r];
-                if (g.parts) {
-                    float* p = g.parts + ((int64_t)split * n_all + n) * g.d + m;
-                    for (int e = 0; e < min(4, g.d - m); ++e) p[e] = v[e];
-                } else {
-                    finish(g, row, n, m, v, factor);
-                }
+            for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r];
+            if (g.parts) {
+                float* p = g.parts + ((int64_t)split * n_all + n) * g.d + m;
+                for (int e = 0; e < min(4, g.d - m); ++e) p[e] = v[e];
+            } else {
+                finish(g, row, n, m, v, factor);
             }
+        }
     }
 }
 
@@ -564,13 +595,18 @@ namespace {
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
-template <bool F16> using LogitsBig = Cfg<F16, 256, 256, 4, 2, 64, 2, false, false>;
-template <bool F16> using LogitsSmall = Cfg<F16, 128, 128, 2, 2, 64, 2, false, false>;
-template <bool F16> using LogitsRow = Cfg<F16, 256, 32, 2, 1, 64, 4, false, false>;
-template <bool F16> using HiddenBig = Cfg<F16, 256, 256, 4, 2, 64, 2, true, false>;
-template <bool F16> using HiddenSmall = Cfg<F16, 128, 128, 2, 2, 64, 2, true, false>;
-template <bool F16> using WeightBig = Cfg<F16, 256, 256, 4, 2, 64, 2, true, true>;
-template <bool F16> using WeightSmall = Cfg<F16, 128, 128, 2, 2, 64, 2, true, true>;
+template <bool F16> using LogitsBig = Cfg<F16, 256, 256, 64, 128, 64, 2, false, false, 4>;
+template <bool F16> using LogitsSmall = Cfg<F16, 128, 128, 64, 64, 64, 2, false, false, 4>;
+template <bool F16> using LogitsRow = Cfg<F16, 256, 32, 64, 32, 64, 4, false, false, 4>;
+template <bool F16> using HiddenBig = Cfg<F16, 256, 256, 64, 128, 64, 2, true, false, 8>;
+template <bool F16> using HiddenSmall = Cfg<F16, 128, 128, 64, 64, 64, 2, true, false, 8>;
+template <bool F16> using WeightBig = Cfg<F16, 256, 256, 128, 64, 64, 2, true, true, 4>;
+template <bool F16> using WeightSmall = Cfg<F16, 128, 128, 64, 64, 64, 2, true, true, 4>;
+
+// Rows up to which G has two planes.  The gradients' products of so few rows take the
+// time of reading W and writing dW (4 V D bytes at 5 TB/s) rather than of their
+// 8 n V D operations (at 1.2 PFLOP/s: n = 120).
+constexpr int kTwoPlaneRows = 64;
 
 enum LogitsTile { kRowTile, kSmallTile, kBigTile };
 
@@ -578,11 +614,12 @@ enum LogitsTile { kRowTile, kSmallTile, kBigTile };
 struct Plan {
     int n, v, d, dtype;
     bool train, dh, dw, pack_w, smooth;
-    int planes, segs;
+    int planes;         // of G
+    bool halves;        // products of half-precision operands
     int64_t dp, ldg;
     int rows, pieces;   // rows of a piece
     LogitsTile tile;
-    int slot_width, slots;
+    int slots;
     bool dh_big, dw_big;
     int dh_splits, dw_splits;
     // byte offsets into the workspace
@@ -618,15 +655,15 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
     p->dw = t.grad_weight != nullptr;
     p->train = p->dh || p->dw;
     p->smooth = t.label_smoothing > 0.0;
-    p->planes = t.dtype == GEFEN_F32 ? 3 : 1;
-    p->segs = t.dtype == GEFEN_F32 ? 6 : 1;
+    p->planes = t.dtype == GEFEN_F32 || t.n <= kTwoPlaneRows ? 2 : 1;
+    p->halves = t.dtype != GEFEN_BF16;
     p->dp = up(t.d, 64);
     p->ldg = up(t.v, kRowAlign);
     p->pack_w = t.dtype == GEFEN_F32 || t.d % 64 != 0 || t.weight_col_stride != 1 || t.weight_row_stride % 8 != 0 ||
                 t.weight_row_stride > kMaxWidth || t.weight_row_stride < t.d || !aligned(t.weight, 16);
     // pieces of rows whose G and slots stay within the limit, of about the same size
     const int64_t limit = t.workspace_limit > 0 ? t.workspace_limit : GEFEN_LCE_DEFAULT_LIMIT;
-    const int64_t row_bytes = (p->train ? p->ldg * 2 * p->planes : 0) + up(t.v, 64) / 64 * 12;
+    const int64_t row_bytes = (p->train ? p->ldg * 2 * p->planes : 0) + up(t.v, kSlot) / kSlot * 12;
     const int64_t all = up(t.n > 0 ? t.n : 1, kRowAlign);
     const int64_t most = limit / row_bytes / kRowAlign * kRowAlign;
     const int64_t fit = most < kRowAlign ? kRowAlign : most;
@@ -637,8 +674,7 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
     const int64_t n = t.n < rows ? (t.n > 0 ? t.n : 1) : rows;
     const int64_t tiles = up(t.v, 256) / 256 * (up(n, 256) / 256);
     p->tile = n <= 32 ? kRowTile : tiles >= kCus / 2 ? kBigTile : kSmallTile;
-    p->slot_width = p->tile == kBigTile ? 128 : 64;
-    p->slots = (int)(up(t.v, p->slot_width) / p->slot_width);
+    p->slots = (int)(up(t.v, kSlot) / kSlot);
     split_rule(t.d, n, up(t.v, 64) / 64, &p->dh_big, &p->dh_splits);
     split_rule(t.d, t.v, up(n, 64) / 64, &p->dw_big, &p->dw_splits);
 
@@ -764,8 +800,15 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     pk.plane = (int64_t)x_rows * p.dp;
     pk.map = map;
     pk.meta = meta;
+    pk.which = 0;
     pk.zero_rows = t.grad_hidden;
     pk.zero_losses = losses;
+    if (pk.f32) {
+        Top tx{static_cast<const float*>(t.hidden), t.hidden_row_stride, t.hidden_col_stride, p.n, p.d, map, meta, 0};
+        hipLaunchKernelGGL(k_top, dim3(p.n < 2048 ? (p.n ? p.n : 1) : 2048), dim3(256), 0, st, tx);
+        Top tw{static_cast<const float*>(t.weight), t.weight_row_stride, t.weight_col_stride, p.v, p.d, nullptr, meta, 1};
+        hipLaunchKernelGGL(k_top, dim3(p.v < 2048 ? p.v : 2048), dim3(256), 0, st, tw);
+    }
     const unsigned pack_y = (unsigned)((p.dp + 2047) / 2048);
     hipLaunchKernelGGL(k_pack, dim3((unsigned)x_rows, pack_y), dim3(256), 0, st, pk);
     if (p.pack_w) {
@@ -779,13 +822,16 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         pw.f32 = pk.f32;
         pw.dst = wp;
         pw.plane = (int64_t)p.v * p.dp;
+        pw.meta = meta;
+        pw.which = 1;
         hipLaunchKernelGGL(k_pack, dim3((unsigned)p.v, pack_y), dim3(256), 0, st, pw);
     }
     Operand w{};
     w.p = p.pack_w ? wp : static_cast<const uint16_t*>(t.weight);
     w.ld = p.pack_w ? p.dp : t.weight_row_stride;
     w.plane = (int64_t)p.v * p.dp;
-    w.finite = pk.f32 ? kPackPlanes - 1 : 0;
+    // segments of the logits' product: low x high, high x low, high x high
+    w.planes = pk.f32 ? 1 | 2 << 2 | 0 << 4 : 0;
     w.rows = p.v;
     w.cols = (int)p.dp;
 
@@ -796,7 +842,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         xo.p = x + (int64_t)from * p.dp;
         xo.ld = p.dp;
         xo.plane = pk.plane;
-        xo.finite = w.finite;
+        xo.planes = pk.f32 ? 2 | 1 << 2 | 0 << 4 : 0;
         xo.rows = p.rows;
         xo.cols = (int)p.dp;
         Logits l{};
@@ -804,7 +850,8 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         l.x = xo;
         l.v = p.v;
         l.steps = (int)(p.dp / 64);
-        l.segs = p.segs;
+        l.segs = pk.f32 ? 3 : 1;
+        l.f32 = pk.f32;
         l.from = from;
         l.most = most;
         l.slots = p.slots;
@@ -818,7 +865,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         l.g_plane = (int64_t)p.rows * p.ldg;
         l.planes = p.planes;
         Grad g{};
-        const bool f16 = t.dtype == GEFEN_F16;
+        const bool f16 = p.halves;
         if (most > 0) {
             if (f16) launch_products<true>(p, 0, l, g, most, st);
             else launch_products<false>(p, 0, l, g, most, st);
@@ -836,11 +883,9 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
             r.g_plane = l.g_plane;
             r.v = p.v;
             r.slots = p.slots;
-            r.slot_width = p.slot_width;
             r.from = from;
             r.most = most;
             r.planes = p.planes;
-            r.f16 = f16;
             r.smoothing = (float)t.label_smoothing;
             // a row per workgroup, or parts of it where the rows do not fill the chip
             const int64_t rows_up = p.train ? up(most, 64) : most;
@@ -848,17 +893,21 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
             const int64_t chunks = p.ldg / 8 / kGradThreads;
             if (parts > chunks) parts = chunks;
             if (parts < 1) parts = 1;
-            hipLaunchKernelGGL(k_gradient_rows, dim3((unsigned)rows_up, (unsigned)parts), dim3(kGradThreads), 0, st, r);
+            const dim3 grid((unsigned)rows_up, (unsigned)parts);
+            if (f16) hipLaunchKernelGGL(k_gradient_rows<true>, grid, dim3(kGradThreads), 0, st, r);
+            else hipLaunchKernelGGL(k_gradient_rows<false>, grid, dim3(kGradThreads), 0, st, r);
         }
         if (!p.train) continue;
         Operand go{};
         go.p = gbuf;
         go.ld = p.ldg;
         go.plane = l.g_plane;
+        // with W or hidden of one plane: low, high; float32: as hidden in the logits' product
+        go.planes = pk.f32 ? 0 | 1 << 2 | 0 << 4 : p.planes == 2 ? 1 | 0 << 2 : 0;
         go.rows = p.rows;
         go.cols = (int)p.ldg;
         g.d = p.d;
-        g.segs = p.segs;
+        g.segs = pk.f32 ? 3 : p.planes;
         g.from = from;
         g.most = most;
         g.map = map;
@@ -883,6 +932,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         }
         if (p.dw) {
             g.a = xo;
+            g.a.planes = w.planes;
             g.b = go;
             g.dh = 0;
             g.n = p.v;

@@ -3,8 +3,8 @@
     loss = linear_cross_entropy(hidden, lm_head.weight, targets)     # F.cross_entropy(hidden @ W^T, targets)
     loss.backward()
 
-The N x V logits never exist: the library keeps 16-bit values of a bounded piece of the
-positions at a time (float32 ones 24 bits) and works on positions that have a loss only.
+The N x V logits never exist: the library keeps 16 bits per logit of a bounded piece of the
+positions at a time (float32 ones 22) and works on positions that have a loss only.
 
 With ``reduction`` "mean" or "sum" and bfloat16 or float32 operands the gradients are
 formed in the forward call, where the kept values still are (three products instead of

@@ -469,8 +469,8 @@ int gefen_scale_gradients(const gefen_gradient_task* tasks, int num_tasks, const
  *   loss_n = lse_n - (1 - e) l[n, y_n] - (e / V) sum_v l[n, v],   lse_n = log sum_v exp l[n, v]
  * with e = label_smoothing; rows whose target is ignore_index have no loss, and nothing
  * they hold is read into a result.  A target outside [0, V) gives a NaN loss (and NaN
- * gradients).  Products accumulate in float32; exp(l - max) is rounded once to 16 bits
- * for the gradients' products (float32 operands keep 24 bits throughout). */
+ * gradients).  Products accumulate in float32; exp(l - max) - target is rounded to dtype
+ * on its way to the gradients (float32 operands keep 22 bits throughout). */
 enum { GEFEN_REDUCE_NONE = 0, GEFEN_REDUCE_MEAN = 1, GEFEN_REDUCE_SUM = 2 };
 /* workspace_limit = 0: what the values kept for the gradients may take */
 #define GEFEN_LCE_DEFAULT_LIMIT ((int64_t)4 << 30)
