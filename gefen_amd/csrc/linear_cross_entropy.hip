@@ -44,6 +44,7 @@
 namespace gefen {
 namespace lce {
 
+constexpr float kLog2E = 1.44269504088896340736f;
 constexpr float kHalfScale = 32768.0f;  // of a half-precision G
 constexpr int kSlot = 64;               // columns that share a maximum
 constexpr int kRowAlign = 256;          // rows of a piece, columns of G
@@ -129,11 +130,13 @@ __device__ __forceinline__ void split_bf16(float x, uint16_t* hi, uint16_t* lo) 
 // is brought down by a product with a power of two (subnormal results are rounded by the
 // hardware), and the mantissa is rounded to nearest.  Relative error 2^-13 down to 2^-14
 // (bf16: 2^-11 down to 2^-62), 2^-27 absolute below.
+// Two of them, low half first; a bf16 one comes scaled by 2^-64 already.
 template <bool F16>
-__device__ __forceinline__ uint16_t pack_exp(float e) {
+__device__ __forceinline__ uint32_t pack_exp2(float a, float b) {
     constexpr int drop = F16 ? 11 : 13;
-    const uint32_t u = __float_as_uint(e * (F16 ? 0x1p-112f : 0x1p-64f));
-    return (uint16_t)((u + ((1u << (drop - 1)) - 1) + ((u >> drop) & 1u)) >> drop);
+    const uint32_t x = __float_as_uint(F16 ? a * 0x1p-112f : a) + (1u << (drop - 1));
+    const uint32_t y = __float_as_uint(F16 ? b * 0x1p-112f : b) + (1u << (drop - 1));
+    return (x >> drop & 0xffffu) | (y >> drop << 16);
 }
 template <bool F16>
 __device__ __forceinline__ float unpack_exp(uint16_t x) {
@@ -156,23 +159,41 @@ struct Top {
     int32_t which;
 };
 __global__ __launch_bounds__(256) void k_top(const Top t) {
-    const int rows = t.map ? t.meta->count : t.n;
+    const uint32_t per = (uint32_t)(t.d + 7) / 8;  // chunks of eight columns a row
+    const int64_t all = (int64_t)(t.map ? t.meta->count : t.n) * per;
     uint32_t top = 0;
-    for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+    auto see = [&](float x) {
+        const uint32_t u = abs_key(x);
+        top = u < 0x7f800000u && u > top ? u : top;
+    };
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < all; q += (int64_t)gridDim.x * 256) {
+        const int64_t r = q / per;
+        const int c = (int)(q - r * per) * 8;
         const float* s = t.src + (int64_t)(t.map ? t.map[r] : r) * t.row_stride;
-        for (int c = threadIdx.x; c < t.d; c += 256) {
-            const uint32_t u = abs_key(s[(int64_t)c * t.col_stride]);
-            top = u < 0x7f800000u && u > top ? u : top;
+        if (t.col_stride == 1 && c + 8 <= t.d) {
+            const AnyVec<float, 8> x = *reinterpret_cast<const AnyVec<float, 8>*>(s + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) see(x.v[e]);
+        } else {
+            for (int e = c; e < min(c + 8, t.d); ++e) see(s[(int64_t)e * t.col_stride]);
         }
     }
+    // one atomic per workgroup: eight thousand on one address took 100 us
+    __shared__ uint32_t part[4];
     top = wave_group_max_u32(top, 64);
-    if ((threadIdx.x & 63) == 0) atomicMax(&t.meta->top[t.which], top);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        top = max(max(part[0], part[1]), max(part[2], part[3]));
+        if (top > 0) atomicMax(&t.meta->top[t.which], top);
+    }
 }
 
 // Rows of a matrix of any strides as the products read them: dp = D rounded up to 64
-// columns, zero-padded, one plane or those of a float32 operand, scaled.  With a map: row r is src row map[r]
-// for r < meta->count and zero up to the next multiple of kRowAlign, and the rows that
-// take no part get a zero gradient and a zero loss.
+// columns, zero-padded, one plane or those of a float32 operand, scaled.  With a map: row
+// r is src row map[r] for r < meta->count and zero up to the next multiple of kRowAlign,
+// and the rows that take no part get a zero gradient and a zero loss.  A thread moves
+// eight columns of a row.
 constexpr int kPackPlanes = 3;  // of a float32 operand: high, low, high where finite
 struct Pack {
     const void* src;
@@ -181,64 +202,65 @@ struct Pack {
     int32_t f32;
     uint16_t* dst;
     int64_t plane;
+    int32_t rows;       // of dst
     const int32_t* map;
     const Meta* meta;
     int32_t which;      // float32: whose largest magnitude in meta->top
-    void* zero_rows;    // [n, d] gradient, rows of d elements of `size` bytes (may be null)
+    void* zero_rows;    // [n, d] gradient (may be null)
     float* zero_losses;  // [n] (may be null)
 };
 __global__ __launch_bounds__(256) void k_pack(const Pack p) {
-    const int r = blockIdx.x;
-    int64_t row = r;
-    bool live = r < p.n;
-    if (p.map) {
-        const int count = p.meta->count;
-        live = r < count;
-        if (r < p.n) row = p.map[r];
-        if (!live && r < p.n) {
-            if (p.zero_losses && threadIdx.x == 0 && blockIdx.y == 0) p.zero_losses[row] = 0.0f;
-            if (p.zero_rows) {
-                const int col = (int)(blockIdx.y * 256 + threadIdx.x) * 8;
-                for (int e = col; e < min(col + 8, p.d); ++e) {
+    const uint32_t per = (uint32_t)p.dp / 8;
+    const int count = p.map ? p.meta->count : p.n;
+    const int ends = p.map ? (count + kRowAlign - 1) / kRowAlign * kRowAlign : p.rows;
+    const int64_t all = (int64_t)(ends > p.n ? ends : p.n) * per;
+    const int ex = p.f32 ? half_exponent(p.meta->top[p.which]) : 0;
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < all; q += (int64_t)gridDim.x * 256) {
+        const int r = (int)(q / per);
+        const int c0 = (int)(q - (int64_t)r * per) * 8;
+        const int64_t row = p.map && r < p.n ? p.map[r] : r;
+        const bool live = r < count;
+        if (p.map && !live && r < p.n) {
+            if (p.zero_losses && c0 == 0) p.zero_losses[row] = 0.0f;
+            if (p.zero_rows)
+                for (int e = c0; e < min(c0 + 8, p.d); ++e) {
                     if (p.f32) static_cast<float*>(p.zero_rows)[row * p.d + e] = 0.0f;
                     else static_cast<uint16_t*>(p.zero_rows)[row * p.d + e] = 0;
                 }
-            }
         }
-        if (r >= (count + kRowAlign - 1) / kRowAlign * kRowAlign) return;
-    }
-    const int c0 = (int)(blockIdx.y * 256 + threadIdx.x) * 8;
-    if (c0 >= p.dp) return;
-    uint16_t out[kPackPlanes][8] = {};
-    if (live) {
-        if (p.f32) {
-            const int ex = half_exponent(p.meta->top[p.which]);
-            const float* s = static_cast<const float*>(p.src) + row * p.row_stride;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (c0 + e < p.d) {
-                    split_half(ldexpf(s[(int64_t)(c0 + e) * p.col_stride], ex), &out[0][e], &out[1][e]);
-                    out[2][e] = (out[0][e] & 0x7c00) == 0x7c00 ? 0 : out[0][e];
-                }
-        } else {
-            const uint16_t* s = static_cast<const uint16_t*>(p.src) + row * p.row_stride;
+        if (r >= ends) continue;
+        Vec<uint16_t, 8> out[kPackPlanes] = {};
+        if (live && p.f32) {
+            const float* s = static_cast<const float*>(p.src) + row * p.row_stride + (int64_t)c0 * p.col_stride;
+            AnyVec<float, 8> x = {};
             if (p.col_stride == 1 && c0 + 8 <= p.d) {
-                const AnyVec<uint16_t, 8> x = *reinterpret_cast<const AnyVec<uint16_t, 8>*>(s + c0);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) out[0][e] = x.v[e];
+                x = *reinterpret_cast<const AnyVec<float, 8>*>(s);
             } else {
-#pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (c0 + e < p.d) out[0][e] = s[(int64_t)(c0 + e) * p.col_stride];
+                    if (c0 + e < p.d) x.v[e] = s[e * p.col_stride];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                split_half(ldexpf(x.v[e], ex), &out[0].v[e], &out[1].v[e]);
+                out[2].v[e] = (out[0].v[e] & 0x7c00) == 0x7c00 ? 0 : out[0].v[e];
+            }
+        } else if (live) {
+            const uint16_t* s = static_cast<const uint16_t*>(p.src) + row * p.row_stride + (int64_t)c0 * p.col_stride;
+            if (p.col_stride == 1 && c0 + 8 <= p.d) {
+                const AnyVec<uint16_t, 8> x = *reinterpret_cast<const AnyVec<uint16_t, 8>*>(s);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) out[0].v[e] = x.v[e];
+            } else {
+                for (int e = 0; e < 8; ++e)
+                    if (c0 + e < p.d) out[0].v[e] = s[e * p.col_stride];
             }
         }
-    }
-    const int planes = p.f32 ? kPackPlanes : 1;
-    for (int k = 0; k < planes; ++k) {
-        Vec<uint16_t, 8> x;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x.v[e] = out[k][e];
-        vstore(p.dst + k * p.plane, (int64_t)r * p.dp + c0, x);
+        uint16_t* d = p.dst + (int64_t)r * p.dp + c0;
+        vstore(d, 0, out[0]);
+        if (p.f32) {
+            vstore(d + p.plane, 0, out[1]);
+            vstore(d + 2 * p.plane, 0, out[2]);
+        }
     }
 }
 
@@ -257,7 +279,10 @@ struct Logits {
     int32_t planes, f32;
 };
 
-template <typename C>
+// What a logits' product keeps for the gradients: nothing, 16 packed bits, two planes.
+enum Keep { kKeepNone, kKeepPacked, kKeepPlanes };
+
+template <typename C, int KEEP>
 __global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
     constexpr int WI = C::WI, WJ = C::WJ;
     __shared__ __attribute__((aligned(1024))) uint16_t smem[C::NST * C::STAGE];
@@ -276,8 +301,11 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
     const int hi = 4 * (lane >> 4);
     const int slot = wm / kSlot;
     static_assert(C::WM == kSlot, "a wave's columns are a slot");
-    if (wm >= a.v && !a.g) return;
-    const int ex = a.f32 ? -half_exponent(a.meta->top[0]) - half_exponent(a.meta->top[1]) : 0;
+    if (wm >= a.v && KEEP == kKeepNone) return;
+    const bool f32 = KEEP != kKeepPacked && a.f32;
+    // exp(x) times 2^-64 when the packed bf16 format takes it as it is
+    constexpr float kDown = KEEP == kKeepPacked && !C::F16 ? 64.0f : 0.0f;
+    const int ex = f32 ? -half_exponent(a.meta->top[0]) - half_exponent(a.meta->top[1]) : 0;
     const bool part = wm + C::WM > a.v;  // the last columns end inside this wave's
 #pragma unroll
     for (int j = 0; j < WJ; ++j) {
@@ -287,7 +315,7 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
         for (int i = 0; i < WI; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                if (a.f32) acc[i][j][r] = ldexpf(acc[i][j][r], ex);
+                if (f32) acc[i][j][r] = ldexpf(acc[i][j][r], ex);
                 if (part && wm + i * 16 + hi + r >= a.v) acc[i][j][r] = -INFINITY;
                 m = fmaxf(m, acc[i][j][r]);  // skips NaN, which the sum of exp keeps
             }
@@ -318,10 +346,12 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
         for (int i = 0; i < WI; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
+                // the difference first: exact where it matters, however large the logits
                 const float x = acc[i][j][r] - ref;
-                acc[i][j][r] = a.f32 ? expf(x) : __expf(x);
+                acc[i][j][r] = f32 ? expf(x) : __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2E, -kDown));
                 s += acc[i][j][r];
             }
+        if (kDown != 0.0f) s *= 0x1p64f;
         s += __shfl_xor(s, 16, 64);
         s += __shfl_xor(s, 32, 64);
         if (n < rows && lane < 16 && wm < a.v) {
@@ -329,23 +359,28 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
             a.stats[at] = make_float2(m, s);
             if (a.sums) a.sums[at] = sum;
         }
-        if (!a.g) continue;
+        if constexpr (KEEP == kKeepNone) continue;
         // rows past the piece's end stay inside the workspace (it holds whole tiles)
         uint16_t* row = a.g + (int64_t)n * a.ldg + wm + hi;
 #pragma unroll
         for (int i = 0; i < WI; ++i) {
-            uint16_t o[2][4];
+            uint16_t* to = row + i * 16;
+            if constexpr (KEEP == kKeepPacked) {
+                *reinterpret_cast<uint2*>(to) = make_uint2(pack_exp2<C::F16>(acc[i][j][0], acc[i][j][1]),
+                                                           pack_exp2<C::F16>(acc[i][j][2], acc[i][j][3]));
+            } else {
+                uint16_t o[2][4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float e = acc[i][j][r];
-                if (a.planes == 1) o[0][r] = pack_exp<C::F16>(e);
-                else if constexpr (C::F16) split_half(e * kHalfScale, &o[0][r], &o[1][r]);
-                else split_bf16(e, &o[0][r], &o[1][r]);
+                for (int r = 0; r < 4; ++r) {
+                    if constexpr (C::F16) split_half(acc[i][j][r] * kHalfScale, &o[0][r], &o[1][r]);
+                    else split_bf16(acc[i][j][r], &o[0][r], &o[1][r]);
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    *reinterpret_cast<uint2*>(to + k * a.g_plane) =
+                        make_uint2((uint32_t)o[k][0] | ((uint32_t)o[k][1] << 16),
+                                   (uint32_t)o[k][2] | ((uint32_t)o[k][3] << 16));
             }
-            for (int k = 0; k < a.planes; ++k)
-                *reinterpret_cast<uint2*>(row + i * 16 + k * a.g_plane) =
-                    make_uint2((uint32_t)o[k][0] | ((uint32_t)o[k][1] << 16),
-                               (uint32_t)o[k][2] | ((uint32_t)o[k][3] << 16));
         }
     }
 }
@@ -410,15 +445,15 @@ __global__ __launch_bounds__(kGradThreads) void k_gradient_rows(const Rows a) {
         st = join_stats(st, part[w]);
         sum += part_sum[w];
     }
-    const float lse = st.x + logf(st.y);
+    // lse = m + log s, kept apart: differences to m stay exact for large logits
+    const float log_s = logf(st.y);
     const int y = a.tgt[a.from + r];
     const float tl = y >= 0 ? a.target_logit[a.from + r] : NAN;
     const float e = a.smoothing;
     const int64_t n = a.map[a.from + r];
     if (a.losses && blockIdx.y == 0 && threadIdx.x == 0) {
-        // (1 - e) (lse - l_y) + e (lse - mean l): the first difference is exact to a rounding
-        float loss = (1.0f - e) * (lse - tl);
-        if (e > 0.0f) loss += e * (lse - sum / (float)a.v);
+        float loss = (1.0f - e) * ((st.x - tl) + log_s);
+        if (e > 0.0f) loss += e * ((st.x - sum / (float)a.v) + log_s);
         a.losses[n] = loss;
     }
     if (!a.g) return;
@@ -430,32 +465,46 @@ __global__ __launch_bounds__(kGradThreads) void k_gradient_rows(const Rows a) {
     const float unit = e > 0.0f ? e / (float)a.v : 0.0f;
     if (y < 0) w = NAN;
     // the target's entry from its own logit: p - 1 without cancellation in 16 bits
-    const float at_target = expm1f(tl - lse) + e - unit;
+    const float at_target = expm1f((tl - st.x) - log_s) + e - unit;
     const float back = F16 && a.planes == 2 ? 1.0f / kHalfScale : 1.0f;
-    for (int c = blockIdx.y * kGradThreads + threadIdx.x; c < chunks; c += gridDim.y * kGradThreads) {
-        const int v0 = c * 8;
-        uint16_t* p = a.g + (int64_t)r * a.ldg + v0;
-        Vec<uint16_t, 8> x[2];
-        if (v0 >= a.v) {
-            x[0] = x[1] = Vec<uint16_t, 8>{};
-        } else {
-            const float f = expf(stats[v0 / kSlot].x - lse) * back;
-            for (int k = 0; k < a.planes; ++k) x[k] = vload<uint16_t, 8>(p + k * a.g_plane, 0);
+    constexpr int kBatch = 4;  // chunks in flight per thread
+    const int stride = gridDim.y * kGradThreads;
+    uint16_t* const row = a.g + (int64_t)r * a.ldg;
+    for (int c0 = blockIdx.y * kGradThreads + threadIdx.x; c0 < chunks; c0 += kBatch * stride) {
+        Vec<uint16_t, 8> x[kBatch][2];
+        float top[kBatch];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float q;
-                if (a.planes == 1) q = F16 ? unpack_exp<true>(x[0].v[i]) : unpack_exp<false>(x[0].v[i]);
-                else if (F16) q = to_f32(f16_t{x[0].v[i]}) + to_f32(f16_t{x[1].v[i]}) * (1.0f / kLowScale);
-                else q = to_f32(bf16_t{x[0].v[i]}) + to_f32(bf16_t{x[1].v[i]});
-                q = q * f - unit;
-                if (v0 + i == y) q = at_target;
-                q = v0 + i < a.v ? q * w : 0.0f;
-                if (a.planes == 1) x[0].v[i] = F16 ? from_f32<f16_t>(q).bits : from_f32<bf16_t>(q).bits;
-                else if (F16) split_half(q, &x[0].v[i], &x[1].v[i]);
-                else split_bf16(q, &x[0].v[i], &x[1].v[i]);
-            }
+        for (int i = 0; i < kBatch; ++i) {
+            const int c = min(c0 + i * stride, chunks - 1);
+            top[i] = stats[min(c * 8, a.v - 1) / kSlot].x;
+            x[i][0] = vload<uint16_t, 8>(row, (int64_t)c * 8);
+            if (a.planes == 2) x[i][1] = vload<uint16_t, 8>(row + a.g_plane, (int64_t)c * 8);
         }
-        for (int k = 0; k < a.planes; ++k) vstore(p + k * a.g_plane, 0, x[k]);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int c = c0 + i * stride, v0 = c * 8;
+            if (c >= chunks) break;
+            const float f = expf((top[i] - st.x) - log_s) * back;
+            Vec<uint16_t, 8>& hi = x[i][0];
+            Vec<uint16_t, 8>& lo = x[i][1];
+            const bool hit = y >= v0 && y < v0 + 8, part = v0 + 8 > a.v;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float q;
+                if (a.planes == 1) q = unpack_exp<F16>(hi.v[e]);
+                else if (F16) q = to_f32(f16_t{hi.v[e]}) + to_f32(f16_t{lo.v[e]}) * (1.0f / kLowScale);
+                else q = to_f32(bf16_t{hi.v[e]}) + to_f32(bf16_t{lo.v[e]});
+                q = q * f - unit;
+                if (hit && v0 + e == y) q = at_target;
+                q *= w;
+                if (part && v0 + e >= a.v) q = 0.0f;
+                if (a.planes == 1) hi.v[e] = F16 ? from_f32<f16_t>(q).bits : from_f32<bf16_t>(q).bits;
+                else if (F16) split_half(q, &hi.v[e], &lo.v[e]);
+                else split_bf16(q, &hi.v[e], &lo.v[e]);
+            }
+            vstore(row, (int64_t)c * 8, hi);
+            if (a.planes == 2) vstore(row + a.g_plane, (int64_t)c * 8, lo);
+        }
     }
 }
 
@@ -475,11 +524,11 @@ __global__ __launch_bounds__(1024) void k_loss(const float* __restrict__ losses,
     }
 }
 
-// A gradient's product: out[n, m] = factor * (prev[n, m] + sum_k A[m, k] B[n, k]) for
-// m < D, rows n of the piece (dh, through the map) or of the vocabulary (dW).
+// A gradient's product: out[n, m] = factor * sum_k A[m, k] B[n, k] for m < D, rows n of
+// the piece (dh, through the map) or of the vocabulary (dW).
 struct Grad {
     Operand a, b;
-    int32_t d, tiles_m, steps, segs, splits;
+    int32_t d, tiles_m, steps, segs;
     int32_t n;              // rows of the result (dW: V); dh: the piece's, from meta
     int32_t dh;             // dh: rows through the map, all of K; dW: K = the piece's rows
     int32_t from, most;
@@ -487,9 +536,11 @@ struct Grad {
     const Meta* meta;
     const float* grad;      // gradient of the loss (null: 1)
     int32_t mean, by_row;   // by_row: G is scaled by 1 / meta->grad_max
-    float* parts;           // [splits][n][d] float32 (splits > 1), to be joined by k_join
-    float* sum;             // running float32 sum over the pieces (null: one piece)
-    int32_t first, last;    // piece of the sum
+    int32_t slots;          // workgroups that fill the chip
+    int32_t most_parts;     // partial tiles that `parts` holds
+    float* parts;           // [cut][tile of the rest][TN][TM]
+    float* sum;             // float32 sum over the pieces (null: one piece)
+    int32_t first;          // piece of the sum
     void* out;
     int32_t dtype;
 };
@@ -502,30 +553,89 @@ __device__ __forceinline__ float grad_factor(const Grad& g) {
     if (g.mean) f = g.meta->count ? f / (float)g.meta->count : 0.0f;
     return f;
 }
-// four results of row n from column m: cnt of them are inside
-__device__ __forceinline__ void finish(const Grad& g, int64_t row, int64_t n, int m, float v[4], float factor) {
-    const int cnt = min(4, g.d - m);
-    if (g.sum) {
-        float* s = g.sum + n * g.d + m;
-        for (int e = 0; e < cnt; ++e) {
-            if (!g.first) v[e] += s[e];
-            if (!g.last) s[e] = v[e];
+
+// How the tiles of a product meet the chip: whole rounds of it tile by tile, and the
+// `rest` of the tiles with K cut into `cuts` equal parts, each left in float32 for k_join.
+// All tiles of one part run together, so that they share what they read (dealing the rest's
+// K steps out evenly instead, as one stretch per workgroup, balances better but left no
+// two workgroups at the same K: dh of 2796 x 2048 over 128256 2.0 ms against 1.63 with two
+// equal parts).  The number of parts is the one of the least estimated time, in K steps of
+// a full chip: rounds times the steps of a part and 4 for its ends, and 0.06 for the
+// traffic of each partial tile.  The rows that take part are only known on the device, so
+// this is worked out there; the host bounds it.
+constexpr int kMostCuts = 16;
+constexpr int kLeastSteps = 4;  // of a part
+struct Deal {
+    int n_all, tiles_n, steps, full, rest;
+};
+template <typename C>
+__device__ __forceinline__ Deal deal_of(const Grad& g) {
+    const int rows = piece_rows(g.meta, g.from, g.most);
+    Deal d;
+    d.n_all = g.dh ? rows : g.n;
+    d.tiles_n = (d.n_all + C::TN - 1) / C::TN;
+    d.steps = g.dh ? g.steps : (rows + C::BK - 1) / C::BK;
+    const int tiles = d.tiles_n * g.tiles_m;
+    d.rest = tiles & (g.slots - 1);  // slots: a power of two
+    d.full = tiles - d.rest;
+    return d;
+}
+__device__ __forceinline__ int cuts_of(const Grad& g, const Deal& d) {
+    int cuts = 1;
+    const float run = (float)(d.steps * g.segs);
+    float best = run + 4.0f;
+    for (int c = 2; c <= kMostCuts && d.rest * c <= g.most_parts && d.steps >= kLeastSteps * c; ++c) {
+        const int rounds = (d.rest * c + g.slots - 1) / g.slots;
+        const float cost = (float)rounds * (run / (float)c + 4.0f) + 0.06f * (float)(d.rest * c);
+        if (cost < best) {
+            best = cost;
+            cuts = c;
         }
-        if (!g.last) return;
     }
+    return cuts;
+}
+
+// cnt (1 to 4) results of output row `row`, from column m, as OUT: added to the sum over
+// the pieces (plain float32), or times the factor in the result's type.
+enum Out { kOutSum, kOutF32, kOut16 };
+template <bool F16, int OUT>
+__device__ __forceinline__ void finish(const Grad& g, int64_t row, int m, int cnt, f32x4 v, float factor) {
     const int64_t at = row * g.d + m;
-    if (g.dtype == GEFEN_F32) {
+    if constexpr (OUT == kOutSum) {
+        float* s = g.sum + at;
+        for (int e = 0; e < cnt; ++e) s[e] = g.first ? v[e] : s[e] + v[e];
+    } else if constexpr (OUT == kOutF32) {
+        v *= factor;
         float* o = static_cast<float*>(g.out) + at;
-        if (cnt == 4) *reinterpret_cast<AnyVec<float, 4>*>(o) = AnyVec<float, 4>{{v[0] * factor, v[1] * factor, v[2] * factor, v[3] * factor}};
-        else for (int e = 0; e < cnt; ++e) o[e] = v[e] * factor;
+        if (cnt == 4) {
+            *reinterpret_cast<AnyVec<float, 4>*>(o) = AnyVec<float, 4>{{v[0], v[1], v[2], v[3]}};
+        } else {
+            for (int e = 0; e < cnt; ++e) o[e] = v[e];
+        }
     } else {
         AnyVec<uint16_t, 4> x;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            x.v[e] = g.dtype == GEFEN_F16 ? from_f32<f16_t>(v[e] * factor).bits : from_f32<bf16_t>(v[e] * factor).bits;
+            x.v[e] = F16 ? from_f32<f16_t>(v[e] * factor).bits : from_f32<bf16_t>(v[e] * factor).bits;
         uint16_t* o = static_cast<uint16_t*>(g.out) + at;
-        if (cnt == 4) *reinterpret_cast<AnyVec<uint16_t, 4>*>(o) = x;
-        else for (int e = 0; e < cnt; ++e) o[e] = x.v[e];
+        if (cnt == 4) {
+            *reinterpret_cast<AnyVec<uint16_t, 4>*>(o) = x;
+        } else {
+            for (int e = 0; e < cnt; ++e) o[e] = x.v[e];
+        }
+    }
+}
+template <typename C, int OUT>
+__device__ __forceinline__ void finish_tile(const Grad& g, int n_all, int m, int n0, const f32x4 (&acc)[C::WI][C::WJ]) {
+    const float factor = grad_factor(g);
+#pragma unroll
+    for (int j = 0; j < C::WJ; ++j) {
+        const int n = n0 + j * 16;
+        if (n >= n_all) continue;
+        const int64_t row = g.dh ? g.map[g.from + n] : n;
+#pragma unroll
+        for (int i = 0; i < C::WI; ++i)
+            if (m + i * 16 < g.d) finish<C::F16, OUT>(g, row, m + i * 16, min(4, g.d - m - i * 16), acc[i][j], factor);
     }
 }
 
@@ -533,60 +643,82 @@ template <typename C>
 __global__ __launch_bounds__(C::TT, C::EU) void k_grad(const Grad g) {
     constexpr int WI = C::WI, WJ = C::WJ;
     __shared__ __attribute__((aligned(1024))) uint16_t smem[C::NST * C::STAGE];
-    const int rows = piece_rows(g.meta, g.from, g.most);
-    const int n_all = g.dh ? rows : g.n;
-    const int tiles_n = (n_all + C::TN - 1) / C::TN;
-    const int live = tiles_n * g.tiles_m * g.splits;
-    if ((int)blockIdx.x >= live) return;
-    const int lb = logical_block(blockIdx.x, live);
-    const int split = lb / (tiles_n * g.tiles_m);
-    int ti, tj;
-    tile_of<C::GROUP_M>(lb - split * tiles_n * g.tiles_m, g.tiles_m, tiles_n, &ti, &tj);
-    const int m0 = ti * C::TM, n0 = tj * C::TN;
-    const int steps = g.dh ? g.steps : (rows + C::BK - 1) / C::BK;
-    const int k0 = (int)((int64_t)steps * split / g.splits), k1 = (int)((int64_t)steps * (split + 1) / g.splits);
-    f32x4 acc[WI][WJ];
-    product_tile<C>(g.a, g.b, m0, n0, k0, k1, g.segs, smem, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = m0 + (wave / C::WAVES_N) * C::WM, wn = n0 + (wave % C::WAVES_N) * C::WN;
-    const float factor = grad_factor(g);
-#pragma unroll
-    for (int j = 0; j < WJ; ++j) {
-        const int n = wn + j * 16 + (lane & 15);
-        if (n >= n_all) continue;
-        const int64_t row = g.dh ? g.map[g.from + n] : n;
-#pragma unroll
-        for (int i = 0; i < WI; ++i) {
-            const int m = wm + i * 16 + 4 * (lane >> 4);
-            if (m >= g.d) continue;
-            float v[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r];
-            if (g.parts) {
-                float* p = g.parts + ((int64_t)split * n_all + n) * g.d + m;
-                for (int e = 0; e < min(4, g.d - m); ++e) p[e] = v[e];
-            } else {
-                finish(g, row, n, m, v, factor);
-            }
-        }
+    const Deal deal = deal_of<C>(g);
+    const int b = blockIdx.x;
+    int u, tile, cut = 0, cuts = 1;
+    if (b < deal.full) {
+        u = tile = logical_block(b, deal.full);
+    } else {
+        cuts = cuts_of(g, deal);
+        if (b >= deal.full + deal.rest * cuts) return;
+        u = logical_block(b - deal.full, deal.rest * cuts);
+        cut = u / deal.rest;
+        tile = deal.full + u - cut * deal.rest;
     }
+    int ti, tj;
+    tile_of<C::GROUP_M>(tile, g.tiles_m, deal.tiles_n, &ti, &tj);
+    const int m0 = ti * C::TM, n0 = tj * C::TN;
+    f32x4 acc[WI][WJ];
+    product_tile<C>(g.a, g.b, m0, n0, (int)((int64_t)deal.steps * cut / cuts),
+                    (int)((int64_t)deal.steps * (cut + 1) / cuts), g.segs, smem, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = (wave / C::WAVES_N) * C::WM + 4 * (lane >> 4), wn = (wave % C::WAVES_N) * C::WN + (lane & 15);
+    if (cuts > 1) {
+        float* p = g.parts + (int64_t)u * (C::TM * C::TN);
+#pragma unroll
+        for (int j = 0; j < WJ; ++j)
+#pragma unroll
+            for (int i = 0; i < WI; ++i)
+                *reinterpret_cast<f32x4*>(p + (wn + j * 16) * C::TM + wm + i * 16) = acc[i][j];
+        return;
+    }
+    if (g.sum) finish_tile<C, kOutSum>(g, deal.n_all, m0 + wm, n0 + wn, acc);
+    else if (C::F16 && g.dtype == GEFEN_F32) finish_tile<C, kOutF32>(g, deal.n_all, m0 + wm, n0 + wn, acc);
+    else finish_tile<C, kOut16>(g, deal.n_all, m0 + wm, n0 + wn, acc);
 }
 
-// The splits of a product added up in order.
+// The parts of the cut tiles added up in order.  blockIdx.x: tile of the rest, blockIdx.y:
+// 1024 of its elements.
+template <typename C>
 __global__ __launch_bounds__(256) void k_join(const Grad g) {
-    const int n_all = g.dh ? piece_rows(g.meta, g.from, g.most) : g.n;
-    const int per = (g.d + 3) / 4;
+    const Deal deal = deal_of<C>(g);
+    const int t = blockIdx.x;
+    if (t >= deal.rest) return;
+    const int cuts = cuts_of(g, deal);
+    if (cuts == 1) return;
+    int ti, tj;
+    tile_of<C::GROUP_M>(deal.full + t, g.tiles_m, deal.tiles_n, &ti, &tj);
+    const int q = (int)(blockIdx.y * 256 + threadIdx.x) * 4;
+    const int n = tj * C::TN + q / C::TM, m = ti * C::TM + q % C::TM;
+    if (n >= deal.n_all || m >= g.d) return;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < cuts; ++c)
+        v += *reinterpret_cast<const f32x4*>(g.parts + ((int64_t)c * deal.rest + t) * (C::TM * C::TN) + q);
+    const int64_t row = g.dh ? g.map[g.from + n] : n;
+    const int cnt = min(4, g.d - m);
     const float factor = grad_factor(g);
-    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < (int64_t)n_all * per; q += (int64_t)gridDim.x * 256) {
-        const int64_t n = q / per;
-        const int m = (int)(q - n * per) * 4;
-        const int cnt = min(4, g.d - m);
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = 0; s < g.splits; ++s) {
-            const float* p = g.parts + ((int64_t)s * n_all + n) * g.d + m;
-            for (int e = 0; e < cnt; ++e) v[e] += p[e];
+    if (g.sum) finish<C::F16, kOutSum>(g, row, m, cnt, v, factor);
+    else if (C::F16 && g.dtype == GEFEN_F32) finish<C::F16, kOutF32>(g, row, m, cnt, v, factor);
+    else finish<C::F16, kOut16>(g, row, m, cnt, v, factor);
+}
+
+// dW from its float32 sum over the pieces.
+template <bool F16>
+__global__ __launch_bounds__(256) void k_convert(const Grad g) {
+    const int64_t all = ((int64_t)g.n * g.d + 3) / 4, numel = (int64_t)g.n * g.d;
+    const float factor = grad_factor(g);
+    const float* sum = g.sum;
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < all; q += (int64_t)gridDim.x * 256) {
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        const int cnt = (int)(numel - q * 4 < 4 ? numel - q * 4 : 4);
+        for (int e = 0; e < cnt; ++e) v[e] = sum[q * 4 + e];
+        if (F16 && g.dtype == GEFEN_F32) {
+            for (int e = 0; e < cnt; ++e) static_cast<float*>(g.out)[q * 4 + e] = v[e] * factor;
+        } else {
+            for (int e = 0; e < cnt; ++e)
+                static_cast<uint16_t*>(g.out)[q * 4 + e] =
+                    F16 ? from_f32<f16_t>(v[e] * factor).bits : from_f32<bf16_t>(v[e] * factor).bits;
         }
-        finish(g, g.dh ? g.map[g.from + n] : n, n, m, v, factor);
     }
 }
 
@@ -621,21 +753,34 @@ struct Plan {
     LogitsTile tile;
     int slots;
     bool dh_big, dw_big;
-    int dh_splits, dw_splits;
+    int dh_parts, dw_parts;
     // byte offsets into the workspace
     size_t o_meta, o_map, o_tgt, o_tlogit, o_losses, o_x, o_w, o_stats, o_sums, o_g, o_wsum, o_parts, bytes;
 };
 
-// Workgroups that fill the chip: one big tile or two small ones per CU.
+// Workgroups that fill the chip: one with a big tile or two with a small one per CU.
 constexpr int kCus = 256;
+constexpr int slots_of(bool big) { return big ? kCus : 2 * kCus; }
 
-void split_rule(int64_t m, int64_t n, int64_t steps, bool* big, int* splits) {
+// Measured: a K step of 64 takes 1.7 us on a chip full of big tiles (256 of 256 x 256)
+// and about 1.06 us on one full of small ones (512 of 128 x 128, half the products).  So
+// big tiles win unless the edges leave more than a fifth of them empty, or there are not
+// steps enough to give every workgroup a few.
+bool big_tile(int64_t m, int64_t n, int64_t steps) {
     const int64_t tb = up(m, 256) / 256 * (up(n, 256) / 256), ts = up(m, 128) / 128 * (up(n, 128) / 128);
-    *big = tb >= kCus / 2 || (m >= 256 && n >= 256 && tb * steps >= kCus * 8);
-    const int64_t tiles = *big ? tb : ts, room = *big ? kCus : 2 * kCus;
-    int64_t s = room / tiles;
-    if (s > steps / 4) s = steps / 4;  // at least four K steps of work per part
-    *splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+    return tb * steps >= kCus * kLeastSteps && ts * 10 > tb * 32;
+}
+// Partial tiles that a product of up to `tiles` tiles of `steps` K steps may leave: four
+// rounds of the chip at most.
+int parts_of(int64_t tiles, int64_t steps, bool big) {
+    const int64_t cuts = steps / kLeastSteps < kMostCuts ? steps / kLeastSteps : kMostCuts;
+    const int64_t rest = tiles < slots_of(big) ? tiles : slots_of(big) - 1;
+    if (cuts < 2) return 0;
+    return (int)(rest * cuts < 4 * slots_of(big) ? rest * cuts : 4 * slots_of(big));
+}
+int64_t tiles_of(int64_t m, int64_t n, bool big) {
+    const int64_t t = big ? 256 : 128;
+    return up(m, t) / t * (up(n, t) / t);
 }
 
 int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* what) {
@@ -675,8 +820,8 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
     const int64_t tiles = up(t.v, 256) / 256 * (up(n, 256) / 256);
     p->tile = n <= 32 ? kRowTile : tiles >= kCus / 2 ? kBigTile : kSmallTile;
     p->slots = (int)(up(t.v, kSlot) / kSlot);
-    split_rule(t.d, n, up(t.v, 64) / 64, &p->dh_big, &p->dh_splits);
-    split_rule(t.d, t.v, up(n, 64) / 64, &p->dw_big, &p->dw_splits);
+    p->dh_big = big_tile(t.d, n, up(t.v, 64) / 64);
+    p->dw_big = big_tile(t.d, t.v, up(n, 64) / 64);
 
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -697,13 +842,11 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
     p->o_sums = p->smooth ? take((size_t)p->rows * p->slots * 4) : at;
     p->o_g = p->train ? take((size_t)p->planes * p->rows * p->ldg * 2) : at;
     p->o_wsum = p->dw && p->pieces > 1 ? take((size_t)p->v * p->d * 4) : at;
-    size_t parts = 0;
-    if (p->dh && p->dh_splits > 1) parts = (size_t)p->dh_splits * (size_t)n * p->d * 4;
-    if (p->dw && p->dw_splits > 1) {
-        const size_t b = (size_t)p->dw_splits * p->v * p->d * 4;
-        parts = b > parts ? b : parts;
-    }
-    p->o_parts = take(parts);
+    p->dh_parts = p->dh ? parts_of(tiles_of(t.d, n, p->dh_big), up(t.v, 64) / 64, p->dh_big) : 0;
+    p->dw_parts = p->dw ? parts_of(tiles_of(t.d, t.v, p->dw_big), up(n, 64) / 64, p->dw_big) : 0;
+    const size_t dh_bytes = (size_t)p->dh_parts * (p->dh_big ? 256 * 256 : 128 * 128) * 4;
+    const size_t dw_bytes = (size_t)p->dw_parts * (p->dw_big ? 256 * 256 : 128 * 128) * 4;
+    p->o_parts = take(dh_bytes > dw_bytes ? dh_bytes : dw_bytes);
     p->bytes = at;
     return GEFEN_OK;
 }
@@ -711,33 +854,41 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
 template <typename C>
 void launch_logits(Logits a, int most, hipStream_t st) {
     a.tiles_m = (a.v + C::TM - 1) / C::TM;
-    const int grid = a.tiles_m * ((most + C::TN - 1) / C::TN);
-    hipLaunchKernelGGL(k_logits<C>, dim3(grid), dim3(C::TT), 0, st, a);
+    const dim3 grid((unsigned)(a.tiles_m * ((most + C::TN - 1) / C::TN))), wg(C::TT);
+    if (!a.g) hipLaunchKernelGGL((k_logits<C, kKeepNone>), grid, wg, 0, st, a);
+    else if (a.planes == 1) hipLaunchKernelGGL((k_logits<C, kKeepPacked>), grid, wg, 0, st, a);
+    else hipLaunchKernelGGL((k_logits<C, kKeepPlanes>), grid, wg, 0, st, a);
 }
+template <bool F16>
+void launch_logits_tile(const Plan& p, const Logits& a, int most, hipStream_t st) {
+    if (p.tile == kBigTile) launch_logits<LogitsBig<F16>>(a, most, st);
+    else if (p.tile == kSmallTile) launch_logits<LogitsSmall<F16>>(a, most, st);
+    else launch_logits<LogitsRow<F16>>(a, most, st);
+}
+// n: the most rows that the device may find
 template <typename C>
 void launch_grad(Grad g, int n, hipStream_t st) {
     g.tiles_m = (g.d + C::TM - 1) / C::TM;
-    const int grid = g.tiles_m * ((n + C::TN - 1) / C::TN) * g.splits;
-    hipLaunchKernelGGL(k_grad<C>, dim3(grid), dim3(C::TT), 0, st, g);
-    if (g.splits > 1) {
-        const int64_t work = ((int64_t)n * ((g.d + 3) / 4) + 255) / 256;
-        hipLaunchKernelGGL(k_join, dim3((unsigned)(work < 8192 ? work : 8192)), dim3(256), 0, st, g);
-    }
+    const int64_t tiles = (int64_t)g.tiles_m * ((n + C::TN - 1) / C::TN);
+    hipLaunchKernelGGL(k_grad<C>, dim3((unsigned)(tiles + g.most_parts)), dim3(C::TT), 0, st, g);
+    if (g.most_parts > 0)
+        hipLaunchKernelGGL(k_join<C>, dim3((unsigned)(tiles < g.slots ? tiles : g.slots - 1), C::TM * C::TN / 1024),
+                           dim3(256), 0, st, g);
 }
-
 template <bool F16>
-void launch_products(const Plan& p, int which, const Logits& l, const Grad& g, int n, hipStream_t st) {
-    if (which == 0) {
-        if (p.tile == kBigTile) launch_logits<LogitsBig<F16>>(l, n, st);
-        else if (p.tile == kSmallTile) launch_logits<LogitsSmall<F16>>(l, n, st);
-        else launch_logits<LogitsRow<F16>>(l, n, st);
-    } else if (which == 1) {
-        if (p.dh_big) launch_grad<HiddenBig<F16>>(g, n, st);
+void launch_grad_tile(Grad g, bool big, int n, hipStream_t st) {
+    g.slots = slots_of(big);
+    if (g.dh) {
+        if (big) launch_grad<HiddenBig<F16>>(g, n, st);
         else launch_grad<HiddenSmall<F16>>(g, n, st);
     } else {
-        if (p.dw_big) launch_grad<WeightBig<F16>>(g, n, st);
+        if (big) launch_grad<WeightBig<F16>>(g, n, st);
         else launch_grad<WeightSmall<F16>>(g, n, st);
     }
+}
+unsigned grid_of(int64_t chunks, int64_t most) {
+    const int64_t wg = (chunks + 255) / 256;
+    return (unsigned)(wg < 1 ? 1 : wg > most ? most : wg);
 }
 
 }  // namespace
@@ -798,6 +949,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     pk.f32 = t.dtype == GEFEN_F32;
     pk.dst = x;
     pk.plane = (int64_t)x_rows * p.dp;
+    pk.rows = x_rows;
     pk.map = map;
     pk.meta = meta;
     pk.which = 0;
@@ -805,12 +957,12 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     pk.zero_losses = losses;
     if (pk.f32) {
         Top tx{static_cast<const float*>(t.hidden), t.hidden_row_stride, t.hidden_col_stride, p.n, p.d, map, meta, 0};
-        hipLaunchKernelGGL(k_top, dim3(p.n < 2048 ? (p.n ? p.n : 1) : 2048), dim3(256), 0, st, tx);
+        const int64_t per = (p.d + 7) / 8;
+        hipLaunchKernelGGL(k_top, dim3(grid_of(p.n * per, 1024)), dim3(256), 0, st, tx);
         Top tw{static_cast<const float*>(t.weight), t.weight_row_stride, t.weight_col_stride, p.v, p.d, nullptr, meta, 1};
-        hipLaunchKernelGGL(k_top, dim3(p.v < 2048 ? p.v : 2048), dim3(256), 0, st, tw);
+        hipLaunchKernelGGL(k_top, dim3(grid_of(p.v * per, 1024)), dim3(256), 0, st, tw);
     }
-    const unsigned pack_y = (unsigned)((p.dp + 2047) / 2048);
-    hipLaunchKernelGGL(k_pack, dim3((unsigned)x_rows, pack_y), dim3(256), 0, st, pk);
+    hipLaunchKernelGGL(k_pack, dim3(grid_of(x_rows * (p.dp / 8), 8192)), dim3(256), 0, st, pk);
     if (p.pack_w) {
         Pack pw{};
         pw.src = t.weight;
@@ -822,9 +974,10 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         pw.f32 = pk.f32;
         pw.dst = wp;
         pw.plane = (int64_t)p.v * p.dp;
+        pw.rows = p.v;
         pw.meta = meta;
         pw.which = 1;
-        hipLaunchKernelGGL(k_pack, dim3((unsigned)p.v, pack_y), dim3(256), 0, st, pw);
+        hipLaunchKernelGGL(k_pack, dim3(grid_of(p.v * (p.dp / 8), 8192)), dim3(256), 0, st, pw);
     }
     Operand w{};
     w.p = p.pack_w ? wp : static_cast<const uint16_t*>(t.weight);
@@ -867,8 +1020,8 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         Grad g{};
         const bool f16 = p.halves;
         if (most > 0) {
-            if (f16) launch_products<true>(p, 0, l, g, most, st);
-            else launch_products<false>(p, 0, l, g, most, st);
+            if (f16) launch_logits_tile<true>(p, l, most, st);
+            else launch_logits_tile<false>(p, l, most, st);
             Rows r{};
             r.stats = l.stats;
             r.sums = l.sums;
@@ -916,19 +1069,17 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         g.mean = t.reduction == GEFEN_REDUCE_MEAN;
         g.by_row = by_row;
         g.dtype = t.dtype;
-        float* parts = reinterpret_cast<float*>(ws + p.o_parts);
+        g.parts = reinterpret_cast<float*>(ws + p.o_parts);
         if (p.dh && most > 0) {
             g.a = w;
             g.b = go;
             g.dh = 1;
             g.n = most;
             g.steps = (p.v + 63) / 64;
-            g.splits = p.dh_splits;
-            g.parts = g.splits > 1 ? parts : nullptr;
-            g.sum = nullptr;
+            g.most_parts = p.dh_parts;
             g.out = t.grad_hidden;
-            if (f16) launch_products<true>(p, 1, l, g, most, st);
-            else launch_products<false>(p, 1, l, g, most, st);
+            if (f16) launch_grad_tile<true>(g, p.dh_big, most, st);
+            else launch_grad_tile<false>(g, p.dh_big, most, st);
         }
         if (p.dw) {
             g.a = xo;
@@ -936,14 +1087,17 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
             g.b = go;
             g.dh = 0;
             g.n = p.v;
-            g.splits = p.dw_splits;
-            g.parts = g.splits > 1 ? parts : nullptr;
             g.sum = p.pieces > 1 ? reinterpret_cast<float*>(ws + p.o_wsum) : nullptr;
             g.first = piece == 0;
-            g.last = piece == p.pieces - 1;
+            g.most_parts = p.dw_parts;
             g.out = t.grad_weight;
-            if (f16) launch_products<true>(p, 2, l, g, p.v, st);
-            else launch_products<false>(p, 2, l, g, p.v, st);
+            if (f16) launch_grad_tile<true>(g, p.dw_big, p.v, st);
+            else launch_grad_tile<false>(g, p.dw_big, p.v, st);
+            if (g.sum && piece == p.pieces - 1) {
+                const dim3 grid(grid_of(((int64_t)p.v * p.d + 3) / 4, 8192));
+                if (f16) hipLaunchKernelGGL(k_convert<true>, grid, dim3(256), 0, st, g);
+                else hipLaunchKernelGGL(k_convert<false>, grid, dim3(256), 0, st, g);
+            }
         }
     }
     if (t.loss)
