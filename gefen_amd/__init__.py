@@ -21,12 +21,11 @@ def __getattr__(name):
         from .gefen_muon import GefenMuon
 
         return GefenMuon
-    if name == "linear_cross_entropy":
-        from .kernels.linear_cross_entropy import linear_cross_entropy
+    if name in ("linear_cross_entropy", "gradient_norm", "clip_gradients", "clip_grad_norm_"):
+        import importlib
 
-        return linear_cross_entropy
-    if name in ("gradient_norm", "clip_gradients", "clip_grad_norm_"):
-        from .kernels import gradient_norm as module
-
-        return getattr(module, name)
+        module = "linear_cross_entropy" if name == "linear_cross_entropy" else "gradient_norm"
+        value = getattr(importlib.import_module("gefen_amd.kernels." + module), name)
+        globals()[name] = value  # found directly from now on
+        return value
     raise AttributeError("module {!r} has no attribute {!r}".format(__name__, name))

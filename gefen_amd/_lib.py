@@ -157,6 +157,24 @@ def load():
     return lib
 
 
+_HOST = None
+
+
+def host():
+    """The host extension with the library's addresses bound; raise if it is not built."""
+    global _HOST
+    if _HOST is None:
+        lib = load()
+        try:
+            from gefen_amd import _gefen_host
+        except ImportError as e:
+            raise ImportError("gefen_amd: the host extension is missing; build it with "
+                              "`python -m gefen_amd.build`.") from e
+        _gefen_host.bind_library({name: ctypes.cast(getattr(lib, name), P).value for name in SIGNATURES})
+        _HOST = _gefen_host
+    return _HOST
+
+
 def check(rc: int, what: str = "") -> None:
     """Raise the Python exception the reference raises for this failure class."""
     if rc == GEFEN_OK:

@@ -107,8 +107,9 @@ def build_test_helpers() -> None:
 
 
 def build_host_ext() -> None:
-    """_gefen_host: the host-side plan checks (csrc/host_plan.cpp), a CPython
-    extension built with the host C++ compiler against torch's headers."""
+    """_gefen_host: the host-side plan checks (csrc/host_plan.cpp) and the host side of the
+    training operators (csrc/host_training.cpp), a CPython extension built with the host
+    C++ compiler against torch's headers (and HIP's, for the type of a stream)."""
     import sysconfig
 
     import torch
@@ -118,12 +119,13 @@ def build_host_ext() -> None:
     out = PKG / ("_gefen_host" + sysconfig.get_config_var("EXT_SUFFIX"))
     tmp = out.with_name(out.name + ".tmp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-shared", "-fPIC", "-std=c++17", "-Wall", "-ffp-contract=off",
-           "-D_GLIBCXX_USE_CXX11_ABI={}".format(int(torch.compiled_with_cxx11_abi())),
-           "-I", sysconfig.get_paths()["include"]]
+           "-D_GLIBCXX_USE_CXX11_ABI={}".format(int(torch.compiled_with_cxx11_abi())), "-D__HIP_PLATFORM_AMD__",
+           "-DUSE_ROCM", "-I", str(REPO / "include"), "-I", sysconfig.get_paths()["include"],
+           "-isystem", str(Path(HIPCC).resolve().parent.parent / "include"), "-isystem", "/opt/rocm/include"]
     for inc in cpp_extension.include_paths():
-        cmd += ["-I", inc]
-    cmd += [str(CSRC / "host_plan.cpp"), "-o", str(tmp), "-L", torch_lib, "-Wl,-rpath," + torch_lib,
-            "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+        cmd += ["-isystem", inc]
+    cmd += [str(CSRC / "host_plan.cpp"), str(CSRC / "host_training.cpp"), "-o", str(tmp), "-L", torch_lib,
+            "-Wl,-rpath," + torch_lib, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)

@@ -23,15 +23,15 @@
 #include <pybind11/pybind11.h>
 #include <torch/csrc/autograd/python_variable.h>
 
-#include <algorithm>
 #include <array>
 #include <cmath>
 #include <cstdint>
 #include <cstring>
-#include <string>
 #include <vector>
 
 namespace py = pybind11;
+
+void register_training(py::module_& m);  // host_training.cpp
 
 namespace {
 
@@ -341,85 +341,6 @@ class PlanCore {
     std::vector<long long> committed_;    // the "step" value written then
 };
 
-// Rows of gefen_gradient_task (include/gefen_hip.h) for a list of gradients, at `table`:
-// src and dst addresses, element count and dtypes.  outs: None (scaled in place) or the
-// list of tensors that receive the scaled gradients.  Returns (k, device): k = -1 when
-// every row is written, else the first tensor whose elements are not one dense run, in
-// the same order in both (the caller makes copies); raises for what no call takes.
-// With `writes`, what is written must not overlap anything else of the call.
-py::tuple gradient_rows(py::list tensors, py::object outs, uintptr_t table, bool writes) {
-    struct Row {
-        uint64_t src, dst;
-        int64_t numel;
-        int32_t src_dtype, dst_dtype;
-    };
-    static_assert(sizeof(Row) == 32, "gefen_gradient_task");
-    struct Span {
-        uint64_t begin, end;
-        size_t task;
-        bool write;
-    };
-    const size_t n = tensors.size();
-    const bool in_place = outs.is_none();
-    py::list out_list = in_place ? py::list() : py::list(outs);
-    if (!in_place && out_list.size() != n)
-        throw py::value_error("Expected as many output tensors as gradients.");
-    int device = -1;
-    auto tensor_at = [&](const py::list& l, size_t k) -> const at::Tensor& {
-        PyObject* o = PyList_GET_ITEM(l.ptr(), static_cast<Py_ssize_t>(k));
-        if (!THPVariable_Check(o))
-            throw py::type_error(std::string("Expected gradients to be torch.Tensor, got ") + Py_TYPE(o)->tp_name);
-        const at::Tensor& t = THPVariable_Unpack(o);
-        if (t.unsafeGetTensorImpl()->is_python_dispatch())
-            throw py::type_error("Expected plain tensors; give the local shards and the norm over all of them.");
-        if (!t.is_cuda()) throw py::value_error("Expected gradients on CUDA, got device " + t.device().str());
-        if (device < 0) device = t.device().index();
-        if (t.device().index() != device) throw py::value_error("Expected all gradients on one device.");
-        if (t.layout() != at::kStrided) throw py::value_error("Expected strided gradients.");
-        return t;
-    };
-    auto code = [](const at::Tensor& t) -> int32_t {
-        switch (t.scalar_type()) {
-            case at::kFloat: return 0;
-            case at::kHalf: return 1;
-            case at::kBFloat16: return 2;
-            default: throw py::value_error("Expected float32, float16 or bfloat16 gradients.");
-        }
-    };
-    std::vector<Span> spans;
-    Row* rows = reinterpret_cast<Row*>(table);
-    for (size_t k = 0; k < n; ++k) {
-        const at::Tensor& t = tensor_at(tensors, k);
-        Row r{reinterpret_cast<uint64_t>(t.data_ptr()), 0, t.numel(), code(t), 0};
-        bool dense = t.is_contiguous() || t.is_non_overlapping_and_dense();
-        r.dst = r.src;
-        r.dst_dtype = r.src_dtype;
-        if (!in_place) {
-            const at::Tensor& o = tensor_at(out_list, k);
-            if (o.sizes() != t.sizes()) throw py::value_error("Expected outputs of the gradients' shapes.");
-            r.dst = reinterpret_cast<uint64_t>(o.data_ptr());
-            r.dst_dtype = code(o);
-            dense = dense && (o.strides() == t.strides() || (o.is_contiguous() && t.is_contiguous()));
-        }
-        if (!dense && r.numel) return py::make_tuple(static_cast<int64_t>(k), device);
-        rows[k] = r;
-        if (writes && r.numel) {
-            const int64_t size[] = {4, 2, 2};
-            const uint64_t src_end = r.src + r.numel * size[r.src_dtype], dst_end = r.dst + r.numel * size[r.dst_dtype];
-            spans.push_back({r.dst, dst_end, k, true});
-            if (r.dst != r.src || dst_end != src_end) spans.push_back({r.src, src_end, k, false});
-        }
-    }
-    std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
-    uint64_t read_end = 0, write_end = 0;
-    for (const Span& s : spans) {
-        if (s.begin < write_end || (s.write && s.begin < read_end))
-            throw py::value_error("Expected gradients that share no memory with what is written.");
-        (s.write ? write_end : read_end) = std::max(s.write ? write_end : read_end, s.end);
-    }
-    return py::make_tuple(static_cast<int64_t>(-1), device);
-}
-
 }  // namespace
 
 PYBIND11_MODULE(_gefen_host, m) {
@@ -431,7 +352,7 @@ PYBIND11_MODULE(_gefen_host, m) {
     key_beta2_ = intern("beta2");
     key_eps_ = intern("eps");
     key_wd_ = intern("weight_decay");
-    m.def("gradient_rows", &gradient_rows);
+    register_training(m);
     py::class_<PlanCore>(m, "PlanCore")
         .def(py::init<py::list, py::list, py::tuple>())
         .def("refresh", &PlanCore::refresh)

@@ -1,0 +1,369 @@
+// Host side of the operators around the optimizer: the task tables of the gradient norm
+// and clipping, and the linear cross entropy with its autograd function.  In C++ because
+// a call on small tensors takes less time on the GPU than its Python form takes to start
+// it (a training call of 48 x 1000 x 96: 160 us from Python).
+//
+// The kernels are reached through the C ABI (include/gefen_hip.h) of the library that
+// gefen_amd/_lib.py has loaded: bind_library() receives the functions' addresses.  Built
+// with the host compiler against torch's headers (no device code).
+
+#include <Python.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <pybind11/pybind11.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <ATen/ATen.h>
+#include <algorithm>
+#include <cstdint>
+#include <stdexcept>
+#include <string>
+#include <vector>
+
+#include "gefen_hip.h"
+
+namespace py = pybind11;
+
+namespace {
+
+struct Library {
+    decltype(&gefen_last_error) last_error;
+    decltype(&gefen_gradient_norm_workspace_size) norm_workspace;
+    decltype(&gefen_gradient_norm) norm;
+    decltype(&gefen_clip_gradients) clip;
+    decltype(&gefen_scale_gradients) scale;
+    decltype(&gefen_linear_cross_entropy_workspace_size) lce_workspace;
+    decltype(&gefen_linear_cross_entropy) lce;
+    decltype(&gefen_scale_by) scale_by;
+};
+Library lib{};
+
+void bind_library(py::dict addresses) {
+    auto at = [&](const char* name) { return addresses[name].cast<uintptr_t>(); };
+    lib.norm_workspace = reinterpret_cast<decltype(lib.norm_workspace)>(at("gefen_gradient_norm_workspace_size"));
+    lib.norm = reinterpret_cast<decltype(lib.norm)>(at("gefen_gradient_norm"));
+    lib.clip = reinterpret_cast<decltype(lib.clip)>(at("gefen_clip_gradients"));
+    lib.scale = reinterpret_cast<decltype(lib.scale)>(at("gefen_scale_gradients"));
+    lib.lce_workspace =
+        reinterpret_cast<decltype(lib.lce_workspace)>(at("gefen_linear_cross_entropy_workspace_size"));
+    lib.lce = reinterpret_cast<decltype(lib.lce)>(at("gefen_linear_cross_entropy"));
+    lib.scale_by = reinterpret_cast<decltype(lib.scale_by)>(at("gefen_scale_by"));
+    lib.last_error = reinterpret_cast<decltype(lib.last_error)>(at("gefen_last_error"));
+}
+void need_library() {
+    if (!lib.last_error) throw std::runtime_error("bind_library() has not been called");
+}
+
+void check(int rc) {
+    if (rc == GEFEN_OK) return;
+    if (rc == GEFEN_EINVAL) throw py::value_error(lib.last_error());
+    throw std::runtime_error(lib.last_error());
+}
+
+int32_t dtype_code(const at::Tensor& t) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return GEFEN_F32;
+        case at::kHalf: return GEFEN_F16;
+        case at::kBFloat16: return GEFEN_BF16;
+        default: return -1;
+    }
+}
+
+gefen_stream_t stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+at::Tensor bytes_on(const at::Tensor& like, size_t n) {
+    return at::empty({static_cast<int64_t>(n)}, like.options().dtype(at::kByte).requires_grad(false));
+}
+
+const at::Tensor& tensor_of(py::handle o, const char* name) {
+    if (!THPVariable_Check(o.ptr()))
+        throw py::type_error(std::string("Expected ") + name + " to be a torch.Tensor, got " + Py_TYPE(o.ptr())->tp_name);
+    return THPVariable_Unpack(o.ptr());
+}
+
+py::object wrap(const at::Tensor& t) { return py::reinterpret_steal<py::object>(THPVariable_Wrap(t)); }
+
+// ------------------------------------------------------------------ gradient norm
+
+// The tasks of a list of gradients (and the list that receives them scaled; None: in
+// place).  bad: the first tensor whose elements are not one dense run, in the same order
+// in both, or -1.  Raises for what no call takes, and, with `writes`, where what is
+// written overlaps anything else of the call.
+struct Tasks {
+    std::vector<gefen_gradient_task> rows;
+    at::Tensor first;
+    int64_t bad = -1;
+};
+Tasks tasks_of(const py::list& tensors, const py::object& outs, bool writes) {
+    struct Span {
+        uint64_t begin, end;
+        bool write;
+    };
+    Tasks out;
+    const size_t n = tensors.size();
+    const bool in_place = outs.is_none();
+    py::list out_list = in_place ? py::list() : py::reinterpret_borrow<py::list>(outs);
+    if (!in_place && out_list.size() != n) throw py::value_error("Expected as many output tensors as gradients.");
+    auto tensor_at = [&](const py::list& l, size_t k) -> const at::Tensor& {
+        const at::Tensor& t = tensor_of(PyList_GET_ITEM(l.ptr(), static_cast<Py_ssize_t>(k)), "gradients");
+        if (t.unsafeGetTensorImpl()->is_python_dispatch())
+            throw py::type_error("Expected plain tensors; give the local shards and the norm over all of them.");
+        if (!t.is_cuda()) throw py::value_error("Expected gradients on CUDA, got device " + t.device().str());
+        if (!out.first.defined()) out.first = t;
+        if (t.device() != out.first.device()) throw py::value_error("Expected all gradients on one device.");
+        if (t.layout() != at::kStrided) throw py::value_error("Expected strided gradients.");
+        if (dtype_code(t) < 0) throw py::value_error("Expected float32, float16 or bfloat16 gradients.");
+        return t;
+    };
+    std::vector<Span> spans;
+    out.rows.resize(n);
+    for (size_t k = 0; k < n; ++k) {
+        const at::Tensor& t = tensor_at(tensors, k);
+        gefen_gradient_task& r = out.rows[k];
+        r.src = r.dst = t.data_ptr();
+        r.numel = t.numel();
+        r.src_dtype = r.dst_dtype = dtype_code(t);
+        bool dense = t.is_contiguous() || t.is_non_overlapping_and_dense();
+        if (!in_place) {
+            const at::Tensor& o = tensor_at(out_list, k);
+            if (o.sizes() != t.sizes()) throw py::value_error("Expected outputs of the gradients' shapes.");
+            r.dst = o.data_ptr();
+            r.dst_dtype = dtype_code(o);
+            dense = dense && (o.strides() == t.strides() || (o.is_contiguous() && t.is_contiguous()));
+        }
+        if (!dense && r.numel && out.bad < 0) out.bad = static_cast<int64_t>(k);
+        if (writes && r.numel && dense) {
+            const int64_t size[] = {4, 2, 2};
+            const uint64_t src = reinterpret_cast<uint64_t>(r.src), dst = reinterpret_cast<uint64_t>(r.dst);
+            const uint64_t src_end = src + r.numel * size[r.src_dtype], dst_end = dst + r.numel * size[r.dst_dtype];
+            spans.push_back({dst, dst_end, true});
+            if (dst != src || dst_end != src_end) spans.push_back({src, src_end, false});
+        }
+    }
+    std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+    uint64_t read_end = 0, write_end = 0;
+    for (const Span& s : spans) {
+        if (s.begin < write_end || (s.write && s.begin < read_end))
+            throw py::value_error("Expected gradients that share no memory with what is written.");
+        uint64_t& end = s.write ? write_end : read_end;
+        end = std::max(end, s.end);
+    }
+    return out;
+}
+
+// The norm, or None where a tensor is not one dense run of elements.
+py::object gradient_norm(py::list tensors, double norm_type) {
+    need_library();
+    Tasks t = tasks_of(tensors, py::none(), false);
+    if (t.bad >= 0) return py::none();
+    const int n = static_cast<int>(t.rows.size());
+    c10::DeviceGuard guard(t.first.device());
+    at::Tensor norm = at::empty({}, t.first.options().dtype(at::kFloat).requires_grad(false));
+    at::Tensor ws = bytes_on(t.first, lib.norm_workspace(t.rows.data(), n));
+    check(lib.norm(t.rows.data(), n, norm_type, norm.data_ptr<float>(), ws.data_ptr(), stream_of(norm)));
+    return wrap(norm);
+}
+
+// Clips (by total_norm, or the norm of these gradients) and returns the norm; None as above.
+py::object clip_gradients(py::list tensors, py::object outs, double max_norm, double norm_type, py::object total_norm) {
+    need_library();
+    Tasks t = tasks_of(tensors, outs, true);
+    if (t.bad >= 0) return py::none();
+    const int n = static_cast<int>(t.rows.size());
+    c10::DeviceGuard guard(t.first.device());
+    if (!total_norm.is_none()) {
+        const at::Tensor& norm = tensor_of(total_norm, "total_norm");
+        check(lib.scale(t.rows.data(), n, norm.data_ptr<float>(), max_norm, stream_of(t.first)));
+        return total_norm;
+    }
+    at::Tensor norm = at::empty({}, t.first.options().dtype(at::kFloat).requires_grad(false));
+    at::Tensor ws = bytes_on(t.first, lib.norm_workspace(t.rows.data(), n));
+    check(lib.clip(t.rows.data(), n, norm_type, max_norm, norm.data_ptr<float>(), ws.data_ptr(), stream_of(norm)));
+    return wrap(norm);
+}
+
+// ------------------------------------------------------------------ linear cross entropy
+
+struct LceOptions {
+    int64_t ignore_index, workspace_limit;
+    double label_smoothing;
+    int64_t reduction;
+};
+
+float* floats(const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+void* data(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// One library call on the current stream.
+void lce_call(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets, const LceOptions& o,
+              const at::Tensor& losses, const at::Tensor& loss, const at::Tensor& grad_hidden,
+              const at::Tensor& grad_weight, const at::Tensor& grad) {
+    at::Tensor h = hidden.dim() == 2 ? hidden : hidden.reshape({-1, hidden.size(-1)});
+    at::Tensor y = targets.contiguous();
+    gefen_linear_cross_entropy_task t{};
+    t.hidden = h.data_ptr();
+    t.weight = weight.data_ptr();
+    t.targets = y.data_ptr();
+    t.losses = floats(losses);
+    t.loss = floats(loss);
+    t.grad_hidden = data(grad_hidden);
+    t.grad_weight = data(grad_weight);
+    t.grad = floats(grad);
+    t.n = h.size(0);
+    t.v = weight.size(0);
+    t.d = weight.size(1);
+    t.hidden_row_stride = h.stride(0);
+    t.hidden_col_stride = h.stride(1);
+    t.weight_row_stride = weight.stride(0);
+    t.weight_col_stride = weight.stride(1);
+    t.ignore_index = o.ignore_index;
+    t.workspace_limit = o.workspace_limit;
+    t.label_smoothing = o.label_smoothing;
+    t.dtype = dtype_code(h);
+    t.targets_int32 = y.scalar_type() == at::kInt;
+    t.reduction = static_cast<int32_t>(o.reduction);
+    const size_t nbytes = lib.lce_workspace(&t);
+    if (nbytes == 0) check(GEFEN_EINVAL);
+    at::Tensor ws = bytes_on(h, nbytes);
+    check(lib.lce(&t, ws.data_ptr(), nbytes, stream_of(h)));
+}
+
+at::Tensor empty_grad(const at::Tensor& like, bool wanted) {
+    return wanted ? at::empty(like.sizes(), like.options().requires_grad(false)) : at::Tensor();
+}
+
+// The loss; gh, gw: the gradients where they are formed here (a reduced loss of bfloat16
+// or float32 operands).  Float16 ones wait for the loss's gradient, so that a loss scale
+// reaches them before they are rounded.
+at::Tensor lce_forward(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
+                       const LceOptions& o, bool need_h, bool need_w, at::Tensor* gh, at::Tensor* gw) {
+    c10::DeviceGuard guard(hidden.device());
+    const auto f32 = hidden.options().dtype(at::kFloat).requires_grad(false);
+    if (o.reduction == GEFEN_REDUCE_NONE) {
+        at::Tensor losses = at::empty(targets.sizes(), f32);
+        lce_call(hidden, weight, targets, o, losses, {}, {}, {}, {});
+        return losses;
+    }
+    at::Tensor loss = at::empty({}, f32);
+    if (hidden.scalar_type() != at::kHalf) {
+        *gh = empty_grad(hidden, need_h);
+        *gw = empty_grad(weight, need_w);
+    }
+    lce_call(hidden, weight, targets, o, {}, loss, *gh, *gw, {});
+    return loss;
+}
+
+class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> {
+   public:
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& hidden, const at::Tensor& weight,
+                              const at::Tensor& targets, int64_t ignore_index, int64_t workspace_limit,
+                              double label_smoothing, int64_t reduction, bool need_h, bool need_w) {
+        at::Tensor gh, gw;
+        at::Tensor result = lce_forward(hidden, weight, targets, {ignore_index, workspace_limit, label_smoothing, reduction},
+                                        need_h, need_w, &gh, &gw);
+        ctx->save_for_backward({hidden, weight, targets});
+        ctx->saved_data["ignore_index"] = ignore_index;
+        ctx->saved_data["workspace_limit"] = workspace_limit;
+        ctx->saved_data["label_smoothing"] = label_smoothing;
+        ctx->saved_data["reduction"] = reduction;
+        ctx->saved_data["need_h"] = need_h;
+        ctx->saved_data["need_w"] = need_w;
+        ctx->saved_data["formed"] = gh.defined() || gw.defined();
+        if (gh.defined()) ctx->saved_data["gh"] = gh;
+        if (gw.defined()) ctx->saved_data["gw"] = gw;
+        return result;
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list grads) {
+        TORCH_CHECK(!c10::GradMode::is_enabled(), "linear_cross_entropy can be differentiated once only");
+        const bool need_h = ctx->saved_data["need_h"].toBool(), need_w = ctx->saved_data["need_w"].toBool();
+        at::Tensor gh, gw;
+        if (grads[0].defined()) {
+            const auto saved = ctx->get_saved_variables();
+            const at::Tensor &hidden = saved[0], &weight = saved[1];
+            c10::DeviceGuard guard(hidden.device());
+            const at::Tensor grad = grads[0].to(at::kFloat).contiguous();
+            if (ctx->saved_data["formed"].toBool()) {
+                // handed over: a second backward of a retained graph forms them again
+                ctx->saved_data["formed"] = false;
+                if (need_h) gh = ctx->saved_data["gh"].toTensor();
+                if (need_w) gw = ctx->saved_data["gw"].toTensor();
+                ctx->saved_data.erase("gh");
+                ctx->saved_data.erase("gw");
+                const int rc = lib.scale_by(data(gh), need_h ? gh.numel() : 0, data(gw), need_w ? gw.numel() : 0,
+                                            dtype_code(hidden), grad.data_ptr<float>(), stream_of(hidden));
+                if (rc != GEFEN_OK) throw std::runtime_error(lib.last_error());
+            } else {
+                gh = empty_grad(hidden, need_h);
+                gw = empty_grad(weight, need_w);
+                lce_call(hidden, weight, saved[2],
+                         {ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["workspace_limit"].toInt(),
+                          ctx->saved_data["label_smoothing"].toDouble(), ctx->saved_data["reduction"].toInt()},
+                         {}, {}, gh, gw, grad);
+            }
+        }
+        return {gh, gw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+std::string shape_of(c10::IntArrayRef s) {
+    std::string out = "(";
+    for (size_t i = 0; i < s.size(); ++i) out += (i ? ", " : "") + std::to_string(s[i]);
+    return out + ")";
+}
+
+py::object linear_cross_entropy(py::handle hidden_, py::handle weight_, py::handle targets_, int64_t ignore_index,
+                                double label_smoothing, int64_t reduction, int64_t workspace_limit) {
+    need_library();
+    const at::Tensor& hidden = tensor_of(hidden_, "hidden");
+    const at::Tensor& weight = tensor_of(weight_, "weight");
+    const at::Tensor& targets = tensor_of(targets_, "targets");
+    auto on_device = [&](const at::Tensor& t, const char* name) {
+        if (!t.is_cuda())
+            throw py::value_error(std::string("Expected ") + name + " to be on CUDA, got device " + t.device().str() + ".");
+        if (t.device() != hidden.device())
+            throw py::value_error(std::string("Expected ") + name + " on " + hidden.device().str() + ", got " +
+                                  t.device().str() + ".");
+        if (t.unsafeGetTensorImpl()->is_python_dispatch() || t.layout() != at::kStrided)
+            throw py::type_error(std::string("Expected ") + name + " to be a plain strided tensor.");
+    };
+    on_device(hidden, "hidden");
+    on_device(weight, "weight");
+    on_device(targets, "targets");
+    if (dtype_code(hidden) < 0)
+        throw py::value_error(std::string("Expected hidden to be float32, float16 or bfloat16, got ") +
+                              c10::toString(hidden.scalar_type()));
+    if (weight.scalar_type() != hidden.scalar_type())
+        throw py::value_error(std::string("Expected weight of hidden's dtype ") + c10::toString(hidden.scalar_type()) +
+                              ", got " + c10::toString(weight.scalar_type()));
+    if (targets.scalar_type() != at::kLong && targets.scalar_type() != at::kInt)
+        throw py::value_error(std::string("Expected targets to be int64 or int32, got ") +
+                              c10::toString(targets.scalar_type()));
+    if (weight.dim() != 2) throw py::value_error("Expected weight to be 2D, got dim=" + std::to_string(weight.dim()));
+    if (hidden.dim() < 1 || hidden.size(-1) != weight.size(1))
+        throw py::value_error("Expected hidden of width " + std::to_string(weight.size(1)) + ", got shape " +
+                              shape_of(hidden.sizes()));
+    if (targets.sizes() != hidden.sizes().slice(0, hidden.dim() - 1))
+        throw py::value_error("Expected targets of shape " + shape_of(hidden.sizes().slice(0, hidden.dim() - 1)) +
+                              ", got " + shape_of(targets.sizes()));
+    if (weight.numel() == 0)
+        throw py::value_error("Expected a non-empty weight, got shape " + shape_of(weight.sizes()));
+    const bool grad = c10::GradMode::is_enabled();
+    const bool need_h = grad && hidden.requires_grad(), need_w = grad && weight.requires_grad();
+    if (need_h || need_w)
+        return wrap(LinearCrossEntropy::apply(hidden, weight, targets, ignore_index, workspace_limit, label_smoothing,
+                                              reduction, need_h, need_w));
+    at::Tensor gh, gw;
+    return wrap(lce_forward(hidden.detach(), weight.detach(), targets,
+                            {ignore_index, workspace_limit, label_smoothing, reduction}, false, false, &gh, &gw));
+}
+
+}  // namespace
+
+void register_training(py::module_& m) {
+    m.def("bind_library", &bind_library);
+    m.def("gradient_norm", &gradient_norm);
+    m.def("clip_gradients", &clip_gradients);
+    m.def("linear_cross_entropy", &linear_cross_entropy);
+}

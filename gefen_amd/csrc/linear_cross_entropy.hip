@@ -37,6 +37,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <utility>
+
 #include "capi_internal.h"
 #include "common.h"
 #include "lce_gemm.h"
@@ -66,50 +68,57 @@ __device__ __forceinline__ int64_t target_at(const void* t, int is32, int64_t n)
     return is32 ? (int64_t) static_cast<const int32_t*>(t)[n] : static_cast<const int64_t*>(t)[n];
 }
 
-// map = the rows that take part, in order, then the ignored ones; targets in that
-// order (-1: not a column, whose loss is NaN).  One workgroup.
-constexpr int kRowsThreads = 1024;
-__global__ __launch_bounds__(kRowsThreads) void k_rows(const void* __restrict__ targets, int is32, int n, int v,
-                                                       int64_t ignore, const float* __restrict__ row_grad,
-                                                       int32_t* __restrict__ map, int32_t* __restrict__ tgt,
-                                                       Meta* __restrict__ meta) {
-    __shared__ int wave_sum[kRowsThreads / 64];
-    __shared__ float wave_max[kRowsThreads / 64];
+// Which rows take part.
+struct Select {
+    const void* targets;
+    int32_t targets_int32, n, v;
+    int64_t ignore;
+    const float* row_grad;  // gradient of each row's loss (null: one for all)
+    int32_t* map;
+    int32_t* tgt;
+    Meta* meta;
+};
+// map = the rows that take part, in order, then the ignored ones; tgt = their targets in
+// that order (-1: not a column, whose loss is NaN; may be null).  One workgroup.
+template <int THREADS>
+__device__ __forceinline__ Meta select_rows(const Select& s, int32_t* map, int32_t* tgt) {
+    __shared__ int wave_sum[THREADS / 64];
+    __shared__ float wave_max[THREADS / 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int base = 0;  // rows that take part before this stretch
-    float gmax = 0.0f;
-    for (int at = 0; at < n; at += kRowsThreads) {
+    Meta m = {0, 0.0f, {0, 0}};
+    for (int at = 0; at < s.n; at += THREADS) {
         const int i = at + (int)threadIdx.x;
-        const int64_t y = i < n ? target_at(targets, is32, i) : ignore;
-        const bool live = i < n && y != ignore;
+        const int64_t y = i < s.n ? target_at(s.targets, s.targets_int32, i) : s.ignore;
+        const bool live = i < s.n && y != s.ignore;
         const uint64_t ball = __ballot(live);
         const int before = __popcll(ball & ((1ull << lane) - 1ull));
         if (lane == 0) wave_sum[wave] = __popcll(ball);
         __syncthreads();
-        int off = 0, all = 0;
-        for (int w = 0; w < kRowsThreads / 64; ++w) {
+        int off = m.count, all = 0;
+        for (int w = 0; w < THREADS / 64; ++w) {
             if (w < wave) off += wave_sum[w];
             all += wave_sum[w];
         }
         if (live) {
-            map[base + off + before] = i;
-            tgt[base + off + before] = (y >= 0 && y < v) ? (int)y : -1;
-            if (row_grad) gmax = nanmax(gmax, fabsf(row_grad[i]));
-        } else if (i < n) {
-            map[n - 1 - (i - base - off - before)] = i;
+            map[off + before] = i;
+            if (tgt) tgt[off + before] = (y >= 0 && y < s.v) ? (int)y : -1;
+            if (s.row_grad) m.grad_max = nanmax(m.grad_max, fabsf(s.row_grad[i]));
+        } else if (i < s.n) {
+            map[s.n - 1 - (i - off - before)] = i;
         }
-        base += all;
+        m.count += all;
         __syncthreads();
     }
-    for (int off = 32; off > 0; off >>= 1) gmax = nanmax(gmax, __shfl_xor(gmax, off, 64));
-    if (lane == 0) wave_max[wave] = gmax;
+    for (int off = 32; off > 0; off >>= 1) m.grad_max = nanmax(m.grad_max, __shfl_xor(m.grad_max, off, 64));
+    if (lane == 0) wave_max[wave] = m.grad_max;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kRowsThreads / 64; ++w) gmax = nanmax(gmax, wave_max[w]);
-        meta->count = base;
-        meta->grad_max = gmax;
-        meta->top[0] = meta->top[1] = 0;
-    }
+    for (int w = 0; w < THREADS / 64; ++w) m.grad_max = nanmax(m.grad_max, wave_max[w]);
+    return m;
+}
+constexpr int kRowsThreads = 1024;
+__global__ __launch_bounds__(kRowsThreads) void k_rows(const Select s) {
+    const Meta m = select_rows<kRowsThreads>(s, s.map, s.tgt);
+    if (threadIdx.x == 0) *s.meta = m;
 }
 
 // x (scaled into half's range) as a half and what it leaves times kLowScale.
@@ -118,6 +127,19 @@ __device__ __forceinline__ void split_half(float x, uint16_t* hi, uint16_t* lo) 
     *hi = h.bits;
     // what is not finite has no remainder worth adding: inf - inf is NaN
     *lo = (h.bits & 0x7c00) == 0x7c00 ? 0 : from_f32<f16_t>((x - to_f32(h)) * kLowScale).bits;
+}
+// The same for what is finite or has no use for the low part (subnormal halves rounded as
+// the conversion instruction does).
+__device__ __forceinline__ uint16_t half_bits(float x) {
+    const _Float16 h = (_Float16)x;
+    uint16_t u;
+    __builtin_memcpy(&u, &h, 2);
+    return u;
+}
+__device__ __forceinline__ void split_half_fast(float x, uint16_t* hi, uint16_t* lo) {
+    const _Float16 h = (_Float16)x;
+    *hi = half_bits(x);
+    *lo = half_bits((x - (float)h) * kLowScale);
 }
 __device__ __forceinline__ void split_bf16(float x, uint16_t* hi, uint16_t* lo) {
     const bf16_t h = from_f32<bf16_t>(x);
@@ -158,7 +180,11 @@ struct Top {
     Meta* meta;
     int32_t which;
 };
-__global__ __launch_bounds__(256) void k_top(const Top t) {
+// Workgroups up to `first` take a, the others b.
+__global__ __launch_bounds__(256) void k_top(const Top a, const Top b, int first) {
+    const bool is_a = (int)blockIdx.x < first;
+    const Top& t = is_a ? a : b;
+    const int block = is_a ? blockIdx.x : blockIdx.x - first, blocks = is_a ? first : gridDim.x - first;
     const uint32_t per = (uint32_t)(t.d + 7) / 8;  // chunks of eight columns a row
     const int64_t all = (int64_t)(t.map ? t.meta->count : t.n) * per;
     uint32_t top = 0;
@@ -166,7 +192,7 @@ __global__ __launch_bounds__(256) void k_top(const Top t) {
         const uint32_t u = abs_key(x);
         top = u < 0x7f800000u && u > top ? u : top;
     };
-    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < all; q += (int64_t)gridDim.x * 256) {
+    for (int64_t q = (int64_t)block * 256 + threadIdx.x; q < all; q += (int64_t)blocks * 256) {
         const int64_t r = q / per;
         const int c = (int)(q - r * per) * 8;
         const float* s = t.src + (int64_t)(t.map ? t.map[r] : r) * t.row_stride;
@@ -209,18 +235,17 @@ struct Pack {
     void* zero_rows;    // [n, d] gradient (may be null)
     float* zero_losses;  // [n] (may be null)
 };
-__global__ __launch_bounds__(256) void k_pack(const Pack p) {
+__device__ __forceinline__ void pack_block(const Pack& p, const int32_t* map, int count, int block, int blocks) {
     const uint32_t per = (uint32_t)p.dp / 8;
-    const int count = p.map ? p.meta->count : p.n;
-    const int ends = p.map ? (count + kRowAlign - 1) / kRowAlign * kRowAlign : p.rows;
+    const int ends = map ? (count + kRowAlign - 1) / kRowAlign * kRowAlign : p.rows;
     const int64_t all = (int64_t)(ends > p.n ? ends : p.n) * per;
     const int ex = p.f32 ? half_exponent(p.meta->top[p.which]) : 0;
-    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < all; q += (int64_t)gridDim.x * 256) {
+    for (int64_t q = (int64_t)block * 256 + threadIdx.x; q < all; q += (int64_t)blocks * 256) {
         const int r = (int)(q / per);
         const int c0 = (int)(q - (int64_t)r * per) * 8;
-        const int64_t row = p.map && r < p.n ? p.map[r] : r;
+        const int64_t row = map && r < p.n ? map[r] : r;
         const bool live = r < count;
-        if (p.map && !live && r < p.n) {
+        if (map && !live && r < p.n) {
             if (p.zero_losses && c0 == 0) p.zero_losses[row] = 0.0f;
             if (p.zero_rows)
                 for (int e = c0; e < min(c0 + 8, p.d); ++e) {
@@ -262,6 +287,28 @@ __global__ __launch_bounds__(256) void k_pack(const Pack p) {
             vstore(d + 2 * p.plane, 0, out[2]);
         }
     }
+}
+
+// hidden by the workgroups up to `first`, weight by the others (if there are any).
+__global__ __launch_bounds__(256) void k_pack(const Pack x, const Pack w, int first) {
+    if ((int)blockIdx.x < first) pack_block(x, x.map, x.meta->count, blockIdx.x, first);
+    else pack_block(w, nullptr, w.n, blockIdx.x - first, gridDim.x - first);
+}
+// The same for few rows without k_rows: every workgroup of hidden selects them for itself
+// (the first one for the kernels that follow), which saves a launch.
+constexpr int kSelfRows = 1024;
+__global__ __launch_bounds__(256) void k_select_pack(const Select s, const Pack x, const Pack w, int first) {
+    __shared__ int32_t map[kSelfRows];
+    if ((int)blockIdx.x >= first) {
+        pack_block(w, nullptr, w.n, blockIdx.x - first, gridDim.x - first);
+        return;
+    }
+    const Meta m = select_rows<256>(s, map, blockIdx.x == 0 ? s.tgt : nullptr);
+    if (blockIdx.x == 0) {
+        for (int i = threadIdx.x; i < s.n; i += 256) s.map[i] = map[i];
+        if (threadIdx.x == 0) *s.meta = m;
+    }
+    pack_block(x, map, m.count, blockIdx.x, first);
 }
 
 // The logits' product of a piece of rows and what is kept of it.
@@ -346,9 +393,10 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
         for (int i = 0; i < WI; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                // the difference first: exact where it matters, however large the logits
-                const float x = acc[i][j][r] - ref;
-                acc[i][j][r] = f32 ? expf(x) : __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2E, -kDown));
+                // the difference first: exact where it matters, however large the logits; the
+                // product's rounding is 2^-24 |x| of exp(x)
+                acc[i][j][r] =
+                    __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r] - ref, kLog2E, -kDown));
                 s += acc[i][j][r];
             }
         if (kDown != 0.0f) s *= 0x1p64f;
@@ -372,7 +420,7 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
                 uint16_t o[2][4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    if constexpr (C::F16) split_half(acc[i][j][r] * kHalfScale, &o[0][r], &o[1][r]);
+                    if constexpr (C::F16) split_half_fast(acc[i][j][r] * kHalfScale, &o[0][r], &o[1][r]);
                     else split_bf16(acc[i][j][r], &o[0][r], &o[1][r]);
                 }
 #pragma unroll
@@ -498,8 +546,8 @@ __global__ __launch_bounds__(kGradThreads) void k_gradient_rows(const Rows a) {
                 if (hit && v0 + e == y) q = at_target;
                 q *= w;
                 if (part && v0 + e >= a.v) q = 0.0f;
-                if (a.planes == 1) hi.v[e] = F16 ? from_f32<f16_t>(q).bits : from_f32<bf16_t>(q).bits;
-                else if (F16) split_half(q, &hi.v[e], &lo.v[e]);
+                if (a.planes == 1) hi.v[e] = F16 ? half_bits(q) : from_f32<bf16_t>(q).bits;
+                else if (F16) split_half_fast(q, &hi.v[e], &lo.v[e]);
                 else split_bf16(q, &hi.v[e], &lo.v[e]);
             }
             vstore(row, (int64_t)c * 8, hi);
@@ -509,20 +557,27 @@ __global__ __launch_bounds__(kGradThreads) void k_gradient_rows(const Rows a) {
 }
 
 // The sum of the rows' losses in float64, over the count for a mean (0 / 0 = NaN
-// where no row takes part, as the mean of nothing is).
-__global__ __launch_bounds__(1024) void k_loss(const float* __restrict__ losses, int n, const Meta* __restrict__ meta,
-                                               int mean, float* __restrict__ out) {
-    __shared__ double part[16];
+// where no row takes part, as the mean of nothing is).  One workgroup.
+struct Loss {
+    const float* losses;
+    int32_t n, mean;
+    const Meta* meta;
+    float* out;  // null: no loss wanted
+};
+template <int THREADS>
+__device__ __forceinline__ void sum_losses(const Loss& l) {
+    __shared__ double part[THREADS / 64];
     double s = 0.0;
-    for (int i = threadIdx.x; i < n; i += 1024) s += (double)losses[i];
+    for (int i = threadIdx.x; i < l.n; i += THREADS) s += (double)l.losses[i];
     for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) s += part[w];
-        *out = (float)(mean ? s / (double)meta->count : s);
+        for (int w = 1; w < THREADS / 64; ++w) s += part[w];
+        *l.out = (float)(l.mean ? s / (double)l.meta->count : s);
     }
 }
+__global__ __launch_bounds__(1024) void k_loss(const Loss l) { sum_losses<1024>(l); }
 
 // A gradient's product: out[n, m] = factor * sum_k A[m, k] B[n, k] for m < D, rows n of
 // the piece (dh, through the map) or of the vocabulary (dW).
@@ -640,11 +695,9 @@ __device__ __forceinline__ void finish_tile(const Grad& g, int n_all, int m, int
 }
 
 template <typename C>
-__global__ __launch_bounds__(C::TT, C::EU) void k_grad(const Grad g) {
+__device__ __forceinline__ void grad_block(const Grad& g, int b, uint16_t* smem) {
     constexpr int WI = C::WI, WJ = C::WJ;
-    __shared__ __attribute__((aligned(1024))) uint16_t smem[C::NST * C::STAGE];
     const Deal deal = deal_of<C>(g);
-    const int b = blockIdx.x;
     int u, tile, cut = 0, cuts = 1;
     if (b < deal.full) {
         u = tile = logical_block(b, deal.full);
@@ -677,12 +730,29 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_grad(const Grad g) {
     else finish_tile<C, kOut16>(g, deal.n_all, m0 + wm, n0 + wn, acc);
 }
 
-// The parts of the cut tiles added up in order.  blockIdx.x: tile of the rest, blockIdx.y:
+// One gradient's product; the last workgroup sums the losses where l.out is given, which
+// saves a launch.
+template <typename C>
+__global__ __launch_bounds__(C::TT, C::EU) void k_grad(const Grad g, const Loss l) {
+    __shared__ __attribute__((aligned(1024))) uint16_t smem[C::NST * C::STAGE];
+    if (l.out && blockIdx.x == gridDim.x - 1) return sum_losses<C::TT>(l);
+    grad_block<C>(g, blockIdx.x, smem);
+}
+// Both products, dh by the workgroups up to `first`.
+template <typename H, typename W>
+__global__ __launch_bounds__(H::TT, H::EU) void k_grads(const Grad h, const Grad w, const Loss l, int first) {
+    static_assert(H::TT == W::TT && H::STAGE == W::STAGE && H::NST == W::NST, "one launch");
+    __shared__ __attribute__((aligned(1024))) uint16_t smem[H::NST * H::STAGE];
+    if (l.out && blockIdx.x == gridDim.x - 1) return sum_losses<H::TT>(l);
+    if ((int)blockIdx.x < first) grad_block<H>(h, blockIdx.x, smem);
+    else grad_block<W>(w, blockIdx.x - first, smem);
+}
+
+// The parts of the cut tiles added up in order.  t: tile of the rest, blockIdx.y:
 // 1024 of its elements.
 template <typename C>
-__global__ __launch_bounds__(256) void k_join(const Grad g) {
+__device__ __forceinline__ void join_block(const Grad& g, int t) {
     const Deal deal = deal_of<C>(g);
-    const int t = blockIdx.x;
     if (t >= deal.rest) return;
     const int cuts = cuts_of(g, deal);
     if (cuts == 1) return;
@@ -700,6 +770,16 @@ __global__ __launch_bounds__(256) void k_join(const Grad g) {
     if (g.sum) finish<C::F16, kOutSum>(g, row, m, cnt, v, factor);
     else if (C::F16 && g.dtype == GEFEN_F32) finish<C::F16, kOutF32>(g, row, m, cnt, v, factor);
     else finish<C::F16, kOut16>(g, row, m, cnt, v, factor);
+}
+
+template <typename C>
+__global__ __launch_bounds__(256) void k_join(const Grad g) {
+    join_block<C>(g, blockIdx.x);
+}
+template <typename H, typename W>
+__global__ __launch_bounds__(256) void k_joins(const Grad h, const Grad w, int first) {
+    if ((int)blockIdx.x < first) join_block<H>(h, blockIdx.x);
+    else join_block<W>(w, blockIdx.x - first);
 }
 
 // dW from its float32 sum over the pieces.
@@ -753,9 +833,10 @@ struct Plan {
     LogitsTile tile;
     int slots;
     bool dh_big, dw_big;
+    bool pair;          // both gradients' products in one launch
     int dh_parts, dw_parts;
     // byte offsets into the workspace
-    size_t o_meta, o_map, o_tgt, o_tlogit, o_losses, o_x, o_w, o_stats, o_sums, o_g, o_wsum, o_parts, bytes;
+    size_t o_meta, o_map, o_tgt, o_tlogit, o_losses, o_x, o_w, o_stats, o_sums, o_g, o_wsum, o_parts, o_dw_parts, bytes;
 };
 
 // Workgroups that fill the chip: one with a big tile or two with a small one per CU.
@@ -770,9 +851,13 @@ bool big_tile(int64_t m, int64_t n, int64_t steps) {
     const int64_t tb = up(m, 256) / 256 * (up(n, 256) / 256), ts = up(m, 128) / 128 * (up(n, 128) / 128);
     return tb * steps >= kCus * kLeastSteps && ts * 10 > tb * 32;
 }
+// K steps that are run in one piece whatever the tiles: joining costs a launch (5 us),
+// what eight steps take where a CU has one small tile.
+constexpr int kUncutSteps = 24;
 // Partial tiles that a product of up to `tiles` tiles of `steps` K steps may leave: four
 // rounds of the chip at most.
-int parts_of(int64_t tiles, int64_t steps, bool big) {
+int parts_of(int64_t tiles, int64_t steps, int segs, bool big) {
+    if (steps * segs <= kUncutSteps) return 0;
     const int64_t cuts = steps / kLeastSteps < kMostCuts ? steps / kLeastSteps : kMostCuts;
     const int64_t rest = tiles < slots_of(big) ? tiles : slots_of(big) - 1;
     if (cuts < 2) return 0;
@@ -842,11 +927,14 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
     p->o_sums = p->smooth ? take((size_t)p->rows * p->slots * 4) : at;
     p->o_g = p->train ? take((size_t)p->planes * p->rows * p->ldg * 2) : at;
     p->o_wsum = p->dw && p->pieces > 1 ? take((size_t)p->v * p->d * 4) : at;
-    p->dh_parts = p->dh ? parts_of(tiles_of(t.d, n, p->dh_big), up(t.v, 64) / 64, p->dh_big) : 0;
-    p->dw_parts = p->dw ? parts_of(tiles_of(t.d, t.v, p->dw_big), up(n, 64) / 64, p->dw_big) : 0;
+    const int segs = t.dtype == GEFEN_F32 ? 3 : p->planes;
+    p->dh_parts = p->dh ? parts_of(tiles_of(t.d, n, p->dh_big), up(t.v, 64) / 64, segs, p->dh_big) : 0;
+    p->dw_parts = p->dw ? parts_of(tiles_of(t.d, t.v, p->dw_big), up(n, 64) / 64, segs, p->dw_big) : 0;
     const size_t dh_bytes = (size_t)p->dh_parts * (p->dh_big ? 256 * 256 : 128 * 128) * 4;
     const size_t dw_bytes = (size_t)p->dw_parts * (p->dw_big ? 256 * 256 : 128 * 128) * 4;
-    p->o_parts = take(dh_bytes > dw_bytes ? dh_bytes : dw_bytes);
+    p->pair = p->dh && p->dw && !p->dh_big && !p->dw_big && p->pieces == 1 && t.n > 0;
+    p->o_parts = take(p->pair ? dh_bytes + dw_bytes : dh_bytes > dw_bytes ? dh_bytes : dw_bytes);
+    p->o_dw_parts = p->o_parts + (p->pair ? dh_bytes : 0);
     p->bytes = at;
     return GEFEN_OK;
 }
@@ -865,26 +953,42 @@ void launch_logits_tile(const Plan& p, const Logits& a, int most, hipStream_t st
     else if (p.tile == kSmallTile) launch_logits<LogitsSmall<F16>>(a, most, st);
     else launch_logits<LogitsRow<F16>>(a, most, st);
 }
-// n: the most rows that the device may find
+// Grids for g.n rows, the most that the device may find.
 template <typename C>
-void launch_grad(Grad g, int n, hipStream_t st) {
-    g.tiles_m = (g.d + C::TM - 1) / C::TM;
-    const int64_t tiles = (int64_t)g.tiles_m * ((n + C::TN - 1) / C::TN);
-    hipLaunchKernelGGL(k_grad<C>, dim3((unsigned)(tiles + g.most_parts)), dim3(C::TT), 0, st, g);
-    if (g.most_parts > 0)
-        hipLaunchKernelGGL(k_join<C>, dim3((unsigned)(tiles < g.slots ? tiles : g.slots - 1), C::TM * C::TN / 1024),
-                           dim3(256), 0, st, g);
+int grad_grid(Grad* g, int* join) {
+    g->tiles_m = (g->d + C::TM - 1) / C::TM;
+    const int tiles = g->tiles_m * ((g->n + C::TN - 1) / C::TN);
+    *join = g->most_parts == 0 ? 0 : tiles < g->slots ? tiles : g->slots - 1;
+    return tiles + g->most_parts;
+}
+template <typename C>
+void launch_grad(Grad g, const Loss& l, hipStream_t st) {
+    int join;
+    const int grid = grad_grid<C>(&g, &join) + (l.out ? 1 : 0);
+    hipLaunchKernelGGL(k_grad<C>, dim3((unsigned)grid), dim3(C::TT), 0, st, g, l);
+    if (join) hipLaunchKernelGGL(k_join<C>, dim3((unsigned)join, C::TM * C::TN / 1024), dim3(256), 0, st, g);
 }
 template <bool F16>
-void launch_grad_tile(Grad g, bool big, int n, hipStream_t st) {
-    g.slots = slots_of(big);
+void launch_grad_tile(Grad g, bool big, const Loss& l, hipStream_t st) {
     if (g.dh) {
-        if (big) launch_grad<HiddenBig<F16>>(g, n, st);
-        else launch_grad<HiddenSmall<F16>>(g, n, st);
+        if (big) launch_grad<HiddenBig<F16>>(g, l, st);
+        else launch_grad<HiddenSmall<F16>>(g, l, st);
     } else {
-        if (big) launch_grad<WeightBig<F16>>(g, n, st);
-        else launch_grad<WeightSmall<F16>>(g, n, st);
+        if (big) launch_grad<WeightBig<F16>>(g, l, st);
+        else launch_grad<WeightSmall<F16>>(g, l, st);
     }
+}
+template <bool F16>
+void launch_grad_pair(Grad h, Grad w, const Loss& l, hipStream_t st) {
+    using H = HiddenSmall<F16>;
+    using W = WeightSmall<F16>;
+    int join_h, join_w;
+    const int first = grad_grid<H>(&h, &join_h);
+    const int grid = first + grad_grid<W>(&w, &join_w) + (l.out ? 1 : 0);
+    hipLaunchKernelGGL((k_grads<H, W>), dim3((unsigned)grid), dim3(H::TT), 0, st, h, w, l, first);
+    if (join_h + join_w)
+        hipLaunchKernelGGL((k_joins<H, W>), dim3((unsigned)(join_h + join_w), H::TM * H::TN / 1024), dim3(256), 0, st,
+                           h, w, join_h);
 }
 unsigned grid_of(int64_t chunks, int64_t most) {
     const int64_t wg = (chunks + 255) / 256;
@@ -936,8 +1040,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     uint16_t* gbuf = reinterpret_cast<uint16_t*>(ws + p.o_g);
     const bool by_row = p.train && t.reduction == GEFEN_REDUCE_NONE;
 
-    hipLaunchKernelGGL(k_rows, dim3(1), dim3(kRowsThreads), 0, st, t.targets, t.targets_int32, p.n, p.v, t.ignore_index,
-                       by_row ? t.grad : nullptr, map, tgt, meta);
+    const Select sel{t.targets, t.targets_int32, p.n, p.v, t.ignore_index, by_row ? t.grad : nullptr, map, tgt, meta};
     const int x_rows = p.rows * p.pieces;
     Pack pk{};
     pk.src = t.hidden;
@@ -955,29 +1058,34 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     pk.which = 0;
     pk.zero_rows = t.grad_hidden;
     pk.zero_losses = losses;
-    if (pk.f32) {
-        Top tx{static_cast<const float*>(t.hidden), t.hidden_row_stride, t.hidden_col_stride, p.n, p.d, map, meta, 0};
-        const int64_t per = (p.d + 7) / 8;
-        hipLaunchKernelGGL(k_top, dim3(grid_of(p.n * per, 1024)), dim3(256), 0, st, tx);
-        Top tw{static_cast<const float*>(t.weight), t.weight_row_stride, t.weight_col_stride, p.v, p.d, nullptr, meta, 1};
-        hipLaunchKernelGGL(k_top, dim3(grid_of(p.v * per, 1024)), dim3(256), 0, st, tw);
-    }
-    hipLaunchKernelGGL(k_pack, dim3(grid_of(x_rows * (p.dp / 8), 8192)), dim3(256), 0, st, pk);
-    if (p.pack_w) {
-        Pack pw{};
-        pw.src = t.weight;
-        pw.row_stride = t.weight_row_stride;
-        pw.col_stride = t.weight_col_stride;
-        pw.n = p.v;
-        pw.d = p.d;
-        pw.dp = (int)p.dp;
-        pw.f32 = pk.f32;
-        pw.dst = wp;
-        pw.plane = (int64_t)p.v * p.dp;
-        pw.rows = p.v;
-        pw.meta = meta;
-        pw.which = 1;
-        hipLaunchKernelGGL(k_pack, dim3(grid_of(p.v * (p.dp / 8), 8192)), dim3(256), 0, st, pw);
+    Pack pw{};
+    pw.src = t.weight;
+    pw.row_stride = t.weight_row_stride;
+    pw.col_stride = t.weight_col_stride;
+    pw.n = p.v;
+    pw.d = p.d;
+    pw.dp = (int)p.dp;
+    pw.dst = wp;
+    pw.f32 = pk.f32;
+    pw.plane = (int64_t)p.v * p.dp;
+    pw.rows = p.v;
+    pw.meta = meta;
+    pw.which = 1;
+    const int pack_x = (int)grid_of(x_rows * (p.dp / 8), 8192);
+    const int pack_w = p.pack_w ? (int)grid_of(p.v * (p.dp / 8), 8192) : 0;
+    if (p.n <= kSelfRows && !pk.f32) {
+        hipLaunchKernelGGL(k_select_pack, dim3((unsigned)(pack_x + pack_w)), dim3(256), 0, st, sel, pk, pw, pack_x);
+    } else {
+        hipLaunchKernelGGL(k_rows, dim3(1), dim3(kRowsThreads), 0, st, sel);
+        if (pk.f32) {
+            const int64_t per = (p.d + 7) / 8;
+            const Top tx{static_cast<const float*>(t.hidden), t.hidden_row_stride, t.hidden_col_stride, p.n, p.d, map, meta, 0};
+            const Top tw{static_cast<const float*>(t.weight), t.weight_row_stride, t.weight_col_stride, p.v, p.d, nullptr,
+                         meta, 1};
+            const int top_x = (int)grid_of(p.n * per, 1024), top_w = (int)grid_of(p.v * per, 1024);
+            hipLaunchKernelGGL(k_top, dim3((unsigned)(top_x + top_w)), dim3(256), 0, st, tx, tw, top_x);
+        }
+        hipLaunchKernelGGL(k_pack, dim3((unsigned)(pack_x + pack_w)), dim3(256), 0, st, pk, pw, pack_x);
     }
     Operand w{};
     w.p = p.pack_w ? wp : static_cast<const uint16_t*>(t.weight);
@@ -988,6 +1096,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     w.rows = p.v;
     w.cols = (int)p.dp;
 
+    Loss loss{losses, p.n, t.reduction == GEFEN_REDUCE_MEAN, meta, t.loss};
     for (int piece = 0; piece < p.pieces; ++piece) {
         const int from = piece * p.rows;
         const int most = p.n - from < p.rows ? (p.n - from > 0 ? p.n - from : 0) : p.rows;
@@ -1069,39 +1178,49 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         g.mean = t.reduction == GEFEN_REDUCE_MEAN;
         g.by_row = by_row;
         g.dtype = t.dtype;
-        g.parts = reinterpret_cast<float*>(ws + p.o_parts);
+        // the loss goes with the last launch of the last piece
+        const bool last = piece == p.pieces - 1;
+        Loss with{};
+        if (last && (p.dw || most > 0)) std::swap(with, loss);
+        g.b = go;
+        Grad h = g, wg = g;
+        h.parts = reinterpret_cast<float*>(ws + p.o_parts);
+        h.most_parts = p.dh_parts;
+        h.slots = slots_of(p.dh_big);
+        h.a = w;
+        h.dh = 1;
+        h.n = most;
+        h.steps = (p.v + 63) / 64;
+        h.out = t.grad_hidden;
+        wg.parts = reinterpret_cast<float*>(ws + p.o_dw_parts);
+        wg.most_parts = p.dw_parts;
+        wg.slots = slots_of(p.dw_big);
+        wg.a = xo;
+        wg.a.planes = w.planes;
+        wg.dh = 0;
+        wg.n = p.v;
+        wg.sum = p.pieces > 1 ? reinterpret_cast<float*>(ws + p.o_wsum) : nullptr;
+        wg.first = piece == 0;
+        wg.out = t.grad_weight;
+        if (p.pair) {
+            if (f16) launch_grad_pair<true>(h, wg, with, st);
+            else launch_grad_pair<false>(h, wg, with, st);
+            continue;
+        }
         if (p.dh && most > 0) {
-            g.a = w;
-            g.b = go;
-            g.dh = 1;
-            g.n = most;
-            g.steps = (p.v + 63) / 64;
-            g.most_parts = p.dh_parts;
-            g.out = t.grad_hidden;
-            if (f16) launch_grad_tile<true>(g, p.dh_big, most, st);
-            else launch_grad_tile<false>(g, p.dh_big, most, st);
+            if (f16) launch_grad_tile<true>(h, p.dh_big, p.dw ? Loss{} : with, st);
+            else launch_grad_tile<false>(h, p.dh_big, p.dw ? Loss{} : with, st);
         }
         if (p.dw) {
-            g.a = xo;
-            g.a.planes = w.planes;
-            g.b = go;
-            g.dh = 0;
-            g.n = p.v;
-            g.sum = p.pieces > 1 ? reinterpret_cast<float*>(ws + p.o_wsum) : nullptr;
-            g.first = piece == 0;
-            g.most_parts = p.dw_parts;
-            g.out = t.grad_weight;
-            if (f16) launch_grad_tile<true>(g, p.dw_big, p.v, st);
-            else launch_grad_tile<false>(g, p.dw_big, p.v, st);
-            if (g.sum && piece == p.pieces - 1) {
+            if (f16) launch_grad_tile<true>(wg, p.dw_big, with, st);
+            else launch_grad_tile<false>(wg, p.dw_big, with, st);
+            if (wg.sum && last) {
                 const dim3 grid(grid_of(((int64_t)p.v * p.d + 3) / 4, 8192));
-                if (f16) hipLaunchKernelGGL(k_convert<true>, grid, dim3(256), 0, st, g);
-                else hipLaunchKernelGGL(k_convert<false>, grid, dim3(256), 0, st, g);
+                if (f16) hipLaunchKernelGGL(k_convert<true>, grid, dim3(256), 0, st, wg);
+                else hipLaunchKernelGGL(k_convert<false>, grid, dim3(256), 0, st, wg);
             }
         }
     }
-    if (t.loss)
-        hipLaunchKernelGGL(k_loss, dim3(1), dim3(1024), 0, st, losses, p.n, meta, t.reduction == GEFEN_REDUCE_MEAN,
-                           t.loss);
+    if (loss.out) hipLaunchKernelGGL(k_loss, dim3(1), dim3(1024), 0, st, loss);
     return launch_status(what);
 }

@@ -15,12 +15,9 @@ from __future__ import annotations
 import math
 from typing import Iterable, List, Optional, Sequence, Union
 
-import numpy as np
 import torch
 
-from gefen_amd import _gefen_host, _lib
-
-from .gefen_hip import check, device_guard, load_extension, stream_of
+from gefen_amd import _lib
 
 __all__ = ["gradient_norm", "clip_gradients", "clip_grad_norm_"]
 
@@ -47,31 +44,15 @@ def _as_list(tensors, name: str) -> List[torch.Tensor]:
     return list(tensors)
 
 
-def _rows(grads: List[torch.Tensor], out: Optional[List[torch.Tensor]], writes: bool):
-    """The task table of a call, and (destination, contiguous stand-in) pairs to copy
-    back for tensors that are not one dense run of elements."""
-    table = np.empty(len(grads), dtype=_lib.GRADIENT_TASK)
-    bad, _ = _gefen_host.gradient_rows(grads, out, table.ctypes.data, writes)
-    if bad < 0:
-        return table, grads, ()
+def _dense(grads: List[torch.Tensor], out: Optional[List[torch.Tensor]] = None):
+    """Contiguous stand-ins for tensors that are not one dense run of elements, and the
+    (destination, stand-in) pairs to copy back."""
     src, dst, back = list(grads), list(grads if out is None else out), []
-    for k in range(bad, len(src)):
-        g, o = src[k], dst[k]
-        if g.is_contiguous() and o.is_contiguous():
-            continue
-        src[k] = g.contiguous()
-        if writes:
-            dst[k] = torch.empty(g.shape, dtype=o.dtype, device=g.device)
+    for k, (g, o) in enumerate(zip(grads, dst)):
+        if not (g.is_contiguous() and o.is_contiguous()):
+            src[k], dst[k] = g.contiguous(), torch.empty(g.shape, dtype=o.dtype, device=g.device)
             back.append((o, dst[k]))
-    bad, _ = _gefen_host.gradient_rows(src, dst if writes else None, table.ctypes.data, writes)
-    assert bad < 0
-    return table, src, back
-
-
-def _workspace(lib, table, device) -> torch.Tensor:
-    """The norm's slot and, 16 bytes on, the library's workspace."""
-    nbytes = int(lib.gefen_gradient_norm_workspace_size(table.ctypes.data, len(table)))
-    return torch.empty(nbytes + 16, dtype=torch.uint8, device=device)
+    return src, dst, back
 
 
 def gradient_norm(gradients: Sequence[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
@@ -83,15 +64,9 @@ def gradient_norm(gradients: Sequence[torch.Tensor], norm_type: float = 2.0) -> 
     grads = _as_list(gradients, "gradients")
     if not grads:
         return torch.zeros(())
-    table, keep, _ = _rows(grads, None, False)
-    lib = load_extension()
-    with device_guard(grads[0]):
-        norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-        ws = _workspace(lib, table, grads[0].device)
-        rc = lib.gefen_gradient_norm(table.ctypes.data, len(table), norm_type, norm.data_ptr(), ws.data_ptr() + 16,
-                                     stream_of(norm))
-    check(rc, "gradient_norm")
-    return norm
+    host = _lib.host()
+    norm = host.gradient_norm(grads, norm_type)
+    return norm if norm is not None else host.gradient_norm(_dense(grads)[0], norm_type)
 
 
 def clip_gradients(gradients: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0, *,
@@ -119,22 +94,14 @@ def clip_gradients(gradients: Sequence[torch.Tensor], max_norm: float, norm_type
         if outs:
             raise ValueError("Expected as many output tensors as gradients.")
         return torch.zeros(()) if total_norm is None else total_norm
-    with torch.no_grad():
-        table, keep, back = _rows(grads, outs, True)
-        lib = load_extension()
-        with device_guard(grads[0]):
-            if total_norm is not None:
-                norm = total_norm
-                rc = lib.gefen_scale_gradients(table.ctypes.data, len(table), norm.data_ptr(), max_norm,
-                                               stream_of(norm))
-            else:
-                norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-                ws = _workspace(lib, table, grads[0].device)
-                rc = lib.gefen_clip_gradients(table.ctypes.data, len(table), norm_type, max_norm, norm.data_ptr(),
-                                              ws.data_ptr() + 16, stream_of(norm))
-            check(rc, "clip_gradients")
-        for dst, tmp in back:
-            dst.copy_(tmp)
+    host = _lib.host()
+    norm = host.clip_gradients(grads, outs, max_norm, norm_type, total_norm)
+    if norm is None:
+        with torch.no_grad():
+            src, dst, back = _dense(grads, outs)
+            norm = host.clip_gradients(src, dst, max_norm, norm_type, total_norm)
+            for o, t in back:
+                o.copy_(t)
     return norm
 
 
