@@ -63,12 +63,14 @@ struct Operand {
 
 constexpr float kLowScale = 2048.0f;  // of half-precision low parts
 
-template <bool F16_, int TM_, int TN_, int WM_, int WN_, int BK_, int NST_, bool AMN_, bool BMN_, int GROUP_M_>
+template <bool F16_, int TM_, int TN_, int WM_, int WN_, int BK_, int NST_, bool AMN_, bool BMN_, int GROUP_M_,
+          bool STREAM_A_ = false>
 struct Cfg {
     static constexpr bool F16 = F16_, AMN = AMN_, BMN = BMN_;
     static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, BK = BK_, NST = NST_;
     static constexpr int WI = WM / 16, WJ = WN / 16;
     static constexpr int WAVES_M = TM / WM, WAVES_N = TN / WN;
+    static constexpr bool STREAM_A = STREAM_A_;  // A is read once by the whole launch
     static constexpr int GROUP_M = GROUP_M_;  // tile rows per band of the tile order
     static constexpr int TT = 64 * WAVES_M * WAVES_N;
     static constexpr int A_ELEMS = TM * BK, B_ELEMS = TN * BK, STAGE = A_ELEMS + B_ELEMS;
@@ -94,13 +96,17 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 // waits for it.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: the compiler sets it before each use of its own
+template <bool STREAM>
 __device__ __forceinline__ void load_to_lds(i32x4 rsrc, int voff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "m0");
+    if constexpr (STREAM)
+        asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(lds), "v"(voff), "s"(rsrc)
+                     : "m0");
+    else asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "m0");
 }
 #pragma clang diagnostic pop
 
 // One operand's side of the K loop.
-template <int ROWS, int BK, int LOADS, int TT, bool MN>
+template <int ROWS, int BK, int LOADS, int TT, bool MN, bool STREAM>
 struct Loader {
     static constexpr int CPR = MN ? ROWS / 8 : BK / 8;  // 16-byte chunks of a tile row
     static_assert(!MN || CPR >= 16, "swizzle_mn");
@@ -137,11 +143,11 @@ struct Loader {
             for (int i = 0; i < LOADS; ++i) {
                 const int r = ((int)threadIdx.x + TT * i) / CPR;
                 const int back = max(k * BK + r - (o.rows - 1), 0);
-                load_to_lds(rsrc, (int)(voff[i] - (int64_t)back * o.ld * 2), l0 + TT * i * 16);
+                load_to_lds<STREAM>(rsrc, (int)(voff[i] - (int64_t)back * o.ld * 2), l0 + TT * i * 16);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) load_to_lds(rsrc, voff[i], l0 + TT * i * 16);
+            for (int i = 0; i < LOADS; ++i) load_to_lds<STREAM>(rsrc, voff[i], l0 + TT * i * 16);
         }
     }
 };
@@ -218,8 +224,8 @@ __device__ __forceinline__ void product_tile(const Operand& A, const Operand& B,
         for (int j = 0; j < WJ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const int per = k_to - k_from, steps = per * segs;
     if (steps <= 0) return;
-    Loader<C::TM, C::BK, C::A_LOADS, C::TT, C::AMN> la;
-    Loader<C::TN, C::BK, C::B_LOADS, C::TT, C::BMN> lb;
+    Loader<C::TM, C::BK, C::A_LOADS, C::TT, C::AMN, C::STREAM_A> la;
+    Loader<C::TN, C::BK, C::B_LOADS, C::TT, C::BMN, false> lb;
     la.init(A, m0);
     lb.init(B, n0);
     int lk = k_from, lseg = 0;  // the next step to load (past the last one: the last again)

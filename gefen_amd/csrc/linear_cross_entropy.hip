@@ -809,7 +809,7 @@ int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
 template <bool F16> using LogitsBig = Cfg<F16, 256, 256, 64, 128, 64, 2, false, false, 4>;
 template <bool F16> using LogitsSmall = Cfg<F16, 128, 128, 64, 64, 64, 2, false, false, 4>;
-template <bool F16> using LogitsRow = Cfg<F16, 256, 32, 64, 32, 64, 4, false, false, 4>;
+template <bool F16> using LogitsRow = Cfg<F16, 128, 32, 64, 32, 64, 4, false, false, 4, true>;
 template <bool F16> using HiddenBig = Cfg<F16, 256, 256, 64, 128, 64, 2, true, false, 8>;
 template <bool F16> using HiddenSmall = Cfg<F16, 128, 128, 64, 64, 64, 2, true, false, 8>;
 template <bool F16> using WeightBig = Cfg<F16, 256, 256, 128, 64, 64, 2, true, true, 4>;
