@@ -58,6 +58,7 @@ struct Meta {
     int32_t count;    // rows that take part
     float grad_max;   // largest |gradient| of a row (per-row gradients)
     uint32_t top[2];  // float32: largest finite magnitude of hidden and weight, as bits
+    float factor[2];  // what the sums of dW and dh are multiplied by
 };
 
 __device__ __forceinline__ int piece_rows(const Meta* m, int from, int most) {
@@ -85,7 +86,7 @@ __device__ __forceinline__ Meta select_rows(const Select& s, int32_t* map, int32
     __shared__ int wave_sum[THREADS / 64];
     __shared__ float wave_max[THREADS / 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    Meta m = {0, 0.0f, {0, 0}};
+    Meta m = {0, 0.0f, {0, 0}, {0.0f, 0.0f}};
     for (int at = 0; at < s.n; at += THREADS) {
         const int i = at + (int)threadIdx.x;
         const int64_t y = i < s.n ? target_at(s.targets, s.targets_int32, i) : s.ignore;
@@ -163,6 +164,18 @@ __device__ __forceinline__ uint32_t pack_exp2(float a, float b) {
 template <bool F16>
 __device__ __forceinline__ float unpack_exp(uint16_t x) {
     return __uint_as_float((uint32_t)x << (F16 ? 11 : 13)) * (F16 ? 0x1p112f : 0x1p64f);
+}
+
+// Packed pairs of 16-bit values of a lane's four rows of MFMA tiles i (a) and i + 1 (b),
+// rearranged so that every lane has eight consecutive rows: those of tile i + (lane / 32)
+// from 8 ((lane / 16) % 2).  Lanes exchange with lanes of the same column only.
+__device__ __forceinline__ uint4 eight_rows(uint2 a, uint2 b) {
+    typedef uint32_t pair __attribute__((ext_vector_type(2)));
+    pair x = __builtin_amdgcn_permlane32_swap(a.x, b.x, false, false);
+    pair y = __builtin_amdgcn_permlane32_swap(a.y, b.y, false, false);
+    x = __builtin_amdgcn_permlane16_swap(x[0], x[1], false, false);
+    y = __builtin_amdgcn_permlane16_swap(y[0], y[1], false, false);
+    return make_uint4(x[0], y[0], x[1], y[1]);
 }
 
 // Exponent that brings a matrix's largest finite magnitude (its bits in `top`) to 2^14.
@@ -409,26 +422,31 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
         }
         if constexpr (KEEP == kKeepNone) continue;
         // rows past the piece's end stay inside the workspace (it holds whole tiles)
-        uint16_t* row = a.g + (int64_t)n * a.ldg + wm + hi;
+        uint16_t* row = a.g + (int64_t)n * a.ldg + wm + 16 * (lane >> 5) + 8 * (lane >> 4 & 1);
 #pragma unroll
-        for (int i = 0; i < WI; ++i) {
-            uint16_t* to = row + i * 16;
-            if constexpr (KEEP == kKeepPacked) {
-                *reinterpret_cast<uint2*>(to) = make_uint2(pack_exp2<C::F16>(acc[i][j][0], acc[i][j][1]),
-                                                           pack_exp2<C::F16>(acc[i][j][2], acc[i][j][3]));
-            } else {
-                uint16_t o[2][4];
+        for (int i = 0; i < WI; i += 2) {
+            uint2 w[2][2];  // [plane][tile]
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if constexpr (C::F16) split_half_fast(acc[i][j][r] * kHalfScale, &o[0][r], &o[1][r]);
-                    else split_bf16(acc[i][j][r], &o[0][r], &o[1][r]);
+            for (int t = 0; t < 2; ++t) {
+                const f32x4 e = acc[i + t][j];
+                if constexpr (KEEP == kKeepPacked) {
+                    w[0][t] = make_uint2(pack_exp2<C::F16>(e[0], e[1]), pack_exp2<C::F16>(e[2], e[3]));
+                } else {
+                    uint16_t o[2][4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if constexpr (C::F16) split_half_fast(e[r] * kHalfScale, &o[0][r], &o[1][r]);
+                        else split_bf16(e[r], &o[0][r], &o[1][r]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        w[k][t] = make_uint2((uint32_t)o[k][0] | ((uint32_t)o[k][1] << 16),
+                                             (uint32_t)o[k][2] | ((uint32_t)o[k][3] << 16));
                 }
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    *reinterpret_cast<uint2*>(to + k * a.g_plane) =
-                        make_uint2((uint32_t)o[k][0] | ((uint32_t)o[k][1] << 16),
-                                   (uint32_t)o[k][2] | ((uint32_t)o[k][3] << 16));
             }
+            *reinterpret_cast<uint4*>(row + i * 16) = eight_rows(w[0][0], w[0][1]);
+            if constexpr (KEEP == kKeepPlanes)
+                *reinterpret_cast<uint4*>(row + i * 16 + a.g_plane) = eight_rows(w[1][0], w[1][1]);
         }
     }
 }
@@ -440,8 +458,10 @@ struct Rows {
     const float* target_logit;
     const int32_t* tgt;
     const int32_t* map;
-    const Meta* meta;
+    Meta* meta;
     const float* row_grad;  // gradient of each row's loss (null: one for all)
+    const float* grad;      // gradient of the loss (null: 1)
+    int32_t mean, dtype;
     float* losses;          // [n], original order
     uint16_t* g;
     int64_t ldg, g_plane;
@@ -463,6 +483,18 @@ __global__ __launch_bounds__(kGradThreads) void k_gradient_rows(const Rows a) {
     const int r = blockIdx.x;
     const int rows = piece_rows(a.meta, a.from, a.most);
     const int chunks = (int)(a.ldg / 8);
+    if (a.g && r == 0 && blockIdx.y == 0 && threadIdx.x < 2) {
+        // of dW (whose other operand is hidden) and dh
+        float f = a.dtype == GEFEN_BF16 ? 1.0f : 1.0f / kHalfScale;
+        if (a.dtype == GEFEN_F32) f = ldexpf(f, -half_exponent(a.meta->top[threadIdx.x]));
+        if (a.row_grad) {
+            f *= a.meta->grad_max;
+        } else {
+            if (a.grad) f *= *a.grad;
+            if (a.mean) f = a.meta->count ? f / (float)a.meta->count : 0.0f;
+        }
+        a.meta->factor[threadIdx.x] = f;
+    }
     if (r >= rows) {  // zero rows up to the end of the last K step of dW
         if (!a.g || r >= (rows + 63) / 64 * 64) return;
         Vec<uint16_t, 8> z = {};
@@ -589,8 +621,6 @@ struct Grad {
     int32_t from, most;
     const int32_t* map;
     const Meta* meta;
-    const float* grad;      // gradient of the loss (null: 1)
-    int32_t mean, by_row;   // by_row: G is scaled by 1 / meta->grad_max
     int32_t slots;          // workgroups that fill the chip
     int32_t most_parts;     // partial tiles that `parts` holds
     float* parts;           // [cut][tile of the rest][TN][TM]
@@ -599,15 +629,6 @@ struct Grad {
     void* out;
     int32_t dtype;
 };
-
-__device__ __forceinline__ float grad_factor(const Grad& g) {
-    float f = g.dtype == GEFEN_BF16 ? 1.0f : 1.0f / kHalfScale;
-    if (g.dtype == GEFEN_F32) f = ldexpf(f, -half_exponent(g.meta->top[g.dh ? 1 : 0]));
-    if (g.by_row) return f * g.meta->grad_max;
-    if (g.grad) f *= *g.grad;
-    if (g.mean) f = g.meta->count ? f / (float)g.meta->count : 0.0f;
-    return f;
-}
 
 // How the tiles of a product meet the chip: whole rounds of it tile by tile, and the
 // `rest` of the tiles with K cut into `cuts` equal parts, each left in float32 for k_join.
@@ -650,16 +671,17 @@ __device__ __forceinline__ int cuts_of(const Grad& g, const Deal& d) {
     return cuts;
 }
 
-// cnt (1 to 4) results of output row `row`, from column m, as OUT: added to the sum over
-// the pieces (plain float32), or times the factor in the result's type.
+// A result goes to the sum over the pieces (plain float32), or times the factor to the
+// output in its type.
 enum Out { kOutSum, kOutF32, kOut16 };
-template <bool F16, int OUT>
-__device__ __forceinline__ void finish(const Grad& g, int64_t row, int m, int cnt, f32x4 v, float factor) {
+// cnt (1 to 4) float32 results of output row `row`, from column m
+template <int OUT>
+__device__ __forceinline__ void finish_f32(const Grad& g, int64_t row, int m, int cnt, f32x4 v, float factor) {
     const int64_t at = row * g.d + m;
     if constexpr (OUT == kOutSum) {
         float* s = g.sum + at;
         for (int e = 0; e < cnt; ++e) s[e] = g.first ? v[e] : s[e] + v[e];
-    } else if constexpr (OUT == kOutF32) {
+    } else {
         v *= factor;
         float* o = static_cast<float*>(g.out) + at;
         if (cnt == 4) {
@@ -667,30 +689,54 @@ __device__ __forceinline__ void finish(const Grad& g, int64_t row, int m, int cn
         } else {
             for (int e = 0; e < cnt; ++e) o[e] = v[e];
         }
-    } else {
-        AnyVec<uint16_t, 4> x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            x.v[e] = F16 ? from_f32<f16_t>(v[e] * factor).bits : from_f32<bf16_t>(v[e] * factor).bits;
-        uint16_t* o = static_cast<uint16_t*>(g.out) + at;
-        if (cnt == 4) {
-            *reinterpret_cast<AnyVec<uint16_t, 4>*>(o) = x;
-        } else {
-            for (int e = 0; e < cnt; ++e) o[e] = x.v[e];
-        }
     }
 }
+template <bool F16>
+__device__ __forceinline__ uint2 round16(f32x4 v, float factor) {
+    uint16_t o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = F16 ? from_f32<f16_t>(v[e] * factor).bits : from_f32<bf16_t>(v[e] * factor).bits;
+    return make_uint2((uint32_t)o[0] | ((uint32_t)o[1] << 16), (uint32_t)o[2] | ((uint32_t)o[3] << 16));
+}
+// cnt (1 to 8 of N) 16-bit results
+template <int N>
+__device__ __forceinline__ void store16(const Grad& g, int64_t row, int m, int cnt, const uint32_t (&w)[N / 2]) {
+    uint16_t* o = static_cast<uint16_t*>(g.out) + row * g.d + m;
+    AnyVec<uint16_t, N> x;
+    __builtin_memcpy(&x, w, sizeof(x));
+    if (cnt >= N) {
+        *reinterpret_cast<AnyVec<uint16_t, N>*>(o) = x;
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (e < cnt) o[e] = x.v[e];
+    }
+}
+// The tile of this wave, from row m of the product and its column n.
 template <typename C, int OUT>
-__device__ __forceinline__ void finish_tile(const Grad& g, int n_all, int m, int n0, const f32x4 (&acc)[C::WI][C::WJ]) {
-    const float factor = grad_factor(g);
+__device__ __forceinline__ void finish_tile(const Grad& g, int n_all, int m0, int n0, float factor,
+                                            const f32x4 (&acc)[C::WI][C::WJ]) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int j = 0; j < C::WJ; ++j) {
-        const int n = n0 + j * 16;
+        const int n = n0 + j * 16 + (lane & 15);
         if (n >= n_all) continue;
         const int64_t row = g.dh ? g.map[g.from + n] : n;
+        if constexpr (OUT == kOut16) {
 #pragma unroll
-        for (int i = 0; i < C::WI; ++i)
-            if (m + i * 16 < g.d) finish<C::F16, OUT>(g, row, m + i * 16, min(4, g.d - m - i * 16), acc[i][j], factor);
+            for (int i = 0; i < C::WI; i += 2) {
+                const uint4 v = eight_rows(round16<C::F16>(acc[i][j], factor), round16<C::F16>(acc[i + 1][j], factor));
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                const int m = m0 + 16 * (i + (lane >> 5)) + 8 * (lane >> 4 & 1);
+                if (m < g.d) store16<8>(g, row, m, g.d - m, w);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < C::WI; ++i) {
+                const int m = m0 + i * 16 + 4 * (lane >> 4);
+                if (m < g.d) finish_f32<OUT>(g, row, m, min(4, g.d - m), acc[i][j], factor);
+            }
+        }
     }
 }
 
@@ -708,6 +754,7 @@ __device__ __forceinline__ void grad_block(const Grad& g, int b, uint16_t* smem)
         cut = u / deal.rest;
         tile = deal.full + u - cut * deal.rest;
     }
+    const float factor = g.meta->factor[g.dh];
     int ti, tj;
     tile_of<C::GROUP_M>(tile, g.tiles_m, deal.tiles_n, &ti, &tj);
     const int m0 = ti * C::TM, n0 = tj * C::TN;
@@ -715,19 +762,18 @@ __device__ __forceinline__ void grad_block(const Grad& g, int b, uint16_t* smem)
     product_tile<C>(g.a, g.b, m0, n0, (int)((int64_t)deal.steps * cut / cuts),
                     (int)((int64_t)deal.steps * (cut + 1) / cuts), g.segs, smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = (wave / C::WAVES_N) * C::WM + 4 * (lane >> 4), wn = (wave % C::WAVES_N) * C::WN + (lane & 15);
+    const int wm = (wave / C::WAVES_N) * C::WM, wn = (wave % C::WAVES_N) * C::WN;
     if (cuts > 1) {
-        float* p = g.parts + (int64_t)u * (C::TM * C::TN);
+        float* p = g.parts + (int64_t)u * (C::TM * C::TN) + (wn + (lane & 15)) * C::TM + wm + 4 * (lane >> 4);
 #pragma unroll
         for (int j = 0; j < WJ; ++j)
 #pragma unroll
-            for (int i = 0; i < WI; ++i)
-                *reinterpret_cast<f32x4*>(p + (wn + j * 16) * C::TM + wm + i * 16) = acc[i][j];
+            for (int i = 0; i < WI; ++i) *reinterpret_cast<f32x4*>(p + j * 16 * C::TM + i * 16) = acc[i][j];
         return;
     }
-    if (g.sum) finish_tile<C, kOutSum>(g, deal.n_all, m0 + wm, n0 + wn, acc);
-    else if (C::F16 && g.dtype == GEFEN_F32) finish_tile<C, kOutF32>(g, deal.n_all, m0 + wm, n0 + wn, acc);
-    else finish_tile<C, kOut16>(g, deal.n_all, m0 + wm, n0 + wn, acc);
+    if (g.sum) finish_tile<C, kOutSum>(g, deal.n_all, m0 + wm, n0 + wn, factor, acc);
+    else if (C::F16 && g.dtype == GEFEN_F32) finish_tile<C, kOutF32>(g, deal.n_all, m0 + wm, n0 + wn, factor, acc);
+    else finish_tile<C, kOut16>(g, deal.n_all, m0 + wm, n0 + wn, factor, acc);
 }
 
 // One gradient's product; the last workgroup sums the losses where l.out is given, which
@@ -766,10 +812,16 @@ __device__ __forceinline__ void join_block(const Grad& g, int t) {
         v += *reinterpret_cast<const f32x4*>(g.parts + ((int64_t)c * deal.rest + t) * (C::TM * C::TN) + q);
     const int64_t row = g.dh ? g.map[g.from + n] : n;
     const int cnt = min(4, g.d - m);
-    const float factor = grad_factor(g);
-    if (g.sum) finish<C::F16, kOutSum>(g, row, m, cnt, v, factor);
-    else if (C::F16 && g.dtype == GEFEN_F32) finish<C::F16, kOutF32>(g, row, m, cnt, v, factor);
-    else finish<C::F16, kOut16>(g, row, m, cnt, v, factor);
+    const float factor = g.meta->factor[g.dh];
+    if (g.sum) {
+        finish_f32<kOutSum>(g, row, m, cnt, v, factor);
+    } else if (C::F16 && g.dtype == GEFEN_F32) {
+        finish_f32<kOutF32>(g, row, m, cnt, v, factor);
+    } else {
+        const uint2 r = round16<C::F16>(v, factor);
+        const uint32_t w[2] = {r.x, r.y};
+        store16<4>(g, row, m, cnt, w);
+    }
 }
 
 template <typename C>
@@ -786,7 +838,7 @@ __global__ __launch_bounds__(256) void k_joins(const Grad h, const Grad w, int f
 template <bool F16>
 __global__ __launch_bounds__(256) void k_convert(const Grad g) {
     const int64_t all = ((int64_t)g.n * g.d + 3) / 4, numel = (int64_t)g.n * g.d;
-    const float factor = grad_factor(g);
+    const float factor = g.meta->factor[0];
     const float* sum = g.sum;
     for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < all; q += (int64_t)gridDim.x * 256) {
         f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -1139,6 +1191,9 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
             r.map = map;
             r.meta = meta;
             r.row_grad = by_row ? t.grad : nullptr;
+            r.grad = by_row ? nullptr : t.grad;
+            r.mean = t.reduction == GEFEN_REDUCE_MEAN;
+            r.dtype = t.dtype;
             r.losses = losses;
             r.g = l.g;
             r.ldg = p.ldg;
@@ -1174,9 +1229,6 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         g.most = most;
         g.map = map;
         g.meta = meta;
-        g.grad = by_row ? nullptr : t.grad;
-        g.mean = t.reduction == GEFEN_REDUCE_MEAN;
-        g.by_row = by_row;
         g.dtype = t.dtype;
         // the loss goes with the last launch of the last piece
         const bool last = piece == p.pieces - 1;
