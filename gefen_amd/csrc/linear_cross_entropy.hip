@@ -87,25 +87,41 @@ __device__ __forceinline__ Meta select_rows(const Select& s, int32_t* map, int32
     __shared__ float wave_max[THREADS / 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     Meta m = {0, 0.0f, {0, 0}, {0.0f, 0.0f}};
-    for (int at = 0; at < s.n; at += THREADS) {
-        const int i = at + (int)threadIdx.x;
-        const int64_t y = i < s.n ? target_at(s.targets, s.targets_int32, i) : s.ignore;
-        const bool live = i < s.n && y != s.ignore;
-        const uint64_t ball = __ballot(live);
-        const int before = __popcll(ball & ((1ull << lane) - 1ull));
-        if (lane == 0) wave_sum[wave] = __popcll(ball);
+    // a wave takes 64 kEach consecutive rows of each stretch, so that one barrier serves
+    // kEach loads in flight
+    constexpr int kEach = 4;
+    for (int at = 0; at < s.n; at += THREADS * kEach) {
+        const int first = at + wave * 64 * kEach + lane;
+        int64_t y[kEach];
+#pragma unroll
+        for (int k = 0; k < kEach; ++k)
+            y[k] = first + 64 * k < s.n ? target_at(s.targets, s.targets_int32, first + 64 * k) : s.ignore;
+        uint64_t ball[kEach];
+        int mine = 0;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            ball[k] = __ballot(y[k] != s.ignore);
+            mine += __popcll(ball[k]);
+        }
+        if (lane == 0) wave_sum[wave] = mine;
         __syncthreads();
         int off = m.count, all = 0;
         for (int w = 0; w < THREADS / 64; ++w) {
             if (w < wave) off += wave_sum[w];
             all += wave_sum[w];
         }
-        if (live) {
-            map[off + before] = i;
-            if (tgt) tgt[off + before] = (y >= 0 && y < s.v) ? (int)y : -1;
-            if (s.row_grad) m.grad_max = nanmax(m.grad_max, fabsf(s.row_grad[i]));
-        } else if (i < s.n) {
-            map[s.n - 1 - (i - off - before)] = i;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const int i = first + 64 * k;
+            const int before = off + __popcll(ball[k] & ((1ull << lane) - 1ull));
+            if (y[k] != s.ignore) {
+                map[before] = i;
+                if (tgt) tgt[before] = (y[k] >= 0 && y[k] < s.v) ? (int)y[k] : -1;
+                if (s.row_grad) m.grad_max = nanmax(m.grad_max, fabsf(s.row_grad[i]));
+            } else if (i < s.n) {
+                map[s.n - 1 - (i - before)] = i;
+            }
+            off += __popcll(ball[k]);
         }
         m.count += all;
         __syncthreads();
@@ -475,8 +491,27 @@ __device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
     return make_float2(m, a.y * expf(a.x - ref) + b.y * expf(b.x - ref));
 }
 
+template <bool STREAM>
+__device__ __forceinline__ Vec<uint16_t, 8> load8(const uint16_t* p) {
+    using R = typename RawVec<16>::type;
+    const R r = STREAM ? __builtin_nontemporal_load(reinterpret_cast<const R*>(p)) : *reinterpret_cast<const R*>(p);
+    Vec<uint16_t, 8> x;
+    __builtin_memcpy(&x, &r, sizeof(x));
+    return x;
+}
+template <bool STREAM>
+__device__ __forceinline__ void store8(uint16_t* p, const Vec<uint16_t, 8>& x) {
+    using R = typename RawVec<16>::type;
+    R r;
+    __builtin_memcpy(&r, &x, sizeof(r));
+    if (STREAM) __builtin_nontemporal_store(r, reinterpret_cast<R*>(p));
+    else *reinterpret_cast<R*>(p) = r;
+}
+
+constexpr int64_t kKeepBytes = 192 << 20;  // of a memory-side cache of 256 MB
 constexpr int kGradThreads = 256;
-template <bool F16>
+// STREAM: G is larger than the memory-side cache holds, and its values go past the caches.
+template <bool F16, bool STREAM>
 __global__ __launch_bounds__(kGradThreads) void k_gradient_rows(const Rows a) {
     __shared__ float2 part[kGradThreads / 64];
     __shared__ float part_sum[kGradThreads / 64];
@@ -557,8 +592,8 @@ __global__ __launch_bounds__(kGradThreads) void k_gradient_rows(const Rows a) {
         for (int i = 0; i < kBatch; ++i) {
             const int c = min(c0 + i * stride, chunks - 1);
             top[i] = stats[min(c * 8, a.v - 1) / kSlot].x;
-            x[i][0] = vload<uint16_t, 8>(row, (int64_t)c * 8);
-            if (a.planes == 2) x[i][1] = vload<uint16_t, 8>(row + a.g_plane, (int64_t)c * 8);
+            x[i][0] = load8<STREAM>(row + (int64_t)c * 8);
+            if (a.planes == 2) x[i][1] = load8<STREAM>(row + a.g_plane + (int64_t)c * 8);
         }
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
@@ -582,8 +617,8 @@ __global__ __launch_bounds__(kGradThreads) void k_gradient_rows(const Rows a) {
                 else if (F16) split_half_fast(q, &hi.v[e], &lo.v[e]);
                 else split_bf16(q, &hi.v[e], &lo.v[e]);
             }
-            vstore(row, (int64_t)c * 8, hi);
-            if (a.planes == 2) vstore(row + a.g_plane, (int64_t)c * 8, lo);
+            store8<STREAM>(row + (int64_t)c * 8, hi);
+            if (a.planes == 2) store8<STREAM>(row + a.g_plane + (int64_t)c * 8, lo);
         }
     }
 }
@@ -1211,8 +1246,10 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
             if (parts > chunks) parts = chunks;
             if (parts < 1) parts = 1;
             const dim3 grid((unsigned)rows_up, (unsigned)parts);
-            if (f16) hipLaunchKernelGGL(k_gradient_rows<true>, grid, dim3(kGradThreads), 0, st, r);
-            else hipLaunchKernelGGL(k_gradient_rows<false>, grid, dim3(kGradThreads), 0, st, r);
+            const bool stream_past = p.train && (int64_t)p.planes * most * p.ldg * 2 > kKeepBytes;
+            auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kGradThreads), 0, st, r); };
+            if (f16) stream_past ? launch(k_gradient_rows<true, true>) : launch(k_gradient_rows<true, false>);
+            else stream_past ? launch(k_gradient_rows<false, true>) : launch(k_gradient_rows<false, false>);
         }
         if (!p.train) continue;
         Operand go{};
