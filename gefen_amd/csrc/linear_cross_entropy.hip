@@ -31,8 +31,9 @@
 // A half-precision G is scaled by 2^15 (and its products by 2^-15), which keeps
 // probabilities down to 1e-9 out of half's subnormals.  float32 runs as two half planes
 // per operand and three products, each matrix scaled by the power of two that brings its
-// largest finite element to 2^14: elements keep 22 bits down to 2^-29 of the largest
-// one, at five times the rate of the float32 matrix instructions.
+// largest finite element to 2^14: elements keep 22 bits down to 2^-28 of the largest
+// one, and what they keep ends at 2^-49 of it (2^-50 for G, whose largest is 1), at five
+// times the rate of the float32 matrix instructions.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
