@@ -7,6 +7,7 @@
 // operation: at full load the clock is set by power, and 16x16x32 ran 8% faster than
 // 32x32x16 on the logits' product).  Each operand is either K-major (a row of it is
 // contiguous along k) or MN-major (stored as its transpose: a row holds one k).
+// A workgroup stays on its CU and takes tile after tile (product_stream).
 // K advances BK at a time through NST LDS stages that are filled straight from
 // global memory (buffer loads with the LDS destination), NST - 1 steps ahead, so an
 // operand takes no registers on its way and one barrier ends a step.
@@ -206,38 +207,49 @@ __device__ __forceinline__ void wait_loads_and_sync() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// acc of the tile at (m0, n0) over K steps [k_from, k_to) of each of `segs` segments:
-// acc[i][j][r] is m = m0 + (wave's) + 16 i + 4 (lane / 16) + r, n = n0 + (wave's) + 16 j +
-// lane % 16.
-template <typename C>
-__device__ __forceinline__ void product_tile(const Operand& A, const Operand& B, int m0, int n0, int k_from, int k_to,
-                                             int segs, uint16_t* smem, f32x4 (&acc)[C::WI][C::WJ]) {
+// A unit of work: the tile at (m0, n0) over K steps [k0, k1) of each segment.
+struct Unit {
+    int m0, n0, k0, k1;
+};
+
+// The units first, first + stride, ... below `total` of this workgroup as one stream of K
+// steps: the loads run ahead across the end of a unit, so that the next one's operands
+// arrive while this one's results are written.  unit_of(u) names unit u; finish(u, unit,
+// acc) takes its sums: acc[i][j][r] is m = m0 + (wave's) + 16 i + 4 (lane / 16) + r, n =
+// n0 + (wave's) + 16 j + lane % 16.  Every unit has a K step at least.
+template <typename C, typename UnitOf, typename Finish>
+__device__ __forceinline__ void product_stream(const Operand& A, const Operand& B, int segs, int first, int total,
+                                               int stride, uint16_t* smem, UnitOf unit_of, Finish finish) {
     constexpr int WI = C::WI, WJ = C::WJ, NST = C::NST, NS = C::BK / 32;
     constexpr int LOADS = C::A_LOADS + C::B_LOADS;
     constexpr int READS = WI * (C::AMN ? 2 : 1) + WJ * (C::BMN ? 2 : 1);   // LDS reads of a slice
     constexpr int PER = (2 * READS + WI * WJ - 1) / (WI * WJ);             // of them after each MFMA
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = (wave / C::WAVES_N) * C::WM, wn = (wave % C::WAVES_N) * C::WN;
-#pragma unroll
-    for (int i = 0; i < WI; ++i)
-#pragma unroll
-        for (int j = 0; j < WJ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const int per = k_to - k_from, steps = per * segs;
-    if (steps <= 0) return;
     Loader<C::TM, C::BK, C::A_LOADS, C::TT, C::AMN, C::STREAM_A> la;
     Loader<C::TN, C::BK, C::B_LOADS, C::TT, C::BMN, false> lb;
-    la.init(A, m0);
-    lb.init(B, n0);
-    int lk = k_from, lseg = 0;  // the next step to load (past the last one: the last again)
+    // the next step to load (past the last one: the last again)
+    int lu = first, lk, lseg = 0;
+    Unit load = unit_of(first);
+    la.init(A, load.m0);
+    lb.init(B, load.n0);
+    lk = load.k0;
     auto issue = [&](int stage) {
         uint16_t* s = smem + stage * C::STAGE;
         la.issue(A, (int64_t)(A.planes >> (2 * lseg) & 3u) * A.plane, lk, s);
         lb.issue(B, (int64_t)(B.planes >> (2 * lseg) & 3u) * B.plane, lk, s + C::A_ELEMS);
-        if (lk + 1 < k_to) {
+        if (lk + 1 < load.k1) {
             ++lk;
         } else if (lseg + 1 < segs) {
-            lk = k_from;
+            lk = load.k0;
             ++lseg;
+        } else if (lu + stride < total) {
+            lu += stride;
+            load = unit_of(lu);
+            la.init(A, load.m0);
+            lb.init(B, load.n0);
+            lk = load.k0;
+            lseg = 0;
         }
     };
     bf16x8 af[2][WI], bf[2][WJ];
@@ -254,39 +266,49 @@ __device__ __forceinline__ void product_tile(const Operand& A, const Operand& B,
 #pragma unroll
     for (int s = 0; s < NST - 1; ++s) issue(s);
     int stage = 0;
-    for (int k = 0; k < steps; ++k) {
-        if (C::F16 && k == steps - per && segs > 1) {
+    for (int u = first; u < total; u += stride) {
+        const Unit unit = unit_of(u);
+        const int per = unit.k1 - unit.k0, steps = per * segs;
+        f32x4 acc[WI][WJ];
 #pragma unroll
-            for (int i = 0; i < WI; ++i)
+        for (int i = 0; i < WI; ++i)
 #pragma unroll
-                for (int j = 0; j < WJ; ++j) acc[i][j] *= 1.0f / kLowScale;
-        }
-        // this step's stage has landed, and every wave is done with the one to fill next
-        wait_loads_and_sync<(NST - 2) * LOADS>();
-        __builtin_amdgcn_sched_barrier(0);
-        issue(stage == 0 ? NST - 1 : stage - 1);
-        read(stage, 0);
+            for (int j = 0; j < WJ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < steps; ++k) {
+            if (C::F16 && k == steps - per && segs > 1) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            if (s + 1 < NS) read(stage, s + 1);
+                for (int i = 0; i < WI; ++i)
 #pragma unroll
-            for (int i = 0; i < WI; ++i)
-#pragma unroll
-                for (int j = 0; j < WJ; ++j) acc[i][j] = mfma<C::F16>(af[s & 1][i], bf[s & 1][j], acc[i][j]);
-        }
-        // the next slice's LDS reads between this slice's MFMAs (0x008 MFMA, 0x100 LDS read)
-        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-#pragma unroll
-            for (int t = 0; t < WI * WJ; ++t) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                if (s + 1 < NS && t * PER < READS) __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+                    for (int j = 0; j < WJ; ++j) acc[i][j] *= 1.0f / kLowScale;
             }
-        __builtin_amdgcn_sched_barrier(0);
-        stage = stage + 1 == NST ? 0 : stage + 1;
+            // this step's stage has landed, and every wave is done with the one to fill next
+            wait_loads_and_sync<(NST - 2) * LOADS>();
+            __builtin_amdgcn_sched_barrier(0);
+            issue(stage == 0 ? NST - 1 : stage - 1);
+            read(stage, 0);
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                if (s + 1 < NS) read(stage, s + 1);
+#pragma unroll
+                for (int i = 0; i < WI; ++i)
+#pragma unroll
+                    for (int j = 0; j < WJ; ++j) acc[i][j] = mfma<C::F16>(af[s & 1][i], bf[s & 1][j], acc[i][j]);
+            }
+            // the next slice's LDS reads between this slice's MFMAs (0x008 MFMA, 0x100 LDS read)
+            __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int t = 0; t < WI * WJ; ++t) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    if (s + 1 < NS && t * PER < READS) __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+                }
+            __builtin_amdgcn_sched_barrier(0);
+            stage = stage + 1 == NST ? 0 : stage + 1;
+        }
+        finish(u, unit, acc);
     }
-    // the last loads (repeats) must have landed before LDS is used again
+    // the last loads (repeats) must have landed before the workgroup gives its LDS back
     wait_loads_and_sync<0>();
 }
 

@@ -359,20 +359,11 @@ struct Logits {
 // What a logits' product keeps for the gradients: nothing, 16 packed bits, two planes.
 enum Keep { kKeepNone, kKeepPacked, kKeepPlanes };
 
+// What becomes of a tile of logits.
 template <typename C, int KEEP>
-__global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
+__device__ __forceinline__ void logits_tile(const Logits& a, int rows, int m0, int n0, int ex,
+                                            f32x4 (&acc)[C::WI][C::WJ]) {
     constexpr int WI = C::WI, WJ = C::WJ;
-    __shared__ __attribute__((aligned(1024))) uint16_t smem[C::NST * C::STAGE];
-    const int rows = piece_rows(a.meta, a.from, a.most);
-    const int tiles_n = (rows + C::TN - 1) / C::TN;
-    const int live = tiles_n * a.tiles_m;
-    if ((int)blockIdx.x >= live) return;
-    int ti, tj;
-    tile_of<C::GROUP_M>(logical_block(blockIdx.x, live), a.tiles_m, tiles_n, &ti, &tj);
-    const int m0 = ti * C::TM, n0 = tj * C::TN;
-    f32x4 acc[WI][WJ];
-    product_tile<C>(a.w, a.x, m0, n0, 0, a.steps, a.segs, smem, acc);
-
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = m0 + (wave / C::WAVES_N) * C::WM, wn = n0 + (wave % C::WAVES_N) * C::WN;
     const int hi = 4 * (lane >> 4);
@@ -382,7 +373,6 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
     const bool f32 = KEEP != kKeepPacked && a.f32;
     // exp(x) times 2^-64 when the packed bf16 format takes it as it is
     constexpr float kDown = KEEP == kKeepPacked && !C::F16 ? 64.0f : 0.0f;
-    const int ex = f32 ? -half_exponent(a.meta->top[0]) - half_exponent(a.meta->top[1]) : 0;
     const bool part = wm + C::WM > a.v;  // the last columns end inside this wave's
 #pragma unroll
     for (int j = 0; j < WJ; ++j) {
@@ -466,6 +456,25 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
                 *reinterpret_cast<uint4*>(row + i * 16 + a.g_plane) = eight_rows(w[1][0], w[1][1]);
         }
     }
+}
+
+template <typename C, int KEEP>
+__global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
+    __shared__ __attribute__((aligned(1024))) uint16_t smem[C::NST * C::STAGE];
+    const int rows = piece_rows(a.meta, a.from, a.most);
+    const int tiles_n = (rows + C::TN - 1) / C::TN;
+    const int live = tiles_n * a.tiles_m;
+    if ((int)blockIdx.x >= live) return;
+    const int ex = a.f32 ? -half_exponent(a.meta->top[0]) - half_exponent(a.meta->top[1]) : 0;
+    auto unit_of = [&](int u) {
+        int ti, tj;
+        tile_of<C::GROUP_M>(logical_block(u, live), a.tiles_m, tiles_n, &ti, &tj);
+        return Unit{ti * C::TM, tj * C::TN, 0, a.steps};
+    };
+    auto finish = [&](int, const Unit& unit, f32x4(&acc)[C::WI][C::WJ]) {
+        logits_tile<C, KEEP>(a, rows, unit.m0, unit.n0, ex, acc);
+    };
+    product_stream<C>(a.w, a.x, a.segs, blockIdx.x, live, gridDim.x, smem, unit_of, finish);
 }
 
 // Loss of each row from its slots, and (g) the row's values turned into G.
@@ -776,40 +785,54 @@ __device__ __forceinline__ void finish_tile(const Grad& g, int n_all, int m0, in
     }
 }
 
+// Worker `b` of `workers` of a product.
 template <typename C>
-__device__ __forceinline__ void grad_block(const Grad& g, int b, uint16_t* smem) {
-    constexpr int WI = C::WI, WJ = C::WJ;
+__device__ __forceinline__ void grad_block(const Grad& g, int b, int workers, uint16_t* smem) {
     const Deal deal = deal_of<C>(g);
-    int u, tile, cut = 0, cuts = 1;
-    if (b < deal.full) {
-        u = tile = logical_block(b, deal.full);
-    } else {
-        cuts = cuts_of(g, deal);
-        if (b >= deal.full + deal.rest * cuts) return;
-        u = logical_block(b - deal.full, deal.rest * cuts);
-        cut = u / deal.rest;
-        tile = deal.full + u - cut * deal.rest;
-    }
+    const int cuts = deal.rest ? cuts_of(g, deal) : 1;
+    const int parts = deal.rest * cuts, total = deal.full + parts;
     const float factor = g.meta->factor[g.dh];
-    int ti, tj;
-    tile_of<C::GROUP_M>(tile, g.tiles_m, deal.tiles_n, &ti, &tj);
-    const int m0 = ti * C::TM, n0 = tj * C::TN;
-    f32x4 acc[WI][WJ];
-    product_tile<C>(g.a, g.b, m0, n0, (int)((int64_t)deal.steps * cut / cuts),
-                    (int)((int64_t)deal.steps * (cut + 1) / cuts), g.segs, smem, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = (wave / C::WAVES_N) * C::WM, wn = (wave % C::WAVES_N) * C::WN;
-    if (cuts > 1) {
-        float* p = g.parts + (int64_t)u * (C::TM * C::TN) + (wn + (lane & 15)) * C::TM + wm + 4 * (lane >> 4);
+    auto unit_of = [&](int u) {
+        int tile, cut = 0;
+        const bool whole = u < deal.full;
+        if (whole) {
+            tile = logical_block(u, deal.full);
+        } else {
+            const int q = logical_block(u - deal.full, parts);
+            cut = q / deal.rest;
+            tile = deal.full + q - cut * deal.rest;
+        }
+        int ti, tj;
+        tile_of<C::GROUP_M>(tile, g.tiles_m, deal.tiles_n, &ti, &tj);
+        return Unit{ti * C::TM, tj * C::TN, whole ? 0 : deal.steps * cut / cuts,
+                    whole ? deal.steps : deal.steps * (cut + 1) / cuts};
+    };
+    auto finish = [&](int u, const Unit& unit, f32x4(&acc)[C::WI][C::WJ]) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int wm = (wave / C::WAVES_N) * C::WM, wn = (wave % C::WAVES_N) * C::WN;
+        if (cuts > 1 && u >= deal.full) {
+            float* p = g.parts + (int64_t)logical_block(u - deal.full, parts) * (C::TM * C::TN) +
+                       (wn + (lane & 15)) * C::TM + wm + 4 * (lane >> 4);
 #pragma unroll
-        for (int j = 0; j < WJ; ++j)
+            for (int j = 0; j < C::WJ; ++j)
 #pragma unroll
-            for (int i = 0; i < WI; ++i) *reinterpret_cast<f32x4*>(p + j * 16 * C::TM + i * 16) = acc[i][j];
-        return;
+                for (int i = 0; i < C::WI; ++i) *reinterpret_cast<f32x4*>(p + j * 16 * C::TM + i * 16) = acc[i][j];
+        } else if (g.sum) {
+            finish_tile<C, kOutSum>(g, deal.n_all, unit.m0 + wm, unit.n0 + wn, factor, acc);
+        } else if (C::F16 && g.dtype == GEFEN_F32) {
+            finish_tile<C, kOutF32>(g, deal.n_all, unit.m0 + wm, unit.n0 + wn, factor, acc);
+        } else {
+            finish_tile<C, kOut16>(g, deal.n_all, unit.m0 + wm, unit.n0 + wn, factor, acc);
+        }
+    };
+    if (deal.steps == 0) {  // dW of no row at all
+        for (int u = b; u < total; u += workers) {
+            f32x4 none[C::WI][C::WJ] = {};
+            finish(u, unit_of(u), none);
+        }
+    } else if (b < total) {
+        product_stream<C>(g.a, g.b, g.segs, b, total, workers, smem, unit_of, finish);
     }
-    if (g.sum) finish_tile<C, kOutSum>(g, deal.n_all, m0 + wm, n0 + wn, factor, acc);
-    else if (C::F16 && g.dtype == GEFEN_F32) finish_tile<C, kOutF32>(g, deal.n_all, m0 + wm, n0 + wn, factor, acc);
-    else finish_tile<C, kOut16>(g, deal.n_all, m0 + wm, n0 + wn, factor, acc);
 }
 
 // One gradient's product; the last workgroup sums the losses where l.out is given, which
@@ -817,17 +840,19 @@ __device__ __forceinline__ void grad_block(const Grad& g, int b, uint16_t* smem)
 template <typename C>
 __global__ __launch_bounds__(C::TT, C::EU) void k_grad(const Grad g, const Loss l) {
     __shared__ __attribute__((aligned(1024))) uint16_t smem[C::NST * C::STAGE];
-    if (l.out && blockIdx.x == gridDim.x - 1) return sum_losses<C::TT>(l);
-    grad_block<C>(g, blockIdx.x, smem);
+    const int workers = gridDim.x - (l.out ? 1 : 0);
+    if ((int)blockIdx.x == workers) return sum_losses<C::TT>(l);
+    grad_block<C>(g, blockIdx.x, workers, smem);
 }
-// Both products, dh by the workgroups up to `first`.
+// Both products, dh by the workers up to `first`.
 template <typename H, typename W>
 __global__ __launch_bounds__(H::TT, H::EU) void k_grads(const Grad h, const Grad w, const Loss l, int first) {
     static_assert(H::TT == W::TT && H::STAGE == W::STAGE && H::NST == W::NST, "one launch");
     __shared__ __attribute__((aligned(1024))) uint16_t smem[H::NST * H::STAGE];
-    if (l.out && blockIdx.x == gridDim.x - 1) return sum_losses<H::TT>(l);
-    if ((int)blockIdx.x < first) grad_block<H>(h, blockIdx.x, smem);
-    else grad_block<W>(w, blockIdx.x - first, smem);
+    const int workers = gridDim.x - (l.out ? 1 : 0);
+    if ((int)blockIdx.x == workers) return sum_losses<H::TT>(l);
+    if ((int)blockIdx.x < first) grad_block<H>(h, blockIdx.x, first, smem);
+    else grad_block<W>(w, blockIdx.x - first, workers - first, smem);
 }
 
 // The parts of the cut tiles added up in order.  t: tile of the rest, blockIdx.y:
@@ -1030,7 +1055,8 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
 template <typename C>
 void launch_logits(Logits a, int most, hipStream_t st) {
     a.tiles_m = (a.v + C::TM - 1) / C::TM;
-    const dim3 grid((unsigned)(a.tiles_m * ((most + C::TN - 1) / C::TN))), wg(C::TT);
+    const int tiles = a.tiles_m * ((most + C::TN - 1) / C::TN), slots = kCus * C::WGS;
+    const dim3 grid((unsigned)(tiles < slots ? tiles : slots)), wg(C::TT);
     if (!a.g) hipLaunchKernelGGL((k_logits<C, kKeepNone>), grid, wg, 0, st, a);
     else if (a.planes == 1) hipLaunchKernelGGL((k_logits<C, kKeepPacked>), grid, wg, 0, st, a);
     else hipLaunchKernelGGL((k_logits<C, kKeepPlanes>), grid, wg, 0, st, a);
@@ -1041,13 +1067,14 @@ void launch_logits_tile(const Plan& p, const Logits& a, int most, hipStream_t st
     else if (p.tile == kSmallTile) launch_logits<LogitsSmall<F16>>(a, most, st);
     else launch_logits<LogitsRow<F16>>(a, most, st);
 }
-// Grids for g.n rows, the most that the device may find.
+// Workers for g.n rows, the most that the device may find.
 template <typename C>
 int grad_grid(Grad* g, int* join) {
     g->tiles_m = (g->d + C::TM - 1) / C::TM;
     const int tiles = g->tiles_m * ((g->n + C::TN - 1) / C::TN);
     *join = g->most_parts == 0 ? 0 : tiles < g->slots ? tiles : g->slots - 1;
-    return tiles + g->most_parts;
+    const int units = tiles + g->most_parts;
+    return units < g->slots ? units : g->slots;
 }
 template <typename C>
 void launch_grad(Grad g, const Loss& l, hipStream_t st) {
