@@ -90,6 +90,8 @@ __device__ __forceinline__ int swizzle_k(int r, int c) { return c ^ ((r >> 1) & 
 __device__ __forceinline__ int swizzle_mn(int r, int c) { return c ^ (((r & 3) | ((r >> 3) & 1) << 2) << 1); }
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+// LDS pointers keep their address space: no check for null on the way to an offset.
+typedef __attribute__((address_space(3))) uint16_t lds_u16;
 
 // 64 lanes' 16 bytes at base + voff to the 1024 LDS bytes at lds.  Written as assembly
 // because the compiler otherwise holds every transposing LDS read back until all such
@@ -133,12 +135,12 @@ struct Loader {
         step = MN ? (int64_t)BK * o.ld : BK;
     }
     // the loads of K step k; MN-major rows past the operand's are read as its last one
-    __device__ __forceinline__ void issue(const Operand& o, int64_t plane_off, int k, uint16_t* lds) const {
+    __device__ __forceinline__ void issue(const Operand& o, int64_t plane_off, int k, lds_u16* lds) const {
         const uint64_t at = reinterpret_cast<uint64_t>(base + plane_off + (int64_t)k * step);
         // raw buffer: every offset below is in bounds, the range covers any of them
         const i32x4 rsrc = {(int)(uint32_t)at, (int)((at >> 32) & 0xffff), 0x7ffffff0, 0x00020000};
-        const uint32_t l0 = __builtin_amdgcn_readfirstlane(
-            (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)(lds + ((int)threadIdx.x >> 6) * 512));
+        const uint32_t l0 =
+            __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds + ((int)threadIdx.x >> 6) * 512));
         if (MN && (k + 1) * BK > o.rows) {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
@@ -164,20 +166,20 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
 
 // Fragment of a K-major tile: rows row0 + lane % 16, k = 32 s + 8 (lane / 16) + 0..7.
 template <int BK>
-__device__ __forceinline__ bf16x8 frag_k(const uint16_t* tile, int row0, int s, int lane) {
+__device__ __forceinline__ bf16x8 frag_k(const lds_u16* tile, int row0, int s, int lane) {
     const int r = lane & 15;
-    return *reinterpret_cast<const bf16x8*>(tile + (row0 + r) * BK + swizzle_k(r, 4 * s + (lane >> 4)) * 8);
+    typedef __attribute__((address_space(3))) bf16x8 lds_v8;
+    return *(const lds_v8*)(tile + (row0 + r) * BK + swizzle_k(r, 4 * s + (lane >> 4)) * 8);
 }
 // Fragment of an MN-major tile of ROWS elements a k: two transposing reads.  In each
 // group of 16 lanes, lane 4 j + q points at k row j, elements 4 q .. 4 q + 3 of a 4 x 16
 // block, and lane i receives element i of the rows 0 .. 3.
 template <int ROWS>
-__device__ __forceinline__ bf16x8 frag_mn(const uint16_t* tile, int row0, int s, int lane) {
+__device__ __forceinline__ bf16x8 frag_mn(const lds_u16* tile, int row0, int s, int lane) {
     typedef __attribute__((address_space(3))) bf16x4 lds_v4;
     const int k = 8 * (lane >> 4) + ((lane & 15) >> 2);  // within the slice of 32
     const int e = row0 + 4 * (lane & 3);
-    const auto* p = (const __attribute__((address_space(3))) uint16_t*)(tile + (32 * s + k) * ROWS +
-                                                                        swizzle_mn(k, e >> 3) * 8 + (e & 7));
+    const lds_u16* p = tile + (32 * s + k) * ROWS + swizzle_mn(k, e >> 3) * 8 + (e & 7);
     const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4*)p);
     const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4*)(p + 4 * ROWS));
     return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -219,7 +221,7 @@ struct Unit {
 // n0 + (wave's) + 16 j + lane % 16.  Every unit has a K step at least.
 template <typename C, typename UnitOf, typename Finish>
 __device__ __forceinline__ void product_stream(const Operand& A, const Operand& B, int segs, int first, int total,
-                                               int stride, uint16_t* smem, UnitOf unit_of, Finish finish) {
+                                               int stride, lds_u16* smem, UnitOf unit_of, Finish finish) {
     constexpr int WI = C::WI, WJ = C::WJ, NST = C::NST, NS = C::BK / 32;
     constexpr int LOADS = C::A_LOADS + C::B_LOADS;
     constexpr int READS = WI * (C::AMN ? 2 : 1) + WJ * (C::BMN ? 2 : 1);   // LDS reads of a slice
@@ -234,8 +236,8 @@ __device__ __forceinline__ void product_stream(const Operand& A, const Operand& 
     la.init(A, load.m0);
     lb.init(B, load.n0);
     lk = load.k0;
-    auto issue = [&](int stage) {
-        uint16_t* s = smem + stage * C::STAGE;
+    auto issue = [&](int stage) __attribute__((always_inline)) {
+        lds_u16* s = smem + stage * C::STAGE;
         la.issue(A, (int64_t)(A.planes >> (2 * lseg) & 3u) * A.plane, lk, s);
         lb.issue(B, (int64_t)(B.planes >> (2 * lseg) & 3u) * B.plane, lk, s + C::A_ELEMS);
         if (lk + 1 < load.k1) {
@@ -253,9 +255,9 @@ __device__ __forceinline__ void product_stream(const Operand& A, const Operand& 
         }
     };
     bf16x8 af[2][WI], bf[2][WJ];
-    auto read = [&](int stage, int s) {
-        const uint16_t* as = smem + stage * C::STAGE;
-        const uint16_t* bs = as + C::A_ELEMS;
+    auto read = [&](int stage, int s) __attribute__((always_inline)) {
+        const lds_u16* as = smem + stage * C::STAGE;
+        const lds_u16* bs = as + C::A_ELEMS;
 #pragma unroll
         for (int i = 0; i < WI; ++i)
             af[s & 1][i] = C::AMN ? frag_mn<C::TM>(as, wm + i * 16, s, lane) : frag_k<C::BK>(as, wm + i * 16, s, lane);

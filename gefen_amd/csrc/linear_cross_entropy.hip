@@ -210,8 +210,9 @@ struct Top {
     Meta* meta;
     int32_t which;
 };
+constexpr int kTopThreads = 1024, kTopGrid = 256;
 // Workgroups up to `first` take a, the others b.
-__global__ __launch_bounds__(256) void k_top(const Top a, const Top b, int first) {
+__global__ __launch_bounds__(kTopThreads) void k_top(const Top a, const Top b, int first) {
     const bool is_a = (int)blockIdx.x < first;
     const Top& t = is_a ? a : b;
     const int block = is_a ? blockIdx.x : blockIdx.x - first, blocks = is_a ? first : gridDim.x - first;
@@ -222,7 +223,7 @@ __global__ __launch_bounds__(256) void k_top(const Top a, const Top b, int first
         const uint32_t u = abs_key(x);
         top = u < 0x7f800000u && u > top ? u : top;
     };
-    for (int64_t q = (int64_t)block * 256 + threadIdx.x; q < all; q += (int64_t)blocks * 256) {
+    for (int64_t q = (int64_t)block * kTopThreads + threadIdx.x; q < all; q += (int64_t)blocks * kTopThreads) {
         const int64_t r = q / per;
         const int c = (int)(q - r * per) * 8;
         const float* s = t.src + (int64_t)(t.map ? t.map[r] : r) * t.row_stride;
@@ -234,13 +235,13 @@ __global__ __launch_bounds__(256) void k_top(const Top a, const Top b, int first
             for (int e = c; e < min(c + 8, t.d); ++e) see(s[(int64_t)e * t.col_stride]);
         }
     }
-    // one atomic per workgroup: eight thousand on one address took 100 us
-    __shared__ uint32_t part[4];
+    // one atomic per workgroup, and few of those: on one address each takes 12 ns
+    __shared__ uint32_t part[kTopThreads / 64];
     top = wave_group_max_u32(top, 64);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
     __syncthreads();
     if (threadIdx.x == 0) {
-        top = max(max(part[0], part[1]), max(part[2], part[3]));
+        for (int w = 1; w < kTopThreads / 64; ++w) top = max(top, part[w]);
         if (top > 0) atomicMax(&t.meta->top[t.which], top);
     }
 }
@@ -466,15 +467,15 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
     const int live = tiles_n * a.tiles_m;
     if ((int)blockIdx.x >= live) return;
     const int ex = a.f32 ? -half_exponent(a.meta->top[0]) - half_exponent(a.meta->top[1]) : 0;
-    auto unit_of = [&](int u) {
+    auto unit_of = [&](int u) __attribute__((always_inline)) {
         int ti, tj;
         tile_of<C::GROUP_M>(logical_block(u, live), a.tiles_m, tiles_n, &ti, &tj);
         return Unit{ti * C::TM, tj * C::TN, 0, a.steps};
     };
-    auto finish = [&](int, const Unit& unit, f32x4(&acc)[C::WI][C::WJ]) {
+    auto finish = [&](int, const Unit& unit, f32x4(&acc)[C::WI][C::WJ]) __attribute__((always_inline)) {
         logits_tile<C, KEEP>(a, rows, unit.m0, unit.n0, ex, acc);
     };
-    product_stream<C>(a.w, a.x, a.segs, blockIdx.x, live, gridDim.x, smem, unit_of, finish);
+    product_stream<C>(a.w, a.x, a.segs, blockIdx.x, live, gridDim.x, (lds_u16*)smem, unit_of, finish);
 }
 
 // Loss of each row from its slots, and (g) the row's values turned into G.
@@ -681,10 +682,11 @@ struct Grad {
 // K steps out evenly instead, as one stretch per workgroup, balances better but left no
 // two workgroups at the same K: dh of 2796 x 2048 over 128256 2.0 ms against 1.63 with two
 // equal parts).  The number of parts is the one of the least estimated time, in K steps of
-// a full chip: rounds times the steps of a part and 4 for its ends, and 0.06 for the
-// traffic of each partial tile.  The rows that take part are only known on the device, so
+// a full chip: rounds times the steps of a part and 4 for its ends, 0.06 for the traffic of
+// each partial tile, and 4 and 0.1 a part for the launch that joins them.  The rows that take part are only known on the device, so
 // this is worked out there; the host bounds it.
-constexpr int kMostCuts = 16;
+constexpr int kMostCuts = 128;
+constexpr int kMostRounds = 4;
 constexpr int kLeastSteps = 4;  // of a part
 struct Deal {
     int n_all, tiles_n, steps, full, rest;
@@ -705,9 +707,12 @@ __device__ __forceinline__ int cuts_of(const Grad& g, const Deal& d) {
     int cuts = 1;
     const float run = (float)(d.steps * g.segs);
     float best = run + 4.0f;
-    for (int c = 2; c <= kMostCuts && d.rest * c <= g.most_parts && d.steps >= kLeastSteps * c; ++c) {
-        const int rounds = (d.rest * c + g.slots - 1) / g.slots;
-        const float cost = (float)rounds * (run / (float)c + 4.0f) + 0.06f * (float)(d.rest * c);
+    for (int rounds = 1; rounds <= kMostRounds; ++rounds) {
+        int c = min(rounds * g.slots, g.most_parts) / d.rest;
+        c = min(min(c, kMostCuts), d.steps / kLeastSteps);
+        if (c < 2) continue;
+        const float cost = (float)((d.rest * c + g.slots - 1) / g.slots) * (run / (float)c + 4.0f) +
+                           0.06f * (float)(d.rest * c) + 0.1f * (float)c + 4.0f;
         if (cost < best) {
             best = cost;
             cuts = c;
@@ -787,12 +792,12 @@ __device__ __forceinline__ void finish_tile(const Grad& g, int n_all, int m0, in
 
 // Worker `b` of `workers` of a product.
 template <typename C>
-__device__ __forceinline__ void grad_block(const Grad& g, int b, int workers, uint16_t* smem) {
+__device__ __forceinline__ void grad_block(const Grad& g, int b, int workers, lds_u16* smem) {
     const Deal deal = deal_of<C>(g);
     const int cuts = deal.rest ? cuts_of(g, deal) : 1;
     const int parts = deal.rest * cuts, total = deal.full + parts;
     const float factor = g.meta->factor[g.dh];
-    auto unit_of = [&](int u) {
+    auto unit_of = [&](int u) __attribute__((always_inline)) {
         int tile, cut = 0;
         const bool whole = u < deal.full;
         if (whole) {
@@ -807,7 +812,7 @@ __device__ __forceinline__ void grad_block(const Grad& g, int b, int workers, ui
         return Unit{ti * C::TM, tj * C::TN, whole ? 0 : deal.steps * cut / cuts,
                     whole ? deal.steps : deal.steps * (cut + 1) / cuts};
     };
-    auto finish = [&](int u, const Unit& unit, f32x4(&acc)[C::WI][C::WJ]) {
+    auto finish = [&](int u, const Unit& unit, f32x4(&acc)[C::WI][C::WJ]) __attribute__((always_inline)) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         const int wm = (wave / C::WAVES_N) * C::WM, wn = (wave % C::WAVES_N) * C::WN;
         if (cuts > 1 && u >= deal.full) {
@@ -842,7 +847,7 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_grad(const Grad g, const Loss 
     __shared__ __attribute__((aligned(1024))) uint16_t smem[C::NST * C::STAGE];
     const int workers = gridDim.x - (l.out ? 1 : 0);
     if ((int)blockIdx.x == workers) return sum_losses<C::TT>(l);
-    grad_block<C>(g, blockIdx.x, workers, smem);
+    grad_block<C>(g, blockIdx.x, workers, (lds_u16*)smem);
 }
 // Both products, dh by the workers up to `first`.
 template <typename H, typename W>
@@ -851,40 +856,55 @@ __global__ __launch_bounds__(H::TT, H::EU) void k_grads(const Grad h, const Grad
     __shared__ __attribute__((aligned(1024))) uint16_t smem[H::NST * H::STAGE];
     const int workers = gridDim.x - (l.out ? 1 : 0);
     if ((int)blockIdx.x == workers) return sum_losses<H::TT>(l);
-    if ((int)blockIdx.x < first) grad_block<H>(h, blockIdx.x, first, smem);
-    else grad_block<W>(w, blockIdx.x - first, workers - first, smem);
+    if ((int)blockIdx.x < first) grad_block<H>(h, blockIdx.x, first, (lds_u16*)smem);
+    else grad_block<W>(w, blockIdx.x - first, workers - first, (lds_u16*)smem);
 }
 
-// The parts of the cut tiles added up in order.  t: tile of the rest, blockIdx.y:
-// 1024 of its elements.
+// The parts of the cut tiles added up, the same way each time: wave w of a workgroup adds
+// parts w, w + 4, ... in order, and the four sums are added in order.  t: tile of the rest,
+// blockIdx.y of kJoinBlocks: every kJoinBlocks-th 256 of its elements.
+constexpr int kJoinBlocks = 64;
 template <typename C>
 __device__ __forceinline__ void join_block(const Grad& g, int t) {
+    __shared__ f32x4 part[4][64];
     const Deal deal = deal_of<C>(g);
     if (t >= deal.rest) return;
     const int cuts = cuts_of(g, deal);
     if (cuts == 1) return;
     int ti, tj;
     tile_of<C::GROUP_M>(deal.full + t, g.tiles_m, deal.tiles_n, &ti, &tj);
-    const int q = (int)(blockIdx.y * 256 + threadIdx.x) * 4;
-    const int n = tj * C::TN + q / C::TM, m = ti * C::TM + q % C::TM;
-    if (n >= deal.n_all || m >= g.d) return;
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c = 0; c < cuts; ++c)
-        v += *reinterpret_cast<const f32x4*>(g.parts + ((int64_t)c * deal.rest + t) * (C::TM * C::TN) + q);
-    const int64_t row = g.dh ? g.map[g.from + n] : n;
-    const int cnt = min(4, g.d - m);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const float factor = g.meta->factor[g.dh];
-    if (g.sum) {
-        finish_f32<kOutSum>(g, row, m, cnt, v, factor);
-    } else if (C::F16 && g.dtype == GEFEN_F32) {
-        finish_f32<kOutF32>(g, row, m, cnt, v, factor);
-    } else {
-        const uint2 r = round16<C::F16>(v, factor);
-        const uint32_t w[2] = {r.x, r.y};
-        store16<4>(g, row, m, cnt, w);
+    for (int chunk = blockIdx.y; chunk < C::TM * C::TN / 256; chunk += kJoinBlocks) {
+        const int q = chunk * 256 + lane * 4;
+        const int n = tj * C::TN + q / C::TM, m = ti * C::TM + q % C::TM;
+        const bool in = n < deal.n_all && m < g.d;
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (in) {
+            const float* p = g.parts + ((int64_t)wave * deal.rest + t) * (C::TM * C::TN) + q;
+#pragma unroll 4
+            for (int c = wave; c < cuts; c += 4, p += (int64_t)4 * deal.rest * (C::TM * C::TN))
+                v += *reinterpret_cast<const f32x4*>(p);
+        }
+        part[wave][lane] = v;
+        __syncthreads();
+        if (wave == 0 && in) {
+            v = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+            const int64_t row = g.dh ? g.map[g.from + n] : n;
+            const int cnt = min(4, g.d - m);
+            if (g.sum) {
+                finish_f32<kOutSum>(g, row, m, cnt, v, factor);
+            } else if (C::F16 && g.dtype == GEFEN_F32) {
+                finish_f32<kOutF32>(g, row, m, cnt, v, factor);
+            } else {
+                const uint2 r = round16<C::F16>(v, factor);
+                const uint32_t w[2] = {r.x, r.y};
+                store16<4>(g, row, m, cnt, w);
+            }
+        }
+        __syncthreads();
     }
 }
-
 template <typename C>
 __global__ __launch_bounds__(256) void k_join(const Grad g) {
     join_block<C>(g, blockIdx.x);
@@ -956,25 +976,31 @@ struct Plan {
 constexpr int kCus = 256;
 constexpr int slots_of(bool big) { return big ? kCus : 2 * kCus; }
 
+// Fewest K steps (of all segments) for big tiles: with one workgroup per CU nothing runs
+// beside the ends of a tile.  Logits of 346 x 81968 in two steps 41 us, small tiles 32; of
+// 2048 x 32000 in eight 96 and 111.  dW of 80 rows (two steps) x 42438 x 3136 142 us, small
+// tiles 121; of 512 rows (eight) x 32000 x 2048 107 and 108.
+constexpr int kBigLogitsSteps = 4, kBigGradSteps = 9;
 // Measured: a K step of 64 takes 1.7 us on a chip full of big tiles (256 of 256 x 256)
 // and about 1.06 us on one full of small ones (512 of 128 x 128, half the products).  So
 // big tiles win unless the edges leave more than a fifth of them empty, or there are not
 // steps enough to give every workgroup a few.
-bool big_tile(int64_t m, int64_t n, int64_t steps) {
+bool big_tile(int64_t m, int64_t n, int64_t steps, int segs) {
+    if (steps * segs < kBigGradSteps) return false;
     const int64_t tb = up(m, 256) / 256 * (up(n, 256) / 256), ts = up(m, 128) / 128 * (up(n, 128) / 128);
     return tb * steps >= kCus * kLeastSteps && ts * 10 > tb * 32;
 }
 // K steps that are run in one piece whatever the tiles: joining costs a launch (5 us),
 // what eight steps take where a CU has one small tile.
 constexpr int kUncutSteps = 24;
-// Partial tiles that a product of up to `tiles` tiles of `steps` K steps may leave: four
+// Partial tiles that a product of up to `tiles` tiles of `steps` K steps may leave: kMostRounds
 // rounds of the chip at most.
 int parts_of(int64_t tiles, int64_t steps, int segs, bool big) {
     if (steps * segs <= kUncutSteps) return 0;
     const int64_t cuts = steps / kLeastSteps < kMostCuts ? steps / kLeastSteps : kMostCuts;
     const int64_t rest = tiles < slots_of(big) ? tiles : slots_of(big) - 1;
     if (cuts < 2) return 0;
-    return (int)(rest * cuts < 4 * slots_of(big) ? rest * cuts : 4 * slots_of(big));
+    return (int)(rest * cuts < kMostRounds * slots_of(big) ? rest * cuts : kMostRounds * slots_of(big));
 }
 int64_t tiles_of(int64_t m, int64_t n, bool big) {
     const int64_t t = big ? 256 : 128;
@@ -1016,10 +1042,13 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
     p->rows = (int)rows;
     const int64_t n = t.n < rows ? (t.n > 0 ? t.n : 1) : rows;
     const int64_t tiles = up(t.v, 256) / 256 * (up(n, 256) / 256);
-    p->tile = n <= 32 ? kRowTile : tiles >= kCus / 2 ? kBigTile : kSmallTile;
+    const int in_segs = t.dtype == GEFEN_F32 ? 3 : 1;
+    p->tile = n <= 32 ? kRowTile
+              : tiles >= kCus / 2 && p->dp / 64 * in_segs >= kBigLogitsSteps ? kBigTile : kSmallTile;
     p->slots = (int)(up(t.v, kSlot) / kSlot);
-    p->dh_big = big_tile(t.d, n, up(t.v, 64) / 64);
-    p->dw_big = big_tile(t.d, t.v, up(n, 64) / 64);
+    const int segs = t.dtype == GEFEN_F32 ? 3 : p->planes;
+    p->dh_big = big_tile(t.d, n, up(t.v, 64) / 64, segs);
+    p->dw_big = big_tile(t.d, t.v, up(n, 64) / 64, segs);
 
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -1040,7 +1069,6 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
     p->o_sums = p->smooth ? take((size_t)p->rows * p->slots * 4) : at;
     p->o_g = p->train ? take((size_t)p->planes * p->rows * p->ldg * 2) : at;
     p->o_wsum = p->dw && p->pieces > 1 ? take((size_t)p->v * p->d * 4) : at;
-    const int segs = t.dtype == GEFEN_F32 ? 3 : p->planes;
     p->dh_parts = p->dh ? parts_of(tiles_of(t.d, n, p->dh_big), up(t.v, 64) / 64, segs, p->dh_big) : 0;
     p->dw_parts = p->dw ? parts_of(tiles_of(t.d, t.v, p->dw_big), up(n, 64) / 64, segs, p->dw_big) : 0;
     const size_t dh_bytes = (size_t)p->dh_parts * (p->dh_big ? 256 * 256 : 128 * 128) * 4;
@@ -1081,7 +1109,7 @@ void launch_grad(Grad g, const Loss& l, hipStream_t st) {
     int join;
     const int grid = grad_grid<C>(&g, &join) + (l.out ? 1 : 0);
     hipLaunchKernelGGL(k_grad<C>, dim3((unsigned)grid), dim3(C::TT), 0, st, g, l);
-    if (join) hipLaunchKernelGGL(k_join<C>, dim3((unsigned)join, C::TM * C::TN / 1024), dim3(256), 0, st, g);
+    if (join) hipLaunchKernelGGL(k_join<C>, dim3((unsigned)join, kJoinBlocks), dim3(256), 0, st, g);
 }
 template <bool F16>
 void launch_grad_tile(Grad g, bool big, const Loss& l, hipStream_t st) {
@@ -1102,7 +1130,7 @@ void launch_grad_pair(Grad h, Grad w, const Loss& l, hipStream_t st) {
     const int grid = first + grad_grid<W>(&w, &join_w) + (l.out ? 1 : 0);
     hipLaunchKernelGGL((k_grads<H, W>), dim3((unsigned)grid), dim3(H::TT), 0, st, h, w, l, first);
     if (join_h + join_w)
-        hipLaunchKernelGGL((k_joins<H, W>), dim3((unsigned)(join_h + join_w), H::TM * H::TN / 1024), dim3(256), 0, st,
+        hipLaunchKernelGGL((k_joins<H, W>), dim3((unsigned)(join_h + join_w), kJoinBlocks), dim3(256), 0, st,
                            h, w, join_h);
 }
 unsigned grid_of(int64_t chunks, int64_t most) {
@@ -1197,8 +1225,8 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
             const Top tx{static_cast<const float*>(t.hidden), t.hidden_row_stride, t.hidden_col_stride, p.n, p.d, map, meta, 0};
             const Top tw{static_cast<const float*>(t.weight), t.weight_row_stride, t.weight_col_stride, p.v, p.d, nullptr,
                          meta, 1};
-            const int top_x = (int)grid_of(p.n * per, 1024), top_w = (int)grid_of(p.v * per, 1024);
-            hipLaunchKernelGGL(k_top, dim3((unsigned)(top_x + top_w)), dim3(256), 0, st, tx, tw, top_x);
+            const int top_x = (int)grid_of(p.n * per / 4, kTopGrid), top_w = (int)grid_of(p.v * per / 4, kTopGrid);
+            hipLaunchKernelGGL(k_top, dim3((unsigned)(top_x + top_w)), dim3(kTopThreads), 0, st, tx, tw, top_x);
         }
         hipLaunchKernelGGL(k_pack, dim3((unsigned)(pack_x + pack_w)), dim3(256), 0, st, pk, pw, pack_x);
     }
