@@ -375,6 +375,12 @@ __device__ __forceinline__ void logits_tile(const Logits& a, int rows, int m0, i
     // exp(x) times 2^-64 when the packed bf16 format takes it as it is
     constexpr float kDown = KEEP == kKeepPacked && !C::F16 ? 64.0f : 0.0f;
     const bool part = wm + C::WM > a.v;  // the last columns end inside this wave's
+    int target[WJ];  // loaded first: among the stores below each would wait for those before it
+#pragma unroll
+    for (int j = 0; j < WJ; ++j) {
+        const int n = wn + j * 16 + (lane & 15);
+        target[j] = n < rows ? a.tgt[a.from + n] - wm : -1;
+    }
 #pragma unroll
     for (int j = 0; j < WJ; ++j) {
         const int n = wn + j * 16 + (lane & 15);
@@ -397,7 +403,7 @@ __device__ __forceinline__ void logits_tile(const Logits& a, int rows, int m0, i
             sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
         }
-        const int y = n < rows ? a.tgt[a.from + n] - wm : -1;
+        const int y = target[j];
         if (y >= 0 && y < C::WM && (y & 12) == hi) {
             float t = 0.0f;
 #pragma unroll
@@ -767,11 +773,16 @@ template <typename C, int OUT>
 __device__ __forceinline__ void finish_tile(const Grad& g, int n_all, int m0, int n0, float factor,
                                             const f32x4 (&acc)[C::WI][C::WJ]) {
     const int lane = threadIdx.x & 63;
+    int rows[C::WJ];  // loaded before the first store
 #pragma unroll
     for (int j = 0; j < C::WJ; ++j) {
-        const int n = n0 + j * 16 + (lane & 15);
-        if (n >= n_all) continue;
-        const int64_t row = g.dh ? g.map[g.from + n] : n;
+        rows[j] = n0 + j * 16 + (lane & 15);
+        if (g.dh && rows[j] < n_all) rows[j] = g.map[g.from + rows[j]];
+    }
+#pragma unroll
+    for (int j = 0; j < C::WJ; ++j) {
+        if (n0 + j * 16 + (lane & 15) >= n_all) continue;
+        const int64_t row = rows[j];
         if constexpr (OUT == kOut16) {
 #pragma unroll
             for (int i = 0; i < C::WI; i += 2) {
@@ -942,7 +953,10 @@ int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
 template <bool F16> using LogitsBig = Cfg<F16, 256, 256, 64, 128, 64, 2, false, false, 4>;
 template <bool F16> using LogitsSmall = Cfg<F16, 128, 128, 64, 64, 64, 2, false, false, 4>;
-template <bool F16> using LogitsRow = Cfg<F16, 128, 32, 64, 32, 64, 4, false, false, 4, true>;
+// For few rows the logits' product is one pass over W: one wave a tile and six stages keep
+// 120 KB a CU in flight (525 MB for one row in 87 us, 6.0 TB/s; tiles of 128 columns in four
+// stages 93 us, three stages 95 us).
+template <bool F16> using LogitsRow = Cfg<F16, 64, 32, 64, 32, 64, 6, false, false, 4, true>;
 template <bool F16> using HiddenBig = Cfg<F16, 256, 256, 64, 128, 64, 2, true, false, 8>;
 template <bool F16> using HiddenSmall = Cfg<F16, 128, 128, 64, 64, 64, 2, true, false, 8>;
 template <bool F16> using WeightBig = Cfg<F16, 256, 256, 128, 64, 64, 2, true, true, 4>;
