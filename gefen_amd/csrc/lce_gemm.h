@@ -19,11 +19,13 @@
 // come out of the transposing ds_read_b64_tr_b16; the XOR spreads both over all banks
 // (no conflicts counted).
 //
-// Measured on products of 8.6e12 bf16 operations, 256 x 256 tiles, normal values:
-// logits [128256, 8192] over K = 4096 1.26 PFLOP/s, dh [4096, 8192] over 128256 1.42,
-// dW [4096, 128256] over 8192 1.28; the vendor's library reached 1.29, 1.24 and 1.05 on
-// the same shapes.  Waves of 128 x 128 (half the waves, a third less LDS traffic) were
-// 20% slower: one wave per SIMD has nothing to cover its waits with.
+// Bound by the matrix cores and the power they draw: the products of 8192 x 128256 x 4096
+// (8.6e12 bf16 operations each) take 6.86 ms for the logits with all that is kept of them
+// (1.25 PFLOP/s), 6.40 ms for dh (1.34) and 7.03 ms for dW (1.22), MFMA busy 61% of the
+// cycles at a clock of 1.9 GHz; the vendor's library reaches 1.29, 1.24 and 1.05 on the
+// bare products.  Waves of 128 x 128 (half the waves, a third less LDS traffic) were 20%
+// slower: one wave per SIMD has nothing to cover its waits with.  Steps of 32 in four or
+// five stages lose to steps of 64 in two (twice the barriers).
 //
 // Operands of more than 16 bits are planes, and a product of them is several segments
 // of one K loop, the small ones first: a float32 value is a half-precision high part and
