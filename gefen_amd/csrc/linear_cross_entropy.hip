@@ -994,15 +994,14 @@ struct Plan {
 constexpr int kCus = 256;
 constexpr int slots_of(bool big) { return big ? kCus : 2 * kCus; }
 
-// Fewest K steps (of all segments) for big tiles: with one workgroup per CU nothing runs
-// beside the ends of a tile.  Logits of 346 x 81968 in two steps 41 us, small tiles 32; of
-// 2048 x 32000 in eight 96 and 111.  dW of 80 rows (two steps) x 42438 x 3136 142 us, small
-// tiles 121; of 512 rows (eight) x 32000 x 2048 107 and 108.
-constexpr int kBigLogitsSteps = 4, kBigGradSteps = 9;
 // Measured: a K step of 64 takes 1.7 us on a chip full of big tiles (256 of 256 x 256)
 // and about 1.06 us on one full of small ones (512 of 128 x 128, half the products).  So
 // big tiles win unless the edges leave more than a fifth of them empty, or there are not
 // steps enough to give every workgroup a few.
+// And unless the steps (of all segments) are few: with one workgroup per CU nothing runs
+// beside the ends of a tile.  dW of 80 rows (two steps) x 42438 x 3136 142 us, with small
+// tiles 121; of 512 rows (eight) x 32000 x 2048 107 and 108.
+constexpr int kBigGradSteps = 9;
 bool big_tile(int64_t m, int64_t n, int64_t steps, int segs) {
     if (steps * segs < kBigGradSteps) return false;
     const int64_t tb = up(m, 256) / 256 * (up(n, 256) / 256), ts = up(m, 128) / 128 * (up(n, 128) / 128);
@@ -1011,6 +1010,23 @@ bool big_tile(int64_t m, int64_t n, int64_t steps, int segs) {
 // K steps that are run in one piece whatever the tiles: joining costs a launch (5 us),
 // what eight steps take where a CU has one small tile.
 constexpr int kUncutSteps = 24;
+// The same for the logits, whose tiles are whole, by an estimate: the times above, and what
+// the ends of a tile take, 7 us a round of big ones and 4 of small ones (256 or fewer small
+// ones, one per CU, run a step in 0.6 us).  Measured, big and small: 3740 x 80744 of width
+// 128 240 us and 267, 2307 x 91309 of width 64 150 and 162, 309 x 110742 of width 256 63 and
+// 48, 80 x 42438 of width 3136 96 and 88, 67 x 97809 of width 1536 115 and 89.  Where the
+// two are within a tenth the estimate may miss: 507 x 16747 of width 4096 106 and 112, and
+// it takes the small ones.
+bool logits_big(int64_t v, int64_t n, int64_t steps) {
+    const int64_t tb = up(v, 256) / 256 * (up(n, 256) / 256), ts = up(v, 128) / 128 * (up(n, 128) / 128);
+    const double s = (double)steps;
+    const double big = (double)((tb + kCus - 1) / kCus) * (1.7 * s + 7.0);
+    const int64_t rest = ts % (2 * kCus);
+    const double small = (double)(ts / (2 * kCus)) * (1.06 * s + 4.0) +
+                         (rest > kCus ? 1.06 * s + 4.0 : rest > 0 ? 0.6 * s + 4.0 : 0.0);
+    return big <= small;
+}
+
 // Partial tiles that a product of up to `tiles` tiles of `steps` K steps may leave: kMostRounds
 // rounds of the chip at most.
 int parts_of(int64_t tiles, int64_t steps, int segs, bool big) {
@@ -1059,10 +1075,8 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
     p->pieces = (int)((all + rows - 1) / rows);
     p->rows = (int)rows;
     const int64_t n = t.n < rows ? (t.n > 0 ? t.n : 1) : rows;
-    const int64_t tiles = up(t.v, 256) / 256 * (up(n, 256) / 256);
-    const int in_segs = t.dtype == GEFEN_F32 ? 3 : 1;
-    p->tile = n <= 32 ? kRowTile
-              : tiles >= kCus / 2 && p->dp / 64 * in_segs >= kBigLogitsSteps ? kBigTile : kSmallTile;
+    const int64_t in_steps = p->dp / 64 * (t.dtype == GEFEN_F32 ? 3 : 1);
+    p->tile = n <= 32 ? kRowTile : logits_big(t.v, n, in_steps) ? kBigTile : kSmallTile;
     p->slots = (int)(up(t.v, kSlot) / kSlot);
     const int segs = t.dtype == GEFEN_F32 ? 3 : p->planes;
     p->dh_big = big_tile(t.d, n, up(t.v, 64) / 64, segs);
