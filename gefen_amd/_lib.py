@@ -123,7 +123,7 @@ class LinearCrossEntropyTask(ctypes.Structure):
     _fields_ += [(name, I64) for name in ("n", "v", "d", "hidden_row_stride", "hidden_col_stride",
                                           "weight_row_stride", "weight_col_stride", "ignore_index",
                                           "workspace_limit")]
-    _fields_ += [("label_smoothing", DBL), ("dtype", I32), ("targets_int32", I32), ("reduction", I32), ("pad", I32)]
+    _fields_ += [("label_smoothing", DBL), ("dtype", I32), ("targets_int32", I32), ("reduction", I32), ("stage", I32)]
 
 
 REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2

@@ -194,10 +194,12 @@ struct LceOptions {
 float* floats(const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 void* data(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-// One library call on the current stream.
+// One library call on the current stream.  A forward stage keeps its workspace in *kept,
+// where all rows fit the limit together (else it is a whole call without gradients, and
+// *kept stays undefined); with *kept defined the call is the backward stage.
 void lce_call(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets, const LceOptions& o,
               const at::Tensor& losses, const at::Tensor& loss, const at::Tensor& grad_hidden,
-              const at::Tensor& grad_weight, const at::Tensor& grad) {
+              const at::Tensor& grad_weight, const at::Tensor& grad, at::Tensor* kept = nullptr) {
     at::Tensor h = hidden.dim() == 2 ? hidden : hidden.reshape({-1, hidden.size(-1)});
     at::Tensor y = targets.contiguous();
     gefen_linear_cross_entropy_task t{};
@@ -222,10 +224,18 @@ void lce_call(const at::Tensor& hidden, const at::Tensor& weight, const at::Tens
     t.dtype = dtype_code(h);
     t.targets_int32 = y.scalar_type() == at::kInt;
     t.reduction = static_cast<int32_t>(o.reduction);
-    const size_t nbytes = lib.lce_workspace(&t);
+    const bool backward = kept && kept->defined();
+    t.stage = backward ? GEFEN_LCE_BACKWARD : kept ? GEFEN_LCE_FORWARD : GEFEN_LCE_WHOLE;
+    size_t nbytes = lib.lce_workspace(&t);
+    const bool keep = kept && nbytes != 0;
+    if (kept && nbytes == 0 && !backward) {
+        t.stage = GEFEN_LCE_WHOLE;
+        nbytes = lib.lce_workspace(&t);
+    }
     if (nbytes == 0) check(GEFEN_EINVAL);
-    at::Tensor ws = bytes_on(h, nbytes);
-    check(lib.lce(&t, ws.data_ptr(), nbytes, stream_of(h)));
+    at::Tensor ws = backward ? *kept : bytes_on(h, nbytes);
+    if (keep) *kept = ws;
+    check(lib.lce(&t, ws.data_ptr(), backward ? ws.numel() : nbytes, stream_of(h)));
 }
 
 at::Tensor empty_grad(const at::Tensor& like, bool wanted) {
@@ -234,22 +244,25 @@ at::Tensor empty_grad(const at::Tensor& like, bool wanted) {
 
 // The loss; gh, gw: the gradients where they are formed here (a reduced loss of bfloat16
 // or float32 operands).  Float16 ones wait for the loss's gradient, so that a loss scale
-// reaches them before they are rounded.
+// reaches them before they are rounded, and so do those of losses that are not reduced;
+// kept is then what they are formed from.
 at::Tensor lce_forward(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
-                       const LceOptions& o, bool need_h, bool need_w, at::Tensor* gh, at::Tensor* gw) {
+                       const LceOptions& o, bool need_h, bool need_w, at::Tensor* gh, at::Tensor* gw,
+                       at::Tensor* kept) {
     c10::DeviceGuard guard(hidden.device());
     const auto f32 = hidden.options().dtype(at::kFloat).requires_grad(false);
     if (o.reduction == GEFEN_REDUCE_NONE) {
         at::Tensor losses = at::empty(targets.sizes(), f32);
-        lce_call(hidden, weight, targets, o, losses, {}, {}, {}, {});
+        lce_call(hidden, weight, targets, o, losses, {}, {}, {}, {}, need_h || need_w ? kept : nullptr);
         return losses;
     }
     at::Tensor loss = at::empty({}, f32);
-    if (hidden.scalar_type() != at::kHalf) {
+    const bool wait = hidden.scalar_type() == at::kHalf && (need_h || need_w);
+    if (!wait) {
         *gh = empty_grad(hidden, need_h);
         *gw = empty_grad(weight, need_w);
     }
-    lce_call(hidden, weight, targets, o, {}, loss, *gh, *gw, {});
+    lce_call(hidden, weight, targets, o, {}, loss, *gh, *gw, {}, wait ? kept : nullptr);
     return loss;
 }
 
@@ -258,9 +271,9 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& hidden, const at::Tensor& weight,
                               const at::Tensor& targets, int64_t ignore_index, int64_t workspace_limit,
                               double label_smoothing, int64_t reduction, bool need_h, bool need_w) {
-        at::Tensor gh, gw;
+        at::Tensor gh, gw, kept;
         at::Tensor result = lce_forward(hidden, weight, targets, {ignore_index, workspace_limit, label_smoothing, reduction},
-                                        need_h, need_w, &gh, &gw);
+                                        need_h, need_w, &gh, &gw, &kept);
         ctx->save_for_backward({hidden, weight, targets});
         ctx->saved_data["ignore_index"] = ignore_index;
         ctx->saved_data["workspace_limit"] = workspace_limit;
@@ -271,6 +284,7 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
         ctx->saved_data["formed"] = gh.defined() || gw.defined();
         if (gh.defined()) ctx->saved_data["gh"] = gh;
         if (gw.defined()) ctx->saved_data["gw"] = gw;
+        if (kept.defined()) ctx->saved_data["kept"] = kept;
         return result;
     }
 
@@ -297,10 +311,17 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
             } else {
                 gh = empty_grad(hidden, need_h);
                 gw = empty_grad(weight, need_w);
+                // used up by the call: a second backward starts from the operands
+                at::Tensor kept;
+                const auto at_kept = ctx->saved_data.find("kept");
+                if (at_kept != ctx->saved_data.end()) {
+                    kept = at_kept->second.toTensor();
+                    ctx->saved_data.erase("kept");
+                }
                 lce_call(hidden, weight, saved[2],
                          {ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["workspace_limit"].toInt(),
                           ctx->saved_data["label_smoothing"].toDouble(), ctx->saved_data["reduction"].toInt()},
-                         {}, {}, gh, gw, grad);
+                         {}, {}, gh, gw, grad, kept.defined() ? &kept : nullptr);
             }
         }
         return {gh, gw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
@@ -354,9 +375,9 @@ py::object linear_cross_entropy(py::handle hidden_, py::handle weight_, py::hand
     if (need_h || need_w)
         return wrap(LinearCrossEntropy::apply(hidden, weight, targets, ignore_index, workspace_limit, label_smoothing,
                                               reduction, need_h, need_w));
-    at::Tensor gh, gw;
+    at::Tensor gh, gw, kept;
     return wrap(lce_forward(hidden.detach(), weight.detach(), targets,
-                            {ignore_index, workspace_limit, label_smoothing, reduction}, false, false, &gh, &gw));
+                            {ignore_index, workspace_limit, label_smoothing, reduction}, false, false, &gh, &gw, &kept));
 }
 
 }  // namespace

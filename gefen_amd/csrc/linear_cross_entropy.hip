@@ -79,6 +79,7 @@ struct Select {
     int32_t* map;
     int32_t* tgt;
     Meta* meta;
+    int32_t again;  // all but grad_max is there from a forward call
 };
 // map = the rows that take part, in order, then the ignored ones; tgt = their targets in
 // that order (-1: not a column, whose loss is NaN; may be null).  One workgroup.
@@ -136,7 +137,9 @@ __device__ __forceinline__ Meta select_rows(const Select& s, int32_t* map, int32
 constexpr int kRowsThreads = 1024;
 __global__ __launch_bounds__(kRowsThreads) void k_rows(const Select s) {
     const Meta m = select_rows<kRowsThreads>(s, s.map, s.tgt);
-    if (threadIdx.x == 0) *s.meta = m;
+    if (threadIdx.x != 0) return;
+    if (s.again) s.meta->grad_max = m.grad_max;
+    else *s.meta = m;
 }
 
 // x (scaled into half's range) as a half and what it leaves times kLowScale.
@@ -977,6 +980,7 @@ enum LogitsTile { kRowTile, kSmallTile, kBigTile };
 struct Plan {
     int n, v, d, dtype;
     bool train, dh, dw, pack_w, smooth;
+    bool forward, backward;  // the stages that this call runs
     int planes;         // of G
     bool halves;        // products of half-precision operands
     int64_t dp, ldg;
@@ -1050,13 +1054,21 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
         return fail_inval("%s: label_smoothing must lie in [0, 1], got %g", what, t.label_smoothing);
     if (t.reduction < GEFEN_REDUCE_NONE || t.reduction > GEFEN_REDUCE_SUM)
         return fail_inval("%s: unknown reduction %d", what, t.reduction);
+    if (t.stage < GEFEN_LCE_WHOLE || t.stage > GEFEN_LCE_BACKWARD) return fail_inval("%s: unknown stage %d", what, t.stage);
+    if (t.stage == GEFEN_LCE_FORWARD && (t.grad_hidden || t.grad_weight))
+        return fail_inval("%s: a forward stage forms no gradients", what);
+    if (t.stage == GEFEN_LCE_BACKWARD && (t.losses || t.loss || (!t.grad_hidden && !t.grad_weight)))
+        return fail_inval("%s: a backward stage forms gradients, and no loss", what);
+    p->forward = t.stage != GEFEN_LCE_BACKWARD;
     p->n = (int)t.n;
     p->v = (int)t.v;
     p->d = (int)t.d;
     p->dtype = t.dtype;
-    p->dh = t.grad_hidden != nullptr;
-    p->dw = t.grad_weight != nullptr;
+    // a forward stage lays its workspace out for either gradient
+    p->dh = t.grad_hidden || t.stage == GEFEN_LCE_FORWARD;
+    p->dw = t.grad_weight || t.stage == GEFEN_LCE_FORWARD;
     p->train = p->dh || p->dw;
+    p->backward = p->train && t.stage != GEFEN_LCE_FORWARD;
     p->smooth = t.label_smoothing > 0.0;
     p->planes = t.dtype == GEFEN_F32 || t.n <= kTwoPlaneRows ? 2 : 1;
     p->halves = t.dtype != GEFEN_BF16;
@@ -1074,6 +1086,7 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
     const int64_t rows = up((all + want - 1) / want, kRowAlign);
     p->pieces = (int)((all + rows - 1) / rows);
     p->rows = (int)rows;
+    if (t.stage && p->pieces > 1) return fail_inval("%s: stages of %d pieces of rows", what, p->pieces);
     const int64_t n = t.n < rows ? (t.n > 0 ? t.n : 1) : rows;
     const int64_t in_steps = p->dp / 64 * (t.dtype == GEFEN_F32 ? 3 : 1);
     p->tile = n <= 32 ? kRowTile : logits_big(t.v, n, in_steps) ? kBigTile : kSmallTile;
@@ -1198,7 +1211,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         return fail_inval("%s: an operand is not aligned to its elements", what);
     if (t.n && !t.losses && !t.loss && !p.train) return fail_inval("%s: nothing to compute", what);
     if (t.loss && t.reduction == GEFEN_REDUCE_NONE) return fail_inval("%s: no reduction for a loss", what);
-    if (t.reduction == GEFEN_REDUCE_NONE && p.train && t.n && !t.grad)
+    if (t.reduction == GEFEN_REDUCE_NONE && p.backward && t.n && !t.grad)
         return fail_inval("%s: gradients without a reduction need one gradient per row", what);
     if (!workspace || workspace_bytes < p.bytes)
         return fail_inval("%s: workspace of %zu bytes, needs %zu", what, workspace_bytes, p.bytes);
@@ -1213,9 +1226,10 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     uint16_t* x = reinterpret_cast<uint16_t*>(ws + p.o_x);
     uint16_t* wp = reinterpret_cast<uint16_t*>(ws + p.o_w);
     uint16_t* gbuf = reinterpret_cast<uint16_t*>(ws + p.o_g);
-    const bool by_row = p.train && t.reduction == GEFEN_REDUCE_NONE;
+    const bool by_row = p.backward && t.reduction == GEFEN_REDUCE_NONE;
 
-    const Select sel{t.targets, t.targets_int32, p.n, p.v, t.ignore_index, by_row ? t.grad : nullptr, map, tgt, meta};
+    const Select sel{t.targets, t.targets_int32, p.n, p.v, t.ignore_index, by_row ? t.grad : nullptr, map, tgt, meta,
+                     !p.forward};
     const int x_rows = p.rows * p.pieces;
     Pack pk{};
     pk.src = t.hidden;
@@ -1248,7 +1262,11 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     pw.which = 1;
     const int pack_x = (int)grid_of(x_rows * (p.dp / 8), 8192);
     const int pack_w = p.pack_w ? (int)grid_of(p.v * (p.dp / 8), 8192) : 0;
-    if (p.n <= kSelfRows && !pk.f32) {
+    if (!p.forward) {
+        // the rows' gradients, and zero for the rows that take no part
+        if (by_row) hipLaunchKernelGGL(k_rows, dim3(1), dim3(kRowsThreads), 0, st, sel);
+        if (p.dh) hipLaunchKernelGGL(k_pack, dim3((unsigned)pack_x), dim3(256), 0, st, pk, pw, pack_x);
+    } else if (p.n <= kSelfRows && !pk.f32) {
         hipLaunchKernelGGL(k_select_pack, dim3((unsigned)(pack_x + pack_w)), dim3(256), 0, st, sel, pk, pw, pack_x);
     } else {
         hipLaunchKernelGGL(k_rows, dim3(1), dim3(kRowsThreads), 0, st, sel);
@@ -1304,8 +1322,10 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         Grad g{};
         const bool f16 = p.halves;
         if (most > 0) {
-            if (f16) launch_logits_tile<true>(p, l, most, st);
-            else launch_logits_tile<false>(p, l, most, st);
+            if (p.forward) {
+                if (f16) launch_logits_tile<true>(p, l, most, st);
+                else launch_logits_tile<false>(p, l, most, st);
+            }
             Rows r{};
             r.stats = l.stats;
             r.sums = l.sums;
@@ -1318,7 +1338,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
             r.mean = t.reduction == GEFEN_REDUCE_MEAN;
             r.dtype = t.dtype;
             r.losses = losses;
-            r.g = l.g;
+            r.g = p.backward ? l.g : nullptr;
             r.ldg = p.ldg;
             r.g_plane = l.g_plane;
             r.v = p.v;
@@ -1328,18 +1348,18 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
             r.planes = p.planes;
             r.smoothing = (float)t.label_smoothing;
             // a row per workgroup, or parts of it where the rows do not fill the chip
-            const int64_t rows_up = p.train ? up(most, 64) : most;
-            int64_t parts = p.train ? 2048 / rows_up : 1;
+            const int64_t rows_up = p.backward ? up(most, 64) : most;
+            int64_t parts = p.backward ? 2048 / rows_up : 1;
             const int64_t chunks = p.ldg / 8 / kGradThreads;
             if (parts > chunks) parts = chunks;
             if (parts < 1) parts = 1;
             const dim3 grid((unsigned)rows_up, (unsigned)parts);
-            const bool stream_past = p.train && (int64_t)p.planes * most * p.ldg * 2 > kKeepBytes;
+            const bool stream_past = p.backward && (int64_t)p.planes * most * p.ldg * 2 > kKeepBytes;
             auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kGradThreads), 0, st, r); };
             if (f16) stream_past ? launch(k_gradient_rows<true, true>) : launch(k_gradient_rows<true, false>);
             else stream_past ? launch(k_gradient_rows<false, true>) : launch(k_gradient_rows<false, false>);
         }
-        if (!p.train) continue;
+        if (!p.backward) continue;
         Operand go{};
         go.p = gbuf;
         go.ld = p.ldg;

@@ -11,7 +11,8 @@ With ``reduction`` "mean" or "sum" and bfloat16 or float32 operands the gradient
 formed in the forward call, where the kept values still are (three products instead of
 four), and backward multiplies them by the loss's own gradient, which costs nothing when
 that is 1.  Float16 gradients are formed in backward, so that a loss scale reaches them
-before they are rounded, and so are those of ``reduction`` "none".
+before they are rounded, and so are those of ``reduction`` "none": the kept values wait for
+backward where all positions fit ``workspace_limit`` together, else they are formed again.
 """
 
 from __future__ import annotations

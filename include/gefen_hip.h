@@ -474,6 +474,11 @@ int gefen_scale_gradients(const gefen_gradient_task* tasks, int num_tasks, const
 enum { GEFEN_REDUCE_NONE = 0, GEFEN_REDUCE_MEAN = 1, GEFEN_REDUCE_SUM = 2 };
 /* workspace_limit = 0: what the values kept for the gradients may take */
 #define GEFEN_LCE_DEFAULT_LIMIT ((int64_t)4 << 30)
+/* A call in two: GEFEN_LCE_FORWARD writes losses and loss (no gradient pointers) and leaves in
+ * the workspace what GEFEN_LCE_BACKWARD forms the gradients from (no loss pointers; the task and
+ * the operands otherwise as they were), once: it overwrites what it reads.  Only where all rows
+ * fit the workspace limit together; otherwise the task is invalid. */
+enum { GEFEN_LCE_WHOLE = 0, GEFEN_LCE_FORWARD = 1, GEFEN_LCE_BACKWARD = 2 };
 
 typedef struct gefen_linear_cross_entropy_task {
     const void* hidden;   /* [n, d], any strides (elements) */
@@ -494,7 +499,7 @@ typedef struct gefen_linear_cross_entropy_task {
     int32_t dtype;            /* of hidden, weight and their gradients */
     int32_t targets_int32;    /* 1: targets are int32 */
     int32_t reduction;        /* the mean is over the rows that have a loss */
-    int32_t pad;
+    int32_t stage;            /* GEFEN_LCE_*: 0 for a whole call */
 } gefen_linear_cross_entropy_task;
 
 /* Bytes of workspace that the call needs (0: invalid task, see gefen_last_error). */

@@ -133,3 +133,25 @@ def test_names_are_exported():
 
     for name in ("linear_cross_entropy", "gradient_norm", "clip_gradients", "clip_grad_norm_"):
         assert name in gefen_amd.__all__ and callable(getattr(gefen_amd, name))
+
+
+@pytest.mark.parametrize("bad", [dict(stage=3), dict(stage=-1), dict(stage=1, grad_hidden=FAKE), dict(stage=2),
+                                 dict(stage=2, grad_hidden=FAKE), dict(stage=2, loss=0),
+                                 dict(stage=2, loss=0, losses=FAKE, grad_weight=FAKE),
+                                 dict(stage=1, n=10000, workspace_limit=1 << 20),
+                                 dict(stage=2, loss=0, grad_weight=FAKE, n=10000, workspace_limit=1 << 20)])
+def test_linear_cross_entropy_refuses_stages(bad):
+    lib = _lib.load()
+    assert size(**bad) == 0
+    assert lib.gefen_linear_cross_entropy(ctypes.byref(task(**bad)), FAKE, 1 << 40, None) == _lib.GEFEN_EINVAL
+
+
+def test_a_backward_stage_fits_the_workspace_of_its_forward_stage():
+    for n, v, d in ((1, 1, 1), (48, 1000, 96), (300, 50257, 768), (2000, 32003, 1001)):
+        for dtype in (_lib.F32, _lib.F16, _lib.BF16):
+            for reduction in (_lib.REDUCE_NONE, _lib.REDUCE_MEAN):
+                k = dict(n=n, v=v, d=d, dtype=dtype, reduction=reduction)
+                loss = 0 if reduction == _lib.REDUCE_NONE else FAKE
+                forward = size(stage=1, loss=loss, **k)
+                for g in (dict(grad_hidden=FAKE), dict(grad_weight=FAKE), dict(grad_hidden=FAKE, grad_weight=FAKE)):
+                    assert 0 < size(stage=2, loss=0, **k, **g) <= forward

@@ -144,3 +144,68 @@ def test_losses_of_a_batch_keep_its_shape():
     assert rows.shape == (3, 4, 5) and rows.dtype == torch.float32
     assert not rows.requires_grad
     assert math.isclose(float(rows.double().mean()), float(lce(h, w, y)), rel_tol=1e-6)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n,v,d,ignored", [(1, 70, 9, 0.0), (60, 900, 64, 0.3), (300, 4100, 200, 0.0),
+                                           (1100, 700, 130, 0.5), (40, 300, 16, 1.0)])
+def test_gradients_of_kept_values_are_those_of_a_second_product(n, v, d, ignored, dtype, reduction):
+    """The first backward starts from what the forward call kept, the second one of a retained
+    graph from the operands, and a call in pieces keeps nothing."""
+    h, w, y = make(n, v, d, dtype, seed=n, ignored=ignored)
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    rows = lce(h, w, y, reduction=reduction, label_smoothing=0.1)
+    c = torch.rand(rows.shape, generator=torch.Generator().manual_seed(2)).cuda() + 0.5
+    if reduction == "mean":
+        c = torch.ones_like(c)
+    kept = torch.autograd.grad(rows, (h, w), grad_outputs=c, retain_graph=True)
+    again = torch.autograd.grad(rows, (h, w), grad_outputs=c)
+    assert torch.equal(kept[0], again[0]) and torch.equal(kept[1], again[1])
+    assert not kept[0][y == -100].any()
+    for i, x in enumerate((h, w)):
+        alone = lce(h if i == 0 else h.detach(), w if i == 1 else w.detach(), y, reduction=reduction,
+                    label_smoothing=0.1)
+        assert torch.equal(alone, rows) or ignored == 1.0
+        assert torch.equal(torch.autograd.grad(alone, x, grad_outputs=c)[0], kept[i])
+
+
+def test_kept_values_outlive_other_calls_and_refuse_changed_operands():
+    h, w, y = make(200, 3000, 96, "f16", seed=4)
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    want = torch.autograd.grad(lce(h, w, y), (h, w))
+    first = lce(h, w, y)
+    second = lce(h * 2, w, y.flip(0))
+    torch.autograd.grad(second, w)
+    got = torch.autograd.grad(first, (h, w))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    loss = lce(h, w, y)
+    with torch.no_grad():
+        w.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_values_are_kept_only_within_the_limit():
+    h, w, y = make(1000, 4096, 64, "f16", seed=6)
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    lce(h, w, y).backward()  # the allocator's first blocks
+    g = h.grad.clone(), w.grad.clone()
+
+    def held(limit):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        loss = lce(h, w, y, workspace_limit=limit)
+        after = torch.cuda.memory_allocated()
+        got = torch.autograd.grad(loss, (h, w))
+        return after - before, got
+
+    much, a = held(None)
+    little, b = held(1 << 20)
+    assert much >= 1000 * 4096 * 2 and little <= 4096
+    for x, z, r in zip(a, b, g):
+        assert torch.equal(x, r)
+        assert torch.allclose(z.float(), r.float(), rtol=2.0 ** -9, atol=2.0 ** -22)
