@@ -254,8 +254,7 @@ __global__ __launch_bounds__(kTopThreads) void k_top(const Top a, const Top b, i
 // Rows of a matrix of any strides as the products read them: dp = D rounded up to 64
 // columns, zero-padded, one plane or those of a float32 operand, scaled.  With a map: row
 // r is src row map[r] for r < meta->count and zero up to the next multiple of kRowAlign,
-// and the rows that take no part get a zero gradient and a zero loss.  A thread moves
-// eight columns of a row.
+// and the rows that take no part get a zero loss.  A thread moves eight columns of a row.
 constexpr int kPackPlanes = 3;  // of a float32 operand: high, low, high where finite
 struct Pack {
     const void* src;
@@ -268,7 +267,6 @@ struct Pack {
     const int32_t* map;
     const Meta* meta;
     int32_t which;      // float32: whose largest magnitude in meta->top
-    void* zero_rows;    // [n, d] gradient (may be null)
     float* zero_losses;  // [n] (may be null)
 };
 __device__ __forceinline__ void pack_block(const Pack& p, const int32_t* map, int count, int block, int blocks) {
@@ -281,14 +279,7 @@ __device__ __forceinline__ void pack_block(const Pack& p, const int32_t* map, in
         const int c0 = (int)(q - (int64_t)r * per) * 8;
         const int64_t row = map && r < p.n ? map[r] : r;
         const bool live = r < count;
-        if (map && !live && r < p.n) {
-            if (p.zero_losses && c0 == 0) p.zero_losses[row] = 0.0f;
-            if (p.zero_rows)
-                for (int e = c0; e < min(c0 + 8, p.d); ++e) {
-                    if (p.f32) static_cast<float*>(p.zero_rows)[row * p.d + e] = 0.0f;
-                    else static_cast<uint16_t*>(p.zero_rows)[row * p.d + e] = 0;
-                }
-        }
+        if (map && !live && r < p.n && p.zero_losses && c0 == 0) p.zero_losses[row] = 0.0f;
         if (r >= ends) continue;
         Vec<uint16_t, 8> out[kPackPlanes] = {};
         if (live && p.f32) {
@@ -507,6 +498,8 @@ struct Rows {
     int64_t ldg, g_plane;
     int32_t v, slots, from, most, planes;
     float smoothing;
+    void* zero_rows;        // [n, zero_bytes]: dh, zero where a row takes no part (may be null)
+    int64_t zero_bytes;     // of a row
 };
 
 __device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
@@ -554,7 +547,13 @@ __global__ __launch_bounds__(kGradThreads) void k_gradient_rows(const Rows a) {
         }
         a.meta->factor[threadIdx.x] = f;
     }
-    if (r >= rows) {  // zero rows up to the end of the last K step of dW
+    if (r >= rows) {
+        if (a.zero_rows && r < a.most) {
+            uint16_t* z = static_cast<uint16_t*>(a.zero_rows) + (int64_t)a.map[a.from + r] * (a.zero_bytes / 2);
+            for (int64_t c = blockIdx.y * kGradThreads + threadIdx.x; c < a.zero_bytes / 2; c += gridDim.y * kGradThreads)
+                z[c] = 0;
+        }
+        // zero rows up to the end of the last K step of dW
         if (!a.g || r >= (rows + 63) / 64 * 64) return;
         Vec<uint16_t, 8> z = {};
         for (int k = 0; k < a.planes; ++k)
@@ -1245,7 +1244,6 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     pk.map = map;
     pk.meta = meta;
     pk.which = 0;
-    pk.zero_rows = t.grad_hidden;
     pk.zero_losses = losses;
     Pack pw{};
     pw.src = t.weight;
@@ -1263,9 +1261,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     const int pack_x = (int)grid_of(x_rows * (p.dp / 8), 8192);
     const int pack_w = p.pack_w ? (int)grid_of(p.v * (p.dp / 8), 8192) : 0;
     if (!p.forward) {
-        // the rows' gradients, and zero for the rows that take no part
         if (by_row) hipLaunchKernelGGL(k_rows, dim3(1), dim3(kRowsThreads), 0, st, sel);
-        if (p.dh) hipLaunchKernelGGL(k_pack, dim3((unsigned)pack_x), dim3(256), 0, st, pk, pw, pack_x);
     } else if (p.n <= kSelfRows && !pk.f32) {
         hipLaunchKernelGGL(k_select_pack, dim3((unsigned)(pack_x + pack_w)), dim3(256), 0, st, sel, pk, pw, pack_x);
     } else {
@@ -1347,6 +1343,8 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
             r.most = most;
             r.planes = p.planes;
             r.smoothing = (float)t.label_smoothing;
+            r.zero_rows = p.backward ? t.grad_hidden : nullptr;
+            r.zero_bytes = (int64_t)p.d * size;
             // a row per workgroup, or parts of it where the rows do not fill the chip
             const int64_t rows_up = p.backward ? up(most, 64) : most;
             int64_t parts = p.backward ? 2048 / rows_up : 1;
