@@ -15,7 +15,7 @@
 // * The logits' product keeps, for every row and slot of 64 columns, the slot's
 //   maximum m and sum of exp(l - m), both float32, and when gradients are wanted
 //   exp(l - m) itself in 16 bits: an unsigned format of its own with three significant
-//   bits more than bf16 (two more than half), so that G is in effect rounded once.
+//   bits more than bf16 (one more than half) and a range beyond that of G.
 // * One pass over those values turns them into G (k_gradient_rows): a row's lse comes
 //   from its slots, and exp(m - lse) scales each slot.  The target's entry is formed in
 //   float32 from its own logit, so that p - 1 of a confident row does not cancel in
@@ -168,22 +168,24 @@ __device__ __forceinline__ void split_bf16(float x, uint16_t* hi, uint16_t* lo) 
     *lo = (h.bits & 0x7f80) == 0x7f80 ? 0 : from_f32<bf16_t>(x - to_f32(h)).bits;
 }
 
-// exp(l - m) in [0, 1] as 16 unsigned bits on its way to G: 4 exponent and 12 mantissa
+// exp(l - m) in [0, 1] as 16 unsigned bits on its way to G: 5 exponent and 11 mantissa
 // bits for a half G, 6 and 10 for a bf16 one, with subnormals.  The float's own exponent
 // is brought down by a product with a power of two (subnormal results are rounded by the
-// hardware), and the mantissa is rounded to nearest.  Relative error 2^-13 down to 2^-14
-// (bf16: 2^-11 down to 2^-62), 2^-27 absolute below.
+// hardware), and the mantissa is rounded to nearest.  Relative error 2^-12 down to 2^-30 and
+// 2^-42 absolute below (bf16: 2^-11 down to 2^-62, 2^-73 below): finer than a half G, which
+// ends at 2^-39.  (With 4 and 12 bits a column 19 nats below the one that leads its slot
+// was lost, and the target's entry, formed on its own, had nothing to balance it.)
 // Two of them, low half first; a bf16 one comes scaled by 2^-64 already.
 template <bool F16>
 __device__ __forceinline__ uint32_t pack_exp2(float a, float b) {
-    constexpr int drop = F16 ? 11 : 13;
-    const uint32_t x = __float_as_uint(F16 ? a * 0x1p-112f : a) + (1u << (drop - 1));
-    const uint32_t y = __float_as_uint(F16 ? b * 0x1p-112f : b) + (1u << (drop - 1));
+    constexpr int drop = F16 ? 12 : 13;
+    const uint32_t x = __float_as_uint(F16 ? a * 0x1p-96f : a) + (1u << (drop - 1));
+    const uint32_t y = __float_as_uint(F16 ? b * 0x1p-96f : b) + (1u << (drop - 1));
     return (x >> drop & 0xffffu) | (y >> drop << 16);
 }
 template <bool F16>
 __device__ __forceinline__ float unpack_exp(uint16_t x) {
-    return __uint_as_float((uint32_t)x << (F16 ? 11 : 13)) * (F16 ? 0x1p112f : 0x1p64f);
+    return __uint_as_float((uint32_t)x << (F16 ? 12 : 13)) * (F16 ? 0x1p96f : 0x1p64f);
 }
 
 // Packed pairs of 16-bit values of a lane's four rows of MFMA tiles i (a) and i + 1 (b),
