@@ -175,12 +175,13 @@ __device__ __forceinline__ void split_bf16(float x, uint16_t* hi, uint16_t* lo) 
 // 2^-42 absolute below (bf16: 2^-11 down to 2^-62, 2^-73 below): finer than a half G, which
 // ends at 2^-39.  (With 4 and 12 bits a column 19 nats below the one that leads its slot
 // was lost, and the target's entry, formed on its own, had nothing to balance it.)
-// Two of them, low half first; a bf16 one comes scaled by 2^-64 already.
+// Two of them, low half first.
 template <bool F16>
 __device__ __forceinline__ uint32_t pack_exp2(float a, float b) {
     constexpr int drop = F16 ? 12 : 13;
-    const uint32_t x = __float_as_uint(F16 ? a * 0x1p-96f : a) + (1u << (drop - 1));
-    const uint32_t y = __float_as_uint(F16 ? b * 0x1p-96f : b) + (1u << (drop - 1));
+    constexpr float down = F16 ? 0x1p-96f : 0x1p-64f;
+    const uint32_t x = __float_as_uint(a * down) + (1u << (drop - 1));
+    const uint32_t y = __float_as_uint(b * down) + (1u << (drop - 1));
     return (x >> drop & 0xffffu) | (y >> drop << 16);
 }
 template <bool F16>
@@ -370,8 +371,6 @@ __device__ __forceinline__ void logits_tile(const Logits& a, int rows, int m0, i
     static_assert(C::WM == kSlot, "a wave's columns are a slot");
     if (wm >= a.v && KEEP == kKeepNone) return;
     const bool f32 = KEEP != kKeepPacked && a.f32;
-    // exp(x) times 2^-64 when the packed bf16 format takes it as it is
-    constexpr float kDown = KEEP == kKeepPacked && !C::F16 ? 64.0f : 0.0f;
     const bool part = wm + C::WM > a.v;  // the last columns end inside this wave's
     int target[WJ];  // loaded first: among the stores below each would wait for those before it
 #pragma unroll
@@ -419,12 +418,11 @@ __device__ __forceinline__ void logits_tile(const Logits& a, int rows, int m0, i
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 // the difference first: exact where it matters, however large the logits; the
-                // product's rounding is 2^-24 |x| of exp(x)
-                acc[i][j][r] =
-                    __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r] - ref, kLog2E, -kDown));
+                // product's rounding is 2^-24 |x| of exp(x) (the kept values' scale comes after
+                // the exponential: as an offset of 64 in its argument it cost the sum 2^-18)
+                acc[i][j][r] = __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * kLog2E);
                 s += acc[i][j][r];
             }
-        if (kDown != 0.0f) s *= 0x1p64f;
         s += __shfl_xor(s, 16, 64);
         s += __shfl_xor(s, 32, 64);
         if (n < rows && lane < 16 && wm < a.v) {
