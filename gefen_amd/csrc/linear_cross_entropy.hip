@@ -57,8 +57,8 @@ constexpr int kMaxWidth = 1 << 20;
 // Device scalars of a call.
 struct Meta {
     int32_t count;    // rows that take part
-    float grad_max;   // largest |gradient| of a row (per-row gradients)
-    uint32_t top[2];  // float32: largest finite magnitude of hidden and weight, as bits
+    float grad_max;   // largest finite |gradient| of a row (per-row gradients)
+    uint32_t top[2];  // largest finite magnitude of hidden and weight, as bits, where they are scaled
     float factor[2];  // what the sums of dW and dh are multiplied by
 };
 
@@ -119,7 +119,10 @@ __device__ __forceinline__ Meta select_rows(const Select& s, int32_t* map, int32
             if (y[k] != s.ignore) {
                 map[before] = i;
                 if (tgt) tgt[before] = (y[k] >= 0 && y[k] < s.v) ? (int)y[k] : -1;
-                if (s.row_grad) m.grad_max = nanmax(m.grad_max, fabsf(s.row_grad[i]));
+                if (s.row_grad) {
+                    const float c = fabsf(s.row_grad[i]);
+                    if (c < INFINITY) m.grad_max = fmaxf(m.grad_max, c);
+                }
             } else if (i < s.n) {
                 map[s.n - 1 - (i - before)] = i;
             }
@@ -206,17 +209,60 @@ __device__ __forceinline__ int half_exponent(uint32_t top) {
     return top == 0 ? 0 : 14 - max((int)(top >> 23) - 127, -112);
 }
 
-// meta->top[which] = the largest finite magnitude of a float32 matrix, as its bits; with
-// a map, of the rows that take part.  Maxima of integers: any order gives the same.
+// The gradient c of a row's loss, where each row has its own.  All are taken relative to 2^E,
+// the largest finite one between 2^(E-1) and 2^E (bfloat16: its factor has to stay a float32,
+// E is 127 at most), and a row that is 2^-s of it has its power of two taken apart, so that a
+// half G, which ends at 2^-39 (two planes: 2^-50), keeps its precision in every row:
+//   * G's row carries w = c 2^-E 2^rest, down to 2^-carry;
+//   * dh's row is multiplied by 2^-rest at the end (exact);
+//   * for dW the row of hidden is (k_shift): its planes keep 2^-28 of hidden's largest element
+//     in full and end at 2^-49 (half: 2^-38).
+// A bfloat16 G has the range to carry all of it.  A gradient that is not finite stays in its
+// own row of G, and so in its row of dh, and in dW, which sums it.
+constexpr int kCarryOne = 4, kCarryTwo = 8, kCarryAll = 1 << 20;
+struct RowWeight {
+    float w;
+    int rest;
+};
+__device__ __forceinline__ int grad_exponent(float top, int carry) {
+    return min(__builtin_amdgcn_frexp_expf(top), carry == kCarryAll ? 127 : 128);
+}
+__device__ __forceinline__ RowWeight row_weight(float c, float top, int carry) {
+    if (c == 0.0f || !(fabsf(c) < INFINITY)) return {c, 0};
+    const int e = grad_exponent(top, carry);
+    const int rest = max(0, e - __builtin_amdgcn_frexp_expf(c) - carry);
+    return {ldexpf(c, rest - e), rest};
+}
+
+// meta->top[which] = the largest finite magnitude of a float32 or half matrix, as the bits
+// of a float32; with a map, of the rows that take part.  Maxima of integers: any order gives
+// the same.
 struct Top {
-    const float* src;
+    const void* src;
     int64_t row_stride, col_stride;
     int32_t n, d;
     const int32_t* map;
     Meta* meta;
-    int32_t which;
+    int32_t which, f16;
 };
 constexpr int kTopThreads = 1024, kTopGrid = 256;
+// the largest finite magnitude of up to eight columns of a row
+template <typename T>
+__device__ __forceinline__ uint32_t top_of_chunk(const T* s, int64_t col_stride, int cols) {
+    uint32_t top = 0;
+    auto see = [&](T x) {
+        const uint32_t u = abs_key(to_f32(x));
+        top = u < 0x7f800000u && u > top ? u : top;
+    };
+    if (col_stride == 1 && cols >= 8) {
+        const AnyVec<T, 8> x = *reinterpret_cast<const AnyVec<T, 8>*>(s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) see(x.v[e]);
+    } else {
+        for (int e = 0; e < min(cols, 8); ++e) see(s[e * col_stride]);
+    }
+    return top;
+}
 // Workgroups up to `first` take a, the others b.
 __global__ __launch_bounds__(kTopThreads) void k_top(const Top a, const Top b, int first) {
     const bool is_a = (int)blockIdx.x < first;
@@ -225,21 +271,12 @@ __global__ __launch_bounds__(kTopThreads) void k_top(const Top a, const Top b, i
     const uint32_t per = (uint32_t)(t.d + 7) / 8;  // chunks of eight columns a row
     const int64_t all = (int64_t)(t.map ? t.meta->count : t.n) * per;
     uint32_t top = 0;
-    auto see = [&](float x) {
-        const uint32_t u = abs_key(x);
-        top = u < 0x7f800000u && u > top ? u : top;
-    };
     for (int64_t q = (int64_t)block * kTopThreads + threadIdx.x; q < all; q += (int64_t)blocks * kTopThreads) {
         const int64_t r = q / per;
         const int c = (int)(q - r * per) * 8;
-        const float* s = t.src + (int64_t)(t.map ? t.map[r] : r) * t.row_stride;
-        if (t.col_stride == 1 && c + 8 <= t.d) {
-            const AnyVec<float, 8> x = *reinterpret_cast<const AnyVec<float, 8>*>(s + c);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) see(x.v[e]);
-        } else {
-            for (int e = c; e < min(c + 8, t.d); ++e) see(s[(int64_t)e * t.col_stride]);
-        }
+        const int64_t at = (int64_t)(t.map ? t.map[r] : r) * t.row_stride + c * t.col_stride;
+        top = max(top, t.f16 ? top_of_chunk(static_cast<const f16_t*>(t.src) + at, t.col_stride, t.d - c)
+                             : top_of_chunk(static_cast<const float*>(t.src) + at, t.col_stride, t.d - c));
     }
     // one atomic per workgroup, and few of those: on one address each takes 12 ns
     __shared__ uint32_t part[kTopThreads / 64];
@@ -271,17 +308,27 @@ struct Pack {
     const Meta* meta;
     int32_t which;      // float32: whose largest magnitude in meta->top
     float* zero_losses;  // [n] (may be null)
+    // SHIFT: rows [from, from + most) that take part again, times their gradients' powers of two
+    const float* row_grad;
+    int32_t from, most, carry;
 };
+template <bool SHIFT = false>
 __device__ __forceinline__ void pack_block(const Pack& p, const int32_t* map, int count, int block, int blocks) {
     const uint32_t per = (uint32_t)p.dp / 8;
-    const int ends = map ? (count + kRowAlign - 1) / kRowAlign * kRowAlign : p.rows;
-    const int64_t all = (int64_t)(ends > p.n ? ends : p.n) * per;
-    const int ex = p.f32 ? half_exponent(p.meta->top[p.which]) : 0;
+    const int first = SHIFT ? p.from : 0;
+    const int ends = SHIFT ? min(count, p.from + p.most)
+                     : map ? (count + kRowAlign - 1) / kRowAlign * kRowAlign
+                           : p.rows;
+    const int64_t all = (int64_t)((SHIFT || ends > p.n ? ends : p.n) - first) * per;
+    const int top = p.f32 || SHIFT ? half_exponent(p.meta->top[p.which]) : 0;
     for (int64_t q = (int64_t)block * 256 + threadIdx.x; q < all; q += (int64_t)blocks * 256) {
-        const int r = (int)(q / per);
-        const int c0 = (int)(q - (int64_t)r * per) * 8;
+        const int up = (int)(q / per);
+        const int r = first + up;
+        const int c0 = (int)(q - (int64_t)up * per) * 8;
         const int64_t row = map && r < p.n ? map[r] : r;
         const bool live = r < count;
+        int ex = top;
+        if (SHIFT) ex -= row_weight(p.row_grad[row], p.meta->grad_max, p.carry).rest;
         if (map && !live && r < p.n && p.zero_losses && c0 == 0) p.zero_losses[row] = 0.0f;
         if (r >= ends) continue;
         Vec<uint16_t, 8> out[kPackPlanes] = {};
@@ -309,6 +356,11 @@ __device__ __forceinline__ void pack_block(const Pack& p, const int32_t* map, in
                 for (int e = 0; e < 8; ++e)
                     if (c0 + e < p.d) out[0].v[e] = s[e * p.col_stride];
             }
+            if (SHIFT) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    out[0].v[e] = from_f32<f16_t>(ldexpf(to_f32(f16_t{out[0].v[e]}), ex)).bits;
+            }
         }
         uint16_t* d = p.dst + (int64_t)r * p.dp + c0;
         vstore(d, 0, out[0]);
@@ -323,6 +375,10 @@ __device__ __forceinline__ void pack_block(const Pack& p, const int32_t* map, in
 __global__ __launch_bounds__(256) void k_pack(const Pack x, const Pack w, int first) {
     if ((int)blockIdx.x < first) pack_block(x, x.map, x.meta->count, blockIdx.x, first);
     else pack_block(w, nullptr, w.n, blockIdx.x - first, gridDim.x - first);
+}
+// Hidden of half-precision products as dW of per-row gradients reads it.
+__global__ __launch_bounds__(256) void k_shift(const Pack x) {
+    pack_block<true>(x, x.map, x.meta->count, blockIdx.x, gridDim.x);
 }
 // The same for few rows without k_rows: every workgroup of hidden selects them for itself
 // (the first one for the kernels that follow), which saves a launch.
@@ -492,7 +548,7 @@ struct Rows {
     Meta* meta;
     const float* row_grad;  // gradient of each row's loss (null: one for all)
     const float* grad;      // gradient of the loss (null: 1)
-    int32_t mean, dtype;
+    int32_t mean, dtype, carry;
     float* losses;          // [n], original order
     uint16_t* g;
     int64_t ldg, g_plane;
@@ -538,14 +594,16 @@ __global__ __launch_bounds__(kGradThreads) void k_gradient_rows(const Rows a) {
     if (a.g && r == 0 && blockIdx.y == 0 && threadIdx.x < 2) {
         // of dW (whose other operand is hidden) and dh
         float f = a.dtype == GEFEN_BF16 ? 1.0f : 1.0f / kHalfScale;
-        if (a.dtype == GEFEN_F32) f = ldexpf(f, -half_exponent(a.meta->top[threadIdx.x]));
+        int ex = 0;
+        if (a.dtype == GEFEN_F32 || (a.dtype == GEFEN_F16 && a.row_grad && threadIdx.x == 0))
+            ex = -half_exponent(a.meta->top[threadIdx.x]);
         if (a.row_grad) {
-            f *= a.meta->grad_max;
+            ex += grad_exponent(a.meta->grad_max, a.carry);
         } else {
             if (a.grad) f *= *a.grad;
             if (a.mean) f = a.meta->count ? f / (float)a.meta->count : 0.0f;
         }
-        a.meta->factor[threadIdx.x] = f;
+        a.meta->factor[threadIdx.x] = ldexpf(f, ex);
     }
     if (r >= rows) {
         if (a.zero_rows && r < a.most) {
@@ -596,10 +654,7 @@ __global__ __launch_bounds__(kGradThreads) void k_gradient_rows(const Rows a) {
     }
     if (!a.g) return;
     float w = F16 ? kHalfScale : 1.0f;
-    if (a.row_grad) {
-        const float g = a.row_grad[n], top = a.meta->grad_max;
-        w *= top == 0.0f ? 0.0f : g / top;
-    }
+    if (a.row_grad) w *= row_weight(a.row_grad[n], a.meta->grad_max, a.carry).w;
     const float unit = e > 0.0f ? e / (float)a.v : 0.0f;
     if (y < 0) w = NAN;
     // the target's entry from its own logit: p - 1 without cancellation in 16 bits
@@ -686,7 +741,15 @@ struct Grad {
     int32_t first;          // piece of the sum
     void* out;
     int32_t dtype;
+    const float* row_grad;  // dh: gradient of each row's loss (null: one for all)
+    int32_t carry;
 };
+// What the sums of an output row are multiplied by.
+template <typename C>
+__device__ __forceinline__ float factor_of(const Grad& g, float factor, int64_t row) {
+    if (C::BMN || !g.row_grad) return factor;  // dW; one gradient for all rows
+    return ldexpf(factor, -row_weight(g.row_grad[row], g.meta->grad_max, g.carry).rest);
+}
 
 // How the tiles of a product meet the chip: whole rounds of it tile by tile, and the
 // `rest` of the tiles with K cut into `cuts` equal parts, each left in float32 for k_join.
@@ -789,10 +852,11 @@ __device__ __forceinline__ void finish_tile(const Grad& g, int n_all, int m0, in
     for (int j = 0; j < C::WJ; ++j) {
         if (n0 + j * 16 + (lane & 15) >= n_all) continue;
         const int64_t row = rows[j];
+        const float f = factor_of<C>(g, factor, row);
         if constexpr (OUT == kOut16) {
 #pragma unroll
             for (int i = 0; i < C::WI; i += 2) {
-                const uint4 v = eight_rows(round16<C::F16>(acc[i][j], factor), round16<C::F16>(acc[i + 1][j], factor));
+                const uint4 v = eight_rows(round16<C::F16>(acc[i][j], f), round16<C::F16>(acc[i + 1][j], f));
                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
                 const int m = m0 + 16 * (i + (lane >> 5)) + 8 * (lane >> 4 & 1);
                 if (m < g.d) store16<8>(g, row, m, g.d - m, w);
@@ -801,7 +865,7 @@ __device__ __forceinline__ void finish_tile(const Grad& g, int n_all, int m0, in
 #pragma unroll
             for (int i = 0; i < C::WI; ++i) {
                 const int m = m0 + i * 16 + 4 * (lane >> 4);
-                if (m < g.d) finish_f32<OUT>(g, row, m, min(4, g.d - m), acc[i][j], factor);
+                if (m < g.d) finish_f32<OUT>(g, row, m, min(4, g.d - m), acc[i][j], f);
             }
         }
     }
@@ -909,12 +973,13 @@ __device__ __forceinline__ void join_block(const Grad& g, int t) {
             v = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
             const int64_t row = g.dh ? g.map[g.from + n] : n;
             const int cnt = min(4, g.d - m);
+            const float f = factor_of<C>(g, factor, row);
             if (g.sum) {
-                finish_f32<kOutSum>(g, row, m, cnt, v, factor);
+                finish_f32<kOutSum>(g, row, m, cnt, v, f);
             } else if (C::F16 && g.dtype == GEFEN_F32) {
-                finish_f32<kOutF32>(g, row, m, cnt, v, factor);
+                finish_f32<kOutF32>(g, row, m, cnt, v, f);
             } else {
-                const uint2 r = round16<C::F16>(v, factor);
+                const uint2 r = round16<C::F16>(v, f);
                 const uint32_t w[2] = {r.x, r.y};
                 store16<4>(g, row, m, cnt, w);
             }
@@ -1226,6 +1291,8 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     uint16_t* wp = reinterpret_cast<uint16_t*>(ws + p.o_w);
     uint16_t* gbuf = reinterpret_cast<uint16_t*>(ws + p.o_g);
     const bool by_row = p.backward && t.reduction == GEFEN_REDUCE_NONE;
+    const bool shift = by_row && p.dw && p.halves;
+    const int carry = !p.halves ? kCarryAll : p.planes == 2 ? kCarryTwo : kCarryOne;
 
     const Select sel{t.targets, t.targets_int32, p.n, p.v, t.ignore_index, by_row ? t.grad : nullptr, map, tgt, meta,
                      !p.forward};
@@ -1245,6 +1312,8 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     pk.meta = meta;
     pk.which = 0;
     pk.zero_losses = losses;
+    pk.row_grad = by_row ? t.grad : nullptr;
+    pk.carry = carry;
     Pack pw{};
     pw.src = t.weight;
     pw.row_stride = t.weight_row_stride;
@@ -1260,6 +1329,9 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     pw.which = 1;
     const int pack_x = (int)grid_of(x_rows * (p.dp / 8), 8192);
     const int pack_w = p.pack_w ? (int)grid_of(p.v * (p.dp / 8), 8192) : 0;
+    const int64_t per = (p.d + 7) / 8;
+    const Top tx{t.hidden, t.hidden_row_stride, t.hidden_col_stride, p.n, p.d, map, meta, 0, t.dtype == GEFEN_F16};
+    const int top_x = (int)grid_of(p.n * per / 4, kTopGrid);
     if (!p.forward) {
         if (by_row) hipLaunchKernelGGL(k_rows, dim3(1), dim3(kRowsThreads), 0, st, sel);
     } else if (p.n <= kSelfRows && !pk.f32) {
@@ -1267,15 +1339,14 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     } else {
         hipLaunchKernelGGL(k_rows, dim3(1), dim3(kRowsThreads), 0, st, sel);
         if (pk.f32) {
-            const int64_t per = (p.d + 7) / 8;
-            const Top tx{static_cast<const float*>(t.hidden), t.hidden_row_stride, t.hidden_col_stride, p.n, p.d, map, meta, 0};
-            const Top tw{static_cast<const float*>(t.weight), t.weight_row_stride, t.weight_col_stride, p.v, p.d, nullptr,
-                         meta, 1};
-            const int top_x = (int)grid_of(p.n * per / 4, kTopGrid), top_w = (int)grid_of(p.v * per / 4, kTopGrid);
+            const Top tw{t.weight, t.weight_row_stride, t.weight_col_stride, p.v, p.d, nullptr, meta, 1, 0};
+            const int top_w = (int)grid_of(p.v * per / 4, kTopGrid);
             hipLaunchKernelGGL(k_top, dim3((unsigned)(top_x + top_w)), dim3(kTopThreads), 0, st, tx, tw, top_x);
         }
         hipLaunchKernelGGL(k_pack, dim3((unsigned)(pack_x + pack_w)), dim3(256), 0, st, pk, pw, pack_x);
     }
+    if (shift && !pk.f32)
+        hipLaunchKernelGGL(k_top, dim3((unsigned)top_x), dim3(kTopThreads), 0, st, tx, tx, top_x);
     Operand w{};
     w.p = p.pack_w ? wp : static_cast<const uint16_t*>(t.weight);
     w.ld = p.pack_w ? p.dp : t.weight_row_stride;
@@ -1333,6 +1404,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
             r.grad = by_row ? nullptr : t.grad;
             r.mean = t.reduction == GEFEN_REDUCE_MEAN;
             r.dtype = t.dtype;
+            r.carry = carry;
             r.losses = losses;
             r.g = p.backward ? l.g : nullptr;
             r.ldg = p.ldg;
@@ -1356,6 +1428,11 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
             auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kGradThreads), 0, st, r); };
             if (f16) stream_past ? launch(k_gradient_rows<true, true>) : launch(k_gradient_rows<true, false>);
             else stream_past ? launch(k_gradient_rows<false, true>) : launch(k_gradient_rows<false, false>);
+            if (shift) {
+                pk.from = from;
+                pk.most = most;
+                hipLaunchKernelGGL(k_shift, dim3(grid_of(most * (p.dp / 8), 8192)), dim3(256), 0, st, pk);
+            }
         }
         if (!p.backward) continue;
         Operand go{};
@@ -1387,6 +1464,8 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         h.n = most;
         h.steps = (p.v + 63) / 64;
         h.out = t.grad_hidden;
+        h.row_grad = by_row ? t.grad : nullptr;
+        h.carry = carry;
         wg.parts = reinterpret_cast<float*>(ws + p.o_dw_parts);
         wg.most_parts = p.dw_parts;
         wg.slots = slots_of(p.dw_big);
