@@ -84,6 +84,7 @@ SIGNATURES = {
     "gefen_linear_cross_entropy_workspace_size": (SZ, [P]),
     "gefen_linear_cross_entropy": (I32, [P, P, SZ, P]),
     "gefen_scale_by": (I32, [P, I64, P, I64, I32, P, P]),
+    "gefen_scale_from_f32": (I32, [P, P, I64, P, P, I64, I32, P, P]),
 }
 
 # numpy mirror of struct gefen_step_task / gefen_muon_task (natural C alignment)
@@ -123,13 +124,14 @@ class LinearCrossEntropyTask(ctypes.Structure):
     _fields_ += [(name, I64) for name in ("n", "v", "d", "hidden_row_stride", "hidden_col_stride",
                                           "weight_row_stride", "weight_col_stride", "ignore_index",
                                           "workspace_limit")]
-    _fields_ += [("label_smoothing", DBL), ("dtype", I32), ("targets_int32", I32), ("reduction", I32), ("stage", I32)]
+    _fields_ += [("label_smoothing", DBL), ("dtype", I32), ("targets_int32", I32), ("reduction", I32), ("stage", I32),
+                 ("grads_f32", I32), ("reserved", I32)]
 
 
 REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2
 STEP_SUMMARY = np.dtype([("launches", np.int32), ("shared", np.int32), ("small", np.int32), ("tables", np.int32)])
 assert PERIOD_TASK.itemsize == 40 and HISTOGRAM_TASK.itemsize == 32
-assert GRADIENT_TASK.itemsize == 32 and ctypes.sizeof(LinearCrossEntropyTask) == 160
+assert GRADIENT_TASK.itemsize == 32 and ctypes.sizeof(LinearCrossEntropyTask) == 168
 assert STEP_TASK.itemsize == 128 and MUON_TASK.itemsize == 72 and MUON_APPLY_TASK.itemsize == 56
 
 _LIB = None

@@ -258,6 +258,19 @@ __global__ __launch_bounds__(kThreads) void k_scale_by(T* a, int64_t na, T* b, i
     }
 }
 
+// Float32 a and b times *factor into a_out and b_out.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_scale_from(const float* a, T* a_out, int64_t na, const float* b, T* b_out,
+                                                         int64_t nb, const float* __restrict__ factor) {
+    const float f = *factor;
+    const int64_t ca = (na + kChunk - 1) / kChunk, cb = (nb + kChunk - 1) / kChunk;
+    for (int64_t c = blockIdx.x; c < ca + cb; c += gridDim.x) {
+        const bool first = c < ca;
+        const int64_t at = (first ? c : c - ca) * kChunk, left = (first ? na : nb) - at;
+        scale_chunk<true>((first ? a : b) + at, (first ? a_out : b_out) + at, left < kChunk ? (int)left : kChunk, f);
+    }
+}
+
 int64_t chunks_of(const gefen_gradient_task& t) { return (t.numel + kChunk - 1) / kChunk; }
 
 // The launches of a call: tables of up to kTable tensors and 2^30 chunks, empty tensors left out.
@@ -466,4 +479,27 @@ extern "C" int gefen_scale_by(void* a, int64_t a_numel, void* b, int64_t b_numel
         hipLaunchKernelGGL(k_scale_by<f16_t>, grid, wg, 0, stream, static_cast<f16_t*>(a), a_numel,
                            static_cast<f16_t*>(b), b_numel, factor);
     return launch_status("gefen_scale_by");
+}
+
+extern "C" int gefen_scale_from_f32(const float* a, void* a_out, int64_t a_numel, const float* b, void* b_out,
+                                    int64_t b_numel, int dtype, const float* factor, gefen_stream_t stream) {
+    const char* what = "gefen_scale_from_f32";
+    if (!valid_dtype(dtype)) return fail_inval("%s: unknown dtype %d", what, dtype);
+    if (a_numel < 0 || b_numel < 0 || (a_numel && (!a || !a_out)) || (b_numel && (!b || !b_out)) || !factor)
+        return fail_inval("%s: null pointer or negative size", what);
+    const int size = dtype_size(dtype);
+    if (!aligned(a, 4) || !aligned(b, 4) || !aligned(a_out, size) || !aligned(b_out, size))
+        return fail_inval("%s: not aligned to its elements", what);
+    const int64_t chunks = (a_numel + kChunk - 1) / kChunk + (b_numel + kChunk - 1) / kChunk;
+    if (!chunks) return GEFEN_OK;
+    const dim3 grid((unsigned)(chunks < kGrid ? chunks : kGrid)), wg(kThreads);
+    auto launch = [&](auto type) {
+        using T = decltype(type);
+        hipLaunchKernelGGL(k_scale_from<T>, grid, wg, 0, stream, a, static_cast<T*>(a_out), a_numel, b,
+                           static_cast<T*>(b_out), b_numel, factor);
+    };
+    if (dtype == GEFEN_F32) launch(0.0f);
+    else if (dtype == GEFEN_BF16) launch(bf16_t{});
+    else launch(f16_t{});
+    return launch_status(what);
 }

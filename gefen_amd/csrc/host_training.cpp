@@ -36,6 +36,7 @@ struct Library {
     decltype(&gefen_linear_cross_entropy_workspace_size) lce_workspace;
     decltype(&gefen_linear_cross_entropy) lce;
     decltype(&gefen_scale_by) scale_by;
+    decltype(&gefen_scale_from_f32) scale_from_f32;
 };
 Library lib{};
 
@@ -49,6 +50,7 @@ void bind_library(py::dict addresses) {
         reinterpret_cast<decltype(lib.lce_workspace)>(at("gefen_linear_cross_entropy_workspace_size"));
     lib.lce = reinterpret_cast<decltype(lib.lce)>(at("gefen_linear_cross_entropy"));
     lib.scale_by = reinterpret_cast<decltype(lib.scale_by)>(at("gefen_scale_by"));
+    lib.scale_from_f32 = reinterpret_cast<decltype(lib.scale_from_f32)>(at("gefen_scale_from_f32"));
     lib.last_error = reinterpret_cast<decltype(lib.last_error)>(at("gefen_last_error"));
 }
 void need_library() {
@@ -194,76 +196,84 @@ struct LceOptions {
 float* floats(const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 void* data(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-// One library call on the current stream.  A forward stage keeps its workspace in *kept,
-// where all rows fit the limit together (else it is a whole call without gradients, and
-// *kept stays undefined); with *kept defined the call is the backward stage.
-void lce_call(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets, const LceOptions& o,
-              const at::Tensor& losses, const at::Tensor& loss, const at::Tensor& grad_hidden,
-              const at::Tensor& grad_weight, const at::Tensor& grad, at::Tensor* kept = nullptr) {
-    at::Tensor h = hidden.dim() == 2 ? hidden : hidden.reshape({-1, hidden.size(-1)});
-    at::Tensor y = targets.contiguous();
+// One library call, to be made on the current stream: the task, and what its addresses
+// belong to.
+struct LceCall {
+    at::Tensor h, y;
     gefen_linear_cross_entropy_task t{};
-    t.hidden = h.data_ptr();
-    t.weight = weight.data_ptr();
-    t.targets = y.data_ptr();
-    t.losses = floats(losses);
-    t.loss = floats(loss);
-    t.grad_hidden = data(grad_hidden);
-    t.grad_weight = data(grad_weight);
-    t.grad = floats(grad);
-    t.n = h.size(0);
-    t.v = weight.size(0);
-    t.d = weight.size(1);
-    t.hidden_row_stride = h.stride(0);
-    t.hidden_col_stride = h.stride(1);
-    t.weight_row_stride = weight.stride(0);
-    t.weight_col_stride = weight.stride(1);
-    t.ignore_index = o.ignore_index;
-    t.workspace_limit = o.workspace_limit;
-    t.label_smoothing = o.label_smoothing;
-    t.dtype = dtype_code(h);
-    t.targets_int32 = y.scalar_type() == at::kInt;
-    t.reduction = static_cast<int32_t>(o.reduction);
-    const bool backward = kept && kept->defined();
-    t.stage = backward ? GEFEN_LCE_BACKWARD : kept ? GEFEN_LCE_FORWARD : GEFEN_LCE_WHOLE;
-    size_t nbytes = lib.lce_workspace(&t);
-    const bool keep = kept && nbytes != 0;
-    if (kept && nbytes == 0 && !backward) {
-        t.stage = GEFEN_LCE_WHOLE;
-        nbytes = lib.lce_workspace(&t);
+
+    LceCall(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets, const LceOptions& o)
+        : h(hidden.dim() == 2 ? hidden : hidden.reshape({-1, hidden.size(-1)})), y(targets.contiguous()) {
+        t.hidden = h.data_ptr();
+        t.weight = weight.data_ptr();
+        t.targets = y.data_ptr();
+        t.n = h.size(0);
+        t.v = weight.size(0);
+        t.d = weight.size(1);
+        t.hidden_row_stride = h.stride(0);
+        t.hidden_col_stride = h.stride(1);
+        t.weight_row_stride = weight.stride(0);
+        t.weight_col_stride = weight.stride(1);
+        t.ignore_index = o.ignore_index;
+        t.workspace_limit = o.workspace_limit;
+        t.label_smoothing = o.label_smoothing;
+        t.dtype = dtype_code(h);
+        t.targets_int32 = y.scalar_type() == at::kInt;
+        t.reduction = static_cast<int32_t>(o.reduction);
     }
-    if (nbytes == 0) check(GEFEN_EINVAL);
-    at::Tensor ws = backward ? *kept : bytes_on(h, nbytes);
-    if (keep) *kept = ws;
-    check(lib.lce(&t, ws.data_ptr(), backward ? ws.numel() : nbytes, stream_of(h)));
+    // The bytes that the stage needs; 0 where it cannot be made.
+    size_t bytes(int stage) {
+        t.stage = stage;
+        return lib.lce_workspace(&t);
+    }
+    void form(const at::Tensor& grad_hidden, const at::Tensor& grad_weight) {
+        t.grad_hidden = data(grad_hidden);
+        t.grad_weight = data(grad_weight);
+        t.grads_f32 = (grad_hidden.defined() ? grad_hidden : grad_weight).scalar_type() == at::kFloat;
+    }
+    // The stage of the last bytes(), or (ws defined) a backward stage on what a forward one left.
+    at::Tensor run(size_t nbytes, at::Tensor ws = {}) {
+        if (nbytes == 0) check(GEFEN_EINVAL);
+        if (!ws.defined()) ws = bytes_on(h, nbytes);
+        check(lib.lce(&t, ws.data_ptr(), ws.numel(), stream_of(h)));
+        return ws;
+    }
+};
+
+at::Tensor empty_grad(const at::Tensor& like, bool wanted, at::ScalarType type) {
+    return wanted ? at::empty(like.sizes(), like.options().dtype(type).requires_grad(false)) : at::Tensor();
 }
 
-at::Tensor empty_grad(const at::Tensor& like, bool wanted) {
-    return wanted ? at::empty(like.sizes(), like.options().requires_grad(false)) : at::Tensor();
-}
-
-// The loss; gh, gw: the gradients where they are formed here (a reduced loss of bfloat16
-// or float32 operands).  Float16 ones wait for the loss's gradient, so that a loss scale
-// reaches them before they are rounded, and so do those of losses that are not reduced;
-// kept is then what they are formed from.
+// The loss, and for its backward pass one of
+//   * kept: what the gradients are formed from, where all rows fit the workspace limit
+//     together.  16-bit gradients wait, so that the loss's own gradient reaches them before
+//     they are rounded, and so do those of losses that are not reduced;
+//   * gh, gw: the gradients, in float32, of a reduced loss: float32 operands, and bfloat16
+//     ones in pieces;
+//   * nothing: they are formed from the operands.
 at::Tensor lce_forward(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
                        const LceOptions& o, bool need_h, bool need_w, at::Tensor* gh, at::Tensor* gw,
                        at::Tensor* kept) {
     c10::DeviceGuard guard(hidden.device());
     const auto f32 = hidden.options().dtype(at::kFloat).requires_grad(false);
-    if (o.reduction == GEFEN_REDUCE_NONE) {
-        at::Tensor losses = at::empty(targets.sizes(), f32);
-        lce_call(hidden, weight, targets, o, losses, {}, {}, {}, {}, need_h || need_w ? kept : nullptr);
-        return losses;
+    const bool reduced = o.reduction != GEFEN_REDUCE_NONE, need = need_h || need_w;
+    const at::ScalarType type = hidden.scalar_type();
+    LceCall c(hidden, weight, targets, o);
+    at::Tensor result = reduced ? at::empty({}, f32) : at::empty(targets.sizes(), f32);
+    (reduced ? c.t.loss : c.t.losses) = floats(result);
+    if (need && !(reduced && type == at::kFloat)) {
+        if (const size_t nbytes = c.bytes(GEFEN_LCE_FORWARD)) {
+            *kept = c.run(nbytes);
+            return result;
+        }
     }
-    at::Tensor loss = at::empty({}, f32);
-    const bool wait = hidden.scalar_type() == at::kHalf && (need_h || need_w);
-    if (!wait) {
-        *gh = empty_grad(hidden, need_h);
-        *gw = empty_grad(weight, need_w);
+    if (need && reduced && type != at::kHalf) {
+        *gh = empty_grad(hidden, need_h, at::kFloat);
+        *gw = empty_grad(weight, need_w, at::kFloat);
+        c.form(*gh, *gw);
     }
-    lce_call(hidden, weight, targets, o, {}, loss, *gh, *gw, {}, wait ? kept : nullptr);
-    return loss;
+    c.run(c.bytes(GEFEN_LCE_WHOLE));
+    return result;
 }
 
 class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> {
@@ -305,12 +315,19 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
                 if (need_w) gw = ctx->saved_data["gw"].toTensor();
                 ctx->saved_data.erase("gh");
                 ctx->saved_data.erase("gw");
-                const int rc = lib.scale_by(data(gh), need_h ? gh.numel() : 0, data(gw), need_w ? gw.numel() : 0,
-                                            dtype_code(hidden), grad.data_ptr<float>(), stream_of(hidden));
-                if (rc != GEFEN_OK) throw std::runtime_error(lib.last_error());
+                const int64_t nh = need_h ? gh.numel() : 0, nw = need_w ? gw.numel() : 0;
+                if (hidden.scalar_type() == at::kFloat) {
+                    check(lib.scale_by(data(gh), nh, data(gw), nw, GEFEN_F32, grad.data_ptr<float>(), stream_of(hidden)));
+                } else {
+                    const at::Tensor fh = gh, fw = gw;
+                    gh = empty_grad(hidden, need_h, hidden.scalar_type());
+                    gw = empty_grad(weight, need_w, hidden.scalar_type());
+                    check(lib.scale_from_f32(floats(fh), data(gh), nh, floats(fw), data(gw), nw, dtype_code(hidden),
+                                             grad.data_ptr<float>(), stream_of(hidden)));
+                }
             } else {
-                gh = empty_grad(hidden, need_h);
-                gw = empty_grad(weight, need_w);
+                gh = empty_grad(hidden, need_h, hidden.scalar_type());
+                gw = empty_grad(weight, need_w, hidden.scalar_type());
                 // used up by the call: a second backward starts from the operands
                 at::Tensor kept;
                 const auto at_kept = ctx->saved_data.find("kept");
@@ -318,10 +335,12 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
                     kept = at_kept->second.toTensor();
                     ctx->saved_data.erase("kept");
                 }
-                lce_call(hidden, weight, saved[2],
-                         {ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["workspace_limit"].toInt(),
-                          ctx->saved_data["label_smoothing"].toDouble(), ctx->saved_data["reduction"].toInt()},
-                         {}, {}, gh, gw, grad, kept.defined() ? &kept : nullptr);
+                LceCall c(hidden, weight, saved[2],
+                          {ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["workspace_limit"].toInt(),
+                           ctx->saved_data["label_smoothing"].toDouble(), ctx->saved_data["reduction"].toInt()});
+                c.form(gh, gw);
+                c.t.grad = grad.data_ptr<float>();
+                c.run(c.bytes(kept.defined() ? GEFEN_LCE_BACKWARD : GEFEN_LCE_WHOLE), kept);
             }
         }
         return {gh, gw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};

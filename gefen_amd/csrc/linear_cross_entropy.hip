@@ -738,9 +738,9 @@ struct Grad {
     int32_t most_parts;     // partial tiles that `parts` holds
     float* parts;           // [cut][tile of the rest][TN][TM]
     float* sum;             // float32 sum over the pieces (null: one piece)
-    int32_t first;          // piece of the sum
+    int32_t first, last;    // pieces of the sum (last: it is the output, in float32)
     void* out;
-    int32_t dtype;
+    int32_t out_f32;
     const float* row_grad;  // dh: gradient of each row's loss (null: one for all)
     int32_t carry;
 };
@@ -796,8 +796,8 @@ __device__ __forceinline__ int cuts_of(const Grad& g, const Deal& d) {
     return cuts;
 }
 
-// A result goes to the sum over the pieces (plain float32), or times the factor to the
-// output in its type.
+// A result goes to the sum over the pieces (plain float32 up to the last one of a float32
+// output), or times the factor to the output in its type.
 enum Out { kOutSum, kOutF32, kOut16 };
 // cnt (1 to 4) float32 results of output row `row`, from column m
 template <int OUT>
@@ -805,7 +805,10 @@ __device__ __forceinline__ void finish_f32(const Grad& g, int64_t row, int m, in
     const int64_t at = row * g.d + m;
     if constexpr (OUT == kOutSum) {
         float* s = g.sum + at;
-        for (int e = 0; e < cnt; ++e) s[e] = g.first ? v[e] : s[e] + v[e];
+        for (int e = 0; e < cnt; ++e) {
+            const float x = g.first ? v[e] : s[e] + v[e];
+            s[e] = g.last ? x * factor : x;
+        }
     } else {
         v *= factor;
         float* o = static_cast<float*>(g.out) + at;
@@ -905,7 +908,7 @@ __device__ __forceinline__ void grad_block(const Grad& g, int b, int workers, ld
                 for (int i = 0; i < C::WI; ++i) *reinterpret_cast<f32x4*>(p + j * 16 * C::TM + i * 16) = acc[i][j];
         } else if (g.sum) {
             finish_tile<C, kOutSum>(g, deal.n_all, unit.m0 + wm, unit.n0 + wn, factor, acc);
-        } else if (C::F16 && g.dtype == GEFEN_F32) {
+        } else if (g.out_f32) {
             finish_tile<C, kOutF32>(g, deal.n_all, unit.m0 + wm, unit.n0 + wn, factor, acc);
         } else {
             finish_tile<C, kOut16>(g, deal.n_all, unit.m0 + wm, unit.n0 + wn, factor, acc);
@@ -976,7 +979,7 @@ __device__ __forceinline__ void join_block(const Grad& g, int t) {
             const float f = factor_of<C>(g, factor, row);
             if (g.sum) {
                 finish_f32<kOutSum>(g, row, m, cnt, v, f);
-            } else if (C::F16 && g.dtype == GEFEN_F32) {
+            } else if (g.out_f32) {
                 finish_f32<kOutF32>(g, row, m, cnt, v, f);
             } else {
                 const uint2 r = round16<C::F16>(v, f);
@@ -997,7 +1000,7 @@ __global__ __launch_bounds__(256) void k_joins(const Grad h, const Grad w, int f
     else join_block<W>(w, blockIdx.x - first);
 }
 
-// dW from its float32 sum over the pieces.
+// 16-bit dW from its float32 sum over the pieces.
 template <bool F16>
 __global__ __launch_bounds__(256) void k_convert(const Grad g) {
     const int64_t all = ((int64_t)g.n * g.d + 3) / 4, numel = (int64_t)g.n * g.d;
@@ -1007,13 +1010,9 @@ __global__ __launch_bounds__(256) void k_convert(const Grad g) {
         f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
         const int cnt = (int)(numel - q * 4 < 4 ? numel - q * 4 : 4);
         for (int e = 0; e < cnt; ++e) v[e] = sum[q * 4 + e];
-        if (F16 && g.dtype == GEFEN_F32) {
-            for (int e = 0; e < cnt; ++e) static_cast<float*>(g.out)[q * 4 + e] = v[e] * factor;
-        } else {
-            for (int e = 0; e < cnt; ++e)
-                static_cast<uint16_t*>(g.out)[q * 4 + e] =
-                    F16 ? from_f32<f16_t>(v[e] * factor).bits : from_f32<bf16_t>(v[e] * factor).bits;
-        }
+        for (int e = 0; e < cnt; ++e)
+            static_cast<uint16_t*>(g.out)[q * 4 + e] =
+                F16 ? from_f32<f16_t>(v[e] * factor).bits : from_f32<bf16_t>(v[e] * factor).bits;
     }
 }
 
@@ -1047,6 +1046,7 @@ struct Plan {
     bool forward, backward;  // the stages that this call runs
     int planes;         // of G
     bool halves;        // products of half-precision operands
+    bool out_f32;       // gradients in float32
     int64_t dp, ldg;
     int rows, pieces;   // rows of a piece
     LogitsTile tile;
@@ -1136,6 +1136,7 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
     p->smooth = t.label_smoothing > 0.0;
     p->planes = t.dtype == GEFEN_F32 || t.n <= kTwoPlaneRows ? 2 : 1;
     p->halves = t.dtype != GEFEN_BF16;
+    p->out_f32 = t.dtype == GEFEN_F32 || t.grads_f32;
     p->dp = up(t.d, 64);
     p->ldg = up(t.v, kRowAlign);
     p->pack_w = t.dtype == GEFEN_F32 || t.d % 64 != 0 || t.weight_col_stride != 1 || t.weight_row_stride % 8 != 0 ||
@@ -1177,7 +1178,8 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
     p->o_stats = take((size_t)p->rows * p->slots * sizeof(float2));
     p->o_sums = p->smooth ? take((size_t)p->rows * p->slots * 4) : at;
     p->o_g = p->train ? take((size_t)p->planes * p->rows * p->ldg * 2) : at;
-    p->o_wsum = p->dw && p->pieces > 1 ? take((size_t)p->v * p->d * 4) : at;
+    // float32 gradients are their own sum over the pieces
+    p->o_wsum = p->dw && p->pieces > 1 && !p->out_f32 ? take((size_t)p->v * p->d * 4) : at;
     p->dh_parts = p->dh ? parts_of(tiles_of(t.d, n, p->dh_big), up(t.v, 64) / 64, segs, p->dh_big) : 0;
     p->dw_parts = p->dw ? parts_of(tiles_of(t.d, t.v, p->dw_big), up(n, 64) / 64, segs, p->dw_big) : 0;
     const size_t dh_bytes = (size_t)p->dh_parts * (p->dh_big ? 256 * 256 : 128 * 128) * 4;
@@ -1269,9 +1271,9 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     const int bad = make_plan(t, &p, what);
     if (bad) return bad;
     if (!t.weight || (t.n && (!t.hidden || !t.targets))) return fail_inval("%s: null input", what);
-    const int size = dtype_size(t.dtype);
-    if (!aligned(t.hidden, size) || !aligned(t.weight, size) || !aligned(t.grad_hidden, size) ||
-        !aligned(t.grad_weight, size) || !aligned(t.targets, t.targets_int32 ? 4 : 8))
+    const int size = dtype_size(t.dtype), grad_size = p.out_f32 ? 4 : 2;
+    if (!aligned(t.hidden, size) || !aligned(t.weight, size) || !aligned(t.grad_hidden, grad_size) ||
+        !aligned(t.grad_weight, grad_size) || !aligned(t.targets, t.targets_int32 ? 4 : 8))
         return fail_inval("%s: an operand is not aligned to its elements", what);
     if (t.n && !t.losses && !t.loss && !p.train) return fail_inval("%s: nothing to compute", what);
     if (t.loss && t.reduction == GEFEN_REDUCE_NONE) return fail_inval("%s: no reduction for a loss", what);
@@ -1416,7 +1418,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
             r.planes = p.planes;
             r.smoothing = (float)t.label_smoothing;
             r.zero_rows = p.backward ? t.grad_hidden : nullptr;
-            r.zero_bytes = (int64_t)p.d * size;
+            r.zero_bytes = (int64_t)p.d * grad_size;
             // a row per workgroup, or parts of it where the rows do not fill the chip
             const int64_t rows_up = p.backward ? up(most, 64) : most;
             int64_t parts = p.backward ? 2048 / rows_up : 1;
@@ -1449,7 +1451,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         g.most = most;
         g.map = map;
         g.meta = meta;
-        g.dtype = t.dtype;
+        g.out_f32 = p.out_f32;
         // the loss goes with the last launch of the last piece
         const bool last = piece == p.pieces - 1;
         Loss with{};
@@ -1473,8 +1475,11 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         wg.a.planes = w.planes;
         wg.dh = 0;
         wg.n = p.v;
-        wg.sum = p.pieces > 1 ? reinterpret_cast<float*>(ws + p.o_wsum) : nullptr;
+        wg.sum = p.pieces == 1 ? nullptr
+                 : p.out_f32   ? static_cast<float*>(t.grad_weight)
+                               : reinterpret_cast<float*>(ws + p.o_wsum);
         wg.first = piece == 0;
+        wg.last = last && p.out_f32;
         wg.out = t.grad_weight;
         if (p.pair) {
             if (f16) launch_grad_pair<true>(h, wg, with, st);
@@ -1488,7 +1493,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         if (p.dw) {
             if (f16) launch_grad_tile<true>(wg, p.dw_big, with, st);
             else launch_grad_tile<false>(wg, p.dw_big, with, st);
-            if (wg.sum && last) {
+            if (wg.sum && last && !p.out_f32) {
                 const dim3 grid(grid_of(((int64_t)p.v * p.d + 3) / 4, 8192));
                 if (f16) hipLaunchKernelGGL(k_convert<true>, grid, dim3(256), 0, st, wg);
                 else hipLaunchKernelGGL(k_convert<false>, grid, dim3(256), 0, st, wg);

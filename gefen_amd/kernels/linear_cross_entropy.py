@@ -7,12 +7,14 @@ The N x V logits never exist: the library keeps 16 bits per logit of a bounded p
 positions at a time (float32 operands: twice as many) and works on positions that have a
 loss only.
 
-With ``reduction`` "mean" or "sum" and bfloat16 or float32 operands the gradients are
-formed in the forward call, where the kept values still are (three products instead of
-four), and backward multiplies them by the loss's own gradient, which costs nothing when
-that is 1.  Float16 gradients are formed in backward, so that a loss scale reaches them
-before they are rounded, and so are those of ``reduction`` "none": the kept values wait for
-backward where all positions fit ``workspace_limit`` together, else they are formed again.
+16-bit gradients, and those of ``reduction`` "none", are formed in backward, so that the
+loss's own gradient (a loss scale, a share of a batch) reaches them before they are rounded:
+the kept values wait for backward where all positions fit ``workspace_limit`` together.  Where
+they do not, bfloat16 gradients of a reduced loss are formed in the forward call and wait in
+float32, and float16 ones and those of "none" take the logits' product again.  Float32
+operands with "mean" or "sum" have their gradients formed in the forward call (three products
+instead of four), and backward multiplies them by the loss's own gradient, which costs nothing
+when that is 1.
 """
 
 from __future__ import annotations
