@@ -88,20 +88,132 @@ py::object wrap(const at::Tensor& t) { return py::reinterpret_steal<py::object>(
 
 // ------------------------------------------------------------------ gradient norm
 
+// The bytes of a tensor's elements: runs of `block` bytes at begin + sum of index x stride.
+struct Layout {
+    struct Dim {
+        int64_t stride, lo, hi;  // bytes; the range of an index (or of the difference of two)
+    };
+    uint64_t begin;
+    int64_t block;
+    std::vector<Dim> dims;
+    explicit Layout(const at::Tensor& t)
+        : begin(reinterpret_cast<uint64_t>(t.data_ptr())), block(static_cast<int64_t>(t.element_size())) {
+        for (int64_t i = 0; i < t.dim(); ++i)
+            if (t.size(i) > 1) dims.push_back({t.stride(i) * block, 0, t.size(i) - 1});
+        std::sort(dims.begin(), dims.end(), [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
+        size_t inner = 0;  // dimensions that only continue the run
+        while (inner < dims.size() && dims[inner].stride == block) block *= dims[inner++].hi + 1;
+        dims.erase(dims.begin(), dims.begin() + inner);
+    }
+};
+// Whether at + sum of stride x index can lie within [least, most], with an index other than 0
+// if `apart`.  dims by descending stride: all but a few values of each index are ruled out by
+// what the smaller strides reach, so nested layouts take a few steps; one that takes too many
+// counts as reaching it.
+struct Reach {
+    std::vector<Layout::Dim> dims;
+    int64_t least, most;
+    int steps = 1 << 16;
+    std::vector<int64_t> lo, hi;  // reached by dims from k on
+    Reach(std::vector<Layout::Dim> all, int64_t least, int64_t most) : least(least), most(most) {
+        std::sort(all.begin(), all.end(),
+                  [](const Layout::Dim& a, const Layout::Dim& b) { return a.stride > b.stride; });
+        for (const Layout::Dim& d : all) {
+            if (!dims.empty() && dims.back().stride == d.stride) {
+                dims.back().lo += d.lo;
+                dims.back().hi += d.hi;
+            } else {
+                dims.push_back(d);
+            }
+        }
+        lo.assign(dims.size() + 1, 0);
+        hi = lo;
+        for (size_t k = dims.size(); k-- > 0;) {
+            lo[k] = lo[k + 1] + dims[k].stride * dims[k].lo;
+            hi[k] = hi[k + 1] + dims[k].stride * dims[k].hi;
+        }
+    }
+    static int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }
+    bool from(size_t k, int64_t at, bool apart) {
+        if (k == dims.size()) return !apart && at >= least && at <= most;
+        const Layout::Dim& d = dims[k];
+        const int64_t first = std::max(d.lo, -floor_div(at + hi[k + 1] - least, d.stride));
+        const int64_t last = std::min(d.hi, floor_div(most - at - lo[k + 1], d.stride));
+        for (int64_t c = first; c <= last; ++c) {
+            if (--steps < 0) return true;
+            if (from(k + 1, at + c * d.stride, apart && c == 0)) return true;
+        }
+        return false;
+    }
+};
+bool share_memory(const Layout& a, const Layout& b) {
+    std::vector<Layout::Dim> dims;  // an expanded dimension adds no memory
+    for (const Layout::Dim& d : a.dims)
+        if (d.stride) dims.push_back(d);
+    for (const Layout::Dim& d : b.dims)
+        if (d.stride) dims.push_back({d.stride, -d.hi, 0});
+    const int64_t apart = static_cast<int64_t>(a.begin - b.begin);
+    return Reach(std::move(dims), 1 - a.block, b.block - 1).from(0, apart, false);
+}
+// Whether two elements of a tensor lie in the same memory.
+bool overlaps_itself(const at::Tensor& t) {
+    if (t.is_contiguous() || t.is_non_overlapping_and_dense()) return false;
+    Layout l(t);
+    std::vector<Layout::Dim> dims;
+    for (size_t k = 0; k < l.dims.size(); ++k) {
+        const Layout::Dim& d = l.dims[k];
+        if (d.stride == 0 || (k > 0 && d.stride == l.dims[k - 1].stride)) return true;
+        dims.push_back({d.stride, -d.hi, d.hi});
+    }
+    return Reach(std::move(dims), 1 - l.block, l.block - 1).from(0, 0, true);
+}
+
+// What a call reads and writes: raises where something written shares memory with anything
+// else, before anything is launched.
+class Accesses {
+   public:
+    void add(const at::Tensor& t, bool write) {
+        if (t.numel() == 0) return;
+        if (write && overlaps_itself(t))
+            throw py::value_error("Expected gradients to write whose elements do not overlap.");
+        int64_t extent = static_cast<int64_t>(t.element_size());
+        for (int64_t i = 0; i < t.dim(); ++i) extent += (t.size(i) - 1) * t.stride(i) * t.element_size();
+        const uint64_t begin = reinterpret_cast<uint64_t>(t.data_ptr());
+        spans_.push_back({begin, begin + extent, write, &t});
+    }
+    void check() {
+        std::sort(spans_.begin(), spans_.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+        std::vector<const Span*> open;  // those that reach past the current one's begin
+        uint64_t reach = 0;
+        for (const Span& s : spans_) {
+            if (s.begin >= reach) open.clear();
+            for (const Span* o : open)
+                if ((s.write || o->write) && s.begin < o->end && share_memory(Layout(*o->t), Layout(*s.t)))
+                    throw py::value_error("Expected gradients that share no memory with what is written.");
+            open.push_back(&s);
+            reach = std::max(reach, s.end);
+        }
+    }
+
+   private:
+    struct Span {
+        uint64_t begin, end;
+        bool write;
+        const at::Tensor* t;
+    };
+    std::vector<Span> spans_;
+};
+
 // The tasks of a list of gradients (and the list that receives them scaled; None: in
 // place).  bad: the first tensor whose elements are not one dense run, in the same order
 // in both, or -1.  Raises for what no call takes, and, with `writes`, where what is
-// written overlaps anything else of the call.
+// written overlaps anything else of the call (total_norm, if given, among it).
 struct Tasks {
     std::vector<gefen_gradient_task> rows;
     at::Tensor first;
     int64_t bad = -1;
 };
-Tasks tasks_of(const py::list& tensors, const py::object& outs, bool writes) {
-    struct Span {
-        uint64_t begin, end;
-        bool write;
-    };
+Tasks tasks_of(const py::list& tensors, const py::object& outs, bool writes, const at::Tensor* total_norm = nullptr) {
     Tasks out;
     const size_t n = tensors.size();
     const bool in_place = outs.is_none();
@@ -118,7 +230,7 @@ Tasks tasks_of(const py::list& tensors, const py::object& outs, bool writes) {
         if (dtype_code(t) < 0) throw py::value_error("Expected float32, float16 or bfloat16 gradients.");
         return t;
     };
-    std::vector<Span> spans;
+    Accesses accesses;
     out.rows.resize(n);
     for (size_t k = 0; k < n; ++k) {
         const at::Tensor& t = tensor_at(tensors, k);
@@ -127,30 +239,21 @@ Tasks tasks_of(const py::list& tensors, const py::object& outs, bool writes) {
         r.numel = t.numel();
         r.src_dtype = r.dst_dtype = dtype_code(t);
         bool dense = t.is_contiguous() || t.is_non_overlapping_and_dense();
+        if (in_place && writes) accesses.add(t, true);
         if (!in_place) {
             const at::Tensor& o = tensor_at(out_list, k);
             if (o.sizes() != t.sizes()) throw py::value_error("Expected outputs of the gradients' shapes.");
             r.dst = o.data_ptr();
             r.dst_dtype = dtype_code(o);
-            dense = dense && (o.strides() == t.strides() || (o.is_contiguous() && t.is_contiguous()));
+            const bool same_order = o.strides() == t.strides() || (o.is_contiguous() && t.is_contiguous());
+            dense = dense && same_order;
+            accesses.add(o, true);
+            if (r.dst != r.src || r.dst_dtype != r.src_dtype || !same_order) accesses.add(t, false);
         }
         if (!dense && r.numel && out.bad < 0) out.bad = static_cast<int64_t>(k);
-        if (writes && r.numel && dense) {
-            const int64_t size[] = {4, 2, 2};
-            const uint64_t src = reinterpret_cast<uint64_t>(r.src), dst = reinterpret_cast<uint64_t>(r.dst);
-            const uint64_t src_end = src + r.numel * size[r.src_dtype], dst_end = dst + r.numel * size[r.dst_dtype];
-            spans.push_back({dst, dst_end, true});
-            if (dst != src || dst_end != src_end) spans.push_back({src, src_end, false});
-        }
     }
-    std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
-    uint64_t read_end = 0, write_end = 0;
-    for (const Span& s : spans) {
-        if (s.begin < write_end || (s.write && s.begin < read_end))
-            throw py::value_error("Expected gradients that share no memory with what is written.");
-        uint64_t& end = s.write ? write_end : read_end;
-        end = std::max(end, s.end);
-    }
+    if (total_norm) accesses.add(*total_norm, false);
+    accesses.check();
     return out;
 }
 
@@ -170,13 +273,13 @@ py::object gradient_norm(py::list tensors, double norm_type) {
 // Clips (by total_norm, or the norm of these gradients) and returns the norm; None as above.
 py::object clip_gradients(py::list tensors, py::object outs, double max_norm, double norm_type, py::object total_norm) {
     need_library();
-    Tasks t = tasks_of(tensors, outs, true);
+    const at::Tensor* given = total_norm.is_none() ? nullptr : &tensor_of(total_norm, "total_norm");
+    Tasks t = tasks_of(tensors, outs, true, given);
     if (t.bad >= 0) return py::none();
     const int n = static_cast<int>(t.rows.size());
     c10::DeviceGuard guard(t.first.device());
-    if (!total_norm.is_none()) {
-        const at::Tensor& norm = tensor_of(total_norm, "total_norm");
-        check(lib.scale(t.rows.data(), n, norm.data_ptr<float>(), max_norm, stream_of(t.first)));
+    if (given) {
+        check(lib.scale(t.rows.data(), n, given->data_ptr<float>(), max_norm, stream_of(t.first)));
         return total_norm;
     }
     at::Tensor norm = at::empty({}, t.first.options().dtype(at::kFloat).requires_grad(false));
