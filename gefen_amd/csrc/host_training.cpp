@@ -210,8 +210,15 @@ class Accesses {
 // written overlaps anything else of the call (total_norm, if given, among it).
 struct Tasks {
     std::vector<gefen_gradient_task> rows;
+    std::vector<const at::Tensor*> written;
     at::Tensor first;
     int64_t bad = -1;
+    // Autograd's count of in-place writes, for what it has saved; the kernels write through
+    // addresses, which it does not see.
+    void count_writes() const {
+        for (const at::Tensor* t : written)
+            if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    }
 };
 Tasks tasks_of(const py::list& tensors, const py::object& outs, bool writes, const at::Tensor* total_norm = nullptr) {
     Tasks out;
@@ -239,9 +246,13 @@ Tasks tasks_of(const py::list& tensors, const py::object& outs, bool writes, con
         r.numel = t.numel();
         r.src_dtype = r.dst_dtype = dtype_code(t);
         bool dense = t.is_contiguous() || t.is_non_overlapping_and_dense();
-        if (in_place && writes) accesses.add(t, true);
+        if (in_place && writes) {
+            accesses.add(t, true);
+            out.written.push_back(&t);
+        }
         if (!in_place) {
             const at::Tensor& o = tensor_at(out_list, k);
+            out.written.push_back(&o);
             if (o.sizes() != t.sizes()) throw py::value_error("Expected outputs of the gradients' shapes.");
             r.dst = o.data_ptr();
             r.dst_dtype = dtype_code(o);
@@ -280,11 +291,13 @@ py::object clip_gradients(py::list tensors, py::object outs, double max_norm, do
     c10::DeviceGuard guard(t.first.device());
     if (given) {
         check(lib.scale(t.rows.data(), n, given->data_ptr<float>(), max_norm, stream_of(t.first)));
+        t.count_writes();
         return total_norm;
     }
     at::Tensor norm = at::empty({}, t.first.options().dtype(at::kFloat).requires_grad(false));
     at::Tensor ws = bytes_on(t.first, lib.norm_workspace(t.rows.data(), n));
     check(lib.clip(t.rows.data(), n, norm_type, max_norm, norm.data_ptr<float>(), ws.data_ptr(), stream_of(norm)));
+    t.count_writes();
     return wrap(norm);
 }
 
