@@ -251,7 +251,8 @@ class PlanCore {
     }
 
     // The advanced step counts of the last successful prepare(): each state's
-    // "step" entry and steps_out (n int64 slots).
+    // "step" entry and steps_out (n int64 slots).  The parameters' versions count the write
+    // (the kernels write through addresses, which autograd does not see).
     void commit(uintptr_t steps_out) {
         int64_t* steps = reinterpret_cast<int64_t*>(steps_out);
         // one int object per distinct step count, shared by the state dicts that take it
@@ -270,6 +271,8 @@ class PlanCore {
             committed_[k] = step_[k];
             if (rc != 0) throw py::error_already_set();
             steps[k] = step_[k];
+            const at::Tensor& p = THPVariable_Unpack(params_[k].ptr());
+            if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
         }
     }
 

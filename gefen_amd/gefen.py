@@ -29,6 +29,7 @@ from typing import Dict, Iterable, List, Optional, Tuple, Union
 import numpy as np
 import torch
 import torch.nn as nn
+from torch.autograd.graph import increment_version
 
 from gefen_amd import _lib
 from gefen_amd import quantization as quantization_module
@@ -449,8 +450,8 @@ def _plan_checks_python(plan, opt):
     """The checks of PlanCore.refresh (gefen_amd/csrc/host_plan.cpp) in Python, for
     a plan with params, pptr, numel, gdtype, grads, gptr, states, state_keys,
     srefs and dev_index (used when the host extension is not built): fills plan.gptr and
-    returns the advanced step counts, or None (changing nothing) when the plan no
-    longer applies."""
+    returns the advanced step counts (the parameters' versions are counted too), or None
+    (changing nothing) when the plan no longer applies."""
     params, pptr, numel, gdtype, grads, gptr = plan.params, plan.pptr, plan.numel, plan.gdtype, plan.grads, plan.gptr
     n = len(params)
     dev = plan.dev_index
@@ -486,6 +487,7 @@ def _plan_checks_python(plan, opt):
         step = st["step"] + 1
         st["step"] = step
         steps.append(step)
+    increment_version(params)  # the launches that follow write them
     return steps
 
 
@@ -508,6 +510,13 @@ def _kernel_weight_decay(lr, weight_decay):
     if not (lr_v > 0.0 and np.isfinite(f) and f != 0.0):
         return None
     return (1.0 - float(f)) / lr_v
+
+
+def _count_writes(items) -> None:
+    """Counts a version of every parameter of (group, param, local param, grad) items, as
+    torch's in-place operations do: the kernels write through addresses, which autograd
+    does not see."""
+    increment_version([t for it in items for t in ((it[1],) if it[2] is it[1] else (it[1], it[2]))])
 
 
 def _distinct(objs):
@@ -986,6 +995,7 @@ class Gefen(torch.optim.Optimizer):
             rc = lib.gefen_step_tasks(tasks.ctypes.data, len(items), tables.data_ptr(),
                                       torch.cuda.current_stream(dev).cuda_stream)
         _lib.check(rc, "gefen_step_tasks")
+        _count_writes(items)
         for local_p, fused_p in copy_back:
             local_p.copy_(fused_p)
         del keep

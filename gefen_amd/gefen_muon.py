@@ -19,8 +19,8 @@ import torch
 import torch.nn as nn
 
 from gefen_amd import _lib
-from gefen_amd.gefen import (Gefen, _DTYPE_CODE, _distinct, _gefen_host, _plan_checks_python, _step_entry,
-                             _kernel_weight_decay, automatic_partition_view)
+from gefen_amd.gefen import (Gefen, _DTYPE_CODE, _count_writes, _distinct, _gefen_host, _kernel_weight_decay,
+                             _plan_checks_python, _step_entry, automatic_partition_view)
 
 EPS = 1e-7
 _SUMSQ_STRIDE = 128  # GEFEN_SUMSQ_STRIDE (include/gefen_hip.h): sum-of-squares entries per momentum task
@@ -291,6 +291,7 @@ class GefenMuon(Gefen):
         with torch.cuda.device(dev):
             rc = lib.gefen_muon_apply_tasks(rest.ctypes.data, len(rest), torch.cuda.current_stream(dev).cuda_stream)
         _lib.check(rc, "gefen_muon_apply_tasks")
+        _count_writes(items)
         for local_p, target in copy_back:
             local_p.copy_(target)
         plain = (not copy_back

@@ -3,12 +3,14 @@
 Same names, argument order, checks and exception types as the reference
 wrappers (automatic_gefen_fused.py:10-489); the work runs in libgefen_hip.so on
 torch's current HIP stream.  The arithmetic is the reference's CPU path, so the
-indices and magnitudes these write equal the ``fused=False`` optimizer's.
+indices and magnitudes these write equal the ``fused=False`` optimizer's.  A
+parameter that is written counts a version, as torch's in-place operations do.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .gefen_hip import check, device_guard, dtype_code, load_extension, stream_of
 
@@ -88,6 +90,7 @@ def automatic_gefen_fused_update_cuda(p, grad_view, m_sign, m_magnitude, stepsiz
             dtype_code(m_magnitude.dtype), st.data_ptr(), cb.data_ptr(), cb.numel(), int(bool(packed_indices)),
             g.shape[0], g.shape[1], float(beta1), float(lr), stream_of(p))
     check(rc, "automatic_gefen_fused_update_cuda")
+    increment_version(p)
 
 
 def automatic_gefen_fused_update_from_vmean_cuda(p, grad_view, m_sign, m_magnitude, vmean, codebook,
@@ -127,6 +130,7 @@ def automatic_gefen_fused_update_from_vmean_cuda(p, grad_view, m_sign, m_magnitu
             int(bool(packed_indices)), g.shape[0], g.shape[1], float(beta1), float(lr),
             float(bias_correction_1), float(bias_correction_2), float(eps), stream_of(p))
     check(rc, "automatic_gefen_fused_update_from_vmean_cuda")
+    increment_version(p)
 
 
 def automatic_gefen_period1_update_cuda(p, grad_flat, m_sign, m_magnitude, vmean, codebook,
@@ -188,6 +192,7 @@ def automatic_gefen_period1_update_cuda(p, grad_flat, m_sign, m_magnitude, vmean
             g.numel(), period_one_divisor, float(beta1), float(beta2), float(lr), float(bias_correction_1),
             float(bias_correction_2), float(eps), stream_of(p))
     check(rc, "automatic_gefen_period1_update_cuda")
+    increment_version(p)
 
 
 def automatic_gefen_muon_momentum_cuda(grad_view, m_sign, m_magnitude, codebook, momentum_update,
