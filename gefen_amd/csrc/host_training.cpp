@@ -13,6 +13,7 @@
 #include <pybind11/pybind11.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <ATen/ATen.h>
 #include <algorithm>
@@ -82,6 +83,14 @@ const at::Tensor& tensor_of(py::handle o, const char* name) {
     if (!THPVariable_Check(o.ptr()))
         throw py::type_error(std::string("Expected ") + name + " to be a torch.Tensor, got " + Py_TYPE(o.ptr())->tp_name);
     return THPVariable_Unpack(o.ptr());
+}
+
+// Raises for a forward-mode tangent, which a call on addresses would drop.
+void no_tangent(const at::Tensor& t, const char* name) {
+    const auto* meta = torch::autograd::impl::get_autograd_meta(t);
+    if (!meta || !meta->fw_grad(/*level=*/0, t).defined()) return;
+    PyErr_Format(PyExc_NotImplementedError, "Expected %s without a forward-mode tangent.", name);
+    throw py::error_already_set();
 }
 
 py::object wrap(const at::Tensor& t) { return py::reinterpret_steal<py::object>(THPVariable_Wrap(t)); }
@@ -235,6 +244,7 @@ Tasks tasks_of(const py::list& tensors, const py::object& outs, bool writes, con
         if (t.device() != out.first.device()) throw py::value_error("Expected all gradients on one device.");
         if (t.layout() != at::kStrided) throw py::value_error("Expected strided gradients.");
         if (dtype_code(t) < 0) throw py::value_error("Expected float32, float16 or bfloat16 gradients.");
+        no_tangent(t, "gradients");
         return t;
     };
     Accesses accesses;
@@ -487,6 +497,8 @@ py::object linear_cross_entropy(py::handle hidden_, py::handle weight_, py::hand
     on_device(hidden, "hidden");
     on_device(weight, "weight");
     on_device(targets, "targets");
+    no_tangent(hidden, "hidden");
+    no_tangent(weight, "weight");
     if (dtype_code(hidden) < 0)
         throw py::value_error(std::string("Expected hidden to be float32, float16 or bfloat16, got ") +
                               c10::toString(hidden.scalar_type()));
