@@ -166,7 +166,7 @@ bool share_memory(const Layout& a, const Layout& b) {
 }
 // Whether two elements of a tensor lie in the same memory.
 bool overlaps_itself(const at::Tensor& t) {
-    if (t.is_contiguous() || t.is_non_overlapping_and_dense()) return false;
+    if (t.is_non_overlapping_and_dense()) return false;
     Layout l(t);
     std::vector<Layout::Dim> dims;
     for (size_t k = 0; k < l.dims.size(); ++k) {
@@ -181,12 +181,17 @@ bool overlaps_itself(const at::Tensor& t) {
 // else, before anything is launched.
 class Accesses {
    public:
+    explicit Accesses(size_t most) { spans_.reserve(most); }
     void add(const at::Tensor& t, bool write) {
         if (t.numel() == 0) return;
-        if (write && overlaps_itself(t))
-            throw py::value_error("Expected gradients to write whose elements do not overlap.");
-        int64_t extent = static_cast<int64_t>(t.element_size());
-        for (int64_t i = 0; i < t.dim(); ++i) extent += (t.size(i) - 1) * t.stride(i) * t.element_size();
+        const int64_t size = static_cast<int64_t>(t.itemsize());
+        int64_t extent = t.numel() * size;
+        if (!t.is_contiguous()) {
+            if (write && overlaps_itself(t))
+                throw py::value_error("Expected gradients to write whose elements do not overlap.");
+            extent = size;
+            for (int64_t i = 0; i < t.dim(); ++i) extent += (t.size(i) - 1) * t.stride(i) * size;
+        }
         const uint64_t begin = reinterpret_cast<uint64_t>(t.data_ptr());
         spans_.push_back({begin, begin + extent, write, &t});
     }
@@ -247,7 +252,7 @@ Tasks tasks_of(const py::list& tensors, const py::object& outs, bool writes, con
         no_tangent(t, "gradients");
         return t;
     };
-    Accesses accesses;
+    Accesses accesses(writes ? 2 * n + 1 : 0);
     out.rows.resize(n);
     for (size_t k = 0; k < n; ++k) {
         const at::Tensor& t = tensor_at(tensors, k);
