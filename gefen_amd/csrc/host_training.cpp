@@ -18,6 +18,7 @@
 #include <ATen/ATen.h>
 #include <algorithm>
 #include <cstdint>
+#include <cstring>
 #include <stdexcept>
 #include <string>
 #include <vector>
@@ -379,7 +380,7 @@ at::Tensor empty_grad(const at::Tensor& like, bool wanted, at::ScalarType type) 
 //   * kept: what the gradients are formed from, where all rows fit the workspace limit
 //     together.  16-bit gradients wait, so that the loss's own gradient reaches them before
 //     they are rounded, and so do those of losses that are not reduced;
-//   * gh, gw: the gradients, in float32, of a reduced loss: float32 operands, and bfloat16
+//   * gh, gw: the gradients, in float32, of a reduced loss: of float32 operands, and bfloat16
 //     ones in pieces or small (kFormSmall);
 //   * nothing: they are formed from the operands.
 // Elements of bfloat16 gradients up to which they are formed in the forward call: rounding
@@ -420,62 +421,58 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
         at::Tensor gh, gw, kept;
         at::Tensor result = lce_forward(hidden, weight, targets, {ignore_index, workspace_limit, label_smoothing, reduction},
                                         need_h, need_w, &gh, &gw, &kept);
-        ctx->save_for_backward({hidden, weight, targets});
-        ctx->saved_data["ignore_index"] = ignore_index;
-        ctx->saved_data["workspace_limit"] = workspace_limit;
-        ctx->saved_data["label_smoothing"] = label_smoothing;
-        ctx->saved_data["reduction"] = reduction;
-        ctx->saved_data["need_h"] = need_h;
-        ctx->saved_data["need_w"] = need_w;
-        ctx->saved_data["formed"] = gh.defined() || gw.defined();
-        if (gh.defined()) ctx->saved_data["gh"] = gh;
-        if (gw.defined()) ctx->saved_data["gw"] = gw;
-        if (kept.defined()) ctx->saved_data["kept"] = kept;
+        // what waits for backward is saved as the operands are: hooks of saved tensors see it
+        ctx->save_for_backward({hidden, weight, targets, gh, gw, kept});
+        int64_t smoothing;
+        std::memcpy(&smoothing, &label_smoothing, 8);
+        ctx->saved_data["options"] =
+            std::vector<int64_t>{ignore_index, workspace_limit, smoothing, reduction, need_h, need_w};
         return result;
     }
 
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                    torch::autograd::variable_list grads) {
         TORCH_CHECK(!c10::GradMode::is_enabled(), "linear_cross_entropy can be differentiated once only");
-        const bool need_h = ctx->saved_data["need_h"].toBool(), need_w = ctx->saved_data["need_w"].toBool();
         at::Tensor gh, gw;
         if (grads[0].defined()) {
+            const std::vector<int64_t> o = ctx->saved_data["options"].toIntVector();
+            const bool need_h = o[4], need_w = o[5];
             const auto saved = ctx->get_saved_variables();
-            const at::Tensor &hidden = saved[0], &weight = saved[1];
+            const at::Tensor &hidden = saved[0], &weight = saved[1], &formed_h = saved[3], &formed_w = saved[4];
+            const at::ScalarType type = hidden.scalar_type();
             c10::DeviceGuard guard(hidden.device());
             const at::Tensor grad = grads[0].to(at::kFloat).contiguous();
-            if (ctx->saved_data["formed"].toBool()) {
-                // handed over: a second backward of a retained graph forms them again
-                ctx->saved_data["formed"] = false;
-                if (need_h) gh = ctx->saved_data["gh"].toTensor();
-                if (need_w) gw = ctx->saved_data["gw"].toTensor();
-                ctx->saved_data.erase("gh");
-                ctx->saved_data.erase("gw");
-                const int64_t nh = need_h ? gh.numel() : 0, nw = need_w ? gw.numel() : 0;
-                if (hidden.scalar_type() == at::kFloat) {
-                    check(lib.scale_by(data(gh), nh, data(gw), nw, GEFEN_F32, grad.data_ptr<float>(), stream_of(hidden)));
+            const float* factor = grad.data_ptr<float>();
+            // kept values are used up by the call and float32 gradients handed over: a second
+            // backward of a retained graph starts from the operands
+            const bool used = ctx->saved_data.count("used");
+            const bool formed = formed_h.defined() || formed_w.defined();
+            if (formed && !used) {
+                const int64_t nh = need_h ? formed_h.numel() : 0, nw = need_w ? formed_w.numel() : 0;
+                if (type == at::kFloat) {
+                    ctx->saved_data["used"] = true;
+                    gh = formed_h;
+                    gw = formed_w;
+                    check(lib.scale_by(data(gh), nh, data(gw), nw, GEFEN_F32, factor, stream_of(hidden)));
                 } else {
-                    const at::Tensor fh = gh, fw = gw;
-                    gh = empty_grad(hidden, need_h, hidden.scalar_type());
-                    gw = empty_grad(weight, need_w, hidden.scalar_type());
-                    check(lib.scale_from_f32(floats(fh), data(gh), nh, floats(fw), data(gw), nw, dtype_code(hidden),
-                                             grad.data_ptr<float>(), stream_of(hidden)));
+                    gh = empty_grad(hidden, need_h, type);
+                    gw = empty_grad(weight, need_w, type);
+                    check(lib.scale_from_f32(floats(formed_h), data(gh), nh, floats(formed_w), data(gw), nw,
+                                             dtype_code(hidden), factor, stream_of(hidden)));
                 }
             } else {
-                gh = empty_grad(hidden, need_h, hidden.scalar_type());
-                gw = empty_grad(weight, need_w, hidden.scalar_type());
-                // used up by the call: a second backward starts from the operands
+                gh = empty_grad(hidden, need_h, type);
+                gw = empty_grad(weight, need_w, type);
                 at::Tensor kept;
-                const auto at_kept = ctx->saved_data.find("kept");
-                if (at_kept != ctx->saved_data.end()) {
-                    kept = at_kept->second.toTensor();
-                    ctx->saved_data.erase("kept");
+                if (!used && saved[5].defined()) {
+                    ctx->saved_data["used"] = true;
+                    kept = saved[5];
                 }
-                LceCall c(hidden, weight, saved[2],
-                          {ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["workspace_limit"].toInt(),
-                           ctx->saved_data["label_smoothing"].toDouble(), ctx->saved_data["reduction"].toInt()});
+                double smoothing;
+                std::memcpy(&smoothing, &o[2], 8);
+                LceCall c(hidden, weight, saved[2], {o[0], o[1], smoothing, o[3]});
                 c.form(gh, gw);
-                c.t.grad = grad.data_ptr<float>();
+                c.t.grad = factor;
                 c.run(c.bytes(kept.defined() ? GEFEN_LCE_BACKWARD : GEFEN_LCE_WHOLE), kept);
             }
         }
