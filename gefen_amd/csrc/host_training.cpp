@@ -358,10 +358,10 @@ struct LceCall {
         t.stage = stage;
         return lib.lce_workspace(&t);
     }
-    void form(const at::Tensor& grad_hidden, const at::Tensor& grad_weight) {
-        t.grad_hidden = data(grad_hidden);
-        t.grad_weight = data(grad_weight);
-        t.grads_f32 = (grad_hidden.defined() ? grad_hidden : grad_weight).scalar_type() == at::kFloat;
+    void form(void* grad_hidden, void* grad_weight, bool f32) {
+        t.grad_hidden = grad_hidden;
+        t.grad_weight = grad_weight;
+        t.grads_f32 = f32;
     }
     // The stage of the last bytes(), or (ws defined) a backward stage on what a forward one left.
     at::Tensor run(size_t nbytes, at::Tensor ws = {}) {
@@ -380,16 +380,24 @@ at::Tensor empty_grad(const at::Tensor& like, bool wanted, at::ScalarType type) 
 //   * kept: what the gradients are formed from, where all rows fit the workspace limit
 //     together.  16-bit gradients wait, so that the loss's own gradient reaches them before
 //     they are rounded, and so do those of losses that are not reduced;
-//   * gh, gw: the gradients, in float32, of a reduced loss: of float32 operands, and bfloat16
-//     ones in pieces or small (kFormSmall);
+//   * gh, gw: the gradients of a reduced loss of float32 operands;
+//   * formed: those of bfloat16 ones in pieces or small (kFormSmall), in float32, hidden's
+//     first (Formed);
 //   * nothing: they are formed from the operands.
 // Elements of bfloat16 gradients up to which they are formed in the forward call: rounding
 // them from float32 moves 8 bytes an element more, and keeping values takes two launches more,
 // 8 us (48 x 1000 x 96: 36 us on the device against 44).
 constexpr int64_t kFormSmall = 4 << 20;
+struct Formed {
+    int64_t nh, nw, at_w, numel;
+    Formed(const at::Tensor& hidden, const at::Tensor& weight, bool need_h, bool need_w)
+        : nh(need_h ? hidden.numel() : 0), nw(need_w ? weight.numel() : 0), at_w((nh + 63) / 64 * 64), numel(at_w + nw) {}
+    float* hidden(const at::Tensor& t) const { return nh ? t.data_ptr<float>() : nullptr; }
+    float* weight(const at::Tensor& t) const { return nw ? t.data_ptr<float>() + at_w : nullptr; }
+};
 at::Tensor lce_forward(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
                        const LceOptions& o, bool need_h, bool need_w, at::Tensor* gh, at::Tensor* gw,
-                       at::Tensor* kept) {
+                       at::Tensor* formed, at::Tensor* kept) {
     c10::DeviceGuard guard(hidden.device());
     const auto f32 = hidden.options().dtype(at::kFloat).requires_grad(false);
     const bool reduced = o.reduction != GEFEN_REDUCE_NONE, need = need_h || need_w;
@@ -404,10 +412,14 @@ at::Tensor lce_forward(const at::Tensor& hidden, const at::Tensor& weight, const
             return result;
         }
     }
-    if (need && reduced && type != at::kHalf) {
-        *gh = empty_grad(hidden, need_h, at::kFloat);
-        *gw = empty_grad(weight, need_w, at::kFloat);
-        c.form(*gh, *gw);
+    if (need && reduced && type == at::kFloat) {
+        *gh = empty_grad(hidden, need_h, type);
+        *gw = empty_grad(weight, need_w, type);
+        c.form(data(*gh), data(*gw), true);
+    } else if (need && reduced && type == at::kBFloat16) {
+        const Formed f(hidden, weight, need_h, need_w);
+        *formed = at::empty({f.numel}, f32);
+        c.form(f.hidden(*formed), f.weight(*formed), true);
     }
     c.run(c.bytes(GEFEN_LCE_WHOLE));
     return result;
@@ -418,11 +430,11 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& hidden, const at::Tensor& weight,
                               const at::Tensor& targets, int64_t ignore_index, int64_t workspace_limit,
                               double label_smoothing, int64_t reduction, bool need_h, bool need_w) {
-        at::Tensor gh, gw, kept;
+        at::Tensor gh, gw, formed, kept;
         at::Tensor result = lce_forward(hidden, weight, targets, {ignore_index, workspace_limit, label_smoothing, reduction},
-                                        need_h, need_w, &gh, &gw, &kept);
+                                        need_h, need_w, &gh, &gw, &formed, &kept);
         // what waits for backward is saved as the operands are: hooks of saved tensors see it
-        ctx->save_for_backward({hidden, weight, targets, gh, gw, kept});
+        ctx->save_for_backward({hidden, weight, targets, gh, gw, formed, kept});
         int64_t smoothing;
         std::memcpy(&smoothing, &label_smoothing, 8);
         ctx->saved_data["options"] =
@@ -438,7 +450,7 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
             const std::vector<int64_t> o = ctx->saved_data["options"].toIntVector();
             const bool need_h = o[4], need_w = o[5];
             const auto saved = ctx->get_saved_variables();
-            const at::Tensor &hidden = saved[0], &weight = saved[1], &formed_h = saved[3], &formed_w = saved[4];
+            const at::Tensor &hidden = saved[0], &weight = saved[1], &formed = saved[5];
             const at::ScalarType type = hidden.scalar_type();
             c10::DeviceGuard guard(hidden.device());
             const at::Tensor grad = grads[0].to(at::kFloat).contiguous();
@@ -446,34 +458,32 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
             // kept values are used up by the call and float32 gradients handed over: a second
             // backward of a retained graph starts from the operands
             const bool used = ctx->saved_data.count("used");
-            const bool formed = formed_h.defined() || formed_w.defined();
-            if (formed && !used) {
-                const int64_t nh = need_h ? formed_h.numel() : 0, nw = need_w ? formed_w.numel() : 0;
-                if (type == at::kFloat) {
-                    ctx->saved_data["used"] = true;
-                    gh = formed_h;
-                    gw = formed_w;
-                    check(lib.scale_by(data(gh), nh, data(gw), nw, GEFEN_F32, factor, stream_of(hidden)));
-                } else {
-                    gh = empty_grad(hidden, need_h, type);
-                    gw = empty_grad(weight, need_w, type);
-                    check(lib.scale_from_f32(floats(formed_h), data(gh), nh, floats(formed_w), data(gw), nw,
-                                             dtype_code(hidden), factor, stream_of(hidden)));
-                }
+            if (type == at::kFloat && !used && (saved[3].defined() || saved[4].defined())) {
+                ctx->saved_data["used"] = true;
+                gh = saved[3];
+                gw = saved[4];
+                check(lib.scale_by(data(gh), need_h ? gh.numel() : 0, data(gw), need_w ? gw.numel() : 0, GEFEN_F32, factor,
+                                   stream_of(hidden)));
             } else {
                 gh = empty_grad(hidden, need_h, type);
                 gw = empty_grad(weight, need_w, type);
-                at::Tensor kept;
-                if (!used && saved[5].defined()) {
-                    ctx->saved_data["used"] = true;
-                    kept = saved[5];
+                if (formed.defined()) {
+                    const Formed f(hidden, weight, need_h, need_w);
+                    check(lib.scale_from_f32(f.hidden(formed), data(gh), f.nh, f.weight(formed), data(gw), f.nw,
+                                             dtype_code(hidden), factor, stream_of(hidden)));
+                } else {
+                    at::Tensor kept;
+                    if (!used && saved[6].defined()) {
+                        ctx->saved_data["used"] = true;
+                        kept = saved[6];
+                    }
+                    double smoothing;
+                    std::memcpy(&smoothing, &o[2], 8);
+                    LceCall c(hidden, weight, saved[2], {o[0], o[1], smoothing, o[3]});
+                    c.form(data(gh), data(gw), false);
+                    c.t.grad = factor;
+                    c.run(c.bytes(kept.defined() ? GEFEN_LCE_BACKWARD : GEFEN_LCE_WHOLE), kept);
                 }
-                double smoothing;
-                std::memcpy(&smoothing, &o[2], 8);
-                LceCall c(hidden, weight, saved[2], {o[0], o[1], smoothing, o[3]});
-                c.form(gh, gw);
-                c.t.grad = factor;
-                c.run(c.bytes(kept.defined() ? GEFEN_LCE_BACKWARD : GEFEN_LCE_WHOLE), kept);
             }
         }
         return {gh, gw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
@@ -529,9 +539,9 @@ py::object linear_cross_entropy(py::handle hidden_, py::handle weight_, py::hand
     if (need_h || need_w)
         return wrap(LinearCrossEntropy::apply(hidden, weight, targets, ignore_index, workspace_limit, label_smoothing,
                                               reduction, need_h, need_w));
-    at::Tensor gh, gw, kept;
     return wrap(lce_forward(hidden.detach(), weight.detach(), targets,
-                            {ignore_index, workspace_limit, label_smoothing, reduction}, false, false, &gh, &gw, &kept));
+                            {ignore_index, workspace_limit, label_smoothing, reduction}, false, false, nullptr, nullptr,
+                            nullptr, nullptr));
 }
 
 }  // namespace
