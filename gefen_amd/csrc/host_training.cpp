@@ -94,6 +94,10 @@ void no_tangent(const at::Tensor& t, const char* name) {
     throw py::error_already_set();
 }
 
+// A tensor whose memory holds its values: a view that stands for the negative of its memory
+// (the imaginary part of a conjugate) is copied.
+at::Tensor as_stored(const at::Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 py::object wrap(const at::Tensor& t) { return py::reinterpret_steal<py::object>(THPVariable_Wrap(t)); }
 
 // ------------------------------------------------------------------ gradient norm
@@ -221,7 +225,7 @@ class Accesses {
 
 // The tasks of a list of gradients (and the list that receives them scaled; None: in
 // place).  bad: the first tensor whose elements are not one dense run, in the same order
-// in both, or -1.  Raises for what no call takes, and, with `writes`, where what is
+// in both, or not what its memory holds, or -1.  Raises for what no call takes, and, with `writes`, where what is
 // written overlaps anything else of the call (total_norm, if given, among it).
 struct Tasks {
     std::vector<gefen_gradient_task> rows;
@@ -261,7 +265,7 @@ Tasks tasks_of(const py::list& tensors, const py::object& outs, bool writes, con
         r.src = r.dst = t.data_ptr();
         r.numel = t.numel();
         r.src_dtype = r.dst_dtype = dtype_code(t);
-        bool dense = t.is_contiguous() || t.is_non_overlapping_and_dense();
+        bool dense = !t.is_neg() && (t.is_contiguous() || t.is_non_overlapping_and_dense());
         if (in_place && writes) {
             accesses.add(t, true);
             out.written.push_back(&t);
@@ -273,7 +277,7 @@ Tasks tasks_of(const py::list& tensors, const py::object& outs, bool writes, con
             r.dst = o.data_ptr();
             r.dst_dtype = dtype_code(o);
             const bool same_order = o.strides() == t.strides() || (o.is_contiguous() && t.is_contiguous());
-            dense = dense && same_order;
+            dense = dense && same_order && !o.is_neg();
             accesses.add(o, true);
             if (r.dst != r.src || r.dst_dtype != r.src_dtype || !same_order) accesses.add(t, false);
         }
@@ -306,7 +310,8 @@ py::object clip_gradients(py::list tensors, py::object outs, double max_norm, do
     const int n = static_cast<int>(t.rows.size());
     c10::DeviceGuard guard(t.first.device());
     if (given) {
-        check(lib.scale(t.rows.data(), n, given->data_ptr<float>(), max_norm, stream_of(t.first)));
+        const at::Tensor norm = as_stored(*given);
+        check(lib.scale(t.rows.data(), n, norm.data_ptr<float>(), max_norm, stream_of(t.first)));
         t.count_writes();
         return total_norm;
     }
@@ -331,21 +336,23 @@ void* data(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 // One library call, to be made on the current stream: the task, and what its addresses
 // belong to.
 struct LceCall {
-    at::Tensor h, y;
+    at::Tensor h, w, y;
     gefen_linear_cross_entropy_task t{};
 
     LceCall(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets, const LceOptions& o)
-        : h(hidden.dim() == 2 ? hidden : hidden.reshape({-1, hidden.size(-1)})), y(targets.contiguous()) {
+        : h(as_stored(hidden.dim() == 2 ? hidden : hidden.reshape({-1, hidden.size(-1)}))),
+          w(as_stored(weight)),
+          y(targets.contiguous()) {
         t.hidden = h.data_ptr();
-        t.weight = weight.data_ptr();
+        t.weight = w.data_ptr();
         t.targets = y.data_ptr();
         t.n = h.size(0);
-        t.v = weight.size(0);
-        t.d = weight.size(1);
+        t.v = w.size(0);
+        t.d = w.size(1);
         t.hidden_row_stride = h.stride(0);
         t.hidden_col_stride = h.stride(1);
-        t.weight_row_stride = weight.stride(0);
-        t.weight_col_stride = weight.stride(1);
+        t.weight_row_stride = w.stride(0);
+        t.weight_col_stride = w.stride(1);
         t.ignore_index = o.ignore_index;
         t.workspace_limit = o.workspace_limit;
         t.label_smoothing = o.label_smoothing;

@@ -45,12 +45,12 @@ def _as_list(tensors, name: str) -> List[torch.Tensor]:
 
 
 def _dense(grads: List[torch.Tensor], out: Optional[List[torch.Tensor]] = None):
-    """Contiguous stand-ins for tensors that are not one dense run of elements, and the
-    (destination, stand-in) pairs to copy back."""
+    """Contiguous stand-ins for tensors that are not one dense run of elements, or stand for
+    the negative of their memory, and the (destination, stand-in) pairs to copy back."""
     src, dst, back = list(grads), list(grads if out is None else out), []
     for k, (g, o) in enumerate(zip(grads, dst)):
-        if not (g.is_contiguous() and o.is_contiguous()):
-            src[k], dst[k] = g.contiguous(), torch.empty(g.shape, dtype=o.dtype, device=g.device)
+        if not (g.is_contiguous() and o.is_contiguous()) or g.is_neg() or o.is_neg():
+            src[k], dst[k] = g.resolve_neg().contiguous(), torch.empty(g.shape, dtype=o.dtype, device=g.device)
             back.append((o, dst[k]))
     return src, dst, back
 
