@@ -30,10 +30,11 @@
 //
 // A half-precision G is scaled by 2^15 (and its products by 2^-15), which keeps
 // probabilities down to 1e-9 out of half's subnormals.  float32 runs as two half planes
-// per operand and three products, each matrix scaled by the power of two that brings its
-// largest finite element to 2^14: elements keep 22 bits down to 2^-28 of the largest
-// one, and what they keep ends at 2^-49 of it (2^-50 for G, whose largest is 1), at five
-// times the rate of the float32 matrix instructions.
+// per operand and three products, weight scaled by the power of two that brings its
+// largest finite element to 2^14 and each row of hidden by its own: elements keep 22 bits
+// down to 2^-28 of the largest one, and what they keep ends at 2^-49 of it (2^-50 for G,
+// whose largest is 1), at five times the rate of the float32 matrix instructions.  dW sums
+// rows, and takes all of hidden at one scale.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -235,8 +236,8 @@ __device__ __forceinline__ RowWeight row_weight(float c, float top, int carry) {
 }
 
 // meta->top[which] = the largest finite magnitude of a float32 or half matrix, as the bits
-// of a float32; with a map, of the rows that take part.  Maxima of integers: any order gives
-// the same.
+// of a float32; with a map, of the rows that take part (rows: each one's own too).  Maxima
+// of integers: any order gives the same.
 struct Top {
     const void* src;
     int64_t row_stride, col_stride;
@@ -244,6 +245,7 @@ struct Top {
     const int32_t* map;
     Meta* meta;
     int32_t which, f16;
+    uint32_t* rows;  // [n] (may be null)
 };
 constexpr int kTopThreads = 1024, kTopGrid = 256;
 // the largest finite magnitude of up to eight columns of a row
@@ -263,20 +265,30 @@ __device__ __forceinline__ uint32_t top_of_chunk(const T* s, int64_t col_stride,
     }
     return top;
 }
-// Workgroups up to `first` take a, the others b.
-__global__ __launch_bounds__(kTopThreads) void k_top(const Top a, const Top b, int first) {
-    const bool is_a = (int)blockIdx.x < first;
-    const Top& t = is_a ? a : b;
-    const int block = is_a ? blockIdx.x : blockIdx.x - first, blocks = is_a ? first : gridDim.x - first;
-    const uint32_t per = (uint32_t)(t.d + 7) / 8;  // chunks of eight columns a row
-    const int64_t all = (int64_t)(t.map ? t.meta->count : t.n) * per;
+__device__ __forceinline__ uint32_t top_of_chunk(const Top& t, int r, int c) {
+    const int64_t at = (int64_t)(t.map ? t.map[r] : r) * t.row_stride + c * t.col_stride;
+    return t.f16 ? top_of_chunk(static_cast<const f16_t*>(t.src) + at, t.col_stride, t.d - c)
+                 : top_of_chunk(static_cast<const float*>(t.src) + at, t.col_stride, t.d - c);
+}
+__device__ __forceinline__ void top_block(const Top& t, int block, int blocks) {
+    const int per = (t.d + 7) / 8;  // chunks of eight columns a row
+    const int rows = t.map ? t.meta->count : t.n;
     uint32_t top = 0;
-    for (int64_t q = (int64_t)block * kTopThreads + threadIdx.x; q < all; q += (int64_t)blocks * kTopThreads) {
-        const int64_t r = q / per;
-        const int c = (int)(q - r * per) * 8;
-        const int64_t at = (int64_t)(t.map ? t.map[r] : r) * t.row_stride + c * t.col_stride;
-        top = max(top, t.f16 ? top_of_chunk(static_cast<const f16_t*>(t.src) + at, t.col_stride, t.d - c)
-                             : top_of_chunk(static_cast<const float*>(t.src) + at, t.col_stride, t.d - c));
+    if (t.rows) {  // a row per wave
+        constexpr int kWaves = kTopThreads / 64;
+        for (int r = block * kWaves + (threadIdx.x >> 6); r < rows; r += blocks * kWaves) {
+            uint32_t own = 0;
+            for (int c = threadIdx.x & 63; c < per; c += 64) own = max(own, top_of_chunk(t, r, c * 8));
+            own = wave_group_max_u32(own, 64);
+            if ((threadIdx.x & 63) == 0) t.rows[r] = own;
+            top = max(top, own);
+        }
+    } else {
+        const int64_t all = (int64_t)rows * per;
+        for (int64_t q = (int64_t)block * kTopThreads + threadIdx.x; q < all; q += (int64_t)blocks * kTopThreads) {
+            const int r = (int)(q / per);
+            top = max(top, top_of_chunk(t, r, (int)(q - (int64_t)r * per) * 8));
+        }
     }
     // one atomic per workgroup, and few of those: on one address each takes 12 ns
     __shared__ uint32_t part[kTopThreads / 64];
@@ -288,11 +300,18 @@ __global__ __launch_bounds__(kTopThreads) void k_top(const Top a, const Top b, i
         if (top > 0) atomicMax(&t.meta->top[t.which], top);
     }
 }
+// Workgroups up to `first` take a, the others b.
+__global__ __launch_bounds__(kTopThreads) void k_top(const Top a, const Top b, int first) {
+    if ((int)blockIdx.x < first) top_block(a, blockIdx.x, first);
+    else top_block(b, blockIdx.x - first, gridDim.x - first);
+}
 
 // Bound by HBM: 8192 x 4096 bf16 rows in 28 us (4.8 TB/s), 50257 x 768 float32 ones and
 // their three planes in 60 (6.4).
 // Rows of a matrix of any strides as the products read them: dp = D rounded up to 64
-// columns, zero-padded, one plane or those of a float32 operand, scaled.  With a map: row
+// columns, zero-padded, one plane or those of a float32 operand, scaled: weight by its largest
+// element, hidden row by row, so that no row's logits depend on the size of another (for dW,
+// which sums rows, all by the largest: k_shift).  With a map: row
 // r is src row map[r] for r < meta->count and zero up to the next multiple of kRowAlign,
 // and the rows that take no part get a zero loss.  A thread moves eight columns of a row.
 constexpr int kPackPlanes = 3;  // of a float32 operand: high, low, high where finite
@@ -308,7 +327,9 @@ struct Pack {
     const Meta* meta;
     int32_t which;      // float32: whose largest magnitude in meta->top
     float* zero_losses;  // [n] (may be null)
-    // SHIFT: rows [from, from + most) that take part again, times their gradients' powers of two
+    const uint32_t* row_top;  // float32 hidden: largest magnitude of each row
+    // SHIFT: rows [from, from + most) that take part again, scaled by the largest element of
+    // all, times their gradients' powers of two (if they have their own)
     const float* row_grad;
     int32_t from, most, carry;
 };
@@ -328,7 +349,8 @@ __device__ __forceinline__ void pack_block(const Pack& p, const int32_t* map, in
         const int64_t row = map && r < p.n ? map[r] : r;
         const bool live = r < count;
         int ex = top;
-        if (SHIFT) ex -= row_weight(p.row_grad[row], p.meta->grad_max, p.carry).rest;
+        if (SHIFT && p.row_grad) ex -= row_weight(p.row_grad[row], p.meta->grad_max, p.carry).rest;
+        if (!SHIFT && p.row_top && live) ex = half_exponent(p.row_top[r]);
         if (map && !live && r < p.n && p.zero_losses && c0 == 0) p.zero_losses[row] = 0.0f;
         if (r >= ends) continue;
         Vec<uint16_t, 8> out[kPackPlanes] = {};
@@ -376,7 +398,8 @@ __global__ __launch_bounds__(256) void k_pack(const Pack x, const Pack w, int fi
     if ((int)blockIdx.x < first) pack_block(x, x.map, x.meta->count, blockIdx.x, first);
     else pack_block(w, nullptr, w.n, blockIdx.x - first, gridDim.x - first);
 }
-// Hidden of half-precision products as dW of per-row gradients reads it.
+// Hidden of half-precision products as dW reads it, where its rows are scaled one by one or
+// have gradients of their own.
 __global__ __launch_bounds__(256) void k_shift(const Pack x) {
     pack_block<true>(x, x.map, x.meta->count, blockIdx.x, gridDim.x);
 }
@@ -409,7 +432,8 @@ struct Logits {
     const Meta* meta;
     uint16_t* g;        // [row][ldg] exp(l - slot maximum), packed or in two planes (null: loss only)
     int64_t ldg, g_plane;
-    int32_t planes, f32;
+    int32_t planes;
+    const uint32_t* row_top;  // float32: largest magnitude of each row of hidden, over all pieces (or null)
 };
 
 // What a logits' product keeps for the gradients: nothing, 16 packed bits, two planes.
@@ -426,13 +450,14 @@ __device__ __forceinline__ void logits_tile(const Logits& a, int rows, int m0, i
     const int slot = wm / kSlot;
     static_assert(C::WM == kSlot, "a wave's columns are a slot");
     if (wm >= a.v && KEEP == kKeepNone) return;
-    const bool f32 = KEEP != kKeepPacked && a.f32;
+    const bool f32 = KEEP != kKeepPacked && a.row_top;
     const bool part = wm + C::WM > a.v;  // the last columns end inside this wave's
-    int target[WJ];  // loaded first: among the stores below each would wait for those before it
+    int target[WJ], down[WJ];  // loaded first: among the stores below each would wait for those before it
 #pragma unroll
     for (int j = 0; j < WJ; ++j) {
         const int n = wn + j * 16 + (lane & 15);
         target[j] = n < rows ? a.tgt[a.from + n] - wm : -1;
+        down[j] = f32 && n < rows ? ex - half_exponent(a.row_top[a.from + n]) : 0;
     }
 #pragma unroll
     for (int j = 0; j < WJ; ++j) {
@@ -442,7 +467,7 @@ __device__ __forceinline__ void logits_tile(const Logits& a, int rows, int m0, i
         for (int i = 0; i < WI; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                if (f32) acc[i][j][r] = ldexpf(acc[i][j][r], ex);
+                if (f32) acc[i][j][r] = ldexpf(acc[i][j][r], down[j]);
                 if (part && wm + i * 16 + hi + r >= a.v) acc[i][j][r] = -INFINITY;
                 m = fmaxf(m, acc[i][j][r]);  // skips NaN, which the sum of exp keeps
             }
@@ -524,7 +549,7 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
     const int tiles_n = (rows + C::TN - 1) / C::TN;
     const int live = tiles_n * a.tiles_m;
     if ((int)blockIdx.x >= live) return;
-    const int ex = a.f32 ? -half_exponent(a.meta->top[0]) - half_exponent(a.meta->top[1]) : 0;
+    const int ex = a.row_top ? -half_exponent(a.meta->top[1]) : 0;  // of weight
     auto unit_of = [&](int u) __attribute__((always_inline)) {
         int ti, tj;
         tile_of<C::GROUP_M>(logical_block(u, live), a.tiles_m, tiles_n, &ti, &tj);
@@ -1055,7 +1080,7 @@ struct Plan {
     bool pair;          // both gradients' products in one launch
     int dh_parts, dw_parts;
     // byte offsets into the workspace
-    size_t o_meta, o_map, o_tgt, o_tlogit, o_losses, o_x, o_w, o_stats, o_sums, o_g, o_wsum, o_parts, o_dw_parts, bytes;
+    size_t o_meta, o_map, o_tgt, o_tlogit, o_losses, o_xtop, o_x, o_w, o_stats, o_sums, o_g, o_wsum, o_parts, o_dw_parts, bytes;
 };
 
 // Workgroups that fill the chip: one with a big tile or two with a small one per CU.
@@ -1173,6 +1198,7 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
     p->o_tgt = take(n_up * 4);
     p->o_tlogit = take(n_up * 4);
     p->o_losses = take(n_up * 4);
+    p->o_xtop = t.dtype == GEFEN_F32 ? take(n_up * 4) : at;
     p->o_x = take((size_t)in_planes * p->rows * p->pieces * p->dp * 2);
     p->o_w = p->pack_w ? take((size_t)in_planes * p->v * p->dp * 2) : at;
     p->o_stats = take((size_t)p->rows * p->slots * sizeof(float2));
@@ -1291,9 +1317,10 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     float* losses = t.losses ? t.losses : reinterpret_cast<float*>(ws + p.o_losses);
     uint16_t* x = reinterpret_cast<uint16_t*>(ws + p.o_x);
     uint16_t* wp = reinterpret_cast<uint16_t*>(ws + p.o_w);
+    uint32_t* x_top = t.dtype == GEFEN_F32 ? reinterpret_cast<uint32_t*>(ws + p.o_xtop) : nullptr;
     uint16_t* gbuf = reinterpret_cast<uint16_t*>(ws + p.o_g);
     const bool by_row = p.backward && t.reduction == GEFEN_REDUCE_NONE;
-    const bool shift = by_row && p.dw && p.halves;
+    const bool shift = p.backward && p.dw && (t.dtype == GEFEN_F32 || (by_row && t.dtype == GEFEN_F16));
     const int carry = !p.halves ? kCarryAll : p.planes == 2 ? kCarryTwo : kCarryOne;
 
     const Select sel{t.targets, t.targets_int32, p.n, p.v, t.ignore_index, by_row ? t.grad : nullptr, map, tgt, meta,
@@ -1314,6 +1341,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     pk.meta = meta;
     pk.which = 0;
     pk.zero_losses = losses;
+    pk.row_top = x_top;
     pk.row_grad = by_row ? t.grad : nullptr;
     pk.carry = carry;
     Pack pw{};
@@ -1332,7 +1360,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     const int pack_x = (int)grid_of(x_rows * (p.dp / 8), 8192);
     const int pack_w = p.pack_w ? (int)grid_of(p.v * (p.dp / 8), 8192) : 0;
     const int64_t per = (p.d + 7) / 8;
-    const Top tx{t.hidden, t.hidden_row_stride, t.hidden_col_stride, p.n, p.d, map, meta, 0, t.dtype == GEFEN_F16};
+    const Top tx{t.hidden, t.hidden_row_stride, t.hidden_col_stride, p.n, p.d, map, meta, 0, t.dtype == GEFEN_F16, x_top};
     const int top_x = (int)grid_of(p.n * per / 4, kTopGrid);
     if (!p.forward) {
         if (by_row) hipLaunchKernelGGL(k_rows, dim3(1), dim3(kRowsThreads), 0, st, sel);
@@ -1341,7 +1369,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
     } else {
         hipLaunchKernelGGL(k_rows, dim3(1), dim3(kRowsThreads), 0, st, sel);
         if (pk.f32) {
-            const Top tw{t.weight, t.weight_row_stride, t.weight_col_stride, p.v, p.d, nullptr, meta, 1, 0};
+            const Top tw{t.weight, t.weight_row_stride, t.weight_col_stride, p.v, p.d, nullptr, meta, 1, 0, nullptr};
             const int top_w = (int)grid_of(p.v * per / 4, kTopGrid);
             hipLaunchKernelGGL(k_top, dim3((unsigned)(top_x + top_w)), dim3(kTopThreads), 0, st, tx, tw, top_x);
         }
@@ -1375,7 +1403,7 @@ extern "C" int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task*
         l.v = p.v;
         l.steps = (int)(p.dp / 64);
         l.segs = pk.f32 ? 3 : 1;
-        l.f32 = pk.f32;
+        l.row_top = x_top;
         l.from = from;
         l.most = most;
         l.slots = p.slots;
