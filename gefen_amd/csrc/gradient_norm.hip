@@ -26,7 +26,7 @@ namespace gefen {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 16384;
+constexpr int kChunk = 16384, kSmallChunk = 2048;
 constexpr int kTable = 128;       // tensors per launch: the table fits the 4 KB of kernel arguments
 constexpr int64_t kKeepBytes = 192 << 20;
 constexpr int kGrid = 2048;         // workgroups of a launch (8 per CU)
@@ -258,16 +258,16 @@ __global__ __launch_bounds__(kThreads) void k_scale_by(T* a, int64_t na, T* b, i
     }
 }
 
-// Float32 a and b times *factor into a_out and b_out.
+// Float32 a and b times *factor into a_out and b_out, in chunks of up to kChunk.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_scale_from(const float* a, T* a_out, int64_t na, const float* b, T* b_out,
-                                                         int64_t nb, const float* __restrict__ factor) {
+                                                         int64_t nb, const float* __restrict__ factor, int chunk) {
     const float f = *factor;
-    const int64_t ca = (na + kChunk - 1) / kChunk, cb = (nb + kChunk - 1) / kChunk;
+    const int64_t ca = (na + chunk - 1) / chunk, cb = (nb + chunk - 1) / chunk;
     for (int64_t c = blockIdx.x; c < ca + cb; c += gridDim.x) {
         const bool first = c < ca;
-        const int64_t at = (first ? c : c - ca) * kChunk, left = (first ? na : nb) - at;
-        scale_chunk<true>((first ? a : b) + at, (first ? a_out : b_out) + at, left < kChunk ? (int)left : kChunk, f);
+        const int64_t at = (first ? c : c - ca) * chunk, left = (first ? na : nb) - at;
+        scale_chunk<true>((first ? a : b) + at, (first ? a_out : b_out) + at, left < chunk ? (int)left : chunk, f);
     }
 }
 
@@ -490,13 +490,15 @@ extern "C" int gefen_scale_from_f32(const float* a, void* a_out, int64_t a_numel
     const int size = dtype_size(dtype);
     if (!aligned(a, 4) || !aligned(b, 4) || !aligned(a_out, size) || !aligned(b_out, size))
         return fail_inval("%s: not aligned to its elements", what);
-    const int64_t chunks = (a_numel + kChunk - 1) / kChunk + (b_numel + kChunk - 1) / kChunk;
+    // few elements are spread over the chip: 101e3 in 7 chunks took 6.2 us, in 50 3.2
+    const int chunk = a_numel + b_numel <= (int64_t)kGrid * kSmallChunk ? kSmallChunk : kChunk;
+    const int64_t chunks = (a_numel + chunk - 1) / chunk + (b_numel + chunk - 1) / chunk;
     if (!chunks) return GEFEN_OK;
     const dim3 grid((unsigned)(chunks < kGrid ? chunks : kGrid)), wg(kThreads);
     auto launch = [&](auto type) {
         using T = decltype(type);
         hipLaunchKernelGGL(k_scale_from<T>, grid, wg, 0, stream, a, static_cast<T*>(a_out), a_numel, b,
-                           static_cast<T*>(b_out), b_numel, factor);
+                           static_cast<T*>(b_out), b_numel, factor, chunk);
     };
     if (dtype == GEFEN_F32) launch(0.0f);
     else if (dtype == GEFEN_BF16) launch(bf16_t{});
