@@ -20,10 +20,10 @@
 // (no conflicts counted).
 //
 // Bound by the matrix cores and the power they draw: the products of 8192 x 128256 x 4096
-// (8.6e12 bf16 operations each) take 6.86 ms for the logits with all that is kept of them
-// (1.25 PFLOP/s), 6.40 ms for dh (1.34) and 7.03 ms for dW (1.22), MFMA busy 61% of the
-// cycles at a clock of 1.9 GHz; the vendor's library reaches 1.29, 1.24 and 1.05 on the
-// bare products.  Waves of 128 x 128 (half the waves, a third less LDS traffic) were 20%
+// (8.6e12 bf16 operations each) take 6.8 to 7.0 ms for the logits with all that is kept of
+// them (1.23 to 1.26 PFLOP/s), 6.4 to 6.6 ms for dh (1.30 to 1.35) and 7.1 to 7.3 ms for dW
+// (1.18 to 1.21), from card to card, MFMA busy 65, 69 and 61% of the cycles at a clock of 1.82
+// to 1.9 GHz; the vendor's library reaches 1.29, 1.24 and 1.05 on the bare products.  Waves of 128 x 128 (half the waves, a third less LDS traffic) were 20%
 // slower: one wave per SIMD has nothing to cover its waits with.  Steps of 32 in four or
 // five stages lose to steps of 64 in two (twice the barriers).
 //

@@ -15,13 +15,17 @@
 // * The logits' product keeps, for every row and slot of 64 columns, the slot's
 //   maximum m and sum of exp(l - m), both float32, and when gradients are wanted
 //   exp(l - m) itself in 16 bits: an unsigned format of its own with three significant
-//   bits more than bf16 (one more than half) and a range beyond that of G.
+//   bits more than bf16 (one more than half; pack_exp2).
 // * One pass over those values turns them into G (k_gradient_rows): a row's lse comes
 //   from its slots, and exp(m - lse) scales each slot.  The target's entry is formed in
 //   float32 from its own logit, so that p - 1 of a confident row does not cancel in
-//   16 bits.  Rounding G to the operands' type is the one rounding below float32 on the
-//   way to the gradients: its errors are independent between the many terms of each sum
-//   and stay below that of the gradients' own rounding.
+//   16 bits.  G is then rounded to the operands' type: with the kept values' smaller one,
+//   the rounding below float32 on the way to the gradients.  Element by element it is up to
+//   half an ulp of each term, so where one term dominates (the row of dW of a token that
+//   occurs once, dh of a row far from its target) it scales the whole row and is as large as
+//   the output's own rounding; over many terms the errors are independent (1.9e-3 of a bf16
+//   gradient in all where the output's rounding alone is 1.7e-3; half 2.6e-4 and 2.1e-4).
+// * 16-bit outputs are rounded once, after the loss's own gradient (factor).
 // * For few rows one term can be most of a sum, and the products wait for W or dW
 //   anyway: G is then two planes, twice the type's bits (kTwoPlaneRows).
 // * Rows are taken in pieces whose G fits a bounded workspace; the logits of a piece
@@ -563,7 +567,8 @@ __global__ __launch_bounds__(C::TT, C::EU) void k_logits(const Logits a) {
 
 // Loss of each row from its slots, and (g) the row's values turned into G: one workgroup a
 // row, or parts of one where the rows are few (each joins the row's slots for itself).
-// Bound by HBM: 8192 x 128256 values read and written in 0.86 ms (4.9 TB/s).
+// Bound by HBM: 8192 x 128256 values read and written in 0.84 ms (5.0 TB/s); the losses alone
+// in 48 us.
 struct Rows {
     const float2* stats;
     const float* sums;
@@ -781,7 +786,7 @@ __device__ __forceinline__ float factor_of(const Grad& g, float factor, int64_t 
 // All tiles of one part run together, so that they share what they read (dealing the rest's
 // K steps out evenly instead, as one stretch per workgroup, balances better but left no
 // two workgroups at the same K: dh of 2796 x 2048 over 128256 2.0 ms against 1.63 with two
-// equal parts).  The number of parts is the one of the least estimated time, in K steps of
+// equal parts; with the number below 1.33).  The number of parts is the one of the least estimated time, in K steps of
 // a full chip: rounds times the steps of a part and 4 for its ends, 0.06 for the traffic of
 // each partial tile, and 4 and 0.1 a part for the launch that joins them.  The rows that take part are only known on the device, so
 // this is worked out there; the host bounds it.
@@ -1057,9 +1062,9 @@ template <bool F16> using HiddenSmall = Cfg<F16, 128, 128, 64, 64, 64, 2, true, 
 template <bool F16> using WeightBig = Cfg<F16, 256, 256, 128, 64, 64, 2, true, true, 4>;
 template <bool F16> using WeightSmall = Cfg<F16, 128, 128, 64, 64, 64, 2, true, true, 4>;
 
-// Rows up to which G has two planes.  The gradients' products of so few rows take the
-// time of reading W and writing dW (4 V D bytes at 5 TB/s) rather than of their
-// 8 n V D operations (at 1.2 PFLOP/s: n = 120).
+// Rows up to which G has two planes.  The gradients' products of so few rows wait for W to
+// be read and dW to be written rather than for their operations: dW of 80 x 42438 x 3136,
+// 266 MB, takes 121 us, and the 8 n V D operations of two planes 71 at 1.2 PFLOP/s.
 constexpr int kTwoPlaneRows = 64;
 
 enum LogitsTile { kRowTile, kSmallTile, kBigTile };

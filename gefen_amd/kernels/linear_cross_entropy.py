@@ -39,7 +39,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     have any strides; targets [...] are int64 or int32.  Positions whose target is
     ``ignore_index`` have no loss and no gradient, whatever they hold, and the mean is
     over the others (NaN where there are none, with zero gradients).  A target outside
-    [0, V) gives a NaN loss.  ``workspace_limit`` bounds the bytes kept for the gradients
+    [0, V) gives a NaN loss.  No position's loss or gradient depends on what another one
+    holds; weight's gradient sums them.  float32 operands are taken in 22 bits, weight's down
+    to 2^-28 of its largest element.  ``workspace_limit`` bounds the bytes kept for the gradients
     at a time (4 GiB by default; at least 256 positions are taken at once).  The loss can
     be differentiated once."""
     code = _REDUCTIONS.get(reduction)

@@ -469,8 +469,15 @@ int gefen_scale_gradients(const gefen_gradient_task* tasks, int num_tasks, const
  *   loss_n = lse_n - (1 - e) l[n, y_n] - (e / V) sum_v l[n, v],   lse_n = log sum_v exp l[n, v]
  * with e = label_smoothing; rows whose target is ignore_index have no loss, and nothing
  * they hold is read into a result.  A target outside [0, V) gives a NaN loss (and NaN
- * gradients).  Products accumulate in float32; exp(l - max) - target is rounded to dtype
- * on its way to the gradients (float32 operands keep 22 bits throughout). */
+ * gradients).  Products accumulate in float32.  On its way to the gradients G = softmax - target
+ * is rounded to dtype (rows above 64), so a gradient is off by half an ulp of each of its terms
+ * and one rounding of its own.  float32 operands are taken in 22 bits: weight's elements down to
+ * 2^-28 of its largest, ending at 2^-49 of that; hidden's likewise of its row's largest (in
+ * grad_weight: of all rows' largest); G down to 2^-28, ending at 2^-50 (float16: 11 bits down to
+ * 2^-29, ending at 2^-39).  With GEFEN_REDUCE_NONE each row of grad_hidden keeps its precision
+ * whatever the rows' gradients are; grad_weight holds float16 rows to 11 bits down to 2^-32 of
+ * the largest gradient and float32 ones to 22 bits down to 2^-36.  A row's gradient that is not
+ * finite reaches its own row of grad_hidden, and grad_weight. */
 enum { GEFEN_REDUCE_NONE = 0, GEFEN_REDUCE_MEAN = 1, GEFEN_REDUCE_SUM = 2 };
 /* workspace_limit = 0: what the values kept for the gradients may take */
 #define GEFEN_LCE_DEFAULT_LIMIT ((int64_t)4 << 30)
