@@ -124,14 +124,14 @@ class LinearCrossEntropyTask(ctypes.Structure):
     _fields_ += [(name, I64) for name in ("n", "v", "d", "hidden_row_stride", "hidden_col_stride",
                                           "weight_row_stride", "weight_col_stride", "ignore_index",
                                           "workspace_limit")]
-    _fields_ += [("label_smoothing", DBL), ("dtype", I32), ("targets_int32", I32), ("reduction", I32), ("stage", I32),
-                 ("grads_f32", I32), ("reserved", I32)]
+    _fields_ += [("label_smoothing", DBL), ("dtype", I32), ("targets_int32", I32), ("reduction", I32), ("stage", I32)]
 
 
 REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2
+LCE_GRADS_F32 = 16
 STEP_SUMMARY = np.dtype([("launches", np.int32), ("shared", np.int32), ("small", np.int32), ("tables", np.int32)])
 assert PERIOD_TASK.itemsize == 40 and HISTOGRAM_TASK.itemsize == 32
-assert GRADIENT_TASK.itemsize == 32 and ctypes.sizeof(LinearCrossEntropyTask) == 168
+assert GRADIENT_TASK.itemsize == 32 and ctypes.sizeof(LinearCrossEntropyTask) == 160
 assert STEP_TASK.itemsize == 128 and MUON_TASK.itemsize == 72 and MUON_APPLY_TASK.itemsize == 56
 
 _LIB = None

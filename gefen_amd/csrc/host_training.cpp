@@ -360,15 +360,16 @@ struct LceCall {
         t.targets_int32 = y.scalar_type() == at::kInt;
         t.reduction = static_cast<int32_t>(o.reduction);
     }
+    int grads = 0;  // GEFEN_LCE_GRADS_F32 or nothing
     // The bytes that the stage needs; 0 where it cannot be made.
     size_t bytes(int stage) {
-        t.stage = stage;
+        t.stage = stage | grads;
         return lib.lce_workspace(&t);
     }
     void form(void* grad_hidden, void* grad_weight, bool f32) {
         t.grad_hidden = grad_hidden;
         t.grad_weight = grad_weight;
-        t.grads_f32 = f32;
+        grads = f32 ? GEFEN_LCE_GRADS_F32 : 0;
     }
     // The stage of the last bytes(), or (ws defined) a backward stage on what a forward one left.
     at::Tensor run(size_t nbytes, at::Tensor ws = {}) {

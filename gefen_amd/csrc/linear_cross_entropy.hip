@@ -1148,25 +1148,26 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
         return fail_inval("%s: label_smoothing must lie in [0, 1], got %g", what, t.label_smoothing);
     if (t.reduction < GEFEN_REDUCE_NONE || t.reduction > GEFEN_REDUCE_SUM)
         return fail_inval("%s: unknown reduction %d", what, t.reduction);
-    if (t.stage < GEFEN_LCE_WHOLE || t.stage > GEFEN_LCE_BACKWARD) return fail_inval("%s: unknown stage %d", what, t.stage);
-    if (t.stage == GEFEN_LCE_FORWARD && (t.grad_hidden || t.grad_weight))
+    const int stage = t.stage & ~GEFEN_LCE_GRADS_F32;
+    if (stage < GEFEN_LCE_WHOLE || stage > GEFEN_LCE_BACKWARD) return fail_inval("%s: unknown stage %d", what, t.stage);
+    if (stage == GEFEN_LCE_FORWARD && (t.grad_hidden || t.grad_weight))
         return fail_inval("%s: a forward stage forms no gradients", what);
-    if (t.stage == GEFEN_LCE_BACKWARD && (t.losses || t.loss || (!t.grad_hidden && !t.grad_weight)))
+    if (stage == GEFEN_LCE_BACKWARD && (t.losses || t.loss || (!t.grad_hidden && !t.grad_weight)))
         return fail_inval("%s: a backward stage forms gradients, and no loss", what);
-    p->forward = t.stage != GEFEN_LCE_BACKWARD;
+    p->forward = stage != GEFEN_LCE_BACKWARD;
     p->n = (int)t.n;
     p->v = (int)t.v;
     p->d = (int)t.d;
     p->dtype = t.dtype;
     // a forward stage lays its workspace out for either gradient
-    p->dh = t.grad_hidden || t.stage == GEFEN_LCE_FORWARD;
-    p->dw = t.grad_weight || t.stage == GEFEN_LCE_FORWARD;
+    p->dh = t.grad_hidden || stage == GEFEN_LCE_FORWARD;
+    p->dw = t.grad_weight || stage == GEFEN_LCE_FORWARD;
     p->train = p->dh || p->dw;
-    p->backward = p->train && t.stage != GEFEN_LCE_FORWARD;
+    p->backward = p->train && stage != GEFEN_LCE_FORWARD;
     p->smooth = t.label_smoothing > 0.0;
     p->planes = t.dtype == GEFEN_F32 || t.n <= kTwoPlaneRows ? 2 : 1;
     p->halves = t.dtype != GEFEN_BF16;
-    p->out_f32 = t.dtype == GEFEN_F32 || t.grads_f32;
+    p->out_f32 = t.dtype == GEFEN_F32 || (t.stage & GEFEN_LCE_GRADS_F32);
     p->dp = up(t.d, 64);
     p->ldg = up(t.v, kRowAlign);
     p->pack_w = t.dtype == GEFEN_F32 || t.d % 64 != 0 || t.weight_col_stride != 1 || t.weight_row_stride % 8 != 0 ||
@@ -1181,7 +1182,7 @@ int make_plan(const gefen_linear_cross_entropy_task& t, Plan* p, const char* wha
     const int64_t rows = up((all + want - 1) / want, kRowAlign);
     p->pieces = (int)((all + rows - 1) / rows);
     p->rows = (int)rows;
-    if (t.stage && p->pieces > 1) return fail_inval("%s: stages of %d pieces of rows", what, p->pieces);
+    if (stage && p->pieces > 1) return fail_inval("%s: stages of %d pieces of rows", what, p->pieces);
     const int64_t n = t.n < rows ? (t.n > 0 ? t.n : 1) : rows;
     const int64_t in_steps = p->dp / 64 * (t.dtype == GEFEN_F32 ? 3 : 1);
     p->tile = n <= 32 ? kRowTile : logits_big(t.v, n, in_steps) ? kBigTile : kSmallTile;

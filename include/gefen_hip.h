@@ -486,6 +486,9 @@ enum { GEFEN_REDUCE_NONE = 0, GEFEN_REDUCE_MEAN = 1, GEFEN_REDUCE_SUM = 2 };
  * the operands otherwise as they were), once: it overwrites what it reads.  Only where all rows
  * fit the workspace limit together; otherwise the task is invalid. */
 enum { GEFEN_LCE_WHOLE = 0, GEFEN_LCE_FORWARD = 1, GEFEN_LCE_BACKWARD = 2 };
+/* Added to the stage: the gradients are float32 whatever dtype, for a caller that multiplies
+ * them before they are rounded (gefen_scale_from_f32). */
+enum { GEFEN_LCE_GRADS_F32 = 16 };
 
 typedef struct gefen_linear_cross_entropy_task {
     const void* hidden;   /* [n, d], any strides (elements) */
@@ -494,7 +497,7 @@ typedef struct gefen_linear_cross_entropy_task {
     const void* targets;  /* [n] contiguous, int64 or int32 */
     float* losses;        /* [n]: loss of each row, 0 where ignored; may be NULL */
     float* loss;          /* the reduced loss; may be NULL (must be for GEFEN_REDUCE_NONE) */
-    void* grad_hidden;    /* [n, d] contiguous, of dtype (or float32, see below); NULL: not wanted */
+    void* grad_hidden;    /* [n, d] contiguous, of dtype (GEFEN_LCE_GRADS_F32: float32); NULL: not wanted */
     void* grad_weight;    /* [v, d] likewise; NULL: not wanted */
     const float* grad;    /* gradient of the loss (device): one value, or one per row for
                            * GEFEN_REDUCE_NONE; NULL: 1 */
@@ -507,9 +510,6 @@ typedef struct gefen_linear_cross_entropy_task {
     int32_t targets_int32;    /* 1: targets are int32 */
     int32_t reduction;        /* the mean is over the rows that have a loss */
     int32_t stage;            /* GEFEN_LCE_*: 0 for a whole call */
-    int32_t grads_f32;        /* 1: the gradients are float32 whatever dtype, for a caller that
-                               * multiplies them before they are rounded (gefen_scale_from_f32) */
-    int32_t reserved;         /* 0 */
 } gefen_linear_cross_entropy_task;
 
 /* Bytes of workspace that the call needs (0: invalid task, see gefen_last_error). */
@@ -521,7 +521,7 @@ int gefen_linear_cross_entropy(const gefen_linear_cross_entropy_task* task, void
  * the gradients of a loss whose own gradient arrives later.  b may be NULL. */
 int gefen_scale_by(void* a, int64_t a_numel, void* b, int64_t b_numel, int dtype, const float* factor,
                    gefen_stream_t stream);
-/* The same of float32 gradients (grads_f32) into others of dtype, rounded once; b may be NULL. */
+/* The same of float32 gradients (GEFEN_LCE_GRADS_F32) into others of dtype, rounded once; b may be NULL. */
 int gefen_scale_from_f32(const float* a, void* a_out, int64_t a_numel, const float* b, void* b_out, int64_t b_numel,
                          int dtype, const float* factor, gefen_stream_t stream);
 

@@ -16,12 +16,18 @@ def test_refusals(a):
     assert _lib.load().gefen_scale_from_f32(*a, None) == _lib.GEFEN_EINVAL
 
 
+@pytest.mark.parametrize("stage", [16 + 3, 8, 32, 17])
+def test_unknown_stages_are_refused(stage):
+    more = dict(grad_hidden=FAKE) if stage == 17 else {}  # a forward stage forms no gradients
+    assert size(stage=stage, **more) == 0
+
+
 def test_nothing_to_do():
     assert _lib.load().gefen_scale_from_f32(None, None, 0, None, None, 0, 2, FAKE, None) == _lib.GEFEN_OK
 
 
 def test_float32_gradients_are_aligned_as_such_and_are_their_own_sum():
-    t = task(grad_hidden=FAKE + 2, grads_f32=1)
+    t = task(grad_hidden=FAKE + 2, stage=_lib.LCE_GRADS_F32)
     assert _lib.load().gefen_linear_cross_entropy(ctypes.byref(t), FAKE, 1 << 40, None) == _lib.GEFEN_EINVAL
     k = dict(n=10000, v=4096, grad_weight=FAKE, workspace_limit=1 << 20)
-    assert size(**k) - size(grads_f32=1, **k) == 4096 * 64 * 4
+    assert size(**k) - size(stage=_lib.LCE_GRADS_F32, **k) == 4096 * 64 * 4
