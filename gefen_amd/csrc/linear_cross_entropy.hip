@@ -310,14 +310,14 @@ __global__ __launch_bounds__(kTopThreads) void k_top(const Top a, const Top b, i
     else top_block(b, blockIdx.x - first, gridDim.x - first);
 }
 
-// Bound by HBM: 8192 x 4096 bf16 rows in 28 us (4.8 TB/s), 50257 x 768 float32 ones and
-// their three planes in 60 (6.4).
 // Rows of a matrix of any strides as the products read them: dp = D rounded up to 64
 // columns, zero-padded, one plane or those of a float32 operand, scaled: weight by its largest
 // element, hidden row by row, so that no row's logits depend on the size of another (for dW,
-// which sums rows, all by the largest: k_shift).  With a map: row
-// r is src row map[r] for r < meta->count and zero up to the next multiple of kRowAlign,
-// and the rows that take no part get a zero loss.  A thread moves eight columns of a row.
+// which sums rows, all by the largest: k_shift).  With a map: row r is src row map[r] for
+// r < meta->count and zero up to the next multiple of kRowAlign, and the rows that take no
+// part get a zero loss.  A thread moves eight columns of a row.
+// Bound by HBM: 8192 x 4096 bf16 rows in 28 us (4.8 TB/s), 50257 x 768 float32 ones and
+// their three planes in 60 (6.4), 8192 x 768 of them again for dW in 15.
 constexpr int kPackPlanes = 3;  // of a float32 operand: high, low, high where finite
 struct Pack {
     const void* src;
@@ -786,10 +786,11 @@ __device__ __forceinline__ float factor_of(const Grad& g, float factor, int64_t 
 // All tiles of one part run together, so that they share what they read (dealing the rest's
 // K steps out evenly instead, as one stretch per workgroup, balances better but left no
 // two workgroups at the same K: dh of 2796 x 2048 over 128256 2.0 ms against 1.63 with two
-// equal parts; with the number below 1.33).  The number of parts is the one of the least estimated time, in K steps of
-// a full chip: rounds times the steps of a part and 4 for its ends, 0.06 for the traffic of
-// each partial tile, and 4 and 0.1 a part for the launch that joins them.  The rows that take part are only known on the device, so
-// this is worked out there; the host bounds it.
+// equal parts; with the number below 1.33).  The number of parts is the one of the least
+// estimated time, in K steps of a full chip: rounds times the steps of a part and 4 for its
+// ends, 0.06 for the traffic of each partial tile, and 4 and 0.1 a part for the launch that
+// joins them.  The rows that take part are only known on the device, so this is worked out
+// there; the host bounds it.
 constexpr int kMostCuts = 128;
 constexpr int kMostRounds = 4;
 constexpr int kLeastSteps = 4;  // of a part
