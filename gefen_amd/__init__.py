@@ -5,11 +5,19 @@
 
 Beside the optimizers, what a training step does around them: ``linear_cross_entropy``
 (the loss of an output matrix with its gradients, without the logits), ``gradient_norm``,
-``clip_gradients`` and ``clip_grad_norm_``.
+``clip_gradients`` and ``clip_grad_norm_``; and what a layer does beside its matrix products:
+``attention``, ``rms_norm`` (with the residual's addition; ``rms_norm_quantized`` with an 8-bit
+output) and ``dropout``.
 """
 
 __all__ = ["Gefen", "GefenMuon", "kernels", "linear_cross_entropy", "gradient_norm", "clip_gradients",
-           "clip_grad_norm_"]
+           "clip_grad_norm_", "attention", "rms_norm", "rms_norm_quantized", "dropout"]
+
+_OPERATORS = {
+    "linear_cross_entropy": "linear_cross_entropy",
+    "gradient_norm": "gradient_norm", "clip_gradients": "gradient_norm", "clip_grad_norm_": "gradient_norm",
+    "attention": "attention", "rms_norm": "rms_norm", "rms_norm_quantized": "rms_norm", "dropout": "dropout",
+}
 
 
 def __getattr__(name):
@@ -21,11 +29,10 @@ def __getattr__(name):
         from .gefen_muon import GefenMuon
 
         return GefenMuon
-    if name in ("linear_cross_entropy", "gradient_norm", "clip_gradients", "clip_grad_norm_"):
+    if name in _OPERATORS:
         import importlib
 
-        module = "linear_cross_entropy" if name == "linear_cross_entropy" else "gradient_norm"
-        value = getattr(importlib.import_module("gefen_amd.kernels." + module), name)
+        value = getattr(importlib.import_module("gefen_amd.kernels." + _OPERATORS[name]), name)
         globals()[name] = value  # found directly from now on
         return value
     raise AttributeError("module {!r} has no attribute {!r}".format(__name__, name))

@@ -85,6 +85,13 @@ SIGNATURES = {
     "gefen_linear_cross_entropy": (I32, [P, P, SZ, P]),
     "gefen_scale_by": (I32, [P, I64, P, I64, I32, P, P]),
     "gefen_scale_from_f32": (I32, [P, P, I64, P, P, I64, I32, P, P]),
+    "gefen_attention_forward": (I32, [P, P]),
+    "gefen_attention_backward_workspace_size": (SZ, [P]),
+    "gefen_attention_backward": (I32, [P, P, SZ, P]),
+    "gefen_rms_norm_forward": (I32, [P, P]),
+    "gefen_rms_norm_backward_workspace_size": (SZ, [P]),
+    "gefen_rms_norm_backward": (I32, [P, P, SZ, P]),
+    "gefen_dropout": (I32, [P, P, P, I64, I32, DBL, P, I64, I64, P]),
 }
 
 # numpy mirror of struct gefen_step_task / gefen_muon_task (natural C alignment)
@@ -127,6 +134,27 @@ class LinearCrossEntropyTask(ctypes.Structure):
     _fields_ += [("label_smoothing", DBL), ("dtype", I32), ("targets_int32", I32), ("reduction", I32), ("stage", I32)]
 
 
+class AttentionTask(ctypes.Structure):
+    """struct gefen_attention_task"""
+
+    _fields_ = [(name, P) for name in ("query", "key", "value", "out", "lse", "grad_out", "grad_query", "grad_key",
+                                       "grad_value", "key_lengths", "offsets")]
+    _fields_ += [(name, I64) for name in ("batch", "queries", "keys", "heads", "kv_heads", "width", "sequences")]
+    _fields_ += [(name, I64 * 3) for name in ("query_strides", "key_strides", "value_strides", "grad_out_strides")]
+    _fields_ += [("scale", DBL), ("dtype", I32), ("causal", I32), ("lengths_int64", I32), ("offsets_int64", I32)]
+
+
+class RmsNormTask(ctypes.Structure):
+    """struct gefen_rms_norm_task"""
+
+    _fields_ = [(name, P) for name in ("x", "residual", "weight", "sum", "y", "scales", "rstd", "grad_y", "grad_sum",
+                                       "grad_x", "grad_residual", "grad_weight", "seed_at")]
+    _fields_ += [(name, I64) for name in ("rows", "width", "x_row_stride", "residual_row_stride",
+                                          "grad_y_row_stride", "grad_sum_row_stride", "seed", "offset")]
+    _fields_ += [("eps", DBL), ("dropout", DBL), ("dtype", I32), ("out", I32)]
+
+
+RMS_SAME, RMS_E4M3, RMS_E5M2 = 0, 1, 2
 REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2
 LCE_GRADS_F32 = 16
 STEP_SUMMARY = np.dtype([("launches", np.int32), ("shared", np.int32), ("small", np.int32), ("tables", np.int32)])

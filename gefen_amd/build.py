@@ -35,7 +35,8 @@ COMMON = [
 LIBS = {
     "libgefen_hip.so": ["capi.cpp", "step.hip", "step_inst_bf16.hip", "step_inst_f16.hip", "step_inst_f32.hip",
                         "step_inst_bf16_f32.hip", "step_inst_f16_f32.hip", "codebook.hip", "period.hip", "ns_gemm.hip",
-                        "newton_schulz.hip", "muon.hip", "gradient_norm.hip", "linear_cross_entropy.hip"],
+                        "newton_schulz.hip", "muon.hip", "gradient_norm.hip", "linear_cross_entropy.hip", "attention.hip",
+                        "rms_norm.hip", "dropout.hip"],
     "libgefen_synth.so": ["capi.cpp", "synthetic.hip"],
 }
 
@@ -108,7 +109,7 @@ def build_test_helpers() -> None:
 
 def build_host_ext() -> None:
     """_gefen_host: the host-side plan checks (csrc/host_plan.cpp) and the host side of the
-    training operators (csrc/host_training.cpp), a CPython extension built with the host
+    training operators (csrc/host_training.cpp, host_layers.cpp), a CPython extension built with the host
     C++ compiler against torch's headers (and HIP's, for the type of a stream)."""
     import sysconfig
 
@@ -124,7 +125,7 @@ def build_host_ext() -> None:
            "-isystem", str(Path(HIPCC).resolve().parent.parent / "include"), "-isystem", "/opt/rocm/include"]
     for inc in cpp_extension.include_paths():
         cmd += ["-isystem", inc]
-    cmd += [str(CSRC / "host_plan.cpp"), str(CSRC / "host_training.cpp"), "-o", str(tmp), "-L", torch_lib,
+    cmd += [str(CSRC / "host_plan.cpp"), str(CSRC / "host_training.cpp"), str(CSRC / "host_layers.cpp"), "-o", str(tmp), "-L", torch_lib,
             "-Wl,-rpath," + torch_lib, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

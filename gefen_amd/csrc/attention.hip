@@ -1,0 +1,723 @@
+// Softmax attention and its gradients.
+//
+//   S_ij = scale q_i . k_j,  L_i = log sum_j exp S_ij,  P_ij = exp(S_ij - L_i),  O_i = sum_j P_ij v_j
+//   D_i = dO_i . O_i,  dS_ij = P_ij (dO_i . v_j - D_i)
+//   dV_j = sum_i P_ij dO_i,  dQ_i = scale sum_j dS_ij k_j,  dK_j = scale sum_i dS_ij q_i
+//
+// Neither S nor P is stored: the forward pass keeps a running maximum and sum per row, and
+// the backward pass forms P again from L.  It takes two kernels, one that owns queries (dQ,
+// and D on its way) and one that owns keys (dK, dV): S and dO v are formed in both, seven
+// products in place of five, and in return every sum has one owner and one order, with no
+// atomics.
+//
+// The heads that share a key head are rows of one problem: row u = query u / G of head
+// u % G of the group (G = heads / kv_heads), so a tile of keys and values is loaded once for
+// all of them, and a single new token still gives G rows.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "attention_tiles.h"
+#include "capi_internal.h"
+#include "common.h"
+
+namespace gefen {
+namespace attn {
+
+constexpr int kThreads = 256;
+constexpr int kCols = 128;   // rows u (or keys) that a workgroup owns, 32 a wave
+constexpr int BN = 64;       // rows of a tile
+constexpr int kRangeParts = 16;
+
+// A tensor [batch, rows, heads, width] with strides in elements.
+struct View {
+    void* p;
+    int64_t batch, row, head;
+};
+
+struct Params {
+    View q, k, v, o, go, gq, gk, gv;
+    float* lse;    // [batch, kv_heads, U], log2 of the sum of exp2(c S): 0 for a row without keys
+    float* delta;  // [batch, kv_heads, U]
+    float* range;  // half precision: [2][batch * kv_heads][kRangeParts] largest norms of rows of v and of go
+    const void* key_lengths;
+    const void* offsets;
+    int32_t lengths64, offsets64, sequences;
+    int32_t batch, queries, keys, kv_heads, group, width, causal;
+    int32_t rows;       // U = queries * group
+    uint32_t div_mul;   // u / group = u * div_mul >> div_shift for u < 2^31
+    int32_t div_shift;
+    float c, scale;     // c = scale * log2(e)
+};
+
+__device__ __forceinline__ int div_group(const Params& a, int u) {
+    return (int)(((uint64_t)(uint32_t)u * a.div_mul) >> a.div_shift);
+}
+__device__ __forceinline__ int clamped(const void* p, int is64, int k, int most) {
+    const int64_t v = is64 ? static_cast<const int64_t*>(p)[k] : (int64_t)static_cast<const int32_t*>(p)[k];
+    return (int)max((int64_t)0, min(v, (int64_t)most));
+}
+
+struct Interval {
+    int lo, hi;
+};
+// The packed sequence that token i belongs to; empty if none.
+__device__ __forceinline__ Interval sequence_of(const Params& a, int i) {
+    int lo = -1, hi = a.sequences;  // offsets[lo] <= i (or lo = -1), and offsets past hi are not
+    while (lo < hi) {
+        const int mid = lo + (hi - lo + 1) / 2;
+        if (clamped(a.offsets, a.offsets64, mid, a.queries) <= i) lo = mid;
+        else hi = mid - 1;
+    }
+    if (lo < 0 || lo >= a.sequences) return {0, 0};
+    const Interval s = {clamped(a.offsets, a.offsets64, lo, a.queries), clamped(a.offsets, a.offsets64, lo + 1, a.queries)};
+    return s.lo <= i && i < s.hi ? s : Interval{0, 0};
+}
+// The keys that query i of sequence b sees.
+__device__ __forceinline__ Interval keys_of(const Params& a, int b, int i) {
+    Interval r = {0, a.keys};
+    if (a.offsets) r = sequence_of(a, i);
+    if (a.key_lengths) r.hi = min(r.hi, clamped(a.key_lengths, a.lengths64, b, a.keys));
+    if (a.causal) r.hi = min(r.hi, i + a.keys - a.queries + 1);
+    return r.hi > r.lo ? r : Interval{0, 0};
+}
+// The queries that see key j.
+__device__ __forceinline__ Interval queries_of(const Params& a, int b, int j) {
+    Interval r = {0, a.queries};
+    if (a.offsets) r = sequence_of(a, j);
+    if (a.key_lengths && j >= clamped(a.key_lengths, a.lengths64, b, a.keys)) return {0, 0};
+    if (a.causal) r.lo = max(r.lo, j - (a.keys - a.queries));
+    return r.hi > r.lo ? r : Interval{0, 0};
+}
+
+// What a wave's columns see of the other side: nothing outside [lo, hi), everything inside
+// [full_lo, full_hi).
+struct Span {
+    int lo, hi, full_lo, full_hi;
+    __device__ __forceinline__ void of(Interval r) {
+        const bool any = r.hi > r.lo;
+        lo = wave_min(any ? r.lo : 0x7fffffff);
+        hi = wave_max(r.hi);
+        full_lo = wave_max(r.lo);
+        full_hi = wave_min(r.hi);
+    }
+    __device__ __forceinline__ bool none(int r0) const { return r0 >= hi || r0 + BN <= lo; }
+    __device__ __forceinline__ bool full(int r0) const { return full_lo <= r0 && r0 + BN <= full_hi; }
+};
+// The span of the workgroup's waves (lo, hi only).
+__device__ __forceinline__ Interval block_span(const Span& s) {
+    __shared__ int part[2][kThreads / 64];
+    if ((threadIdx.x & 63) == 0) {
+        part[0][threadIdx.x >> 6] = s.lo;
+        part[1][threadIdx.x >> 6] = s.hi;
+    }
+    __syncthreads();
+    Interval r = {part[0][0], part[1][0]};
+    for (int w = 1; w < kThreads / 64; ++w) {
+        r.lo = min(r.lo, part[0][w]);
+        r.hi = max(r.hi, part[1][w]);
+    }
+    return r;
+}
+
+// Rows of a view: of keys, or (GROUPED) rows u of queries.
+template <typename T, bool GROUPED>
+struct Rows {
+    const T* base;
+    int64_t row, head;
+    int count;
+    __device__ __forceinline__ Rows(const Params& a, const View& v, int b, int hk)
+        : base(static_cast<const T*>(v.p) + b * v.batch + (int64_t)hk * (GROUPED ? a.group : 1) * v.head),
+          row(v.row),
+          head(v.head),
+          count(GROUPED ? a.rows : a.keys) {}
+    __device__ __forceinline__ const T* at(const Params& a, int u) const {
+        if constexpr (GROUPED) {
+            const int i = div_group(a, u);
+            return base + i * row + (u - i * a.group) * head;
+        } else {
+            return base + u * row;
+        }
+    }
+};
+
+// A tile on its way from global memory to LDS.  Rows past the last one are read as the last.
+template <typename T, int DP>
+struct Stage {
+    static constexpr int CPR = Tile<T, BN, DP>::CPR, LOADS = BN * CPR / kThreads, EPC = Elem<T>::EPC;
+    u32x4 r[LOADS];
+    template <bool GROUPED>
+    __device__ __forceinline__ void load(const Params& a, const Rows<T, GROUPED>& rows, int r0) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int q = (int)threadIdx.x + kThreads * i, row = q / CPR, c = q % CPR;
+            const int n = a.width - c * EPC;
+            r[i] = n > 0 ? load_chunk(rows.at(a, min(r0 + row, rows.count - 1)) + c * EPC, n) : u32x4{0u, 0u, 0u, 0u};
+        }
+    }
+    __device__ __forceinline__ void store(const Tile<T, BN, DP>& t) const {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int q = (int)threadIdx.x + kThreads * i;
+            t.put(q / CPR, q % CPR, r[i]);
+        }
+    }
+};
+
+// A lane's row as the right side of the rows products.
+template <typename T, int DP>
+struct Column {
+    static constexpr int EPC = Elem<T>::EPC, STEPS = DP / (2 * EPC);
+    u32x4 c[STEPS];
+    __device__ __forceinline__ void load(const T* row, int width, int lane) {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const int at = (2 * s + (lane >> 5)) * EPC;
+            c[s] = at < width ? load_chunk(row + at, width - at) : u32x4{0u, 0u, 0u, 0u};
+        }
+    }
+    // sum of this half's products with another row, float32
+    __device__ __forceinline__ float dot(const Column& o) const {
+        float sum = 0.0f;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int i = 0; i < EPC; ++i) sum = __builtin_fmaf(elem(c[s], i), elem(o.c[s], i), sum);
+        return sum;
+    }
+    __device__ __forceinline__ static float elem(u32x4 v, int i) {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(v[i]);
+        else return Elem<T>::value((uint16_t)(v[i / 2] >> (16 * (i & 1))));
+    }
+};
+
+template <typename T, int DP>
+__device__ __forceinline__ f32x16 rows_product(const Tile<T, BN, DP>& t, int r0, const Column<T, DP>& x, int lane) {
+    f32x16 acc = {};
+#pragma unroll
+    for (int c = 0; c < Column<T, DP>::STEPS; ++c) acc = mma_rows<T>(t.row_chunk(r0, c, lane), x.c[c], acc);
+    return acc;
+}
+// The row of a tile that register i of a rows product holds.
+__device__ __forceinline__ int row_of(int r0, int i, int lane) { return r0 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4; }
+__device__ __forceinline__ bool within(int r, Interval s) { return (uint32_t)(r - s.lo) < (uint32_t)(s.hi - s.lo); }
+
+// acc[d, n] times f into a row of width elements.
+template <typename T, int DT>
+__device__ __forceinline__ void store_column(T* row, const f32x16 (&acc)[DT], float f, int width, int lane) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int d = row_of(32 * dt, i, lane);
+            if (d < width)
+                store4(row + d, acc[dt][i] * f, acc[dt][i + 1] * f, acc[dt][i + 2] * f, acc[dt][i + 3] * f, width - d);
+        }
+}
+
+// Half precision keeps 2^-14 .. 65504 at full precision, so what is rounded to it is brought
+// there by powers of two that are taken out again: probabilities by 2^14 in the backward pass
+// and 2^6 in the forward one (whose running maximum may lag by 2^8), and dO v - D by the
+// bound that the rows' norms give.
+template <typename T>
+constexpr bool kHalf = std::is_same<T, f16_t>::value;
+constexpr float kLag = 8.0f;
+template <typename T>
+constexpr float kForwardShift = kHalf<T> ? 6.0f : 0.0f;
+template <typename T>
+constexpr float kBackwardShift = kHalf<T> ? 14.0f : 0.0f;
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) k_forward(Params a) {
+    using TileT = Tile<T, BN, DP>;
+    constexpr int DT = DP / 32;
+    __shared__ __attribute__((aligned(16))) char smem[2 * TileT::BYTES];
+    const TileT kt{(typename TileT::lds_t*)smem}, vt{(typename TileT::lds_t*)(smem + TileT::BYTES)};
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // the rows that see most keys first
+    const int heads = a.batch * a.kv_heads, tiles = (a.rows + kCols - 1) / kCols;
+    const int bh = blockIdx.x % heads, tile = tiles - 1 - blockIdx.x / heads;
+    const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
+    const int u = tile * kCols + wave * 32 + (lane & 31), uc = min(u, a.rows - 1);
+    const Interval seen = keys_of(a, b, div_group(a, uc));
+    Span span;
+    span.of(seen);
+    const Interval all = block_span(span);
+
+    const Rows<T, true> queries(a, a.q, b, hk);
+    const Rows<T, false> keys(a, a.k, b, hk), values(a, a.v, b, hk);
+    Column<T, DP> q;
+    q.load(queries.at(a, uc), a.width, lane);
+    f32x16 acc[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
+    float top = -INFINITY, sum = 0.0f;
+
+    auto tile_step = [&](auto partial, int k0) __attribute__((always_inline)) {
+        constexpr bool PARTIAL = decltype(partial)::value;
+        f32x16 s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[t] = rows_product(kt, 32 * t, q, lane);
+        float most = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (PARTIAL && !within(row_of(k0 + 32 * t, i, lane), seen)) s[t][i] = -INFINITY;
+                most = fmaxf(most, s[t][i]);
+            }
+        most = fmaxf(most, other_half(most)) * a.c;
+        if (__any(most > top + kLag)) {
+            const float next = fmaxf(top, most);
+            const float f = __builtin_amdgcn_exp2f(top - (next == -INFINITY ? 0.0f : next));
+            top = next;
+            sum *= f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) acc[dt] *= f;
+        }
+        const float shift = kForwardShift<T> - (top == -INFINITY ? 0.0f : top);
+        bool bad = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.c, shift));
+                if (PARTIAL && !within(row_of(k0 + 32 * t, i, lane), seen)) p = 0.0f;
+                s[t][i] = p;
+                sum += p;
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const PFrag<T> p = pack<T>(s[t], c);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+                    acc[dt] = vt.template mma_columns<PARTIAL>(p, 32 * t + 16 * c, 32 * dt, lane, acc[dt], &bad);
+            }
+        }
+        if (PARTIAL && __any(bad)) vt.template add_nonfinite<false>(acc, BN, seen.lo - k0, seen.hi - k0, lane);
+    };
+
+    if (all.hi > all.lo) {
+        Stage<T, DP> sk, sv;
+        int k0 = all.lo / BN * BN;
+        sk.load(a, keys, k0);
+        sv.load(a, values, k0);
+        for (; k0 < all.hi; k0 += BN) {
+            __syncthreads();
+            sk.store(kt);
+            sv.store(vt);
+            __syncthreads();
+            if (k0 + BN < all.hi) {
+                sk.load(a, keys, k0 + BN);
+                sv.load(a, values, k0 + BN);
+            }
+            if (span.none(k0)) continue;
+            if (span.full(k0)) tile_step(std::false_type{}, k0);
+            else tile_step(std::true_type{}, k0);
+        }
+    }
+    sum += other_half(sum);
+    if (u >= a.rows) return;
+    const bool empty = seen.hi <= seen.lo;
+    const int i = div_group(a, u);
+    T* out = static_cast<T*>(a.o.p) + b * a.o.batch + i * a.o.row + (int64_t)(hk * a.group + u - i * a.group) * a.o.head;
+    store_column(out, acc, empty ? 1.0f : 1.0f / sum, a.width, lane);
+    if (a.lse && lane < 32)
+        a.lse[(int64_t)bh * a.rows + u] = empty ? 0.0f : top + __builtin_amdgcn_logf(sum) - kForwardShift<T>;
+}
+
+// The power of two that brings values of up to `most` into [-1, 1].
+__device__ __forceinline__ float into_one(float most) {
+    if (!(most > 0.0f) || most > 3.0e38f) return 1.0f;
+    int e;
+    frexpf(most, &e);
+    return ldexpf(1.0f, min(max(-e, -120), 120));
+}
+// The largest row norm of v (which = 0) or of go (1) in (batch, key head) bh.
+__device__ __forceinline__ float largest_norm(const Params& a, int which, int bh) {
+    const float* r = a.range + ((int64_t)which * a.batch * a.kv_heads + bh) * kRangeParts;
+    float m = 0.0f;
+    for (int k = 0; k < kRangeParts; ++k) m = fmaxf(m, r[k]);
+    return m;
+}
+
+// Largest norms of the rows of v that take part, and of go, for half precision; 16 lanes a row.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_range(Params a) {
+    const int heads = a.batch * a.kv_heads, which = blockIdx.y, part = blockIdx.x % kRangeParts,
+              bh = blockIdx.x / kRangeParts;
+    const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
+    const Rows<T, true> grads(a, a.go, b, hk);
+    const Rows<T, false> values(a, a.v, b, hk);
+    int rows = which ? a.rows : a.keys;
+    if (!which && a.key_lengths) rows = clamped(a.key_lengths, a.lengths64, b, a.keys);
+    const int c = (threadIdx.x & 15) * Elem<T>::EPC;
+    float most = 0.0f;
+    for (int r = part * (kThreads / 16) + (threadIdx.x >> 4); r < rows; r += kRangeParts * (kThreads / 16)) {
+        const T* row = which ? grads.at(a, r) : values.at(a, r);
+        float sq = 0.0f;
+        if (c < a.width) {
+            const u32x4 x = load_chunk(row + c, a.width - c);
+#pragma unroll
+            for (int i = 0; i < Elem<T>::EPC; ++i) {
+                const float e = Column<T, 128>::elem(x, i);
+                sq = __builtin_fmaf(e, e, sq);
+            }
+        }
+        for (int off = 8; off > 0; off >>= 1) sq += __shfl_xor(sq, off, 64);
+        if (sq < INFINITY) most = fmaxf(most, sq);  // what is not finite reaches its results anyway
+    }
+    most = fmaxf(most, __shfl_xor(most, 16, 64));
+    most = fmaxf(most, __shfl_xor(most, 32, 64));
+    __shared__ float part_most[kThreads / 64];
+    if ((threadIdx.x & 63) == 0) part_most[threadIdx.x >> 6] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kThreads / 64; ++w) most = fmaxf(most, part_most[w]);
+        a.range[((int64_t)which * heads + bh) * kRangeParts + part] = sqrtf(most);
+    }
+}
+
+// dQ, and D for the other kernel.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) k_backward_queries(Params a) {
+    using TileT = Tile<T, BN, DP>;
+    constexpr int DT = DP / 32;
+    __shared__ __attribute__((aligned(16))) char smem[2 * TileT::BYTES];
+    const TileT kt{(typename TileT::lds_t*)smem}, vt{(typename TileT::lds_t*)(smem + TileT::BYTES)};
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int heads = a.batch * a.kv_heads, tiles = (a.rows + kCols - 1) / kCols;
+    const int bh = blockIdx.x % heads, tile = tiles - 1 - blockIdx.x / heads;
+    const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
+    const int u = tile * kCols + wave * 32 + (lane & 31), uc = min(u, a.rows - 1);
+    const Interval seen = keys_of(a, b, div_group(a, uc));
+    Span span;
+    span.of(seen);
+    const Interval all = block_span(span);
+
+    const Rows<T, false> keys(a, a.k, b, hk), values(a, a.v, b, hk);
+    Column<T, DP> q, go;
+    go.load(Rows<T, true>(a, a.go, b, hk).at(a, uc), a.width, lane);
+    q.load(Rows<T, true>(a, a.o, b, hk).at(a, uc), a.width, lane);
+    float delta = go.dot(q);
+    delta += other_half(delta);
+    if (lane < 32 && u < a.rows) a.delta[(int64_t)bh * a.rows + u] = delta;
+    q.load(Rows<T, true>(a, a.q, b, hk).at(a, uc), a.width, lane);
+    const float shift = kBackwardShift<T> - a.lse[(int64_t)bh * a.rows + uc];
+    float unit = 1.0f;
+    if constexpr (kHalf<T>) {
+        float norm = go.dot(go);
+        norm = sqrtf(norm + other_half(norm));
+        unit = into_one(2.0f * norm * largest_norm(a, 0, bh));
+    }
+    f32x16 acc[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
+
+    auto tile_step = [&](auto partial, int k0) __attribute__((always_inline)) {
+        constexpr bool PARTIAL = decltype(partial)::value;
+        bool bad = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x16 s = rows_product(kt, 32 * t, q, lane);
+            const f32x16 dp = rows_product(vt, 32 * t, go, lane);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, shift));
+                float ds = kHalf<T> ? p * ((dp[i] - delta) * unit) : p * (dp[i] - delta);
+                if (PARTIAL && !within(row_of(k0 + 32 * t, i, lane), seen)) ds = 0.0f;
+                s[i] = ds;
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const PFrag<T> ds = pack<T>(s, c);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+                    acc[dt] = kt.template mma_columns<PARTIAL>(ds, 32 * t + 16 * c, 32 * dt, lane, acc[dt], &bad);
+            }
+        }
+        if (PARTIAL && __any(bad)) kt.template add_nonfinite<true>(acc, BN, seen.lo - k0, seen.hi - k0, lane);
+    };
+
+    if (all.hi > all.lo) {
+        Stage<T, DP> sk, sv;
+        int k0 = all.lo / BN * BN;
+        sk.load(a, keys, k0);
+        sv.load(a, values, k0);
+        for (; k0 < all.hi; k0 += BN) {
+            __syncthreads();
+            sk.store(kt);
+            sv.store(vt);
+            __syncthreads();
+            if (k0 + BN < all.hi) {
+                sk.load(a, keys, k0 + BN);
+                sv.load(a, values, k0 + BN);
+            }
+            if (span.none(k0)) continue;
+            if (span.full(k0)) tile_step(std::false_type{}, k0);
+            else tile_step(std::true_type{}, k0);
+        }
+    }
+    if (u >= a.rows) return;
+    const int i = div_group(a, u);
+    T* out = static_cast<T*>(a.gq.p) + b * a.gq.batch + i * a.gq.row + (int64_t)(hk * a.group + u - i * a.group) * a.gq.head;
+    store_column(out, acc, kHalf<T> ? a.scale * (1.0f / 16384.0f) / unit : a.scale, a.width, lane);
+}
+
+// dK and dV.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) k_backward_keys(Params a) {
+    using TileT = Tile<T, BN, DP>;
+    constexpr int DT = DP / 32;
+    __shared__ __attribute__((aligned(16))) char smem[2 * TileT::BYTES];
+    __shared__ __attribute__((aligned(16))) float row_stats[2][BN];
+    const TileT qt{(typename TileT::lds_t*)smem}, gt{(typename TileT::lds_t*)(smem + TileT::BYTES)};
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // the keys that most rows see first
+    const int heads = a.batch * a.kv_heads;
+    const int bh = blockIdx.x % heads, tile = blockIdx.x / heads;
+    const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
+    const int j = tile * kCols + wave * 32 + (lane & 31), jc = min(j, a.keys - 1);
+    Interval seen = queries_of(a, b, jc);
+    seen.lo *= a.group;
+    seen.hi *= a.group;
+    Span span;
+    span.of(seen);
+    const Interval all = block_span(span);
+
+    const Rows<T, true> queries(a, a.q, b, hk), grads(a, a.go, b, hk);
+    Column<T, DP> k, v;
+    k.load(Rows<T, false>(a, a.k, b, hk).at(a, jc), a.width, lane);
+    v.load(Rows<T, false>(a, a.v, b, hk).at(a, jc), a.width, lane);
+    float unit = 1.0f;
+    if constexpr (kHalf<T>) unit = into_one(2.0f * largest_norm(a, 0, bh) * largest_norm(a, 1, bh));
+    f32x16 dk[DT], dv[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) dk[dt] = dv[dt] = f32x16{};
+
+    auto tile_step = [&](auto partial, int u0) __attribute__((always_inline)) {
+        constexpr bool PARTIAL = decltype(partial)::value;
+        bool bad_q = false, bad_g = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x16 s = rows_product(qt, 32 * t, k, lane);
+            f32x16 dp = rows_product(gt, 32 * t, v, lane);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int r = row_of(32 * t, i, lane);
+                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, kBackwardShift<T> - row_stats[0][r]));
+                const float d = dp[i] - row_stats[1][r];
+                float ds = kHalf<T> ? p * (d * unit) : p * d;
+                if (PARTIAL && !within(u0 + r, seen)) p = ds = 0.0f;
+                s[i] = p;
+                dp[i] = ds;
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const PFrag<T> p = pack<T>(s, c), ds = pack<T>(dp, c);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    dv[dt] = gt.template mma_columns<PARTIAL>(p, 32 * t + 16 * c, 32 * dt, lane, dv[dt], &bad_g);
+                    dk[dt] = qt.template mma_columns<PARTIAL>(ds, 32 * t + 16 * c, 32 * dt, lane, dk[dt], &bad_q);
+                }
+            }
+        }
+        if (PARTIAL && __any(bad_g)) gt.template add_nonfinite<false>(dv, BN, seen.lo - u0, seen.hi - u0, lane);
+        if (PARTIAL && __any(bad_q)) qt.template add_nonfinite<true>(dk, BN, seen.lo - u0, seen.hi - u0, lane);
+    };
+
+    if (all.hi > all.lo) {
+        Stage<T, DP> sq, sg;
+        const int which = threadIdx.x / BN, r = threadIdx.x % BN;  // row_stats: two quarters of the threads
+        const float* stats = (which ? a.delta : a.lse) + (int64_t)bh * a.rows;
+        float stat = 0.0f;
+        int u0 = all.lo / BN * BN;
+        sq.load(a, queries, u0);
+        sg.load(a, grads, u0);
+        if (which < 2) stat = stats[min(u0 + r, a.rows - 1)];
+        for (; u0 < all.hi; u0 += BN) {
+            __syncthreads();
+            sq.store(qt);
+            sg.store(gt);
+            if (which < 2) row_stats[which][r] = stat;
+            __syncthreads();
+            if (u0 + BN < all.hi) {
+                sq.load(a, queries, u0 + BN);
+                sg.load(a, grads, u0 + BN);
+                if (which < 2) stat = stats[min(u0 + BN + r, a.rows - 1)];
+            }
+            if (span.none(u0)) continue;
+            if (span.full(u0)) tile_step(std::false_type{}, u0);
+            else tile_step(std::true_type{}, u0);
+        }
+    }
+    if (j >= a.keys) return;
+    T* gk = static_cast<T*>(a.gk.p) + b * a.gk.batch + j * a.gk.row + hk * a.gk.head;
+    T* gv = static_cast<T*>(a.gv.p) + b * a.gv.batch + j * a.gv.row + hk * a.gv.head;
+    store_column(gk, dk, kHalf<T> ? a.scale * (1.0f / 16384.0f) / unit : a.scale, a.width, lane);
+    store_column(gv, dv, kHalf<T> ? 1.0f / 16384.0f : 1.0f, a.width, lane);
+}
+
+// ------------------------------------------------------------------ host side
+
+enum Pass { kForwardPass, kQueriesPass, kKeysPass };
+
+template <typename T, int DP>
+int launch(Pass pass, const Params& a, hipStream_t st) {
+    const int64_t heads = (int64_t)a.batch * a.kv_heads;
+    const int64_t cols = pass == kKeysPass ? a.keys : a.rows;
+    const dim3 grid((uint32_t)(heads * ((cols + kCols - 1) / kCols)));
+    if (pass == kForwardPass) k_forward<T, DP><<<grid, kThreads, 0, st>>>(a);
+    else if (pass == kQueriesPass) k_backward_queries<T, DP><<<grid, kThreads, 0, st>>>(a);
+    else k_backward_keys<T, DP><<<grid, kThreads, 0, st>>>(a);
+    return launch_status("attention");
+}
+template <typename T>
+int launch_width(Pass pass, const Params& a, hipStream_t st) {
+    if (a.width <= 32) return launch<T, 32>(pass, a, st);
+    if (a.width <= 64) return launch<T, 64>(pass, a, st);
+    if (a.width <= 96) return launch<T, 96>(pass, a, st);
+    return launch<T, 128>(pass, a, st);
+}
+int launch_type(int dtype, Pass pass, const Params& a, hipStream_t st) {
+    if (dtype == GEFEN_F32) return launch_width<float>(pass, a, st);
+    if (dtype == GEFEN_F16) return launch_width<f16_t>(pass, a, st);
+    return launch_width<bf16_t>(pass, a, st);
+}
+
+int64_t stat_count(const gefen_attention_task& t) { return t.batch * t.queries * t.heads; }
+int64_t round16(int64_t floats) { return (floats + 3) / 4 * 4; }
+
+// Checks what does not depend on the direction.
+int check_task(const gefen_attention_task* t) {
+    if (!t) return fail_inval("attention: no task");
+    if (!valid_dtype(t->dtype)) return fail_inval("attention: unknown dtype %d", t->dtype);
+    if (t->batch < 0 || t->queries < 0 || t->keys < 0 || t->heads < 1 || t->kv_heads < 1)
+        return fail_inval("attention: sizes must not be negative, and there is a head at least");
+    if (t->heads % t->kv_heads) return fail_inval("attention: heads must be a multiple of kv_heads");
+    if (t->width < 1 || t->width > GEFEN_ATTENTION_MAX_WIDTH)
+        return fail_inval("attention: width must be 1 to %d, got %lld", GEFEN_ATTENTION_MAX_WIDTH, (long long)t->width);
+    const int64_t most = (int64_t)1 << 30;
+    if (t->batch > most || t->queries > most || t->keys > most || t->heads > 65536)
+        return fail_inval("attention: sizes out of range");
+    const int64_t group = t->heads / t->kv_heads, pairs = t->batch * t->kv_heads;
+    if (t->queries * group > most || pairs > most || pairs * ((t->queries * group + kCols - 1) / kCols) > 0x7fffffff ||
+        pairs * ((t->keys + kCols - 1) / kCols) > 0x7fffffff)
+        return fail_inval("attention: sizes out of range");
+    if (!(t->scale >= 0.0) || !isfinite(t->scale)) return fail_inval("attention: scale must be finite and not negative");
+    if (t->offsets && (t->batch != 1 || t->queries != t->keys || t->sequences < 0 || t->sequences > most))
+        return fail_inval("attention: packed sequences are one batch of as many queries as keys");
+    if (t->offsets && t->key_lengths) return fail_inval("attention: either offsets or key_lengths");
+    if (t->key_lengths && !aligned(t->key_lengths, t->lengths_int64 ? 8 : 4))
+        return fail_inval("attention: key_lengths must be aligned");
+    if (t->offsets && !aligned(t->offsets, t->offsets_int64 ? 8 : 4))
+        return fail_inval("attention: offsets must be aligned");
+    return GEFEN_OK;
+}
+int check_tensor(const gefen_attention_task& t, const void* p, int64_t numel, const char* name) {
+    if (numel && !p) return fail_inval("attention: %s is missing", name);
+    if (!aligned(p, dtype_size(t.dtype))) return fail_inval("attention: %s must be aligned to its elements", name);
+    return GEFEN_OK;
+}
+int check_floats(const void* p, const char* name) {
+    if (!p || !aligned(p, 4)) return fail_inval("attention: %s must be aligned float32 memory", name);
+    return GEFEN_OK;
+}
+
+Params params_of(const gefen_attention_task& t) {
+    Params a{};
+    auto view = [](const void* p, const int64_t* s) { return View{const_cast<void*>(p), s[0], s[1], s[2]}; };
+    auto dense = [&](void* p, int64_t rows, int64_t heads) {
+        return View{p, rows * heads * t.width, heads * t.width, t.width};
+    };
+    a.q = view(t.query, t.query_strides);
+    a.k = view(t.key, t.key_strides);
+    a.v = view(t.value, t.value_strides);
+    a.go = view(t.grad_out, t.grad_out_strides);
+    a.o = dense(t.out, t.queries, t.heads);
+    a.gq = dense(t.grad_query, t.queries, t.heads);
+    a.gk = dense(t.grad_key, t.keys, t.kv_heads);
+    a.gv = dense(t.grad_value, t.keys, t.kv_heads);
+    a.lse = t.lse;
+    a.key_lengths = t.key_lengths;
+    a.offsets = t.offsets;
+    a.lengths64 = t.lengths_int64;
+    a.offsets64 = t.offsets_int64;
+    a.sequences = (int32_t)t.sequences;
+    a.batch = (int32_t)t.batch;
+    a.queries = (int32_t)t.queries;
+    a.keys = (int32_t)t.keys;
+    a.kv_heads = (int32_t)t.kv_heads;
+    a.group = (int32_t)(t.heads / t.kv_heads);
+    a.width = (int32_t)t.width;
+    a.causal = t.causal;
+    a.rows = a.queries * a.group;
+    // 2^(31 + s) / group rounded up, s = ceil(log2 group): exact quotients below 2^31
+    int s = 0;
+    while ((1 << s) < a.group) ++s;
+    a.div_shift = 31 + s;
+    a.div_mul = (uint32_t)((((uint64_t)1 << a.div_shift) + a.group - 1) / a.group);
+    a.scale = (float)t.scale;
+    a.c = (float)(t.scale * 1.4426950408889634);
+    return a;
+}
+
+}  // namespace attn
+}  // namespace gefen
+
+using namespace gefen;
+using namespace gefen::attn;
+
+extern "C" size_t gefen_attention_backward_workspace_size(const gefen_attention_task* task) {
+    if (check_task(task) != GEFEN_OK) return 0;
+    const int64_t range = task->dtype == GEFEN_F16 ? 2 * task->batch * task->kv_heads * kRangeParts : 0;
+    return (size_t)(round16(stat_count(*task)) + round16(range) + 4) * 4;
+}
+
+extern "C" int gefen_attention_forward(const gefen_attention_task* task, gefen_stream_t stream) {
+    if (int rc = check_task(task)) return rc;
+    const gefen_attention_task& t = *task;
+    const int64_t nq = t.batch * t.queries * t.heads * t.width, nk = t.batch * t.keys * t.kv_heads * t.width;
+    if (int rc = check_tensor(t, t.query, nq, "query")) return rc;
+    if (int rc = check_tensor(t, t.key, nk, "key")) return rc;
+    if (int rc = check_tensor(t, t.value, nk, "value")) return rc;
+    if (int rc = check_tensor(t, t.out, nq, "out")) return rc;
+    if (t.lse && !aligned(t.lse, 4)) return fail_inval("attention: lse must be aligned float32 memory");
+    if (nq == 0) return GEFEN_OK;
+    return launch_type(t.dtype, kForwardPass, params_of(t), static_cast<hipStream_t>(stream));
+}
+
+extern "C" int gefen_attention_backward(const gefen_attention_task* task, void* workspace, size_t workspace_bytes,
+                                        gefen_stream_t stream) {
+    if (int rc = check_task(task)) return rc;
+    const gefen_attention_task& t = *task;
+    const int64_t nq = t.batch * t.queries * t.heads * t.width, nk = t.batch * t.keys * t.kv_heads * t.width;
+    if (int rc = check_tensor(t, t.query, nq, "query")) return rc;
+    if (int rc = check_tensor(t, t.key, nk, "key")) return rc;
+    if (int rc = check_tensor(t, t.value, nk, "value")) return rc;
+    if (int rc = check_tensor(t, t.out, nq, "out")) return rc;
+    if (int rc = check_tensor(t, t.grad_out, nq, "grad_out")) return rc;
+    if (int rc = check_tensor(t, t.grad_query, nq, "grad_query")) return rc;
+    const bool key_grads = t.grad_key || t.grad_value;
+    if (int rc = check_tensor(t, t.grad_key, key_grads ? nk : 0, "grad_key")) return rc;
+    if (int rc = check_tensor(t, t.grad_value, key_grads ? nk : 0, "grad_value")) return rc;
+    if (nq)
+        if (int rc = check_floats(t.lse, "lse")) return rc;
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < gefen_attention_backward_workspace_size(task))
+        return fail_inval("attention: workspace too small, missing or not aligned to 16 bytes");
+    Params a = params_of(t);
+    a.delta = static_cast<float*>(workspace);
+    a.range = a.delta + round16(stat_count(t));
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (t.dtype == GEFEN_F16 && nq && nk) {
+        k_range<f16_t><<<dim3((uint32_t)(t.batch * t.kv_heads * kRangeParts), 2), kThreads, 0, st>>>(a);
+        if (int rc = launch_status("attention")) return rc;
+    }
+    if (nq)
+        if (int rc = launch_type(t.dtype, kQueriesPass, a, st)) return rc;
+    if (nk && key_grads)
+        if (int rc = launch_type(t.dtype, kKeysPass, a, st)) return rc;
+    return GEFEN_OK;
+}

@@ -1,0 +1,229 @@
+// Tiles of the attention kernels (attention.hip), gfx950.
+//
+// Every product of attention and of its gradients is taken with one side in registers and
+// the other in LDS, 32 x 32 at a time (v_mfma_f32_32x32x16 of 16-bit operands,
+// v_mfma_f32_32x32x2_f32 of float32 ones):
+//
+//   rows:     acc[m, n] += sum_k tile[m, k] x[n, k]      k along the head's width
+//   columns:  acc[d, n] += sum_m tile[m, d] p[m, n]      m along the tile's rows
+//
+// A lane owns one n (lane % 32) throughout: a query in the forward pass and in dQ, a key in
+// dK and dV.  The accumulator of a rows product holds p[m, n] for m = 8 (i / 4) + 4 h + i % 4
+// (i = 0..15, h = lane / 32), and the columns product takes it as it lies: the order of m
+// within a matrix instruction is free as long as both sides agree, so the tile's side is read
+// in that order (16-bit: two transposing ds_read_b64_tr_b16, four rows each) and p never
+// moves between lanes.  The softmax's maximum and sum need one exchange, between the halves.
+//
+// A tile is BN rows of DP elements, DP the head's width rounded up to 32 with zeros, and rows
+// are padded so that row reads (16 bytes of 8 rows at a time) and transposing reads (4 rows x
+// 32 bytes) spread over all banks.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "common.h"
+
+namespace gefen {
+namespace attn {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct Elem {
+    static constexpr int EPC = 16 / sizeof(T);           // elements of a 16-byte chunk
+    static constexpr int PAD = sizeof(T) == 2 ? 16 : 8;  // elements between rows of a tile
+    using Raw = typename RawVec<sizeof(T)>::type;        // what LDS holds
+    __device__ __forceinline__ static float value(Raw r) {
+        T t;
+        __builtin_memcpy(&t, &r, sizeof(T));
+        return to_f32(t);
+    }
+};
+
+// A rows product's step: 2 x EPC elements of k, lane half h holding k = 2 EPC c + EPC h + 0..
+template <typename T>
+__device__ __forceinline__ f32x16 mma_rows(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            c = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(f32x4, a)[i], __builtin_bit_cast(f32x4, b)[i], c,
+                                                     0, 0, 0);
+        return c;
+    } else if constexpr (__is_same(T, f16_t)) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                      0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                       0, 0);
+    }
+}
+
+// Sixteen rows of p as the columns product takes them.
+template <typename T>
+struct PFrag {
+    u32x4 v;
+};
+template <>
+struct PFrag<float> {
+    float v[8];
+};
+template <typename T>
+__device__ __forceinline__ PFrag<T> pack(const f32x16& p, int chunk) {
+    PFrag<T> out;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) out.v[i] = p[8 * chunk + i];
+    } else if constexpr (__is_same(T, f16_t)) {
+        f16x8 t;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = (_Float16)p[8 * chunk + i];
+        out.v = __builtin_bit_cast(u32x4, t);
+    } else {
+        bf16x8 t;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = (__bf16)p[8 * chunk + i];
+        out.v = __builtin_bit_cast(u32x4, t);
+    }
+    return out;
+}
+
+// Zeros in place of what is not finite; true if there was any.
+template <typename T>
+__device__ __forceinline__ bool drop_nonfinite(uint32_t& x) {
+    if constexpr (sizeof(T) == 4) {
+        const bool bad = (x & 0x7f800000u) == 0x7f800000u;
+        x = bad ? 0u : x;
+        return bad;
+    } else {
+        constexpr uint32_t e = __is_same(T, f16_t) ? 0x7c00u : 0x7f80u;
+        const bool lo = (x & e) == e, hi = (x & (e << 16)) == (e << 16);
+        x &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
+        return lo | hi;
+    }
+}
+
+template <typename T, int BN, int DP>
+struct Tile {
+    static constexpr int EPC = Elem<T>::EPC, LD = DP + Elem<T>::PAD;
+    static constexpr int BYTES = BN * LD * (int)sizeof(T);
+    static constexpr int CPR = DP / EPC;  // chunks of a row
+    // LDS pointers keep their address space
+    typedef __attribute__((address_space(3))) typename Elem<T>::Raw lds_t;
+    typedef __attribute__((address_space(3))) u32x4 lds_chunk;
+    lds_t* p;
+
+    __device__ __forceinline__ void put(int row, int c, u32x4 v) const { *(lds_chunk*)(p + row * LD + c * EPC) = v; }
+
+    // chunk c of the rows product's left side: row r0 + lane % 32
+    __device__ __forceinline__ u32x4 row_chunk(int r0, int c, int lane) const {
+        return *(const lds_chunk*)(p + (r0 + (lane & 31)) * LD + (2 * c + (lane >> 5)) * EPC);
+    }
+    // acc[d0 + .., n] += sum over rows r0 .. r0 + 15.  CHECK: what is not finite counts as
+    // zero, and *bad tells.
+    template <bool CHECK>
+    __device__ __forceinline__ f32x16 mma_columns(const PFrag<T>& b, int r0, int d0, int lane, f32x16 acc,
+                                                  bool* bad) const {
+        const int h = lane >> 5;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                uint32_t a = p[(r0 + 8 * (i / 4) + 4 * h + i % 4) * LD + d0 + (lane & 31)];
+                if (CHECK) *bad |= drop_nonfinite<T>(a);
+                acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a), b.v[i], acc, 0, 0, 0);
+            }
+            return acc;
+        } else {
+            // in each group of 16 lanes, lane 4 j + q points at row j, elements 4 q .. 4 q + 3
+            typedef __attribute__((address_space(3))) bf16x4 lds_v4;
+            const int row = r0 + 4 * h + ((lane & 15) >> 2);
+            const int col = d0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+            lds_t* at = p + row * LD + col;
+            const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4*)at);
+            const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4*)(at + 8 * LD));
+            u32x4 a = __builtin_bit_cast(u32x4, bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+            if (CHECK) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t x = a[i];
+                    *bad |= drop_nonfinite<T>(x);
+                    a[i] = x;
+                }
+            }
+            if constexpr (__is_same(T, f16_t))
+                return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b.v),
+                                                              acc, 0, 0, 0);
+            else
+                return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                               __builtin_bit_cast(bf16x8, b.v), acc, 0, 0, 0);
+        }
+    }
+    // What the checked product has left out, for the rows in [lo, hi) that this lane's column
+    // sees: infinities as they are, or (AS_NAN) NaN for any.
+    template <bool AS_NAN, int DT>
+    __device__ __forceinline__ void add_nonfinite(f32x16 (&acc)[DT], int rows, int lo, int hi, int lane) const {
+        const int h = lane >> 5;
+#pragma unroll 1
+        for (int r = 0; r < rows; ++r) {
+            const bool seen = r >= lo && r < hi;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float v = Elem<T>::value(p[r * LD + 32 * dt + 8 * (i / 4) + 4 * h + i % 4]);
+                    const bool bad = (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u;
+                    if (bad && seen) acc[dt][i] += AS_NAN ? __uint_as_float(0x7fc00000u) : v;
+                }
+        }
+    }
+};
+
+// EPC elements from p, of which the first `n` exist (n >= 1); zeros for the others.
+template <typename T>
+__device__ __forceinline__ u32x4 load_chunk(const T* p, int n) {
+    constexpr int EPC = Elem<T>::EPC;
+    if (n >= EPC) return *reinterpret_cast<const typename RawAny<16, sizeof(T)>::type*>(p);
+    u32x4 out = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < EPC; ++i) {
+        if (i < n) {
+            if constexpr (sizeof(T) == 4) out[i] = __float_as_uint(p[i]);
+            else out[i / 2] |= (uint32_t)p[i].bits << (16 * (i & 1));
+        }
+    }
+    return out;
+}
+
+// Four consecutive elements of which the first `n` exist.
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d, int n) {
+    const AnyVec<T, 4> v = {{from_f32<T>(a), from_f32<T>(b), from_f32<T>(c), from_f32<T>(d)}};
+    if (n >= 4) {
+        using R = typename RawAny<sizeof(T) * 4, sizeof(T)>::type;
+        typename RawVec<sizeof(T) * 4>::type r;
+        __builtin_memcpy(&r, &v, sizeof(r));
+        *reinterpret_cast<R*>(p) = r;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < n) p[i] = v.v[i];
+    }
+}
+
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+__device__ __forceinline__ int wave_min(int v) {
+    for (int off = 32; off > 0; off >>= 1) v = min(v, __shfl_xor(v, off, 64));
+    return v;
+}
+__device__ __forceinline__ int wave_max(int v) {
+    for (int off = 32; off > 0; off >>= 1) v = max(v, __shfl_xor(v, off, 64));
+    return v;
+}
+
+}  // namespace attn
+}  // namespace gefen

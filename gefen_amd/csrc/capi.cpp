@@ -56,5 +56,7 @@ extern "C" size_t gefen_struct_size(int which) {
            : which == 2 ? sizeof(gefen_muon_apply_task)
            : which == 3 ? sizeof(gefen_gradient_task)
            : which == 4 ? sizeof(gefen_linear_cross_entropy_task)
+           : which == 5 ? sizeof(gefen_attention_task)
+           : which == 6 ? sizeof(gefen_rms_norm_task)
                         : 0;
 }

@@ -32,6 +32,7 @@
 namespace py = pybind11;
 
 void register_training(py::module_& m);  // host_training.cpp
+void register_layers(py::module_& m);    // host_layers.cpp
 
 namespace {
 
@@ -356,6 +357,7 @@ PYBIND11_MODULE(_gefen_host, m) {
     key_eps_ = intern("eps");
     key_wd_ = intern("weight_decay");
     register_training(m);
+    register_layers(m);
     py::class_<PlanCore>(m, "PlanCore")
         .def(py::init<py::list, py::list, py::tuple>())
         .def("refresh", &PlanCore::refresh)

@@ -7,30 +7,23 @@
 // gefen_amd/_lib.py has loaded: bind_library() receives the functions' addresses.  Built
 // with the host compiler against torch's headers (no device code).
 
-#include <Python.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <pybind11/pybind11.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/autograd/variable.h>
-
-#include <ATen/ATen.h>
 #include <algorithm>
-#include <cstdint>
 #include <cstring>
-#include <stdexcept>
-#include <string>
 #include <vector>
 
-#include "gefen_hip.h"
+#include "host_common.h"
 
-namespace py = pybind11;
+void bind_layers(const py::dict& addresses);  // host_layers.cpp
+
+namespace gefen_host {
+decltype(&gefen_last_error) last_error = nullptr;
+}
 
 namespace {
 
+using namespace gefen_host;
+
 struct Library {
-    decltype(&gefen_last_error) last_error;
     decltype(&gefen_gradient_norm_workspace_size) norm_workspace;
     decltype(&gefen_gradient_norm) norm;
     decltype(&gefen_clip_gradients) clip;
@@ -53,52 +46,9 @@ void bind_library(py::dict addresses) {
     lib.lce = reinterpret_cast<decltype(lib.lce)>(at("gefen_linear_cross_entropy"));
     lib.scale_by = reinterpret_cast<decltype(lib.scale_by)>(at("gefen_scale_by"));
     lib.scale_from_f32 = reinterpret_cast<decltype(lib.scale_from_f32)>(at("gefen_scale_from_f32"));
-    lib.last_error = reinterpret_cast<decltype(lib.last_error)>(at("gefen_last_error"));
+    bind_layers(addresses);
+    last_error = reinterpret_cast<decltype(last_error)>(at("gefen_last_error"));
 }
-void need_library() {
-    if (!lib.last_error) throw std::runtime_error("bind_library() has not been called");
-}
-
-void check(int rc) {
-    if (rc == GEFEN_OK) return;
-    if (rc == GEFEN_EINVAL) throw py::value_error(lib.last_error());
-    throw std::runtime_error(lib.last_error());
-}
-
-int32_t dtype_code(const at::Tensor& t) {
-    switch (t.scalar_type()) {
-        case at::kFloat: return GEFEN_F32;
-        case at::kHalf: return GEFEN_F16;
-        case at::kBFloat16: return GEFEN_BF16;
-        default: return -1;
-    }
-}
-
-gefen_stream_t stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-
-at::Tensor bytes_on(const at::Tensor& like, size_t n) {
-    return at::empty({static_cast<int64_t>(n)}, like.options().dtype(at::kByte).requires_grad(false));
-}
-
-const at::Tensor& tensor_of(py::handle o, const char* name) {
-    if (!THPVariable_Check(o.ptr()))
-        throw py::type_error(std::string("Expected ") + name + " to be a torch.Tensor, got " + Py_TYPE(o.ptr())->tp_name);
-    return THPVariable_Unpack(o.ptr());
-}
-
-// Raises for a forward-mode tangent, which a call on addresses would drop.
-void no_tangent(const at::Tensor& t, const char* name) {
-    const auto* meta = torch::autograd::impl::get_autograd_meta(t);
-    if (!meta || !meta->fw_grad(/*level=*/0, t).defined()) return;
-    PyErr_Format(PyExc_NotImplementedError, "Expected %s without a forward-mode tangent.", name);
-    throw py::error_already_set();
-}
-
-// A tensor whose memory holds its values: a view that stands for the negative of its memory
-// (the imaginary part of a conjugate) is copied.
-at::Tensor as_stored(const at::Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
-
-py::object wrap(const at::Tensor& t) { return py::reinterpret_steal<py::object>(THPVariable_Wrap(t)); }
 
 // ------------------------------------------------------------------ gradient norm
 
@@ -330,9 +280,6 @@ struct LceOptions {
     int64_t reduction;
 };
 
-float* floats(const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
-void* data(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-
 // One library call, to be made on the current stream: the task, and what its addresses
 // belong to.
 struct LceCall {
@@ -379,10 +326,6 @@ struct LceCall {
         return ws;
     }
 };
-
-at::Tensor empty_grad(const at::Tensor& like, bool wanted, at::ScalarType type) {
-    return wanted ? at::empty(like.sizes(), like.options().dtype(type).requires_grad(false)) : at::Tensor();
-}
 
 // The loss, and for its backward pass one of
 //   * kept: what the gradients are formed from, where all rows fit the workspace limit
@@ -498,30 +441,15 @@ class LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> 
     }
 };
 
-std::string shape_of(c10::IntArrayRef s) {
-    std::string out = "(";
-    for (size_t i = 0; i < s.size(); ++i) out += (i ? ", " : "") + std::to_string(s[i]);
-    return out + ")";
-}
-
 py::object linear_cross_entropy(py::handle hidden_, py::handle weight_, py::handle targets_, int64_t ignore_index,
                                 double label_smoothing, int64_t reduction, int64_t workspace_limit) {
     need_library();
     const at::Tensor& hidden = tensor_of(hidden_, "hidden");
     const at::Tensor& weight = tensor_of(weight_, "weight");
     const at::Tensor& targets = tensor_of(targets_, "targets");
-    auto on_device = [&](const at::Tensor& t, const char* name) {
-        if (!t.is_cuda())
-            throw py::value_error(std::string("Expected ") + name + " to be on CUDA, got device " + t.device().str() + ".");
-        if (t.device() != hidden.device())
-            throw py::value_error(std::string("Expected ") + name + " on " + hidden.device().str() + ", got " +
-                                  t.device().str() + ".");
-        if (t.unsafeGetTensorImpl()->is_python_dispatch() || t.layout() != at::kStrided)
-            throw py::type_error(std::string("Expected ") + name + " to be a plain strided tensor.");
-    };
-    on_device(hidden, "hidden");
-    on_device(weight, "weight");
-    on_device(targets, "targets");
+    plain_on(hidden, "hidden", hidden);
+    plain_on(weight, "weight", hidden);
+    plain_on(targets, "targets", hidden);
     no_tangent(hidden, "hidden");
     no_tangent(weight, "weight");
     if (dtype_code(hidden) < 0)

@@ -525,6 +525,87 @@ int gefen_scale_by(void* a, int64_t a_numel, void* b, int64_t b_numel, int dtype
 int gefen_scale_from_f32(const float* a, void* a_out, int64_t a_numel, const float* b, void* b_out, int64_t b_numel,
                          int dtype, const float* factor, gefen_stream_t stream);
 
+/* ------------------------------------------------------------------ attention
+ * Softmax attention of query [batch, queries, heads, width] over key and value
+ * [batch, keys, kv_heads, width], heads a multiple of kv_heads (query head h reads key head
+ * h / (heads / kv_heads)):
+ *   S_ij = scale q_i . k_j,  P_ij = exp(S_ij) / sum over the keys that i sees,  O_i = sum_j P_ij v_j
+ * Query i of sequence b sees key j where j < key_lengths[b], and (causal) j <= i + keys - queries;
+ * with offsets, the tokens of one batch are packed sequences [offsets[s], offsets[s + 1]) and i
+ * sees keys of its own sequence only.  A query without keys has a zero output and no gradient.
+ * Products accumulate in float32 and the softmax is float32; P and dS are rounded to dtype on
+ * their way into the second products (float16: scaled into its range, P down to 2^-28 (backward),
+ * dS down to 2^-28 of the bound that the norms of the rows of value and grad_out give, one bound
+ * a query in grad_query, one a key head in grad_key).  What a query does not see does not reach
+ * it, whatever it holds, nor the other way round.  Every sum has a fixed order. */
+enum { GEFEN_ATTENTION_MAX_WIDTH = 128 };
+typedef struct gefen_attention_task {
+    const void* query;
+    const void* key;
+    const void* value;
+    void* out;            /* [batch, queries, heads, width] contiguous: written by forward, read by backward */
+    float* lse;           /* [batch * queries * heads]: written by forward (NULL: not wanted) for backward */
+    const void* grad_out; /* backward from here on */
+    void* grad_query;     /* contiguous, as query, key and value */
+    void* grad_key;       /* this and the next: NULL both where they are not wanted */
+    void* grad_value;
+    const void* key_lengths; /* device, int32 or int64 [batch]; NULL: keys.  Taken into [0, keys] */
+    const void* offsets;     /* device, int32 or int64 [sequences + 1], ascending; NULL: not packed */
+    int64_t batch, queries, keys, heads, kv_heads, width, sequences;
+    int64_t query_strides[3], key_strides[3], value_strides[3], grad_out_strides[3]; /* batch, token, head: elements */
+    double scale;            /* not negative */
+    int32_t dtype, causal, lengths_int64, offsets_int64;
+} gefen_attention_task;
+
+int gefen_attention_forward(const gefen_attention_task* task, gefen_stream_t stream);
+/* Bytes of workspace (16-byte aligned) that gefen_attention_backward needs; 0: invalid task. */
+size_t gefen_attention_backward_workspace_size(const gefen_attention_task* task);
+int gefen_attention_backward(const gefen_attention_task* task, void* workspace, size_t workspace_bytes,
+                             gefen_stream_t stream);
+
+/* ------------------------------------------------------------------ norm of a residual stream
+ *   s = residual + dropout(x),  r = (mean s^2 + eps)^(-1/2),  y = s r weight
+ * and its gradient (see gefen_dropout for the mask; element e = row * width + column).  Forward
+ * works on s before its rounding to dtype, backward on the stored s and the stored r.  With
+ * GEFEN_RMS_E4M3 or _E5M2, y is 8-bit floating point: y = q * scales[row], the row's largest
+ * value at the largest of the format (448, 57344). */
+enum { GEFEN_RMS_SAME = 0, GEFEN_RMS_E4M3 = 1, GEFEN_RMS_E5M2 = 2 };
+enum { GEFEN_RMS_MAX_WIDTH = 32768 };
+typedef struct gefen_rms_norm_task {
+    const void* x;           /* [rows, width]; backward: s (x itself without a residual) */
+    const void* residual;    /* NULL: none */
+    const void* weight;      /* [width] */
+    void* sum;               /* s, contiguous; NULL: not wanted */
+    void* y;                 /* contiguous */
+    float* scales;           /* [rows], 8-bit output only */
+    float* rstd;             /* [rows]: r, written by forward (NULL: not wanted) for backward */
+    const void* grad_y;      /* backward from here on */
+    const void* grad_sum;    /* NULL: none */
+    void* grad_x;            /* contiguous; each of the three may be NULL */
+    void* grad_residual;     /* the gradient of s */
+    void* grad_weight;
+    const int64_t* seed_at;  /* device; NULL: seed */
+    int64_t rows, width, x_row_stride, residual_row_stride, grad_y_row_stride, grad_sum_row_stride;
+    int64_t seed, offset;
+    double eps, dropout;
+    int32_t dtype, out;
+} gefen_rms_norm_task;
+
+int gefen_rms_norm_forward(const gefen_rms_norm_task* task, gefen_stream_t stream);
+size_t gefen_rms_norm_backward_workspace_size(const gefen_rms_norm_task* task);
+/* workspace: 16-byte aligned; only for grad_weight. */
+int gefen_rms_norm_backward(const gefen_rms_norm_task* task, void* workspace, size_t workspace_bytes,
+                            gefen_stream_t stream);
+
+/* ------------------------------------------------------------------ dropout
+ * y_e = residual_e + m_e x_e / (1 - p), numel contiguous elements; residual may be NULL.  p is
+ * taken to the nearest multiple of 2^-16; m_e = 1 where the 16 bits of element e are at least
+ * 65536 p: half e % 2 (0: the low one) of word (e % 8) / 2 of Philox4x32-10 with the 64-bit key
+ * seed and the counter (e / 8, offset).  What is dropped counts as zero whatever it holds.  The
+ * gradient of x is the same call on the gradient of y, without residual. */
+int gefen_dropout(const void* x, const void* residual, void* y, int64_t numel, int dtype, double p,
+                  const int64_t* seed_at, int64_t seed, int64_t offset, gefen_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
