@@ -143,25 +143,95 @@ struct Rows {
     }
 };
 
-// A tile on its way from global memory to LDS.  Rows past the last one are read as the last.
-template <typename T, int DP>
-struct Stage {
-    static constexpr int CPR = Tile<T, BN, DP>::CPR, LOADS = BN * CPR / kThreads, EPC = Elem<T>::EPC;
-    u32x4 r[LOADS];
+// Fills a tile.  Rows past the last one are read as the last.  ASYNC: rows are 16-byte
+// aligned and a width of whole chunks (what lies behind the width is cleared once, by
+// clear_tiles); issue() starts the loads and the caller waits for them.  Otherwise issue()
+// takes the rows into registers and land() writes them.
+template <typename T, int DP, bool ASYNC>
+struct Filler {
+    using TileT = Tile<T, BN, DP>;
+    static constexpr int CPR = TileT::CPR, LOADS = BN * CPR / kThreads, EPC = Elem<T>::EPC;
+    u32x4 r[ASYNC ? 1 : LOADS];
     template <bool GROUPED>
-    __device__ __forceinline__ void load(const Params& a, const Rows<T, GROUPED>& rows, int r0) {
+    __device__ __forceinline__ void issue(const Params& a, const Rows<T, GROUPED>& rows, int r0, const TileT& t) {
+        const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(t.p + ((int)threadIdx.x >> 6) * 64 * EPC));
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const int q = (int)threadIdx.x + kThreads * i, row = q / CPR, c = q % CPR;
+            const int q = (int)threadIdx.x + kThreads * i, row = q / CPR;
+            const int c = (q % CPR) ^ (ASYNC ? chunk_xor(row, CPR) : 0);
             const int n = a.width - c * EPC;
-            r[i] = n > 0 ? load_chunk(rows.at(a, min(r0 + row, rows.count - 1)) + c * EPC, n) : u32x4{0u, 0u, 0u, 0u};
+            const T* at = rows.at(a, min(r0 + row, rows.count - 1)) + c * EPC;
+            if constexpr (ASYNC) {
+                if (n > 0) load_to_lds<16>(at, lds + i * kThreads * 16);
+            } else {
+                r[i] = n > 0 ? load_chunk(at, n) : u32x4{0u, 0u, 0u, 0u};
+            }
         }
     }
-    __device__ __forceinline__ void store(const Tile<T, BN, DP>& t) const {
+    __device__ __forceinline__ void land(const TileT& t) const {
+        if constexpr (!ASYNC) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int q = (int)threadIdx.x + kThreads * i;
-            t.put(q / CPR, q % CPR, r[i]);
+            for (int i = 0; i < LOADS; ++i) {
+                const int q = (int)threadIdx.x + kThreads * i;
+                t.put(q / CPR, q % CPR, r[i]);
+            }
+        }
+    }
+};
+
+// The tiles of two operands, twice: one pair is filled while the other is worked on.
+template <typename T, int DP, bool ASYNC, bool GROUPED>
+struct Pipe {
+    using TileT = Tile<T, BN, DP>;
+    static constexpr int BYTES = 4 * TileT::BYTES;
+    const Params& a;
+    Rows<T, GROUPED> x, y;
+    typename TileT::lds_t* base;
+    Filler<T, DP, ASYNC> fx, fy;
+
+    __device__ __forceinline__ Pipe(const Params& a, const View& vx, const View& vy, int b, int hk, char* smem)
+        : a(a), x(a, vx, b, hk), y(a, vy, b, hk), base((typename TileT::lds_t*)smem) {
+        if (ASYNC && a.width < DP) {
+            __attribute__((address_space(3))) u32x4* p = (__attribute__((address_space(3))) u32x4*)base;
+            for (int i = threadIdx.x; i < BYTES / 16; i += kThreads) p[i] = u32x4{0u, 0u, 0u, 0u};
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ TileT tile(int buffer, int which) const {
+        return TileT{base + (2 * buffer + which) * TileT::ELEMS};
+    }
+    __device__ __forceinline__ void issue(int r0, int buffer) {
+        fx.issue(a, x, r0, tile(buffer, 0));
+        fy.issue(a, y, r0, tile(buffer, 1));
+    }
+    __device__ __forceinline__ void land(int buffer) const {
+        fx.land(tile(buffer, 0));
+        fy.land(tile(buffer, 1));
+    }
+    // step(r0, first tile, second tile, buffer) for the tiles of [all.lo, all.hi); more(r0,
+    // buffer) loads what else the step needs.
+    template <typename More, typename Step>
+    __device__ __forceinline__ void run(Interval all, More more, Step step) {
+        if (all.hi <= all.lo) return;
+        int r0 = all.lo / BN * BN;
+        issue(r0, 0);
+        more(r0, 0);
+        if (!ASYNC) land(0);
+        auto one = [&](auto which) __attribute__((always_inline)) {
+            constexpr int buffer = decltype(which)::value;
+            // this buffer has landed, and every wave is done with the other one
+            wait_loads_and_sync();
+            const bool next = r0 + BN < all.hi;
+            if (next) {
+                issue(r0 + BN, 1 - buffer);
+                more(r0 + BN, 1 - buffer);
+            }
+            step(r0, tile(buffer, 0), tile(buffer, 1), buffer);
+            if (!ASYNC && next) land(1 - buffer);
+            r0 += BN;
+            return next;
+        };
+        while (one(std::integral_constant<int, 0>{}) && one(std::integral_constant<int, 1>{})) {
         }
     }
 };
@@ -229,12 +299,12 @@ constexpr float kForwardShift = kHalf<T> ? 6.0f : 0.0f;
 template <typename T>
 constexpr float kBackwardShift = kHalf<T> ? 14.0f : 0.0f;
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) k_forward(Params a) {
+template <typename T, int DP, bool ASYNC>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_forward(Params a) {
     using TileT = Tile<T, BN, DP>;
+    using PipeT = Pipe<T, DP, ASYNC, false>;
     constexpr int DT = DP / 32;
-    __shared__ __attribute__((aligned(16))) char smem[2 * TileT::BYTES];
-    const TileT kt{(typename TileT::lds_t*)smem}, vt{(typename TileT::lds_t*)(smem + TileT::BYTES)};
+    extern __shared__ __attribute__((aligned(1024))) char smem[];  // PipeT::BYTES
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     // the rows that see most keys first
     const int heads = a.batch * a.kv_heads, tiles = (a.rows + kCols - 1) / kCols;
@@ -247,7 +317,7 @@ __global__ void __launch_bounds__(kThreads) k_forward(Params a) {
     const Interval all = block_span(span);
 
     const Rows<T, true> queries(a, a.q, b, hk);
-    const Rows<T, false> keys(a, a.k, b, hk), values(a, a.v, b, hk);
+    PipeT pipe(a, a.k, a.v, b, hk, smem);
     Column<T, DP> q;
     q.load(queries.at(a, uc), a.width, lane);
     f32x16 acc[DT];
@@ -255,7 +325,7 @@ __global__ void __launch_bounds__(kThreads) k_forward(Params a) {
     for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
     float top = -INFINITY, sum = 0.0f;
 
-    auto tile_step = [&](auto partial, int k0) __attribute__((always_inline)) {
+    auto tile_step = [&](auto partial, int k0, const TileT& kt, const TileT& vt) __attribute__((always_inline)) {
         constexpr bool PARTIAL = decltype(partial)::value;
         f32x16 s[2];
 #pragma unroll
@@ -299,25 +369,11 @@ __global__ void __launch_bounds__(kThreads) k_forward(Params a) {
         if (PARTIAL && __any(bad)) vt.template add_nonfinite<false>(acc, BN, seen.lo - k0, seen.hi - k0, lane);
     };
 
-    if (all.hi > all.lo) {
-        Stage<T, DP> sk, sv;
-        int k0 = all.lo / BN * BN;
-        sk.load(a, keys, k0);
-        sv.load(a, values, k0);
-        for (; k0 < all.hi; k0 += BN) {
-            __syncthreads();
-            sk.store(kt);
-            sv.store(vt);
-            __syncthreads();
-            if (k0 + BN < all.hi) {
-                sk.load(a, keys, k0 + BN);
-                sv.load(a, values, k0 + BN);
-            }
-            if (span.none(k0)) continue;
-            if (span.full(k0)) tile_step(std::false_type{}, k0);
-            else tile_step(std::true_type{}, k0);
-        }
-    }
+    pipe.run(all, [](int, int) {}, [&](int k0, const TileT& kt, const TileT& vt, int) __attribute__((always_inline)) {
+        if (span.none(k0)) return;
+        if (span.full(k0)) tile_step(std::false_type{}, k0, kt, vt);
+        else tile_step(std::true_type{}, k0, kt, vt);
+    });
     sum += other_half(sum);
     if (u >= a.rows) return;
     const bool empty = seen.hi <= seen.lo;
@@ -381,12 +437,12 @@ __global__ void __launch_bounds__(kThreads) k_range(Params a) {
 }
 
 // dQ, and D for the other kernel.
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) k_backward_queries(Params a) {
+template <typename T, int DP, bool ASYNC>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_queries(Params a) {
     using TileT = Tile<T, BN, DP>;
+    using PipeT = Pipe<T, DP, ASYNC, false>;
     constexpr int DT = DP / 32;
-    __shared__ __attribute__((aligned(16))) char smem[2 * TileT::BYTES];
-    const TileT kt{(typename TileT::lds_t*)smem}, vt{(typename TileT::lds_t*)(smem + TileT::BYTES)};
+    extern __shared__ __attribute__((aligned(1024))) char smem[];  // PipeT::BYTES
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int heads = a.batch * a.kv_heads, tiles = (a.rows + kCols - 1) / kCols;
     const int bh = blockIdx.x % heads, tile = tiles - 1 - blockIdx.x / heads;
@@ -397,7 +453,7 @@ __global__ void __launch_bounds__(kThreads) k_backward_queries(Params a) {
     span.of(seen);
     const Interval all = block_span(span);
 
-    const Rows<T, false> keys(a, a.k, b, hk), values(a, a.v, b, hk);
+    PipeT pipe(a, a.k, a.v, b, hk, smem);
     Column<T, DP> q, go;
     go.load(Rows<T, true>(a, a.go, b, hk).at(a, uc), a.width, lane);
     q.load(Rows<T, true>(a, a.o, b, hk).at(a, uc), a.width, lane);
@@ -416,7 +472,7 @@ __global__ void __launch_bounds__(kThreads) k_backward_queries(Params a) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
 
-    auto tile_step = [&](auto partial, int k0) __attribute__((always_inline)) {
+    auto tile_step = [&](auto partial, int k0, const TileT& kt, const TileT& vt) __attribute__((always_inline)) {
         constexpr bool PARTIAL = decltype(partial)::value;
         bool bad = false;
 #pragma unroll
@@ -441,25 +497,11 @@ __global__ void __launch_bounds__(kThreads) k_backward_queries(Params a) {
         if (PARTIAL && __any(bad)) kt.template add_nonfinite<true>(acc, BN, seen.lo - k0, seen.hi - k0, lane);
     };
 
-    if (all.hi > all.lo) {
-        Stage<T, DP> sk, sv;
-        int k0 = all.lo / BN * BN;
-        sk.load(a, keys, k0);
-        sv.load(a, values, k0);
-        for (; k0 < all.hi; k0 += BN) {
-            __syncthreads();
-            sk.store(kt);
-            sv.store(vt);
-            __syncthreads();
-            if (k0 + BN < all.hi) {
-                sk.load(a, keys, k0 + BN);
-                sv.load(a, values, k0 + BN);
-            }
-            if (span.none(k0)) continue;
-            if (span.full(k0)) tile_step(std::false_type{}, k0);
-            else tile_step(std::true_type{}, k0);
-        }
-    }
+    pipe.run(all, [](int, int) {}, [&](int k0, const TileT& kt, const TileT& vt, int) __attribute__((always_inline)) {
+        if (span.none(k0)) return;
+        if (span.full(k0)) tile_step(std::false_type{}, k0, kt, vt);
+        else tile_step(std::true_type{}, k0, kt, vt);
+    });
     if (u >= a.rows) return;
     const int i = div_group(a, u);
     T* out = static_cast<T*>(a.gq.p) + b * a.gq.batch + i * a.gq.row + (int64_t)(hk * a.group + u - i * a.group) * a.gq.head;
@@ -467,13 +509,13 @@ __global__ void __launch_bounds__(kThreads) k_backward_queries(Params a) {
 }
 
 // dK and dV.
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) k_backward_keys(Params a) {
+template <typename T, int DP, bool ASYNC>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && DP < 96 ? 2 : 1) k_backward_keys(Params a) {
     using TileT = Tile<T, BN, DP>;
+    using PipeT = Pipe<T, DP, ASYNC, true>;
     constexpr int DT = DP / 32;
-    __shared__ __attribute__((aligned(16))) char smem[2 * TileT::BYTES];
-    __shared__ __attribute__((aligned(16))) float row_stats[2][BN];
-    const TileT qt{(typename TileT::lds_t*)smem}, gt{(typename TileT::lds_t*)(smem + TileT::BYTES)};
+    extern __shared__ __attribute__((aligned(1024))) char smem[];  // PipeT::BYTES
+    __shared__ __attribute__((aligned(16))) float row_stats[2][2][BN];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     // the keys that most rows see first
     const int heads = a.batch * a.kv_heads;
@@ -487,7 +529,7 @@ __global__ void __launch_bounds__(kThreads) k_backward_keys(Params a) {
     span.of(seen);
     const Interval all = block_span(span);
 
-    const Rows<T, true> queries(a, a.q, b, hk), grads(a, a.go, b, hk);
+    PipeT pipe(a, a.q, a.go, b, hk, smem);
     Column<T, DP> k, v;
     k.load(Rows<T, false>(a, a.k, b, hk).at(a, jc), a.width, lane);
     v.load(Rows<T, false>(a, a.v, b, hk).at(a, jc), a.width, lane);
@@ -497,18 +539,19 @@ __global__ void __launch_bounds__(kThreads) k_backward_keys(Params a) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) dk[dt] = dv[dt] = f32x16{};
 
-    auto tile_step = [&](auto partial, int u0) __attribute__((always_inline)) {
+    auto tile_step = [&](auto partial, int u0, const TileT& qt, const TileT& gt,
+                         const float (&stats)[2][BN]) __attribute__((always_inline)) {
         constexpr bool PARTIAL = decltype(partial)::value;
         bool bad_q = false, bad_g = false;
-#pragma unroll
+#pragma unroll 1
         for (int t = 0; t < 2; ++t) {
             f32x16 s = rows_product(qt, 32 * t, k, lane);
             f32x16 dp = rows_product(gt, 32 * t, v, lane);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int r = row_of(32 * t, i, lane);
-                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, kBackwardShift<T> - row_stats[0][r]));
-                const float d = dp[i] - row_stats[1][r];
+                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, kBackwardShift<T> - stats[0][r]));
+                const float d = dp[i] - stats[1][r];
                 float ds = kHalf<T> ? p * (d * unit) : p * d;
                 if (PARTIAL && !within(u0 + r, seen)) p = ds = 0.0f;
                 s[i] = p;
@@ -528,31 +571,18 @@ __global__ void __launch_bounds__(kThreads) k_backward_keys(Params a) {
         if (PARTIAL && __any(bad_q)) qt.template add_nonfinite<true>(dk, BN, seen.lo - u0, seen.hi - u0, lane);
     };
 
-    if (all.hi > all.lo) {
-        Stage<T, DP> sq, sg;
-        const int which = threadIdx.x / BN, r = threadIdx.x % BN;  // row_stats: two quarters of the threads
-        const float* stats = (which ? a.delta : a.lse) + (int64_t)bh * a.rows;
-        float stat = 0.0f;
-        int u0 = all.lo / BN * BN;
-        sq.load(a, queries, u0);
-        sg.load(a, grads, u0);
-        if (which < 2) stat = stats[min(u0 + r, a.rows - 1)];
-        for (; u0 < all.hi; u0 += BN) {
-            __syncthreads();
-            sq.store(qt);
-            sg.store(gt);
-            if (which < 2) row_stats[which][r] = stat;
-            __syncthreads();
-            if (u0 + BN < all.hi) {
-                sq.load(a, queries, u0 + BN);
-                sg.load(a, grads, u0 + BN);
-                if (which < 2) stat = stats[min(u0 + BN + r, a.rows - 1)];
-            }
-            if (span.none(u0)) continue;
-            if (span.full(u0)) tile_step(std::false_type{}, u0);
-            else tile_step(std::true_type{}, u0);
-        }
-    }
+    // two waves' 64 lanes take the rows' L and D along
+    const float* stats = (wave ? a.delta : a.lse) + (int64_t)bh * a.rows;
+    const uint32_t stats_lds =
+        __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) float*)&row_stats[0][wave & 1][0]);
+    auto more = [&](int u0, int buffer) __attribute__((always_inline)) {
+        if (wave < 2) load_to_lds<4>(stats + min(u0 + lane, a.rows - 1), stats_lds + buffer * (uint32_t)sizeof(row_stats[0]));
+    };
+    pipe.run(all, more, [&](int u0, const TileT& qt, const TileT& gt, int buffer) __attribute__((always_inline)) {
+        if (span.none(u0)) return;
+        if (span.full(u0)) tile_step(std::false_type{}, u0, qt, gt, row_stats[buffer]);
+        else tile_step(std::true_type{}, u0, qt, gt, row_stats[buffer]);
+    });
     if (j >= a.keys) return;
     T* gk = static_cast<T*>(a.gk.p) + b * a.gk.batch + j * a.gk.row + hk * a.gk.head;
     T* gv = static_cast<T*>(a.gv.p) + b * a.gv.batch + j * a.gv.row + hk * a.gv.head;
@@ -564,22 +594,34 @@ __global__ void __launch_bounds__(kThreads) k_backward_keys(Params a) {
 
 enum Pass { kForwardPass, kQueriesPass, kKeysPass };
 
-template <typename T, int DP>
+template <typename T, int DP, bool ASYNC>
 int launch(Pass pass, const Params& a, hipStream_t st) {
     const int64_t heads = (int64_t)a.batch * a.kv_heads;
     const int64_t cols = pass == kKeysPass ? a.keys : a.rows;
     const dim3 grid((uint32_t)(heads * ((cols + kCols - 1) / kCols)));
-    if (pass == kForwardPass) k_forward<T, DP><<<grid, kThreads, 0, st>>>(a);
-    else if (pass == kQueriesPass) k_backward_queries<T, DP><<<grid, kThreads, 0, st>>>(a);
-    else k_backward_keys<T, DP><<<grid, kThreads, 0, st>>>(a);
+    constexpr int lds = Pipe<T, DP, ASYNC, false>::BYTES;
+    if (pass == kForwardPass) k_forward<T, DP, ASYNC><<<grid, kThreads, lds, st>>>(a);
+    else if (pass == kQueriesPass) k_backward_queries<T, DP, ASYNC><<<grid, kThreads, lds, st>>>(a);
+    else k_backward_keys<T, DP, ASYNC><<<grid, kThreads, lds, st>>>(a);
     return launch_status("attention");
+}
+// Whether a tensor's rows are whole 16-byte chunks.
+bool chunked(const Params& a, const View& v, int size) {
+    return aligned(v.p, 16) && a.width * size % 16 == 0 && v.batch * size % 16 == 0 && v.row * size % 16 == 0 &&
+           v.head * size % 16 == 0;
+}
+template <typename T, int DP>
+int launch_filler(Pass pass, const Params& a, hipStream_t st) {
+    const bool keys = pass == kKeysPass;
+    const bool async = chunked(a, keys ? a.q : a.k, sizeof(T)) && chunked(a, keys ? a.go : a.v, sizeof(T));
+    return async ? launch<T, DP, true>(pass, a, st) : launch<T, DP, false>(pass, a, st);
 }
 template <typename T>
 int launch_width(Pass pass, const Params& a, hipStream_t st) {
-    if (a.width <= 32) return launch<T, 32>(pass, a, st);
-    if (a.width <= 64) return launch<T, 64>(pass, a, st);
-    if (a.width <= 96) return launch<T, 96>(pass, a, st);
-    return launch<T, 128>(pass, a, st);
+    if (a.width <= 32) return launch_filler<T, 32>(pass, a, st);
+    if (a.width <= 64) return launch_filler<T, 64>(pass, a, st);
+    if (a.width <= 96) return launch_filler<T, 96>(pass, a, st);
+    return launch_filler<T, 128>(pass, a, st);
 }
 int launch_type(int dtype, Pass pass, const Params& a, hipStream_t st) {
     if (dtype == GEFEN_F32) return launch_width<float>(pass, a, st);

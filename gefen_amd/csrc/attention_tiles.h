@@ -14,9 +14,13 @@
 // in that order (16-bit: two transposing ds_read_b64_tr_b16, four rows each) and p never
 // moves between lanes.  The softmax's maximum and sum need one exchange, between the halves.
 //
-// A tile is BN rows of DP elements, DP the head's width rounded up to 32 with zeros, and rows
-// are padded so that row reads (16 bytes of 8 rows at a time) and transposing reads (4 rows x
-// 32 bytes) spread over all banks.
+// A tile is BN rows of DP elements, DP the head's width rounded up to 32 with zeros.  It is
+// filled straight from global memory (loads with the LDS destination: no registers on the
+// way), where a wave's 64 lanes write 1024 contiguous bytes; so rows are not padded, but the
+// 16-byte chunks of a row are permuted by an XOR with bits of the row, and a lane fetches the
+// chunk that belongs at its place.  The XOR spreads what one read takes at a time over all 64
+// banks: 16 rows of one chunk, and 4 rows of four neighbouring ones (the transposing read).
+// Heads whose rows are no whole aligned chunks come through registers (ASYNC false).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -36,9 +40,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 template <typename T>
 struct Elem {
-    static constexpr int EPC = 16 / sizeof(T);           // elements of a 16-byte chunk
-    static constexpr int PAD = sizeof(T) == 2 ? 16 : 8;  // elements between rows of a tile
-    using Raw = typename RawVec<sizeof(T)>::type;        // what LDS holds
+    static constexpr int EPC = 16 / sizeof(T);     // elements of a 16-byte chunk
+    using Raw = typename RawVec<sizeof(T)>::type;  // what LDS holds
     __device__ __forceinline__ static float value(Raw r) {
         T t;
         __builtin_memcpy(&t, &r, sizeof(T));
@@ -108,23 +111,34 @@ __device__ __forceinline__ bool drop_nonfinite(uint32_t& x) {
     }
 }
 
+// The XOR of row r's chunks, `chunks` a row.
+constexpr __device__ __forceinline__ int chunk_xor(int r, int chunks) {
+    return chunks % 16 == 0  ? (r & 3) << 2 | ((r >> 2) & 3)
+           : chunks % 8 == 0 ? ((r >> 1) & 1) << 2 | ((r >> 2) & 3)
+                             : (r >> 2) & 3;
+}
+
 template <typename T, int BN, int DP>
 struct Tile {
-    static constexpr int EPC = Elem<T>::EPC, LD = DP + Elem<T>::PAD;
-    static constexpr int BYTES = BN * LD * (int)sizeof(T);
+    static constexpr int EPC = Elem<T>::EPC, LD = DP;
+    static constexpr int ELEMS = BN * LD, BYTES = ELEMS * (int)sizeof(T);
     static constexpr int CPR = DP / EPC;  // chunks of a row
     // LDS pointers keep their address space
     typedef __attribute__((address_space(3))) typename Elem<T>::Raw lds_t;
     typedef __attribute__((address_space(3))) u32x4 lds_chunk;
     lds_t* p;
 
-    __device__ __forceinline__ void put(int row, int c, u32x4 v) const { *(lds_chunk*)(p + row * LD + c * EPC) = v; }
-
-    // chunk c of the rows product's left side: row r0 + lane % 32
-    __device__ __forceinline__ u32x4 row_chunk(int r0, int c, int lane) const {
-        return *(const lds_chunk*)(p + (r0 + (lane & 31)) * LD + (2 * c + (lane >> 5)) * EPC);
+    // element d of row r
+    __device__ __forceinline__ static int place(int r, int d) {
+        return r * LD + ((d / EPC) ^ chunk_xor(r, CPR)) * EPC + d % EPC;
     }
-    // acc[d0 + .., n] += sum over rows r0 .. r0 + 15.  CHECK: what is not finite counts as
+    __device__ __forceinline__ void put(int row, int c, u32x4 v) const { *(lds_chunk*)(p + place(row, c * EPC)) = v; }
+
+    // chunk c of the rows product's left side: row r0 + lane % 32 (r0 a multiple of 32)
+    __device__ __forceinline__ u32x4 row_chunk(int r0, int c, int lane) const {
+        return *(const lds_chunk*)(p + r0 * LD + place(lane & 31, (2 * c + (lane >> 5)) * EPC));
+    }
+    // acc[d0 + .., n] += sum over rows r0 .. r0 + 15 (r0 a multiple of 16).  CHECK: what is not finite counts as
     // zero, and *bad tells.
     template <bool CHECK>
     __device__ __forceinline__ f32x16 mma_columns(const PFrag<T>& b, int r0, int d0, int lane, f32x16 acc,
@@ -133,7 +147,7 @@ struct Tile {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                uint32_t a = p[(r0 + 8 * (i / 4) + 4 * h + i % 4) * LD + d0 + (lane & 31)];
+                uint32_t a = p[r0 * LD + place(8 * (i / 4) + 4 * h + i % 4, d0 + (lane & 31))];
                 if (CHECK) *bad |= drop_nonfinite<T>(a);
                 acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a), b.v[i], acc, 0, 0, 0);
             }
@@ -141,11 +155,10 @@ struct Tile {
         } else {
             // in each group of 16 lanes, lane 4 j + q points at row j, elements 4 q .. 4 q + 3
             typedef __attribute__((address_space(3))) bf16x4 lds_v4;
-            const int row = r0 + 4 * h + ((lane & 15) >> 2);
+            const int row = 4 * h + ((lane & 15) >> 2);
             const int col = d0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-            lds_t* at = p + row * LD + col;
-            const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4*)at);
-            const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4*)(at + 8 * LD));
+            const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4*)(p + r0 * LD + place(row, col)));
+            const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4*)(p + r0 * LD + place(row + 8, col)));
             u32x4 a = __builtin_bit_cast(u32x4, bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
             if (CHECK) {
 #pragma unroll
@@ -175,13 +188,32 @@ struct Tile {
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float v = Elem<T>::value(p[r * LD + 32 * dt + 8 * (i / 4) + 4 * h + i % 4]);
+                    const float v = Elem<T>::value(p[place(r, 32 * dt + 8 * (i / 4) + 4 * h + i % 4)]);
                     const bool bad = (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u;
                     if (bad && seen) acc[dt][i] += AS_NAN ? __uint_as_float(0x7fc00000u) : v;
                 }
         }
     }
 };
+
+// BYTES from each active lane's address to its place after lds (wave-uniform): lane * BYTES.
+// Written as assembly because the compiler otherwise holds every transposing LDS read back
+// until all such loads in flight have landed; it has no register result, and
+// wait_loads_and_sync waits for it.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: the compiler sets it before each use of its own
+template <int BYTES>
+__device__ __forceinline__ void load_to_lds(const void* at, uint32_t lds) {
+    static_assert(BYTES == 4 || BYTES == 16, "");
+    if constexpr (BYTES == 16)
+        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(at) : "m0");
+    else asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(at) : "m0");
+}
+#pragma clang diagnostic pop
+// This wave's loads to LDS have landed and its LDS reads are done, then the barrier.
+__device__ __forceinline__ void wait_loads_and_sync() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
 
 // EPC elements from p, of which the first `n` exist (n >= 1); zeros for the others.
 template <typename T>
