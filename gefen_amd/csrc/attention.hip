@@ -103,19 +103,21 @@ struct Span {
         full_lo = wave_max(r.lo);
         full_hi = wave_min(r.hi);
     }
-    __device__ __forceinline__ bool none(int r0) const { return r0 >= hi || r0 + BN <= lo; }
-    __device__ __forceinline__ bool full(int r0) const { return full_lo <= r0 && r0 + BN <= full_hi; }
+    // of the n rows from r0 on
+    __device__ __forceinline__ bool none(int r0, int n) const { return r0 >= hi || r0 + n <= lo; }
+    __device__ __forceinline__ bool full(int r0, int n) const { return full_lo <= r0 && r0 + n <= full_hi; }
 };
 // The span of the workgroup's waves (lo, hi only).
+template <int THREADS>
 __device__ __forceinline__ Interval block_span(const Span& s) {
-    __shared__ int part[2][kThreads / 64];
+    __shared__ int part[2][THREADS / 64];
     if ((threadIdx.x & 63) == 0) {
         part[0][threadIdx.x >> 6] = s.lo;
         part[1][threadIdx.x >> 6] = s.hi;
     }
     __syncthreads();
     Interval r = {part[0][0], part[1][0]};
-    for (int w = 1; w < kThreads / 64; ++w) {
+    for (int w = 1; w < THREADS / 64; ++w) {
         r.lo = min(r.lo, part[0][w]);
         r.hi = max(r.hi, part[1][w]);
     }
@@ -147,22 +149,25 @@ struct Rows {
 // aligned and a width of whole chunks (what lies behind the width is cleared once, by
 // clear_tiles); issue() starts the loads and the caller waits for them.  Otherwise issue()
 // takes the rows into registers and land() writes them.
-template <typename T, int DP, bool ASYNC>
+template <typename T, int ROWS, int DP, bool ASYNC, int THREADS>
 struct Filler {
-    using TileT = Tile<T, BN, DP>;
-    static constexpr int CPR = TileT::CPR, LOADS = BN * CPR / kThreads, EPC = Elem<T>::EPC;
+    using TileT = Tile<T, ROWS, DP>;
+    static constexpr int CPR = TileT::CPR, CHUNKS = ROWS * CPR, EPC = Elem<T>::EPC;
+    static constexpr int LOADS = (CHUNKS + THREADS - 1) / THREADS;
+    static_assert(CHUNKS % 64 == 0, "whole waves");
     u32x4 r[ASYNC ? 1 : LOADS];
     template <bool GROUPED>
     __device__ __forceinline__ void issue(const Params& a, const Rows<T, GROUPED>& rows, int r0, const TileT& t) {
         const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(t.p + ((int)threadIdx.x >> 6) * 64 * EPC));
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            const int q = (int)threadIdx.x + kThreads * i, row = q / CPR;
+            const int q = (int)threadIdx.x + THREADS * i, row = q / CPR;
+            if (CHUNKS % THREADS && q >= CHUNKS) continue;
             const int c = (q % CPR) ^ (ASYNC ? chunk_xor(row, CPR) : 0);
             const int n = a.width - c * EPC;
             const T* at = rows.at(a, min(r0 + row, rows.count - 1)) + c * EPC;
             if constexpr (ASYNC) {
-                if (n > 0) load_to_lds<16>(at, lds + i * kThreads * 16);
+                if (n > 0) load_to_lds<16>(at, lds + i * THREADS * 16);
             } else {
                 r[i] = n > 0 ? load_chunk(at, n) : u32x4{0u, 0u, 0u, 0u};
             }
@@ -172,29 +177,34 @@ struct Filler {
         if constexpr (!ASYNC) {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
-                const int q = (int)threadIdx.x + kThreads * i;
+                const int q = (int)threadIdx.x + THREADS * i;
+                if (CHUNKS % THREADS && q >= CHUNKS) continue;
                 t.put(q / CPR, q % CPR, r[i]);
             }
         }
     }
 };
+// Zeros behind the rows' width, which asynchronous loads leave as they are.
+template <int THREADS>
+__device__ __forceinline__ void clear_tiles(char* smem, int bytes) {
+    typedef __attribute__((address_space(3))) u32x4 lds_chunk;
+    lds_chunk* p = (lds_chunk*)smem;
+    for (int i = threadIdx.x; i < bytes / 16; i += THREADS) p[i] = u32x4{0u, 0u, 0u, 0u};
+}
 
-// The tiles of two operands, twice: one pair is filled while the other is worked on.
-template <typename T, int DP, bool ASYNC, bool GROUPED>
+// The tiles of keys and values, twice: one pair is filled while the other is worked on.
+template <typename T, int DP, bool ASYNC>
 struct Pipe {
     using TileT = Tile<T, BN, DP>;
     static constexpr int BYTES = 4 * TileT::BYTES;
     const Params& a;
-    Rows<T, GROUPED> x, y;
+    Rows<T, false> x, y;
     typename TileT::lds_t* base;
-    Filler<T, DP, ASYNC> fx, fy;
+    Filler<T, BN, DP, ASYNC, kThreads> fx, fy;
 
     __device__ __forceinline__ Pipe(const Params& a, const View& vx, const View& vy, int b, int hk, char* smem)
         : a(a), x(a, vx, b, hk), y(a, vy, b, hk), base((typename TileT::lds_t*)smem) {
-        if (ASYNC && a.width < DP) {
-            __attribute__((address_space(3))) u32x4* p = (__attribute__((address_space(3))) u32x4*)base;
-            for (int i = threadIdx.x; i < BYTES / 16; i += kThreads) p[i] = u32x4{0u, 0u, 0u, 0u};
-        }
+        if (ASYNC && a.width < DP) clear_tiles<kThreads>(smem, BYTES);
         __syncthreads();
     }
     __device__ __forceinline__ TileT tile(int buffer, int which) const {
@@ -208,25 +218,20 @@ struct Pipe {
         fx.land(tile(buffer, 0));
         fy.land(tile(buffer, 1));
     }
-    // step(r0, first tile, second tile, buffer) for the tiles of [all.lo, all.hi); more(r0,
-    // buffer) loads what else the step needs.
-    template <typename More, typename Step>
-    __device__ __forceinline__ void run(Interval all, More more, Step step) {
+    // step(r0, keys, values) for the tiles of [all.lo, all.hi).
+    template <typename Step>
+    __device__ __forceinline__ void run(Interval all, Step step) {
         if (all.hi <= all.lo) return;
         int r0 = all.lo / BN * BN;
         issue(r0, 0);
-        more(r0, 0);
         if (!ASYNC) land(0);
         auto one = [&](auto which) __attribute__((always_inline)) {
             constexpr int buffer = decltype(which)::value;
             // this buffer has landed, and every wave is done with the other one
             wait_loads_and_sync();
             const bool next = r0 + BN < all.hi;
-            if (next) {
-                issue(r0 + BN, 1 - buffer);
-                more(r0 + BN, 1 - buffer);
-            }
-            step(r0, tile(buffer, 0), tile(buffer, 1), buffer);
+            if (next) issue(r0 + BN, 1 - buffer);
+            step(r0, tile(buffer, 0), tile(buffer, 1));
             if (!ASYNC && next) land(1 - buffer);
             r0 += BN;
             return next;
@@ -263,8 +268,8 @@ struct Column {
     }
 };
 
-template <typename T, int DP>
-__device__ __forceinline__ f32x16 rows_product(const Tile<T, BN, DP>& t, int r0, const Column<T, DP>& x, int lane) {
+template <typename T, int ROWS, int DP>
+__device__ __forceinline__ f32x16 rows_product(const Tile<T, ROWS, DP>& t, int r0, const Column<T, DP>& x, int lane) {
     f32x16 acc = {};
 #pragma unroll
     for (int c = 0; c < Column<T, DP>::STEPS; ++c) acc = mma_rows<T>(t.row_chunk(r0, c, lane), x.c[c], acc);
@@ -302,7 +307,7 @@ constexpr float kBackwardShift = kHalf<T> ? 14.0f : 0.0f;
 template <typename T, int DP, bool ASYNC>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_forward(Params a) {
     using TileT = Tile<T, BN, DP>;
-    using PipeT = Pipe<T, DP, ASYNC, false>;
+    using PipeT = Pipe<T, DP, ASYNC>;
     constexpr int DT = DP / 32;
     extern __shared__ __attribute__((aligned(1024))) char smem[];  // PipeT::BYTES
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -314,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_forward(Pa
     const Interval seen = keys_of(a, b, div_group(a, uc));
     Span span;
     span.of(seen);
-    const Interval all = block_span(span);
+    const Interval all = block_span<kThreads>(span);
 
     const Rows<T, true> queries(a, a.q, b, hk);
     PipeT pipe(a, a.k, a.v, b, hk, smem);
@@ -369,9 +374,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_forward(Pa
         if (PARTIAL && __any(bad)) vt.template add_nonfinite<false>(acc, BN, seen.lo - k0, seen.hi - k0, lane);
     };
 
-    pipe.run(all, [](int, int) {}, [&](int k0, const TileT& kt, const TileT& vt, int) __attribute__((always_inline)) {
-        if (span.none(k0)) return;
-        if (span.full(k0)) tile_step(std::false_type{}, k0, kt, vt);
+    pipe.run(all, [&](int k0, const TileT& kt, const TileT& vt) __attribute__((always_inline)) {
+        if (span.none(k0, BN)) return;
+        if (span.full(k0, BN)) tile_step(std::false_type{}, k0, kt, vt);
         else tile_step(std::true_type{}, k0, kt, vt);
     });
     sum += other_half(sum);
@@ -440,7 +445,7 @@ __global__ void __launch_bounds__(kThreads) k_range(Params a) {
 template <typename T, int DP, bool ASYNC>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_queries(Params a) {
     using TileT = Tile<T, BN, DP>;
-    using PipeT = Pipe<T, DP, ASYNC, false>;
+    using PipeT = Pipe<T, DP, ASYNC>;
     constexpr int DT = DP / 32;
     extern __shared__ __attribute__((aligned(1024))) char smem[];  // PipeT::BYTES
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -451,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
     const Interval seen = keys_of(a, b, div_group(a, uc));
     Span span;
     span.of(seen);
-    const Interval all = block_span(span);
+    const Interval all = block_span<kThreads>(span);
 
     PipeT pipe(a, a.k, a.v, b, hk, smem);
     Column<T, DP> q, go;
@@ -497,9 +502,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
         if (PARTIAL && __any(bad)) kt.template add_nonfinite<true>(acc, BN, seen.lo - k0, seen.hi - k0, lane);
     };
 
-    pipe.run(all, [](int, int) {}, [&](int k0, const TileT& kt, const TileT& vt, int) __attribute__((always_inline)) {
-        if (span.none(k0)) return;
-        if (span.full(k0)) tile_step(std::false_type{}, k0, kt, vt);
+    pipe.run(all, [&](int k0, const TileT& kt, const TileT& vt) __attribute__((always_inline)) {
+        if (span.none(k0, BN)) return;
+        if (span.full(k0, BN)) tile_step(std::false_type{}, k0, kt, vt);
         else tile_step(std::true_type{}, k0, kt, vt);
     });
     if (u >= a.rows) return;
@@ -508,15 +513,30 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
     store_column(out, acc, kHalf<T> ? a.scale * (1.0f / 16384.0f) / unit : a.scale, a.width, lane);
 }
 
-// dK and dV.
+// dK and dV.  The accumulators of both beside a lane's key and value leave no room for a
+// second wave on a SIMD, so two waves share 32 keys: the first forms P, dV += P dO and leaves
+// P (rounded, as it enters that product) in LDS, the second forms dP, dS = P (dP - D) and dK
+// += dS Q, one step of KS rows behind.
+constexpr int kKeyThreads = 512;
+constexpr int KS = 32;
+template <typename T, int DP>
+struct KeysLds {
+    using TileT = Tile<T, KS, DP>;
+    static constexpr int RING = 3;  // steps in LDS: the next one's loads, the first waves', the second waves'
+    static constexpr int P_CHUNKS = KS * 32 * (int)sizeof(T) / 16;  // of P of 32 keys
+    static constexpr int TILES = 2 * RING * TileT::BYTES, P = 2 * 4 * P_CHUNKS * 16, STATS = 2 * RING * KS * 4;
+    static constexpr int BYTES = TILES + P + STATS;
+};
 template <typename T, int DP, bool ASYNC>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && DP < 96 ? 2 : 1) k_backward_keys(Params a) {
-    using TileT = Tile<T, BN, DP>;
-    using PipeT = Pipe<T, DP, ASYNC, true>;
-    constexpr int DT = DP / 32;
-    extern __shared__ __attribute__((aligned(1024))) char smem[];  // PipeT::BYTES
-    __shared__ __attribute__((aligned(16))) float row_stats[2][2][BN];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__global__ void __launch_bounds__(kKeyThreads, 2) k_backward_keys(Params a) {
+    using Lds = KeysLds<T, DP>;
+    using TileT = typename Lds::TileT;
+    typedef __attribute__((address_space(3))) float lds_float;
+    typedef __attribute__((address_space(3))) u32x4 lds_chunk;
+    constexpr int DT = DP / 32, PV = Lds::P_CHUNKS / 64;  // chunks of P a lane
+    extern __shared__ __attribute__((aligned(1024))) char smem[];  // Lds::BYTES
+    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3;
+    const bool second = threadIdx.x >= kKeyThreads / 2;
     // the keys that most rows see first
     const int heads = a.batch * a.kv_heads;
     const int bh = blockIdx.x % heads, tile = blockIdx.x / heads;
@@ -527,67 +547,124 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && DP < 96 ? 2 : 1) k
     seen.hi *= a.group;
     Span span;
     span.of(seen);
-    const Interval all = block_span(span);
+    const Interval all = block_span<kKeyThreads>(span);
 
-    PipeT pipe(a, a.q, a.go, b, hk, smem);
-    Column<T, DP> k, v;
-    k.load(Rows<T, false>(a, a.k, b, hk).at(a, jc), a.width, lane);
-    v.load(Rows<T, false>(a, a.v, b, hk).at(a, jc), a.width, lane);
+    const Rows<T, true> queries(a, a.q, b, hk), grads(a, a.go, b, hk);
+    if (ASYNC && a.width < DP) clear_tiles<kKeyThreads>(smem, Lds::TILES);
+    __syncthreads();
+    Column<T, DP> x;  // the key, or (second) the value
+    x.load(second ? Rows<T, false>(a, a.v, b, hk).at(a, jc) : Rows<T, false>(a, a.k, b, hk).at(a, jc), a.width, lane);
     float unit = 1.0f;
     if constexpr (kHalf<T>) unit = into_one(2.0f * largest_norm(a, 0, bh) * largest_norm(a, 1, bh));
-    f32x16 dk[DT], dv[DT];
+    f32x16 acc[DT];  // dV, or (second) dK
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) dk[dt] = dv[dt] = f32x16{};
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
 
-    auto tile_step = [&](auto partial, int u0, const TileT& qt, const TileT& gt,
-                         const float (&stats)[2][BN]) __attribute__((always_inline)) {
+    typename TileT::lds_t* const tiles = (typename TileT::lds_t*)smem;
+    lds_chunk* const probs = (lds_chunk*)(smem + Lds::TILES) + wave * Lds::P_CHUNKS + lane;  // + 4 P_CHUNKS the other step's
+    lds_float* const stats = (lds_float*)(smem + Lds::TILES + Lds::P);
+    Filler<T, KS, DP, ASYNC, kKeyThreads> fq, fg;
+    auto query_tile = [&](int slot) { return TileT{tiles + 2 * slot * TileT::ELEMS}; };
+    auto grad_tile = [&](int slot) { return TileT{tiles + (2 * slot + 1) * TileT::ELEMS}; };
+    auto issue = [&](int u0, int slot) __attribute__((always_inline)) {
+        fq.issue(a, queries, u0, query_tile(slot));
+        fg.issue(a, grads, u0, grad_tile(slot));
+        // two half waves take the rows' L and D along
+        const int w = threadIdx.x >> 6;
+        if (w < 2 && lane < KS)
+            load_to_lds<4>((w ? a.delta : a.lse) + (int64_t)bh * a.rows + min(u0 + lane, a.rows - 1),
+                           __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(stats + (2 * slot + w) * KS)));
+    };
+    auto land = [&](int slot) __attribute__((always_inline)) {
+        fq.land(query_tile(slot));
+        fg.land(grad_tile(slot));
+    };
+
+    auto first_step = [&](auto partial, int u0, int slot, int parity) __attribute__((always_inline)) {
         constexpr bool PARTIAL = decltype(partial)::value;
-        bool bad_q = false, bad_g = false;
-#pragma unroll 1
-        for (int t = 0; t < 2; ++t) {
-            f32x16 s = rows_product(qt, 32 * t, k, lane);
-            f32x16 dp = rows_product(gt, 32 * t, v, lane);
+        const TileT qt = query_tile(slot), gt = grad_tile(slot);
+        f32x16 s = rows_product(qt, 0, x, lane);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int r = row_of(32 * t, i, lane);
-                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, kBackwardShift<T> - stats[0][r]));
-                const float d = dp[i] - stats[1][r];
-                float ds = kHalf<T> ? p * (d * unit) : p * d;
-                if (PARTIAL && !within(u0 + r, seen)) p = ds = 0.0f;
-                s[i] = p;
-                dp[i] = ds;
-            }
+        for (int i = 0; i < 16; ++i) {
+            const int r = row_of(0, i, lane);
+            s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, kBackwardShift<T> - stats[2 * slot * KS + r]));
+            if (PARTIAL && !within(u0 + r, seen)) s[i] = 0.0f;
+        }
+        bool bad = false;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const PFrag<T> p = pack<T>(s, c), ds = pack<T>(dp, c);
+        for (int c = 0; c < 2; ++c) {
+            const PFrag<T> p = pack<T>(s, c);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    dv[dt] = gt.template mma_columns<PARTIAL>(p, 32 * t + 16 * c, 32 * dt, lane, dv[dt], &bad_g);
-                    dk[dt] = qt.template mma_columns<PARTIAL>(ds, 32 * t + 16 * c, 32 * dt, lane, dk[dt], &bad_q);
-                }
+            for (int k = 0; k < PV / 2; ++k)
+                probs[parity * 4 * Lds::P_CHUNKS + (PV / 2 * c + k) * 64] = reinterpret_cast<const u32x4*>(&p)[k];
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+                acc[dt] = gt.template mma_columns<PARTIAL>(p, 16 * c, 32 * dt, lane, acc[dt], &bad);
+        }
+        if (PARTIAL && __any(bad)) gt.template add_nonfinite<false>(acc, KS, seen.lo - u0, seen.hi - u0, lane);
+    };
+    auto second_step = [&](auto partial, int u0, int slot, int parity) __attribute__((always_inline)) {
+        constexpr bool PARTIAL = decltype(partial)::value;
+        const TileT qt = query_tile(slot), gt = grad_tile(slot);
+        f32x16 ds = rows_product(gt, 0, x, lane);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            PFrag<T> p;
+#pragma unroll
+            for (int k = 0; k < PV / 2; ++k)
+                reinterpret_cast<u32x4*>(&p)[k] = probs[parity * 4 * Lds::P_CHUNKS + (PV / 2 * c + k) * 64];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = row_of(0, 8 * c + i, lane);
+                float d = ds[8 * c + i] - stats[(2 * slot + 1) * KS + r];
+                if (kHalf<T>) d *= unit;
+                d *= unpacked(p, i);
+                ds[8 * c + i] = PARTIAL && !within(u0 + r, seen) ? 0.0f : d;
             }
         }
-        if (PARTIAL && __any(bad_g)) gt.template add_nonfinite<false>(dv, BN, seen.lo - u0, seen.hi - u0, lane);
-        if (PARTIAL && __any(bad_q)) qt.template add_nonfinite<true>(dk, BN, seen.lo - u0, seen.hi - u0, lane);
+        bool bad = false;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const PFrag<T> p = pack<T>(ds, c);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+                acc[dt] = qt.template mma_columns<PARTIAL>(p, 16 * c, 32 * dt, lane, acc[dt], &bad);
+        }
+        if (PARTIAL && __any(bad)) qt.template add_nonfinite<true>(acc, KS, seen.lo - u0, seen.hi - u0, lane);
     };
 
-    // two waves' 64 lanes take the rows' L and D along
-    const float* stats = (wave ? a.delta : a.lse) + (int64_t)bh * a.rows;
-    const uint32_t stats_lds =
-        __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) float*)&row_stats[0][wave & 1][0]);
-    auto more = [&](int u0, int buffer) __attribute__((always_inline)) {
-        if (wave < 2) load_to_lds<4>(stats + min(u0 + lane, a.rows - 1), stats_lds + buffer * (uint32_t)sizeof(row_stats[0]));
-    };
-    pipe.run(all, more, [&](int u0, const TileT& qt, const TileT& gt, int buffer) __attribute__((always_inline)) {
-        if (span.none(u0)) return;
-        if (span.full(u0)) tile_step(std::false_type{}, u0, qt, gt, row_stats[buffer]);
-        else tile_step(std::true_type{}, u0, qt, gt, row_stats[buffer]);
-    });
+    if (all.hi > all.lo) {
+        int u0 = all.lo / KS * KS, slot = 0, parity = 0;
+        issue(u0, 0);
+        if (!ASYNC) land(0);
+        for (;; u0 += KS) {
+            // this step has landed, P of the last one is there, and every wave is done with the
+            // slot to fill next
+            wait_loads_and_sync();
+            const bool more = u0 + KS < all.hi, now = u0 < all.hi;
+            const int next = slot == Lds::RING - 1 ? 0 : slot + 1, last = slot == 0 ? Lds::RING - 1 : slot - 1;
+            if (more) issue(u0 + KS, next);
+            const int at = second ? u0 - KS : u0;
+            if ((second ? at >= all.lo / KS * KS : now) && !span.none(at, KS)) {
+                if (second) {
+                    if (span.full(at, KS)) second_step(std::false_type{}, at, last, parity ^ 1);
+                    else second_step(std::true_type{}, at, last, parity ^ 1);
+                } else {
+                    if (span.full(at, KS)) first_step(std::false_type{}, at, slot, parity);
+                    else first_step(std::true_type{}, at, slot, parity);
+                }
+            }
+            if (!ASYNC && more) land(next);
+            if (!now) break;
+            slot = next;
+            parity ^= 1;
+        }
+    }
     if (j >= a.keys) return;
-    T* gk = static_cast<T*>(a.gk.p) + b * a.gk.batch + j * a.gk.row + hk * a.gk.head;
-    T* gv = static_cast<T*>(a.gv.p) + b * a.gv.batch + j * a.gv.row + hk * a.gv.head;
-    store_column(gk, dk, kHalf<T> ? a.scale * (1.0f / 16384.0f) / unit : a.scale, a.width, lane);
-    store_column(gv, dv, kHalf<T> ? 1.0f / 16384.0f : 1.0f, a.width, lane);
+    const View& out = second ? a.gk : a.gv;
+    T* row = static_cast<T*>(out.p) + b * out.batch + j * out.row + hk * out.head;
+    const float down = kHalf<T> ? 1.0f / 16384.0f : 1.0f;
+    store_column(row, acc, second ? a.scale * down / unit : down, a.width, lane);
 }
 
 // ------------------------------------------------------------------ host side
@@ -599,10 +676,10 @@ int launch(Pass pass, const Params& a, hipStream_t st) {
     const int64_t heads = (int64_t)a.batch * a.kv_heads;
     const int64_t cols = pass == kKeysPass ? a.keys : a.rows;
     const dim3 grid((uint32_t)(heads * ((cols + kCols - 1) / kCols)));
-    constexpr int lds = Pipe<T, DP, ASYNC, false>::BYTES;
+    constexpr int lds = Pipe<T, DP, ASYNC>::BYTES;
     if (pass == kForwardPass) k_forward<T, DP, ASYNC><<<grid, kThreads, lds, st>>>(a);
     else if (pass == kQueriesPass) k_backward_queries<T, DP, ASYNC><<<grid, kThreads, lds, st>>>(a);
-    else k_backward_keys<T, DP, ASYNC><<<grid, kThreads, lds, st>>>(a);
+    else k_backward_keys<T, DP, ASYNC><<<grid, kKeyThreads, KeysLds<T, DP>::BYTES, st>>>(a);
     return launch_status("attention");
 }
 // Whether a tensor's rows are whole 16-byte chunks.

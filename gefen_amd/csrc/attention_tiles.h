@@ -73,7 +73,7 @@ struct PFrag {
     u32x4 v;
 };
 template <>
-struct PFrag<float> {
+struct alignas(16) PFrag<float> {
     float v[8];
 };
 template <typename T>
@@ -94,6 +94,13 @@ __device__ __forceinline__ PFrag<T> pack(const f32x16& p, int chunk) {
         out.v = __builtin_bit_cast(u32x4, t);
     }
     return out;
+}
+
+// Element i of them as float32.
+template <typename T>
+__device__ __forceinline__ float unpacked(const PFrag<T>& p, int i) {
+    if constexpr (sizeof(T) == 4) return p.v[i];
+    else return Elem<T>::value((uint16_t)(p.v[i / 2] >> (16 * (i & 1))));
 }
 
 // Zeros in place of what is not finite; true if there was any.
