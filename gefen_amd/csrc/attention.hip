@@ -39,8 +39,8 @@ struct View {
 
 struct Params {
     View q, k, v, o, go, gq, gk, gv;
-    float* lse;    // [batch, kv_heads, U], log2 of the sum of exp2(c S): 0 for a row without keys
-    float* delta;  // [batch, kv_heads, U]
+    float* lse;    // [batch, heads, queries], log2 of the sum of exp2(c S): 0 for a row without keys
+    float* delta;  // [batch, heads, queries]
     float* range;  // half precision: [2][batch * kv_heads][kRangeParts] largest norms of rows of v and of go
     const void* key_lengths;
     const void* offsets;
@@ -103,25 +103,30 @@ struct Span {
         full_lo = wave_max(r.lo);
         full_hi = wave_min(r.hi);
     }
-    // of the n rows from r0 on
-    __device__ __forceinline__ bool none(int r0, int n) const { return r0 >= hi || r0 + n <= lo; }
-    __device__ __forceinline__ bool full(int r0, int n) const { return full_lo <= r0 && r0 + n <= full_hi; }
+    // of the tile from r0 on
+    __device__ __forceinline__ bool none(int r0) const { return r0 >= hi || r0 + BN <= lo; }
+    __device__ __forceinline__ bool full(int r0) const { return full_lo <= r0 && r0 + BN <= full_hi; }
 };
 // The span of the workgroup's waves (lo, hi only).
-template <int THREADS>
 __device__ __forceinline__ Interval block_span(const Span& s) {
-    __shared__ int part[2][THREADS / 64];
+    __shared__ int part[2][kThreads / 64];
     if ((threadIdx.x & 63) == 0) {
         part[0][threadIdx.x >> 6] = s.lo;
         part[1][threadIdx.x >> 6] = s.hi;
     }
     __syncthreads();
     Interval r = {part[0][0], part[1][0]};
-    for (int w = 1; w < THREADS / 64; ++w) {
+    for (int w = 1; w < kThreads / 64; ++w) {
         r.lo = min(r.lo, part[0][w]);
         r.hi = max(r.hi, part[1][w]);
     }
-    return r;
+    return {uniform(r.lo), uniform(r.hi)};
+}
+
+// Place of row u in lse and delta.
+__device__ __forceinline__ int64_t stat_at(const Params& a, int bh, int u) {
+    const int i = div_group(a, u);
+    return ((int64_t)bh * a.group + u - i * a.group) * a.queries + i;
 }
 
 // Rows of a view: of keys, or (GROUPED) rows u of queries.
@@ -145,95 +150,136 @@ struct Rows {
     }
 };
 
-// Fills a tile.  Rows past the last one are read as the last.  ASYNC: rows are 16-byte
-// aligned and a width of whole chunks (what lies behind the width is cleared once, by
-// clear_tiles); issue() starts the loads and the caller waits for them.  Otherwise issue()
-// takes the rows into registers and land() writes them.
+// Fills two tiles, one behind the other, from rows r0 .. of two operands.  ASYNC: rows are
+// 16-byte aligned and a width of whole chunks (what lies behind the width is cleared once); issue() starts LOADS loads of a wave, for which the caller waits, each lane at
+// an offset of its own that stays the same from tile to tile.  What lies behind the last row
+// is left as it is: no step takes a row that it does not see.  Otherwise (ASYNC false) issue()
+// takes the rows into registers, the last one again behind it, and land() writes them.
 template <typename T, int ROWS, int DP, bool ASYNC, int THREADS>
 struct Filler {
     using TileT = Tile<T, ROWS, DP>;
-    static constexpr int CPR = TileT::CPR, CHUNKS = ROWS * CPR, EPC = Elem<T>::EPC;
-    static constexpr int LOADS = (CHUNKS + THREADS - 1) / THREADS;
-    static_assert(CHUNKS % 64 == 0, "whole waves");
+    static constexpr int CPR = TileT::CPR, CHUNKS = ROWS * CPR, EPC = Elem<T>::EPC, LOADS = 2 * CHUNKS / THREADS;
+    static_assert(LOADS * THREADS == 2 * CHUNKS && CHUNKS % 64 == 0, "whole loads, whole waves a tile");
+    static constexpr uint32_t kBehind = 0xffffffffu;  // the offset of a chunk behind the width
+    const int64_t row_x, row_y;                       // elements (ASYNC: ROWS of them are less than 2^30 bytes)
+    const int width, count;
+    const uint32_t lds;
+    uint32_t off[ASYNC ? LOADS : 1];
     u32x4 r[ASYNC ? 1 : LOADS];
-    template <bool GROUPED>
-    __device__ __forceinline__ void issue(const Params& a, const Rows<T, GROUPED>& rows, int r0, const TileT& t) {
-        const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(t.p + ((int)threadIdx.x >> 6) * 64 * EPC));
+
+    // base: of the first tile, in LDS
+    __device__ __forceinline__ Filler(const View& x, const View& y, int width, int count, typename TileT::lds_t* base)
+        : row_x(x.row),
+          row_y(y.row),
+          width(width),
+          count(count),
+          lds(uniform((int)(uint32_t)(uintptr_t)(base + ((int)threadIdx.x >> 6) * 64 * EPC))) {
+        if constexpr (ASYNC) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int q = (int)threadIdx.x + THREADS * i, row = q / CPR;
-            if (CHUNKS % THREADS && q >= CHUNKS) continue;
-            const int c = (q % CPR) ^ (ASYNC ? chunk_xor(row, CPR) : 0);
-            const int n = a.width - c * EPC;
-            const T* at = rows.at(a, min(r0 + row, rows.count - 1)) + c * EPC;
-            if constexpr (ASYNC) {
-                if (n > 0) load_to_lds<16>(at, lds + i * THREADS * 16);
-            } else {
-                r[i] = n > 0 ? load_chunk(at, n) : u32x4{0u, 0u, 0u, 0u};
+            for (int i = 0; i < LOADS; ++i) {
+                const int c = chunk(i, threadIdx.x) * EPC;
+                off[i] = c < width
+                             ? (uint32_t)((row(i, threadIdx.x) * (int)(second(i) ? row_y : row_x) + c) * (int)sizeof(T))
+                             : kBehind;
             }
         }
     }
+    // load i of thread t
+    __device__ __forceinline__ static int id(int i, int t) { return t + THREADS * i; }
+    // whether it belongs to y (the same for a wave)
+    __device__ __forceinline__ static bool second(int i) {
+        if (THREADS * (i + 1) <= CHUNKS) return false;
+        if (THREADS * i >= CHUNKS) return true;
+        return uniform(id(i, threadIdx.x)) >= CHUNKS;
+    }
+    __device__ __forceinline__ static int row(int i, int t) { return (unsigned)id(i, t) % CHUNKS / CPR; }
+    __device__ __forceinline__ static int chunk(int i, int t) {
+        return ((unsigned)id(i, t) % CPR) ^ (ASYNC ? chunk_xor(row(i, t), CPR) : 0);
+    }
+    // x, y: row 0 of the operands
+    __device__ __forceinline__ void issue(const T* x, const T* y, int r0, uint32_t tile_bytes) {
+        int t = threadIdx.x;
+        if constexpr (ASYNC) {
+            x += r0 * row_x;
+            y += r0 * row_y;
+            const uint32_t to = lds + tile_bytes;
+            const bool tail = r0 + ROWS > count;
+            asm volatile("" : "+v"(t));  // rows are not kept in registers for the last tile's sake
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                bool have = off[i] != kBehind;
+                if (tail) have = have && r0 + row(i, t) < count;
+                if (have) load_to_lds(second(i) ? y : x, off[i], to + i * THREADS * 16);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int n = width - chunk(i, t) * EPC;
+                const T* at = (second(i) ? y : x) + min(r0 + row(i, t), count - 1) * (second(i) ? row_y : row_x);
+                r[i] = n > 0 ? load_chunk(at + chunk(i, t) * EPC, n) : u32x4{0u, 0u, 0u, 0u};
+            }
+        }
+    }
+    // t: the first tile
     __device__ __forceinline__ void land(const TileT& t) const {
         if constexpr (!ASYNC) {
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const int q = (int)threadIdx.x + THREADS * i;
-                if (CHUNKS % THREADS && q >= CHUNKS) continue;
-                t.put(q / CPR, q % CPR, r[i]);
-            }
+            for (int i = 0; i < LOADS; ++i)
+                TileT{t.p + (second(i) ? TileT::ELEMS : 0)}.put(row(i, threadIdx.x), chunk(i, threadIdx.x), r[i]);
         }
     }
 };
-// Zeros behind the rows' width, which asynchronous loads leave as they are.
-template <int THREADS>
-__device__ __forceinline__ void clear_tiles(char* smem, int bytes) {
-    typedef __attribute__((address_space(3))) u32x4 lds_chunk;
-    lds_chunk* p = (lds_chunk*)smem;
-    for (int i = threadIdx.x; i < bytes / 16; i += THREADS) p[i] = u32x4{0u, 0u, 0u, 0u};
-}
-
-// The tiles of keys and values, twice: one pair is filled while the other is worked on.
+// The tiles of two operands, twice: one pair is filled while the other is worked on.
 template <typename T, int DP, bool ASYNC>
 struct Pipe {
     using TileT = Tile<T, BN, DP>;
     static constexpr int BYTES = 4 * TileT::BYTES;
-    const Params& a;
-    Rows<T, false> x, y;
     typename TileT::lds_t* base;
-    Filler<T, BN, DP, ASYNC, kThreads> fx, fy;
+    Filler<T, BN, DP, ASYNC, kThreads> fill;
+    const T *x, *y;  // row 0 of the operands
 
-    __device__ __forceinline__ Pipe(const Params& a, const View& vx, const View& vy, int b, int hk, char* smem)
-        : a(a), x(a, vx, b, hk), y(a, vy, b, hk), base((typename TileT::lds_t*)smem) {
-        if (ASYNC && a.width < DP) clear_tiles<kThreads>(smem, BYTES);
+    __device__ __forceinline__ Pipe(const View& vx, const View& vy, const T* x, const T* y, int width, int count, char* smem)
+        : base((typename TileT::lds_t*)smem), fill(vx, vy, width, count, base), x(x), y(y) {
+        if (ASYNC && width < DP) {  // zeros behind the rows' width, which the loads leave as they are
+            typedef __attribute__((address_space(3))) u32x4 lds_chunk;
+            lds_chunk* p = (lds_chunk*)base;
+            for (int i = threadIdx.x; i < BYTES / 16; i += kThreads) p[i] = u32x4{0u, 0u, 0u, 0u};
+        }
         __syncthreads();
     }
     __device__ __forceinline__ TileT tile(int buffer, int which) const {
         return TileT{base + (2 * buffer + which) * TileT::ELEMS};
     }
-    __device__ __forceinline__ void issue(int r0, int buffer) {
-        fx.issue(a, x, r0, tile(buffer, 0));
-        fy.issue(a, y, r0, tile(buffer, 1));
-    }
-    __device__ __forceinline__ void land(int buffer) const {
-        fx.land(tile(buffer, 0));
-        fy.land(tile(buffer, 1));
-    }
-    // step(r0, keys, values) for the tiles of [all.lo, all.hi).
-    template <typename Step>
-    __device__ __forceinline__ void run(Interval all, Step step) {
+    // step(r0, first tile, second tile, buffer) for the tiles of [all.lo, all.hi) of `heads`
+    // heads, head_x and head_y elements apart; more(head, r0, buffer) loads what else the step
+    // needs.
+    template <typename More, typename Step>
+    __device__ __forceinline__ void run(Interval all, int heads, int64_t head_x, int64_t head_y, More more, Step step) {
         if (all.hi <= all.lo) return;
-        int r0 = all.lo / BN * BN;
-        issue(r0, 0);
-        if (!ASYNC) land(0);
+        const int start = all.lo / BN * BN;
+        int r0 = start, head = 0;
+        fill.issue(x, y, r0, 0);
+        more(head, r0, 0);
+        fill.land(tile(0, 0));
         auto one = [&](auto which) __attribute__((always_inline)) {
             constexpr int buffer = decltype(which)::value;
             // this buffer has landed, and every wave is done with the other one
             wait_loads_and_sync();
-            const bool next = r0 + BN < all.hi;
-            if (next) issue(r0 + BN, 1 - buffer);
-            step(r0, tile(buffer, 0), tile(buffer, 1));
-            if (!ASYNC && next) land(1 - buffer);
+            const int now = r0;
             r0 += BN;
+            if (r0 >= all.hi) {
+                r0 = start;
+                ++head;
+                x += head_x;
+                y += head_y;
+            }
+            const bool next = head < heads;
+            if (next) {
+                fill.issue(x, y, r0, (1 - buffer) * 2 * TileT::BYTES);
+                more(head, r0, 1 - buffer);
+            }
+            step(now, tile(buffer, 0), tile(buffer, 1), buffer);
+            if (next) fill.land(tile(1 - buffer, 0));
             return next;
         };
         while (one(std::integral_constant<int, 0>{}) && one(std::integral_constant<int, 1>{})) {
@@ -319,10 +365,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_forward(Pa
     const Interval seen = keys_of(a, b, div_group(a, uc));
     Span span;
     span.of(seen);
-    const Interval all = block_span<kThreads>(span);
+    const Interval all = block_span(span);
 
     const Rows<T, true> queries(a, a.q, b, hk);
-    PipeT pipe(a, a.k, a.v, b, hk, smem);
+    const Rows<T, false> keys(a, a.k, b, hk), values(a, a.v, b, hk);
+    PipeT pipe(a.k, a.v, keys.base, values.base, a.width, a.keys, smem);
     Column<T, DP> q;
     q.load(queries.at(a, uc), a.width, lane);
     f32x16 acc[DT];
@@ -353,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_forward(Pa
             for (int dt = 0; dt < DT; ++dt) acc[dt] *= f;
         }
         const float shift = kForwardShift<T> - (top == -INFINITY ? 0.0f : top);
-        bool bad = false;
+        uint32_t bad = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -371,14 +418,15 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_forward(Pa
                     acc[dt] = vt.template mma_columns<PARTIAL>(p, 32 * t + 16 * c, 32 * dt, lane, acc[dt], &bad);
             }
         }
-        if (PARTIAL && __any(bad)) vt.template add_nonfinite<false>(acc, BN, seen.lo - k0, seen.hi - k0, lane);
+        if (PARTIAL && __any((bad & kBadBits<T>) != 0)) vt.template add_nonfinite<false>(acc, BN, seen.lo - k0, seen.hi - k0, lane);
     };
 
-    pipe.run(all, [&](int k0, const TileT& kt, const TileT& vt) __attribute__((always_inline)) {
-        if (span.none(k0, BN)) return;
-        if (span.full(k0, BN)) tile_step(std::false_type{}, k0, kt, vt);
+    auto step = [&](int k0, const TileT& kt, const TileT& vt, int) __attribute__((always_inline)) {
+        if (span.none(k0)) return;
+        if (span.full(k0)) tile_step(std::false_type{}, k0, kt, vt);
         else tile_step(std::true_type{}, k0, kt, vt);
-    });
+    };
+    pipe.run(all, 1, 0, 0, [](int, int, int) {}, step);
     sum += other_half(sum);
     if (u >= a.rows) return;
     const bool empty = seen.hi <= seen.lo;
@@ -386,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_forward(Pa
     T* out = static_cast<T*>(a.o.p) + b * a.o.batch + i * a.o.row + (int64_t)(hk * a.group + u - i * a.group) * a.o.head;
     store_column(out, acc, empty ? 1.0f : 1.0f / sum, a.width, lane);
     if (a.lse && lane < 32)
-        a.lse[(int64_t)bh * a.rows + u] = empty ? 0.0f : top + __builtin_amdgcn_logf(sum) - kForwardShift<T>;
+        a.lse[stat_at(a, bh, u)] = empty ? 0.0f : top + __builtin_amdgcn_logf(sum) - kForwardShift<T>;
 }
 
 // The power of two that brings values of up to `most` into [-1, 1].
@@ -456,17 +504,18 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
     const Interval seen = keys_of(a, b, div_group(a, uc));
     Span span;
     span.of(seen);
-    const Interval all = block_span<kThreads>(span);
+    const Interval all = block_span(span);
 
-    PipeT pipe(a, a.k, a.v, b, hk, smem);
+    const Rows<T, false> keys(a, a.k, b, hk), values(a, a.v, b, hk);
+    PipeT pipe(a.k, a.v, keys.base, values.base, a.width, a.keys, smem);
     Column<T, DP> q, go;
     go.load(Rows<T, true>(a, a.go, b, hk).at(a, uc), a.width, lane);
     q.load(Rows<T, true>(a, a.o, b, hk).at(a, uc), a.width, lane);
     float delta = go.dot(q);
     delta += other_half(delta);
-    if (lane < 32 && u < a.rows) a.delta[(int64_t)bh * a.rows + u] = delta;
+    if (lane < 32 && u < a.rows) a.delta[stat_at(a, bh, u)] = delta;
     q.load(Rows<T, true>(a, a.q, b, hk).at(a, uc), a.width, lane);
-    const float shift = kBackwardShift<T> - a.lse[(int64_t)bh * a.rows + uc];
+    const float shift = kBackwardShift<T> - a.lse[stat_at(a, bh, uc)];
     float unit = 1.0f;
     if constexpr (kHalf<T>) {
         float norm = go.dot(go);
@@ -479,8 +528,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
 
     auto tile_step = [&](auto partial, int k0, const TileT& kt, const TileT& vt) __attribute__((always_inline)) {
         constexpr bool PARTIAL = decltype(partial)::value;
-        bool bad = false;
-#pragma unroll
+        uint32_t bad = 0;
+#pragma unroll 1
         for (int t = 0; t < 2; ++t) {
             f32x16 s = rows_product(kt, 32 * t, q, lane);
             const f32x16 dp = rows_product(vt, 32 * t, go, lane);
@@ -499,172 +548,107 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
                     acc[dt] = kt.template mma_columns<PARTIAL>(ds, 32 * t + 16 * c, 32 * dt, lane, acc[dt], &bad);
             }
         }
-        if (PARTIAL && __any(bad)) kt.template add_nonfinite<true>(acc, BN, seen.lo - k0, seen.hi - k0, lane);
+        if (PARTIAL && __any((bad & kBadBits<T>) != 0)) kt.template add_nonfinite<true>(acc, BN, seen.lo - k0, seen.hi - k0, lane);
     };
 
-    pipe.run(all, [&](int k0, const TileT& kt, const TileT& vt) __attribute__((always_inline)) {
-        if (span.none(k0, BN)) return;
-        if (span.full(k0, BN)) tile_step(std::false_type{}, k0, kt, vt);
+    auto step = [&](int k0, const TileT& kt, const TileT& vt, int) __attribute__((always_inline)) {
+        if (span.none(k0)) return;
+        if (span.full(k0)) tile_step(std::false_type{}, k0, kt, vt);
         else tile_step(std::true_type{}, k0, kt, vt);
-    });
+    };
+    pipe.run(all, 1, 0, 0, [](int, int, int) {}, step);
     if (u >= a.rows) return;
     const int i = div_group(a, u);
     T* out = static_cast<T*>(a.gq.p) + b * a.gq.batch + i * a.gq.row + (int64_t)(hk * a.group + u - i * a.group) * a.gq.head;
     store_column(out, acc, kHalf<T> ? a.scale * (1.0f / 16384.0f) / unit : a.scale, a.width, lane);
 }
 
-// dK and dV.  The accumulators of both beside a lane's key and value leave no room for a
-// second wave on a SIMD, so two waves share 32 keys: the first forms P, dV += P dO and leaves
-// P (rounded, as it enters that product) in LDS, the second forms dP, dS = P (dP - D) and dK
-// += dS Q, one step of KS rows behind.
-constexpr int kKeyThreads = 512;
-constexpr int KS = 32;
-template <typename T, int DP>
-struct KeysLds {
-    using TileT = Tile<T, KS, DP>;
-    static constexpr int RING = 3;  // steps in LDS: the next one's loads, the first waves', the second waves'
-    static constexpr int P_CHUNKS = KS * 32 * (int)sizeof(T) / 16;  // of P of 32 keys
-    static constexpr int TILES = 2 * RING * TileT::BYTES, P = 2 * 4 * P_CHUNKS * 16, STATS = 2 * RING * KS * 4;
-    static constexpr int BYTES = TILES + P + STATS;
-};
-template <typename T, int DP, bool ASYNC>
-__global__ void __launch_bounds__(kKeyThreads, 2) k_backward_keys(Params a) {
-    using Lds = KeysLds<T, DP>;
-    using TileT = typename Lds::TileT;
-    typedef __attribute__((address_space(3))) float lds_float;
-    typedef __attribute__((address_space(3))) u32x4 lds_chunk;
-    constexpr int DT = DP / 32, PV = Lds::P_CHUNKS / 64;  // chunks of P a lane
-    extern __shared__ __attribute__((aligned(1024))) char smem[];  // Lds::BYTES
-    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3;
-    const bool second = threadIdx.x >= kKeyThreads / 2;
-    // the keys that most rows see first
-    const int heads = a.batch * a.kv_heads;
-    const int bh = blockIdx.x % heads, tile = blockIdx.x / heads;
+// dK, or (VALUES) dV.  Together they would need 4 products instead of 5, but their
+// accumulators beside a lane's key and value leave no room for a second wave on a SIMD, and
+// that costs more: at 8192 causal tokens of 32 / 8 heads of 128 one kernel for both took 2022
+// us alone on its SIMDs and 1369 us as pairs of waves that hand P over through LDS.
+template <typename T, int DP, bool ASYNC, bool VALUES>
+__device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile, char* smem) {
+    using TileT = Tile<T, BN, DP>;
+    constexpr int DT = DP / 32;
+    __shared__ __attribute__((aligned(16))) float row_stats[2][2][BN];  // L and D of each buffer's rows
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
     const int j = tile * kCols + wave * 32 + (lane & 31), jc = min(j, a.keys - 1);
-    Interval seen = queries_of(a, b, jc);
-    seen.lo *= a.group;
-    seen.hi *= a.group;
+    const Interval seen = queries_of(a, b, jc);
     Span span;
     span.of(seen);
-    const Interval all = block_span<kKeyThreads>(span);
+    const Interval all = block_span(span);
 
     const Rows<T, true> queries(a, a.q, b, hk), grads(a, a.go, b, hk);
-    if (ASYNC && a.width < DP) clear_tiles<kKeyThreads>(smem, Lds::TILES);
-    __syncthreads();
-    Column<T, DP> x;  // the key, or (second) the value
-    x.load(second ? Rows<T, false>(a, a.v, b, hk).at(a, jc) : Rows<T, false>(a, a.k, b, hk).at(a, jc), a.width, lane);
+    Pipe<T, DP, ASYNC> pipe(a.q, a.go, queries.base, grads.base, a.width, a.queries, smem);
+    Column<T, DP> k, v;
+    k.load(Rows<T, false>(a, a.k, b, hk).at(a, jc), a.width, lane);
+    if (!VALUES) v.load(Rows<T, false>(a, a.v, b, hk).at(a, jc), a.width, lane);
     float unit = 1.0f;
-    if constexpr (kHalf<T>) unit = into_one(2.0f * largest_norm(a, 0, bh) * largest_norm(a, 1, bh));
-    f32x16 acc[DT];  // dV, or (second) dK
+    if constexpr (kHalf<T> && !VALUES) unit = into_one(2.0f * largest_norm(a, 0, bh) * largest_norm(a, 1, bh));
+    f32x16 acc[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
 
-    typename TileT::lds_t* const tiles = (typename TileT::lds_t*)smem;
-    lds_chunk* const probs = (lds_chunk*)(smem + Lds::TILES) + wave * Lds::P_CHUNKS + lane;  // + 4 P_CHUNKS the other step's
-    lds_float* const stats = (lds_float*)(smem + Lds::TILES + Lds::P);
-    Filler<T, KS, DP, ASYNC, kKeyThreads> fq, fg;
-    auto query_tile = [&](int slot) { return TileT{tiles + 2 * slot * TileT::ELEMS}; };
-    auto grad_tile = [&](int slot) { return TileT{tiles + (2 * slot + 1) * TileT::ELEMS}; };
-    auto issue = [&](int u0, int slot) __attribute__((always_inline)) {
-        fq.issue(a, queries, u0, query_tile(slot));
-        fg.issue(a, grads, u0, grad_tile(slot));
-        // two half waves take the rows' L and D along
-        const int w = threadIdx.x >> 6;
-        if (w < 2 && lane < KS)
-            load_to_lds<4>((w ? a.delta : a.lse) + (int64_t)bh * a.rows + min(u0 + lane, a.rows - 1),
-                           __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(stats + (2 * slot + w) * KS)));
-    };
-    auto land = [&](int slot) __attribute__((always_inline)) {
-        fq.land(query_tile(slot));
-        fg.land(grad_tile(slot));
-    };
-
-    auto first_step = [&](auto partial, int u0, int slot, int parity) __attribute__((always_inline)) {
+    auto tile_step = [&](auto partial, int i0, const TileT& qt, const TileT& gt, int buffer) __attribute__((always_inline)) {
         constexpr bool PARTIAL = decltype(partial)::value;
-        const TileT qt = query_tile(slot), gt = grad_tile(slot);
-        f32x16 s = rows_product(qt, 0, x, lane);
+        const TileT& into = VALUES ? gt : qt;
+        uint32_t bad = 0;
+#pragma unroll 1
+        for (int t = 0; t < BN / 32; ++t) {
+            f32x16 s = rows_product(qt, 32 * t, k, lane), dp;
+            if (!VALUES) dp = rows_product(gt, 32 * t, v, lane);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int r = row_of(0, i, lane);
-            s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, kBackwardShift<T> - stats[2 * slot * KS + r]));
-            if (PARTIAL && !within(u0 + r, seen)) s[i] = 0.0f;
-        }
-        bool bad = false;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const PFrag<T> p = pack<T>(s, c);
-#pragma unroll
-            for (int k = 0; k < PV / 2; ++k)
-                probs[parity * 4 * Lds::P_CHUNKS + (PV / 2 * c + k) * 64] = reinterpret_cast<const u32x4*>(&p)[k];
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-                acc[dt] = gt.template mma_columns<PARTIAL>(p, 16 * c, 32 * dt, lane, acc[dt], &bad);
-        }
-        if (PARTIAL && __any(bad)) gt.template add_nonfinite<false>(acc, KS, seen.lo - u0, seen.hi - u0, lane);
-    };
-    auto second_step = [&](auto partial, int u0, int slot, int parity) __attribute__((always_inline)) {
-        constexpr bool PARTIAL = decltype(partial)::value;
-        const TileT qt = query_tile(slot), gt = grad_tile(slot);
-        f32x16 ds = rows_product(gt, 0, x, lane);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            PFrag<T> p;
-#pragma unroll
-            for (int k = 0; k < PV / 2; ++k)
-                reinterpret_cast<u32x4*>(&p)[k] = probs[parity * 4 * Lds::P_CHUNKS + (PV / 2 * c + k) * 64];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = row_of(0, 8 * c + i, lane);
-                float d = ds[8 * c + i] - stats[(2 * slot + 1) * KS + r];
-                if (kHalf<T>) d *= unit;
-                d *= unpacked(p, i);
-                ds[8 * c + i] = PARTIAL && !within(u0 + r, seen) ? 0.0f : d;
-            }
-        }
-        bool bad = false;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const PFrag<T> p = pack<T>(ds, c);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-                acc[dt] = qt.template mma_columns<PARTIAL>(p, 16 * c, 32 * dt, lane, acc[dt], &bad);
-        }
-        if (PARTIAL && __any(bad)) qt.template add_nonfinite<true>(acc, KS, seen.lo - u0, seen.hi - u0, lane);
-    };
-
-    if (all.hi > all.lo) {
-        int u0 = all.lo / KS * KS, slot = 0, parity = 0;
-        issue(u0, 0);
-        if (!ASYNC) land(0);
-        for (;; u0 += KS) {
-            // this step has landed, P of the last one is there, and every wave is done with the
-            // slot to fill next
-            wait_loads_and_sync();
-            const bool more = u0 + KS < all.hi, now = u0 < all.hi;
-            const int next = slot == Lds::RING - 1 ? 0 : slot + 1, last = slot == 0 ? Lds::RING - 1 : slot - 1;
-            if (more) issue(u0 + KS, next);
-            const int at = second ? u0 - KS : u0;
-            if ((second ? at >= all.lo / KS * KS : now) && !span.none(at, KS)) {
-                if (second) {
-                    if (span.full(at, KS)) second_step(std::false_type{}, at, last, parity ^ 1);
-                    else second_step(std::true_type{}, at, last, parity ^ 1);
-                } else {
-                    if (span.full(at, KS)) first_step(std::false_type{}, at, slot, parity);
-                    else first_step(std::true_type{}, at, slot, parity);
+            for (int i = 0; i < 16; ++i) {
+                const int r = row_of(32 * t, i, lane);
+                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, kBackwardShift<T> - row_stats[buffer][0][r]));
+                if (!VALUES) {
+                    const float d = dp[i] - row_stats[buffer][1][r];
+                    p *= kHalf<T> ? d * unit : d;
                 }
+                s[i] = PARTIAL && !within(i0 + r, seen) ? 0.0f : p;
             }
-            if (!ASYNC && more) land(next);
-            if (!now) break;
-            slot = next;
-            parity ^= 1;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const PFrag<T> p = pack<T>(s, c);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+                    acc[dt] = into.template mma_columns<PARTIAL>(p, 32 * t + 16 * c, 32 * dt, lane, acc[dt], &bad);
+            }
         }
-    }
+        if (PARTIAL && __any((bad & kBadBits<T>) != 0))
+            into.template add_nonfinite<!VALUES>(acc, BN, seen.lo - i0, seen.hi - i0, lane);
+    };
+    auto step = [&](int i0, const TileT& qt, const TileT& gt, int buffer) __attribute__((always_inline)) {
+        if (span.none(i0)) return;
+        if (span.full(i0)) tile_step(std::false_type{}, i0, qt, gt, buffer);
+        else tile_step(std::true_type{}, i0, qt, gt, buffer);
+    };
+    // a wave's 64 lanes take the rows' L along, another one's D
+    const float* const stats = (wave & 1 ? a.delta : a.lse) + (int64_t)bh * a.group * a.queries + lane;
+    const uint32_t stats_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) float*)&row_stats[0][wave & 1][0];
+    auto more = [&](int head, int i0, int buffer) __attribute__((always_inline)) {
+        if (wave < (VALUES ? 1 : 2) && i0 + lane < a.queries)
+            load_to_lds<4>(stats + (int64_t)head * a.queries + i0, stats_lds + buffer * (uint32_t)sizeof(row_stats[0]));
+    };
+    pipe.run(all, a.group, a.q.head, a.go.head, more, step);
     if (j >= a.keys) return;
-    const View& out = second ? a.gk : a.gv;
+    const View& out = VALUES ? a.gv : a.gk;
     T* row = static_cast<T*>(out.p) + b * out.batch + j * out.row + hk * out.head;
     const float down = kHalf<T> ? 1.0f / 16384.0f : 1.0f;
-    store_column(row, acc, second ? a.scale * down / unit : down, a.width, lane);
+    store_column(row, acc, VALUES ? down : a.scale * down / unit, a.width, lane);
+}
+// The workgroups of dK (the longer ones), then those of dV; of each the keys first that most
+// rows see.
+template <typename T, int DP, bool ASYNC>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_keys(Params a) {
+    extern __shared__ __attribute__((aligned(1024))) char smem[];  // Pipe::BYTES
+    const int heads = a.batch * a.kv_heads, half = gridDim.x / 2;
+    const bool values = blockIdx.x >= half;
+    const int block = values ? blockIdx.x - half : blockIdx.x;
+    if (values) backward_keys<T, DP, ASYNC, true>(a, block % heads, block / heads, smem);
+    else backward_keys<T, DP, ASYNC, false>(a, block % heads, block / heads, smem);
 }
 
 // ------------------------------------------------------------------ host side
@@ -674,18 +658,18 @@ enum Pass { kForwardPass, kQueriesPass, kKeysPass };
 template <typename T, int DP, bool ASYNC>
 int launch(Pass pass, const Params& a, hipStream_t st) {
     const int64_t heads = (int64_t)a.batch * a.kv_heads;
-    const int64_t cols = pass == kKeysPass ? a.keys : a.rows;
-    const dim3 grid((uint32_t)(heads * ((cols + kCols - 1) / kCols)));
+    const int64_t tiles = ((pass == kKeysPass ? a.keys : a.rows) + kCols - 1) / kCols;
+    const uint32_t grid = (uint32_t)(heads * tiles);
     constexpr int lds = Pipe<T, DP, ASYNC>::BYTES;
     if (pass == kForwardPass) k_forward<T, DP, ASYNC><<<grid, kThreads, lds, st>>>(a);
     else if (pass == kQueriesPass) k_backward_queries<T, DP, ASYNC><<<grid, kThreads, lds, st>>>(a);
-    else k_backward_keys<T, DP, ASYNC><<<grid, kKeyThreads, KeysLds<T, DP>::BYTES, st>>>(a);
+    else k_backward_keys<T, DP, ASYNC><<<2 * grid, kThreads, lds, st>>>(a);
     return launch_status("attention");
 }
-// Whether a tensor's rows are whole 16-byte chunks.
+// Whether a tensor's rows are whole 16-byte chunks at distances that a tile's offsets hold.
 bool chunked(const Params& a, const View& v, int size) {
     return aligned(v.p, 16) && a.width * size % 16 == 0 && v.batch * size % 16 == 0 && v.row * size % 16 == 0 &&
-           v.head * size % 16 == 0;
+           v.head * size % 16 == 0 && v.row < (int64_t)1 << 22;
 }
 template <typename T, int DP>
 int launch_filler(Pass pass, const Params& a, hipStream_t st) {
@@ -723,7 +707,7 @@ int check_task(const gefen_attention_task* t) {
         return fail_inval("attention: sizes out of range");
     const int64_t group = t->heads / t->kv_heads, pairs = t->batch * t->kv_heads;
     if (t->queries * group > most || pairs > most || pairs * ((t->queries * group + kCols - 1) / kCols) > 0x7fffffff ||
-        pairs * ((t->keys + kCols - 1) / kCols) > 0x7fffffff)
+        pairs * ((t->keys + kCols - 1) / kCols) > 0x3fffffff)
         return fail_inval("attention: sizes out of range");
     if (!(t->scale >= 0.0) || !isfinite(t->scale)) return fail_inval("attention: scale must be finite and not negative");
     if (t->offsets && (t->batch != 1 || t->queries != t->keys || t->sequences < 0 || t->sequences > most))

@@ -73,7 +73,7 @@ struct PFrag {
     u32x4 v;
 };
 template <>
-struct alignas(16) PFrag<float> {
+struct PFrag<float> {
     float v[8];
 };
 template <typename T>
@@ -96,26 +96,19 @@ __device__ __forceinline__ PFrag<T> pack(const f32x16& p, int chunk) {
     return out;
 }
 
-// Element i of them as float32.
+// Zeros in place of what is not finite; *bad gets bits of kBadBits where there was any.  The
+// largest exponent plus its lowest bit carries into the sign's place.
 template <typename T>
-__device__ __forceinline__ float unpacked(const PFrag<T>& p, int i) {
-    if constexpr (sizeof(T) == 4) return p.v[i];
-    else return Elem<T>::value((uint16_t)(p.v[i / 2] >> (16 * (i & 1))));
-}
-
-// Zeros in place of what is not finite; true if there was any.
+constexpr uint32_t kBadBits = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
 template <typename T>
-__device__ __forceinline__ bool drop_nonfinite(uint32_t& x) {
-    if constexpr (sizeof(T) == 4) {
-        const bool bad = (x & 0x7f800000u) == 0x7f800000u;
-        x = bad ? 0u : x;
-        return bad;
-    } else {
-        constexpr uint32_t e = __is_same(T, f16_t) ? 0x7c00u : 0x7f80u;
-        const bool lo = (x & e) == e, hi = (x & (e << 16)) == (e << 16);
-        x &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
-        return lo | hi;
-    }
+__device__ __forceinline__ uint32_t drop_nonfinite(uint32_t x, uint32_t* bad) {
+    constexpr uint32_t e = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, f16_t) ? 0x7c007c00u : 0x7f807f80u;
+    constexpr uint32_t one = sizeof(T) == 4 ? 0x00800000u : __is_same(T, f16_t) ? 0x04000400u : 0x00800080u;
+    const uint32_t t = ((x & e) + one) & kBadBits<T>;
+    *bad |= t;
+    if constexpr (sizeof(T) == 4) return x & ~(uint32_t)((int32_t)t >> 31);
+    const uint32_t m = t >> 15;
+    return x & ~((m << 16) - m);
 }
 
 // The XOR of row r's chunks, `chunks` a row.
@@ -146,16 +139,16 @@ struct Tile {
         return *(const lds_chunk*)(p + r0 * LD + place(lane & 31, (2 * c + (lane >> 5)) * EPC));
     }
     // acc[d0 + .., n] += sum over rows r0 .. r0 + 15 (r0 a multiple of 16).  CHECK: what is not finite counts as
-    // zero, and *bad tells.
+    // zero, and *bad tells (kBadBits).
     template <bool CHECK>
     __device__ __forceinline__ f32x16 mma_columns(const PFrag<T>& b, int r0, int d0, int lane, f32x16 acc,
-                                                  bool* bad) const {
+                                                  uint32_t* bad) const {
         const int h = lane >> 5;
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 uint32_t a = p[r0 * LD + place(8 * (i / 4) + 4 * h + i % 4, d0 + (lane & 31))];
-                if (CHECK) *bad |= drop_nonfinite<T>(a);
+                if (CHECK) a = drop_nonfinite<T>(a, bad);
                 acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a), b.v[i], acc, 0, 0, 0);
             }
             return acc;
@@ -169,11 +162,7 @@ struct Tile {
             u32x4 a = __builtin_bit_cast(u32x4, bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
             if (CHECK) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t x = a[i];
-                    *bad |= drop_nonfinite<T>(x);
-                    a[i] = x;
-                }
+                for (int i = 0; i < 4; ++i) a[i] = drop_nonfinite<T>(a[i], bad);
             }
             if constexpr (__is_same(T, f16_t))
                 return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b.v),
@@ -203,7 +192,8 @@ struct Tile {
     }
 };
 
-// BYTES from each active lane's address to its place after lds (wave-uniform): lane * BYTES.
+// BYTES from each active lane's address (or base, wave-uniform, + offset bytes) to its place
+// after lds (wave-uniform): lane * BYTES.
 // Written as assembly because the compiler otherwise holds every transposing LDS read back
 // until all such loads in flight have landed; it has no register result, and
 // wait_loads_and_sync waits for it.
@@ -212,9 +202,18 @@ struct Tile {
 template <int BYTES>
 __device__ __forceinline__ void load_to_lds(const void* at, uint32_t lds) {
     static_assert(BYTES == 4 || BYTES == 16, "");
+    lds = __builtin_amdgcn_readfirstlane((int)lds);
     if constexpr (BYTES == 16)
         asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(at) : "m0");
     else asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(at) : "m0");
+}
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t lds) {
+    const uint64_t b = reinterpret_cast<uint64_t>(base);
+    const uint64_t s = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32 |
+                       (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)),
+                 "v"(offset), "s"(s)
+                 : "m0");
 }
 #pragma clang diagnostic pop
 // This wave's loads to LDS have landed and its LDS reads are done, then the barrier.
@@ -255,6 +254,7 @@ __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d,
 }
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ int wave_min(int v) {
     for (int off = 32; off > 0; off >>= 1) v = min(v, __shfl_xor(v, off, 64));
     return v;

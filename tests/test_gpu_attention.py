@@ -16,8 +16,7 @@ share a key head):
 * D_i is formed of the rounded output: its error is that of the output times |dO|, and a sum;
 * dS = P (dP - D) has the errors of its factors, u of its own, and in float16 2^-25 of a
   spacing at 2^14 of the bound B = 4 |dO_i| max |v_j| (a power of two at most twice
-  2 |dO_i| max |v_j|): 2^-39 B, with the largest row's |dO| for dK;
-* dK's dS takes P as rounded for dV: another u (float16: and 2^-39) times dP - D."""
+  2 |dO_i| max |v_j|): 2^-39 B, with the largest row's |dO| for dK."""
 
 import math
 
@@ -99,13 +98,12 @@ def definition(q, k, v, go, seen, dtype, scale=None):
     ebig = (go.abs() * eo).sum(2, keepdim=True) + (d + 2) * F * (go * o).abs().sum(2, keepdim=True)
     ds = p * (dp - big)
     eds = p * (delta * (dp - big).abs() + edp + ebig + 4 * F * (dp.abs() + big.abs())) + up * ds.abs()
-    eds_k = eds + up * ds.abs()
+    eds_k = eds
     if half:
         vmax = v.norm(dim=2).amax(1)[:, None, None] if sk else zero
         bound = 4 * go.norm(dim=2, keepdim=True) * vmax
         edv = edv + 2.0 ** -39 * torch.bmm(T(seen.double()), go.abs()) + 2.0 ** -25
-        eds = eds + mask(2.0 ** -39 * bound)
-        eds_k = eds_k + mask(2.0 ** -39 * (bound.amax(1, keepdim=True) + (dp - big).abs()))
+        eds, eds_k = eds + mask(2.0 ** -39 * bound), eds + mask(2.0 ** -39 * bound.amax(1, keepdim=True))
     dq, dk = scale * torch.bmm(ds, k), scale * torch.bmm(T(ds), q)
     edq = scale * (torch.bmm(eds, k.abs()) + (n + 6) * F * torch.bmm(ds.abs(), k.abs())) + u * dq.abs()
     edk = scale * (torch.bmm(T(eds_k), q.abs()) + (m + 6) * F * torch.bmm(T(ds.abs()), q.abs())) + u * dk.abs()
