@@ -85,7 +85,8 @@ SIGNATURES = {
     "gefen_linear_cross_entropy": (I32, [P, P, SZ, P]),
     "gefen_scale_by": (I32, [P, I64, P, I64, I32, P, P]),
     "gefen_scale_from_f32": (I32, [P, P, I64, P, P, I64, I32, P, P]),
-    "gefen_attention_forward": (I32, [P, P]),
+    "gefen_attention_forward_workspace_size": (SZ, [P]),
+    "gefen_attention_forward": (I32, [P, P, SZ, P]),
     "gefen_attention_backward_workspace_size": (SZ, [P]),
     "gefen_attention_backward": (I32, [P, P, SZ, P]),
     "gefen_rms_norm_forward": (I32, [P, P]),

@@ -50,6 +50,12 @@ struct Params {
     uint32_t div_mul;   // u / group = u * div_mul >> div_shift for u < 2^31
     int32_t div_shift;
     float c, scale;     // c = scale * log2(e)
+    // A workgroup's tiles are split into `parts`; with more than one, part k leaves its sums in
+    // float32 at partial + k * partial_stride (dV: behind the parts of dK), laid out as the
+    // result, and its lse (forward) at partial_lse + k * stats.
+    int32_t parts;
+    float *partial, *partial_lse;
+    int64_t partial_stride, stats;
 };
 
 __device__ __forceinline__ int div_group(const Params& a, int u) {
@@ -250,14 +256,22 @@ struct Pipe {
     __device__ __forceinline__ TileT tile(int buffer, int which) const {
         return TileT{base + (2 * buffer + which) * TileT::ELEMS};
     }
-    // step(r0, first tile, second tile, buffer) for the tiles of [all.lo, all.hi) of `heads`
-    // heads, head_x and head_y elements apart; more(head, r0, buffer) loads what else the step
-    // needs.
+    // step(r0, first tile, second tile, buffer) for this part of the tiles of [all.lo, all.hi)
+    // of `heads` heads, head_x and head_y elements apart; more(head, r0, buffer) loads what else
+    // the step needs.
     template <typename More, typename Step>
-    __device__ __forceinline__ void run(Interval all, int heads, int64_t head_x, int64_t head_y, More more, Step step) {
+    __device__ __forceinline__ void run(Interval all, int heads, int64_t head_x, int64_t head_y, int part, int parts,
+                                        More more, Step step) {
         if (all.hi <= all.lo) return;
-        const int start = all.lo / BN * BN;
-        int r0 = start, head = 0;
+        const int start = all.lo / BN * BN, each = (all.hi - start + BN - 1) / BN;  // tiles of a head
+        const int64_t tiles = (int64_t)each * heads;
+        int left = (int)(tiles * (part + 1) / parts);
+        const int first = (int)(tiles * part / parts);
+        left -= first;
+        if (left <= 0) return;
+        int head = first / each, r0 = start + (first - head * each) * BN;
+        x += head * head_x;
+        y += head * head_y;
         fill.issue(x, y, r0, 0);
         more(head, r0, 0);
         fill.land(tile(0, 0));
@@ -273,7 +287,7 @@ struct Pipe {
                 x += head_x;
                 y += head_y;
             }
-            const bool next = head < heads;
+            const bool next = --left > 0;
             if (next) {
                 fill.issue(x, y, r0, (1 - buffer) * 2 * TileT::BYTES);
                 more(head, r0, 1 - buffer);
@@ -345,6 +359,7 @@ __device__ __forceinline__ void store_column(T* row, const f32x16 (&acc)[DT], fl
 template <typename T>
 constexpr bool kHalf = std::is_same<T, f16_t>::value;
 constexpr float kLag = 8.0f;
+constexpr float kAllInfinite = -3.4028235e38f;  // lse of a part whose keys all score -inf
 template <typename T>
 constexpr float kForwardShift = kHalf<T> ? 6.0f : 0.0f;
 template <typename T>
@@ -359,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_forward(Pa
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     // the rows that see most keys first
     const int heads = a.batch * a.kv_heads, tiles = (a.rows + kCols - 1) / kCols;
-    const int bh = blockIdx.x % heads, tile = tiles - 1 - blockIdx.x / heads;
+    const int bh = blockIdx.x % heads, part = blockIdx.x / heads % a.parts, tile = tiles - 1 - blockIdx.x / heads / a.parts;
     const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
     const int u = tile * kCols + wave * 32 + (lane & 31), uc = min(u, a.rows - 1);
     const Interval seen = keys_of(a, b, div_group(a, uc));
@@ -426,15 +441,69 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_forward(Pa
         if (span.full(k0)) tile_step(std::false_type{}, k0, kt, vt);
         else tile_step(std::true_type{}, k0, kt, vt);
     };
-    pipe.run(all, 1, 0, 0, [](int, int, int) {}, step);
+    pipe.run(all, 1, 0, 0, part, a.parts, [](int, int, int) {}, step);
     sum += other_half(sum);
     if (u >= a.rows) return;
     const bool empty = seen.hi <= seen.lo;
     const int i = div_group(a, u);
-    T* out = static_cast<T*>(a.o.p) + b * a.o.batch + i * a.o.row + (int64_t)(hk * a.group + u - i * a.group) * a.o.head;
-    store_column(out, acc, empty ? 1.0f : 1.0f / sum, a.width, lane);
+    const int64_t at = b * a.o.batch + i * a.o.row + (int64_t)(hk * a.group + u - i * a.group) * a.o.head;
+    if (a.parts > 1) {
+        // a part's own result; a part without keys, or whose scores are all -inf, weighs nothing
+        store_column(a.partial + part * a.partial_stride + at, acc, sum == 0.0f ? 0.0f : 1.0f / sum, a.width, lane);
+        if (lane < 32)
+            a.partial_lse[part * a.stats + stat_at(a, bh, u)] =
+                empty ? -INFINITY : sum == 0.0f ? kAllInfinite : top + __builtin_amdgcn_logf(sum) - kForwardShift<T>;
+        return;
+    }
+    store_column(static_cast<T*>(a.o.p) + at, acc, empty ? 1.0f : 1.0f / sum, a.width, lane);
     if (a.lse && lane < 32)
         a.lse[stat_at(a, bh, u)] = empty ? 0.0f : top + __builtin_amdgcn_logf(sum) - kForwardShift<T>;
+}
+
+// The parts of a row of the output together: 32 lanes a row, four elements each.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_join_forward(Params a) {
+    const int64_t row = (int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32;  // [batch, query, head]
+    const int heads = a.kv_heads * a.group;
+    if (row >= (int64_t)a.batch * a.queries * heads) return;
+    const int64_t bi = row / heads;
+    const int h = (int)(row - bi * heads), b = (int)(bi / a.queries), i = (int)(bi - (int64_t)b * a.queries);
+    const int64_t stat = ((int64_t)b * heads + h) * a.queries + i;
+    float most = -INFINITY;
+    for (int p = 0; p < a.parts; ++p) most = fmaxf(most, a.partial_lse[p * a.stats + stat]);
+    const int d = (threadIdx.x & 31) * 4;
+    float sum = 0.0f, out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p = 0; p < a.parts; ++p) {
+        const float lse = a.partial_lse[p * a.stats + stat];
+        if (lse == -INFINITY) continue;  // no keys
+        const float w = __builtin_amdgcn_exp2f(lse - most);
+        sum += w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (d + k < a.width) out[k] = __builtin_fmaf(w, a.partial[p * a.partial_stride + row * a.width + d + k], out[k]);
+    }
+    const bool empty = sum == 0.0f;
+    // keys, but none of a finite score
+    const float f = empty ? 1.0f : most == kAllInfinite ? __uint_as_float(0x7fc00000u) : 1.0f / sum;
+    if (d < a.width)
+        store4(static_cast<T*>(a.o.p) + row * a.width + d, out[0] * f, out[1] * f, out[2] * f, out[3] * f, a.width - d);
+    if (a.lse && d == 0) a.lse[stat] = empty ? 0.0f : (most + __builtin_amdgcn_logf(sum)) + (f != f ? f : 0.0f);
+}
+
+// The sum of the parts, in their order.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) k_join_sums(const float* partial, int parts, int64_t stride, int64_t numel,
+                                                        T* out) {
+    const int64_t e = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4;
+    if (e >= numel) return;
+    const int have = (int)min((int64_t)4, numel - e);
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p = 0; p < parts; ++p) {
+        const u32x4 x = load_chunk(partial + p * stride + e, have);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] += __uint_as_float(x[k]);
+    }
+    store4(out + e, sum[0], sum[1], sum[2], sum[3], have);
 }
 
 // The power of two that brings values of up to `most` into [-1, 1].
@@ -498,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
     extern __shared__ __attribute__((aligned(1024))) char smem[];  // PipeT::BYTES
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int heads = a.batch * a.kv_heads, tiles = (a.rows + kCols - 1) / kCols;
-    const int bh = blockIdx.x % heads, tile = tiles - 1 - blockIdx.x / heads;
+    const int bh = blockIdx.x % heads, part = blockIdx.x / heads % a.parts, tile = tiles - 1 - blockIdx.x / heads / a.parts;
     const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
     const int u = tile * kCols + wave * 32 + (lane & 31), uc = min(u, a.rows - 1);
     const Interval seen = keys_of(a, b, div_group(a, uc));
@@ -513,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
     q.load(Rows<T, true>(a, a.o, b, hk).at(a, uc), a.width, lane);
     float delta = go.dot(q);
     delta += other_half(delta);
-    if (lane < 32 && u < a.rows) a.delta[stat_at(a, bh, u)] = delta;
+    if (lane < 32 && u < a.rows && part == 0) a.delta[stat_at(a, bh, u)] = delta;
     q.load(Rows<T, true>(a, a.q, b, hk).at(a, uc), a.width, lane);
     const float shift = kBackwardShift<T> - a.lse[stat_at(a, bh, uc)];
     float unit = 1.0f;
@@ -556,11 +625,13 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
         if (span.full(k0)) tile_step(std::false_type{}, k0, kt, vt);
         else tile_step(std::true_type{}, k0, kt, vt);
     };
-    pipe.run(all, 1, 0, 0, [](int, int, int) {}, step);
+    pipe.run(all, 1, 0, 0, part, a.parts, [](int, int, int) {}, step);
     if (u >= a.rows) return;
     const int i = div_group(a, u);
-    T* out = static_cast<T*>(a.gq.p) + b * a.gq.batch + i * a.gq.row + (int64_t)(hk * a.group + u - i * a.group) * a.gq.head;
-    store_column(out, acc, kHalf<T> ? a.scale * (1.0f / 16384.0f) / unit : a.scale, a.width, lane);
+    const int64_t at = b * a.gq.batch + i * a.gq.row + (int64_t)(hk * a.group + u - i * a.group) * a.gq.head;
+    const float f = kHalf<T> ? a.scale * (1.0f / 16384.0f) / unit : a.scale;
+    if (a.parts > 1) store_column(a.partial + part * a.partial_stride + at, acc, f, a.width, lane);
+    else store_column(static_cast<T*>(a.gq.p) + at, acc, f, a.width, lane);
 }
 
 // dK, or (VALUES) dV.  Together they would need 4 products instead of 5, but their
@@ -568,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
 // that costs more: at 8192 causal tokens of 32 / 8 heads of 128 one kernel for both took 2022
 // us alone on its SIMDs and 1369 us as pairs of waves that hand P over through LDS.
 template <typename T, int DP, bool ASYNC, bool VALUES>
-__device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile, char* smem) {
+__device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile, int part, char* smem) {
     using TileT = Tile<T, BN, DP>;
     constexpr int DT = DP / 32;
     __shared__ __attribute__((aligned(16))) float row_stats[2][2][BN];  // L and D of each buffer's rows
@@ -632,12 +703,14 @@ __device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile,
         if (wave < (VALUES ? 1 : 2) && i0 + lane < a.queries)
             load_to_lds<4>(stats + (int64_t)head * a.queries + i0, stats_lds + buffer * (uint32_t)sizeof(row_stats[0]));
     };
-    pipe.run(all, a.group, a.q.head, a.go.head, more, step);
+    pipe.run(all, a.group, a.q.head, a.go.head, part, a.parts, more, step);
     if (j >= a.keys) return;
     const View& out = VALUES ? a.gv : a.gk;
-    T* row = static_cast<T*>(out.p) + b * out.batch + j * out.row + hk * out.head;
-    const float down = kHalf<T> ? 1.0f / 16384.0f : 1.0f;
-    store_column(row, acc, VALUES ? down : a.scale * down / unit, a.width, lane);
+    const int64_t at = b * out.batch + j * out.row + hk * out.head;
+    const float down = kHalf<T> ? 1.0f / 16384.0f : 1.0f, f = VALUES ? down : a.scale * down / unit;
+    if (a.parts > 1)
+        store_column(a.partial + (part + (VALUES ? a.parts : 0)) * a.partial_stride + at, acc, f, a.width, lane);
+    else store_column(static_cast<T*>(out.p) + at, acc, f, a.width, lane);
 }
 // The workgroups of dK (the longer ones), then those of dV; of each the keys first that most
 // rows see.
@@ -647,8 +720,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_k
     const int heads = a.batch * a.kv_heads, half = gridDim.x / 2;
     const bool values = blockIdx.x >= half;
     const int block = values ? blockIdx.x - half : blockIdx.x;
-    if (values) backward_keys<T, DP, ASYNC, true>(a, block % heads, block / heads, smem);
-    else backward_keys<T, DP, ASYNC, false>(a, block % heads, block / heads, smem);
+    const int bh = block % heads, part = block / heads % a.parts, tile = block / heads / a.parts;
+    if (values) backward_keys<T, DP, ASYNC, true>(a, bh, tile, part, smem);
+    else backward_keys<T, DP, ASYNC, false>(a, bh, tile, part, smem);
 }
 
 // ------------------------------------------------------------------ host side
@@ -659,11 +733,23 @@ template <typename T, int DP, bool ASYNC>
 int launch(Pass pass, const Params& a, hipStream_t st) {
     const int64_t heads = (int64_t)a.batch * a.kv_heads;
     const int64_t tiles = ((pass == kKeysPass ? a.keys : a.rows) + kCols - 1) / kCols;
-    const uint32_t grid = (uint32_t)(heads * tiles);
+    const uint32_t grid = (uint32_t)(heads * tiles * a.parts);
     constexpr int lds = Pipe<T, DP, ASYNC>::BYTES;
     if (pass == kForwardPass) k_forward<T, DP, ASYNC><<<grid, kThreads, lds, st>>>(a);
     else if (pass == kQueriesPass) k_backward_queries<T, DP, ASYNC><<<grid, kThreads, lds, st>>>(a);
     else k_backward_keys<T, DP, ASYNC><<<2 * grid, kThreads, lds, st>>>(a);
+    if (int rc = launch_status("attention")) return rc;
+    if (a.parts == 1) return GEFEN_OK;
+    if (pass == kForwardPass) {
+        const int64_t rows = (int64_t)a.batch * a.queries * a.kv_heads * a.group;
+        k_join_forward<T><<<(uint32_t)((rows + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st>>>(a);
+    } else {
+        const View* const out[2] = {pass == kQueriesPass ? &a.gq : &a.gk, &a.gv};
+        for (int k = 0; k < (pass == kKeysPass ? 2 : 1); ++k)
+            k_join_sums<T><<<(uint32_t)((a.partial_stride / 4 + kThreads - 1) / kThreads + 1), kThreads, 0, st>>>(
+                a.partial + k * a.parts * a.partial_stride, a.parts, a.partial_stride, out[k]->batch * a.batch,
+                static_cast<T*>(out[k]->p));
+    }
     return launch_status("attention");
 }
 // Whether a tensor's rows are whole 16-byte chunks at distances that a tile's offsets hold.
@@ -692,6 +778,39 @@ int launch_type(int dtype, Pass pass, const Params& a, hipStream_t st) {
 
 int64_t stat_count(const gefen_attention_task& t) { return t.batch * t.queries * t.heads; }
 int64_t round16(int64_t floats) { return (floats + 3) / 4 * 4; }
+int64_t out_count(Pass pass, const gefen_attention_task& t) {
+    return t.batch * t.width * (pass == kKeysPass ? t.keys * t.kv_heads : t.queries * t.heads);
+}
+
+// Into how many parts a workgroup's tiles are split.  The chip holds kSlots workgroups: few of
+// them leave it idle, and where rows differ in what they see (causal ones by half on
+// average), as many as it holds wait for the longest.  A part has four tiles at least, for
+// its sums go through memory.
+int parts_of(Pass pass, const gefen_attention_task& t) {
+    const int64_t slots = t.dtype == GEFEN_F32 ? 256 : 512, group = t.heads / t.kv_heads;
+    const int64_t cols = pass == kKeysPass ? t.keys : t.queries * group;
+    const int64_t tiles = pass == kKeysPass ? group * ((t.queries + BN - 1) / BN) : (t.keys + BN - 1) / BN;
+    const int64_t wgs = t.batch * t.kv_heads * ((cols + kCols - 1) / kCols) * (pass == kKeysPass ? 2 : 1);
+    if (wgs == 0 || tiles == 0) return 1;
+    const int64_t uneven = t.causal || t.offsets ? 2 : 1;
+    int64_t parts = (2 * slots * uneven / 2 + wgs - 1) / wgs;
+    parts = parts < tiles / 4 ? parts : tiles / 4;
+    return (int)(parts < 1 ? 1 : parts > 32 ? 32 : parts);
+}
+// Floats of the parts' results and (forward) lse.
+int64_t partial_count(Pass pass, const gefen_attention_task& t) {
+    const int parts = parts_of(pass, t);
+    if (parts == 1) return 0;
+    return parts * (round16(out_count(pass, t)) * (pass == kKeysPass ? 2 : 1) +
+                    (pass == kForwardPass ? round16(stat_count(t)) : 0));
+}
+void set_parts(Pass pass, const gefen_attention_task& t, float* memory, Params* a) {
+    a->parts = parts_of(pass, t);
+    a->partial = memory;
+    a->partial_stride = round16(out_count(pass, t));
+    a->partial_lse = memory + a->parts * a->partial_stride;
+    a->stats = round16(stat_count(t));
+}
 
 // Checks what does not depend on the direction.
 int check_task(const gefen_attention_task* t) {
@@ -706,8 +825,9 @@ int check_task(const gefen_attention_task* t) {
     if (t->batch > most || t->queries > most || t->keys > most || t->heads > 65536)
         return fail_inval("attention: sizes out of range");
     const int64_t group = t->heads / t->kv_heads, pairs = t->batch * t->kv_heads;
-    if (t->queries * group > most || pairs > most || pairs * ((t->queries * group + kCols - 1) / kCols) > 0x7fffffff ||
-        pairs * ((t->keys + kCols - 1) / kCols) > 0x3fffffff)
+    const int64_t most_blocks = 0x7fffffff / 64;
+    if (t->queries * group > most || pairs > most || pairs * ((t->queries * group + kCols - 1) / kCols) > most_blocks ||
+        pairs * ((t->keys + kCols - 1) / kCols) > most_blocks)
         return fail_inval("attention: sizes out of range");
     if (!(t->scale >= 0.0) || !isfinite(t->scale)) return fail_inval("attention: scale must be finite and not negative");
     if (t->offsets && (t->batch != 1 || t->queries != t->keys || t->sequences < 0 || t->sequences > most))
@@ -773,30 +893,48 @@ Params params_of(const gefen_attention_task& t) {
 using namespace gefen;
 using namespace gefen::attn;
 
-extern "C" size_t gefen_attention_backward_workspace_size(const gefen_attention_task* task) {
+namespace {
+int check_workspace(const void* workspace, size_t bytes, size_t need) {
+    if (need && (!workspace || !aligned(workspace, 16) || bytes < need))
+        return fail_inval("attention: workspace too small, missing or not aligned to 16 bytes");
+    return GEFEN_OK;
+}
+}  // namespace
+
+extern "C" size_t gefen_attention_forward_workspace_size(const gefen_attention_task* task) {
     if (check_task(task) != GEFEN_OK) return 0;
-    const int64_t range = task->dtype == GEFEN_F16 ? 2 * task->batch * task->kv_heads * kRangeParts : 0;
-    return (size_t)(round16(stat_count(*task)) + round16(range) + 4) * 4;
+    return (size_t)partial_count(kForwardPass, *task) * 4;
 }
 
-extern "C" int gefen_attention_forward(const gefen_attention_task* task, gefen_stream_t stream) {
+extern "C" int gefen_attention_forward(const gefen_attention_task* task, void* workspace, size_t workspace_bytes,
+                                       gefen_stream_t stream) {
     if (int rc = check_task(task)) return rc;
     const gefen_attention_task& t = *task;
-    const int64_t nq = t.batch * t.queries * t.heads * t.width, nk = t.batch * t.keys * t.kv_heads * t.width;
+    const int64_t nq = out_count(kForwardPass, t), nk = out_count(kKeysPass, t);
     if (int rc = check_tensor(t, t.query, nq, "query")) return rc;
     if (int rc = check_tensor(t, t.key, nk, "key")) return rc;
     if (int rc = check_tensor(t, t.value, nk, "value")) return rc;
     if (int rc = check_tensor(t, t.out, nq, "out")) return rc;
     if (t.lse && !aligned(t.lse, 4)) return fail_inval("attention: lse must be aligned float32 memory");
+    if (int rc = check_workspace(workspace, workspace_bytes, gefen_attention_forward_workspace_size(task))) return rc;
     if (nq == 0) return GEFEN_OK;
-    return launch_type(t.dtype, kForwardPass, params_of(t), static_cast<hipStream_t>(stream));
+    Params a = params_of(t);
+    set_parts(kForwardPass, t, static_cast<float*>(workspace), &a);
+    return launch_type(t.dtype, kForwardPass, a, static_cast<hipStream_t>(stream));
+}
+
+extern "C" size_t gefen_attention_backward_workspace_size(const gefen_attention_task* task) {
+    if (check_task(task) != GEFEN_OK) return 0;
+    const int64_t range = task->dtype == GEFEN_F16 ? 2 * task->batch * task->kv_heads * kRangeParts : 0;
+    const int64_t q = partial_count(kQueriesPass, *task), k = partial_count(kKeysPass, *task);
+    return (size_t)(round16(stat_count(*task)) + round16(range) + (q > k ? q : k) + 4) * 4;
 }
 
 extern "C" int gefen_attention_backward(const gefen_attention_task* task, void* workspace, size_t workspace_bytes,
                                         gefen_stream_t stream) {
     if (int rc = check_task(task)) return rc;
     const gefen_attention_task& t = *task;
-    const int64_t nq = t.batch * t.queries * t.heads * t.width, nk = t.batch * t.keys * t.kv_heads * t.width;
+    const int64_t nq = out_count(kForwardPass, t), nk = out_count(kKeysPass, t);
     if (int rc = check_tensor(t, t.query, nq, "query")) return rc;
     if (int rc = check_tensor(t, t.key, nk, "key")) return rc;
     if (int rc = check_tensor(t, t.value, nk, "value")) return rc;
@@ -808,19 +946,24 @@ extern "C" int gefen_attention_backward(const gefen_attention_task* task, void* 
     if (int rc = check_tensor(t, t.grad_value, key_grads ? nk : 0, "grad_value")) return rc;
     if (nq)
         if (int rc = check_floats(t.lse, "lse")) return rc;
-    if (!workspace || !aligned(workspace, 16) || workspace_bytes < gefen_attention_backward_workspace_size(task))
-        return fail_inval("attention: workspace too small, missing or not aligned to 16 bytes");
+    if (int rc = check_workspace(workspace, workspace_bytes, gefen_attention_backward_workspace_size(task))) return rc;
     Params a = params_of(t);
     a.delta = static_cast<float*>(workspace);
     a.range = a.delta + round16(stat_count(t));
+    // the two passes follow each other: their parts share the memory behind
+    float* const parts = a.range + (t.dtype == GEFEN_F16 ? round16(2 * t.batch * t.kv_heads * kRangeParts) : 0);
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (t.dtype == GEFEN_F16 && nq && nk) {
         k_range<f16_t><<<dim3((uint32_t)(t.batch * t.kv_heads * kRangeParts), 2), kThreads, 0, st>>>(a);
         if (int rc = launch_status("attention")) return rc;
     }
-    if (nq)
+    if (nq) {
+        set_parts(kQueriesPass, t, parts, &a);
         if (int rc = launch_type(t.dtype, kQueriesPass, a, st)) return rc;
-    if (nk && key_grads)
+    }
+    if (nk && key_grads) {
+        set_parts(kKeysPass, t, parts, &a);
         if (int rc = launch_type(t.dtype, kKeysPass, a, st)) return rc;
+    }
     return GEFEN_OK;
 }

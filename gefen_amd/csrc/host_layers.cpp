@@ -14,6 +14,7 @@ namespace {
 using namespace gefen_host;
 
 struct Library {
+    decltype(&gefen_attention_forward_workspace_size) attention_forward_workspace;
     decltype(&gefen_attention_forward) attention_forward;
     decltype(&gefen_attention_backward_workspace_size) attention_workspace;
     decltype(&gefen_attention_backward) attention_backward;
@@ -136,7 +137,10 @@ at::Tensor attention_forward(const at::Tensor& query, const at::Tensor& key, con
         *lse = at::empty({c.t.batch * c.t.queries * c.t.heads}, query.options().dtype(at::kFloat).requires_grad(false));
         c.t.lse = floats(*lse);
     }
-    check(lib.attention_forward(&c.t, stream_of(query)));
+    at::Tensor ws;
+    const size_t bytes = lib.attention_forward_workspace(&c.t);
+    if (bytes) ws = bytes_on(query, bytes);
+    check(lib.attention_forward(&c.t, data(ws), bytes, stream_of(query)));
     return out;
 }
 
@@ -495,6 +499,8 @@ py::object dropout(py::handle x_, py::handle residual_, double p, py::handle see
 
 void bind_layers(const py::dict& addresses) {
     auto at = [&](const char* name) { return addresses[name].cast<uintptr_t>(); };
+    lib.attention_forward_workspace =
+        reinterpret_cast<decltype(lib.attention_forward_workspace)>(at("gefen_attention_forward_workspace_size"));
     lib.attention_forward = reinterpret_cast<decltype(lib.attention_forward)>(at("gefen_attention_forward"));
     lib.attention_workspace =
         reinterpret_cast<decltype(lib.attention_workspace)>(at("gefen_attention_backward_workspace_size"));

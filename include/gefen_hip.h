@@ -557,8 +557,11 @@ typedef struct gefen_attention_task {
     int32_t dtype, causal, lengths_int64, offsets_int64;
 } gefen_attention_task;
 
-int gefen_attention_forward(const gefen_attention_task* task, gefen_stream_t stream);
-/* Bytes of workspace (16-byte aligned) that gefen_attention_backward needs; 0: invalid task. */
+/* Bytes of workspace (16-byte aligned) that gefen_attention_forward needs; may be 0. */
+size_t gefen_attention_forward_workspace_size(const gefen_attention_task* task);
+int gefen_attention_forward(const gefen_attention_task* task, void* workspace, size_t workspace_bytes,
+                            gefen_stream_t stream);
+/* The same of gefen_attention_backward; 0: invalid task. */
 size_t gefen_attention_backward_workspace_size(const gefen_attention_task* task);
 int gefen_attention_backward(const gefen_attention_task* task, void* workspace, size_t workspace_bytes,
                              gefen_stream_t stream);

@@ -52,7 +52,7 @@ def test_struct_mirrors():
 def test_attention_refuses(bad):
     lib = _lib.load()
     t = attention_task(**bad)
-    assert lib.gefen_attention_forward(ctypes.byref(t), None) == _lib.GEFEN_EINVAL
+    assert lib.gefen_attention_forward(ctypes.byref(t), FAKE, 1 << 40, None) == _lib.GEFEN_EINVAL
     assert lib.gefen_last_error()
     assert lib.gefen_attention_backward(ctypes.byref(t), FAKE, 1 << 40, None) == _lib.GEFEN_EINVAL
 
@@ -67,11 +67,18 @@ def test_attention_backward_refuses():
     for bad in (dict(lse=0), dict(grad_out=0), dict(grad_query=0), dict(grad_key=0), dict(grad_value=0),
                 dict(grad_key=FAKE + 1)):
         assert lib.gefen_attention_backward(ctypes.byref(attention_task(**bad)), FAKE, n, None) == _lib.GEFEN_EINVAL
-    assert lib.gefen_attention_forward(None, None) == _lib.GEFEN_EINVAL
+    assert lib.gefen_attention_forward(None, FAKE, 1 << 40, None) == _lib.GEFEN_EINVAL
     assert lib.gefen_attention_backward(None, FAKE, n, None) == _lib.GEFEN_EINVAL
     assert lib.gefen_attention_backward_workspace_size(None) == 0
+    assert lib.gefen_attention_forward_workspace_size(None) == 0
+    # few rows over many keys are split, and their parts need a workspace
+    t = attention_task(queries=1, keys=8192)
+    n = int(lib.gefen_attention_forward_workspace_size(ctypes.byref(t)))
+    assert n >= 2 * 2 * 8 * 64 * 4
+    for ws, size in ((FAKE, n - 1), (None, n), (FAKE + 8, n)):
+        assert lib.gefen_attention_forward(ctypes.byref(t), ws, size, None) == _lib.GEFEN_EINVAL
     # nothing to do
-    assert lib.gefen_attention_forward(ctypes.byref(attention_task(batch=0)), None) == _lib.GEFEN_OK
+    assert lib.gefen_attention_forward(ctypes.byref(attention_task(batch=0)), None, 0, None) == _lib.GEFEN_OK
     assert lib.gefen_attention_backward(ctypes.byref(attention_task(batch=0)), FAKE, 1 << 20, None) == _lib.GEFEN_OK
 
 

@@ -264,6 +264,39 @@ def test_an_infinite_value_stays_infinite_where_it_is_seen():
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_scores_of_minus_infinity(dtype):
+    """Keys that score -inf weigh nothing, also where a whole part of a long axis is of them; a query
+    whose keys all score -inf has no softmax."""
+    b, sk = 1, 1100
+    q, k, v, go = make(dtype, b, 3, sk, 2, 1, 32)
+    q = q.abs()
+    for first, last in ((0, 700), (300, 1100), (64, 128)):
+        k2 = k.clone()
+        k2[:, first:last] = -math.inf
+        seen = visible(b, 3, sk)
+        seen[:, :, first:last] = False
+        with torch.no_grad():
+            out = attention(q, k2, v)
+        want, bounds = definition(q, k, v, go, seen, dtype)
+        within(out, want[0], bounds[0], "out")
+    with torch.no_grad():
+        assert bool(torch.isnan(attention(q, torch.full_like(k, -math.inf), v)).all())
+        some = attention(q, torch.full_like(k, -math.inf), v, key_lengths=torch.tensor([0], device="cuda"))
+        assert not bool(some.any())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("b,sq,sk,h,hk,d,causal", [(1, 2, 4100, 4, 1, 64, True), (3, 1, 2050, 8, 8, 128, False),
+                                                   (1, 1500, 70, 8, 2, 40, False), (1, 1300, 1300, 2, 1, 96, True)])
+def test_few_rows_over_a_long_axis(dtype, b, sq, sk, h, hk, d, causal):
+    q, k, v, go = make(dtype, b, sq, sk, h, hk, d)
+    compare(dtype, q, k, v, go, visible(b, sq, sk, causal), causal=causal)
+    lengths = [sk // 3 + 7, 0, sk][:b]
+    compare(dtype, q, k, v, go, visible(b, sq, sk, causal, lengths), causal=causal,
+            key_lengths=torch.tensor(lengths, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 def test_strides_orders_and_alignment(dtype):
     b, s, h, hk, d = 2, 75, 4, 2, 40
     q, k, v, go = make(dtype, b, s, s, h, hk, d)
