@@ -258,34 +258,40 @@ struct Pipe {
     }
     // step(r0, first tile, second tile, buffer) for this part of the tiles of [all.lo, all.hi)
     // of `heads` heads, head_x and head_y elements apart; more(head, r0, buffer) loads what else
-    // the step needs.
-    template <typename More, typename Step>
+    // the step needs, and land(buffer) writes what of it is in registers.  The heads of a tile
+    // follow each other, and the tiles (DOWN: from the last to the first): causal workgroups see
+    // a common beginning of that order, and those that run side by side read the same rows at
+    // about the same time, from their XCD's L2.
+    template <bool DOWN, typename More, typename Land, typename Step>
     __device__ __forceinline__ void run(Interval all, int heads, int64_t head_x, int64_t head_y, int part, int parts,
-                                        More more, Step step) {
+                                        More more, Land land, Step step) {
         if (all.hi <= all.lo) return;
-        const int start = all.lo / BN * BN, each = (all.hi - start + BN - 1) / BN;  // tiles of a head
-        const int64_t tiles = (int64_t)each * heads;
-        int left = (int)(tiles * (part + 1) / parts);
-        const int first = (int)(tiles * part / parts);
-        left -= first;
+        const int start = all.lo / BN * BN, count = (all.hi - start + BN - 1) / BN;
+        // parts share the heads out, and where there are more of them than heads the tiles too
+        const int by_head = min(parts, heads), by_tile = parts / by_head;
+        const int head0 = part % by_head * heads / by_head, heads_here = (part % by_head + 1) * heads / by_head - head0;
+        const int tile0 = part / by_head * count / by_tile, tiles = (part / by_head + 1) * count / by_tile - tile0;
+        int left = part < by_head * by_tile ? tiles * heads_here : 0;
         if (left <= 0) return;
-        int head = first / each, r0 = start + (first - head * each) * BN;
+        int head = head0, r0 = start + (DOWN ? count - 1 - tile0 : tile0) * BN;
         x += head * head_x;
         y += head * head_y;
         fill.issue(x, y, r0, 0);
         more(head, r0, 0);
         fill.land(tile(0, 0));
+        land(0);
         auto one = [&](auto which) __attribute__((always_inline)) {
             constexpr int buffer = decltype(which)::value;
             // this buffer has landed, and every wave is done with the other one
             wait_loads_and_sync();
             const int now = r0;
-            r0 += BN;
-            if (r0 >= all.hi) {
-                r0 = start;
-                ++head;
-                x += head_x;
-                y += head_y;
+            x += head_x;
+            y += head_y;
+            if (++head == head0 + heads_here) {
+                head = head0;
+                x -= heads_here * head_x;
+                y -= heads_here * head_y;
+                r0 += DOWN ? -BN : BN;
             }
             const bool next = --left > 0;
             if (next) {
@@ -293,7 +299,10 @@ struct Pipe {
                 more(head, r0, 1 - buffer);
             }
             step(now, tile(buffer, 0), tile(buffer, 1), buffer);
-            if (next) fill.land(tile(1 - buffer, 0));
+            if (next) {
+                fill.land(tile(1 - buffer, 0));
+                land(1 - buffer);
+            }
             return next;
         };
         while (one(std::integral_constant<int, 0>{}) && one(std::integral_constant<int, 1>{})) {
@@ -329,8 +338,8 @@ struct Column {
 };
 
 template <typename T, int ROWS, int DP>
-__device__ __forceinline__ f32x16 rows_product(const Tile<T, ROWS, DP>& t, int r0, const Column<T, DP>& x, int lane) {
-    f32x16 acc = {};
+__device__ __forceinline__ f32x16 rows_product(const Tile<T, ROWS, DP>& t, int r0, const Column<T, DP>& x, int lane,
+                                               f32x16 acc = {}) {
 #pragma unroll
     for (int c = 0; c < Column<T, DP>::STEPS; ++c) acc = mma_rows<T>(t.row_chunk(r0, c, lane), x.c[c], acc);
     return acc;
@@ -441,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_forward(Pa
         if (span.full(k0)) tile_step(std::false_type{}, k0, kt, vt);
         else tile_step(std::true_type{}, k0, kt, vt);
     };
-    pipe.run(all, 1, 0, 0, part, a.parts, [](int, int, int) {}, step);
+    pipe.template run<false>(all, 1, 0, 0, part, a.parts, [](int, int, int) {}, [](int) {}, step);
     sum += other_half(sum);
     if (u >= a.rows) return;
     const bool empty = seen.hi <= seen.lo;
@@ -601,11 +610,17 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
 #pragma unroll 1
         for (int t = 0; t < 2; ++t) {
             f32x16 s = rows_product(kt, 32 * t, q, lane);
-            const f32x16 dp = rows_product(vt, 32 * t, go, lane);
+            f32x16 dp = {};
+            if constexpr (DP <= 64) {  // wide heads took 7% longer this way
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dp[i] = -delta;
+            }
+            dp = rows_product(vt, 32 * t, go, lane, dp);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, shift));
-                float ds = kHalf<T> ? p * ((dp[i] - delta) * unit) : p * (dp[i] - delta);
+                const float d = DP <= 64 ? dp[i] : dp[i] - delta;
+                float ds = p * (kHalf<T> ? d * unit : d);
                 if (PARTIAL && !within(row_of(k0 + 32 * t, i, lane), seen)) ds = 0.0f;
                 s[i] = ds;
             }
@@ -625,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
         if (span.full(k0)) tile_step(std::false_type{}, k0, kt, vt);
         else tile_step(std::true_type{}, k0, kt, vt);
     };
-    pipe.run(all, 1, 0, 0, part, a.parts, [](int, int, int) {}, step);
+    pipe.template run<false>(all, 1, 0, 0, part, a.parts, [](int, int, int) {}, [](int) {}, step);
     if (u >= a.rows) return;
     const int i = div_group(a, u);
     const int64_t at = b * a.gq.batch + i * a.gq.row + (int64_t)(hk * a.group + u - i * a.group) * a.gq.head;
@@ -642,7 +657,12 @@ template <typename T, int DP, bool ASYNC, bool VALUES>
 __device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile, int part, char* smem) {
     using TileT = Tile<T, BN, DP>;
     constexpr int DT = DP / 32;
-    __shared__ __attribute__((aligned(16))) float row_stats[2][2][BN];  // L and D of each buffer's rows
+    // L / c and D of each buffer's rows, which the products subtract: as terms of their own, or
+    // (float32) as numbers to start from
+    constexpr bool TERMS = sizeof(T) == 2;
+    __shared__ u32x4 row_terms[TERMS ? 2 : 1][2][TERMS ? BN : 1];
+    __shared__ __attribute__((aligned(16))) float row_starts[TERMS ? 1 : 2][2][TERMS ? 1 : BN];
+    constexpr int UNROLL = VALUES || DP <= 64 ? 2 : 1;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
     const int j = tile * kCols + wave * 32 + (lane & 31), jc = min(j, a.keys - 1);
@@ -656,6 +676,13 @@ __device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile,
     Column<T, DP> k, v;
     k.load(Rows<T, false>(a, a.k, b, hk).at(a, jc), a.width, lane);
     if (!VALUES) v.load(Rows<T, false>(a, a.v, b, hk).at(a, jc), a.width, lane);
+    // S - L / c is formed, and c applied after; with a c that is as good as zero, -L with a key of zeros
+    float c = a.c, over = 1.0f / a.c;
+    if (!(a.c > 5.4e-20f)) {
+        c = over = 1.0f;
+#pragma unroll
+        for (int i = 0; i < Column<T, DP>::STEPS; ++i) k.c[i] = u32x4{0u, 0u, 0u, 0u};
+    }
     float unit = 1.0f;
     if constexpr (kHalf<T> && !VALUES) unit = into_one(2.0f * largest_norm(a, 0, bh) * largest_norm(a, 1, bh));
     f32x16 acc[DT];
@@ -666,18 +693,26 @@ __device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile,
         constexpr bool PARTIAL = decltype(partial)::value;
         const TileT& into = VALUES ? gt : qt;
         uint32_t bad = 0;
-#pragma unroll 1
+#pragma unroll UNROLL
         for (int t = 0; t < BN / 32; ++t) {
-            f32x16 s = rows_product(qt, 32 * t, k, lane), dp;
-            if (!VALUES) dp = rows_product(gt, 32 * t, v, lane);
+            f32x16 s = {}, dp = {};
+            if constexpr (TERMS) {
+                s = RowTerm{(RowTerm::lds_chunk*)row_terms[buffer][0]}.subtract(32 * t, lane, s);
+                if (!VALUES) dp = RowTerm{(RowTerm::lds_chunk*)row_terms[buffer][1]}.subtract(32 * t, lane, dp);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[i] = row_starts[buffer][0][row_of(32 * t, i, lane)];
+                    if (!VALUES) dp[i] = row_starts[buffer][1][row_of(32 * t, i, lane)];
+                }
+            }
+            s = rows_product(qt, 32 * t, k, lane, s);
+            if (!VALUES) dp = rows_product(gt, 32 * t, v, lane, dp);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int r = row_of(32 * t, i, lane);
-                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, kBackwardShift<T> - row_stats[buffer][0][r]));
-                if (!VALUES) {
-                    const float d = dp[i] - row_stats[buffer][1][r];
-                    p *= kHalf<T> ? d * unit : d;
-                }
+                float p = __builtin_amdgcn_exp2f(kHalf<T> ? __builtin_fmaf(s[i], c, kBackwardShift<T>) : s[i] * c);
+                if (!VALUES) p *= kHalf<T> ? dp[i] * unit : dp[i];
                 s[i] = PARTIAL && !within(i0 + r, seen) ? 0.0f : p;
             }
 #pragma unroll
@@ -698,12 +733,18 @@ __device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile,
     };
     // a wave's 64 lanes take the rows' L along, another one's D
     const float* const stats = (wave & 1 ? a.delta : a.lse) + (int64_t)bh * a.group * a.queries + lane;
-    const uint32_t stats_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) float*)&row_stats[0][wave & 1][0];
-    auto more = [&](int head, int i0, int buffer) __attribute__((always_inline)) {
-        if (wave < (VALUES ? 1 : 2) && i0 + lane < a.queries)
-            load_to_lds<4>(stats + (int64_t)head * a.queries + i0, stats_lds + buffer * (uint32_t)sizeof(row_stats[0]));
+    const bool takes = wave < (VALUES ? 1 : 2);
+    float taken = 0.0f;
+    auto more = [&](int head, int i0, int) __attribute__((always_inline)) {
+        if (takes && i0 + lane < a.queries) taken = stats[(int64_t)head * a.queries + i0];
     };
-    pipe.run(all, a.group, a.q.head, a.go.head, part, a.parts, more, step);
+    auto land = [&](int buffer) __attribute__((always_inline)) {
+        if (!takes) return;
+        const float x = wave ? taken : taken * over;
+        if constexpr (TERMS) row_terms[buffer][wave][lane] = RowTerm::split(x);
+        else row_starts[buffer][wave][lane] = -x;
+    };
+    pipe.template run<true>(all, a.group, a.q.head, a.go.head, part, a.parts, more, land, step);
     if (j >= a.keys) return;
     const View& out = VALUES ? a.gv : a.gk;
     const int64_t at = b * out.batch + j * out.row + hk * out.head;
@@ -782,18 +823,20 @@ int64_t out_count(Pass pass, const gefen_attention_task& t) {
     return t.batch * t.width * (pass == kKeysPass ? t.keys * t.kv_heads : t.queries * t.heads);
 }
 
-// Into how many parts a workgroup's tiles are split.  The chip holds kSlots workgroups: few of
-// them leave it idle, and where rows differ in what they see (causal ones by half on
-// average), as many as it holds wait for the longest.  A part has four tiles at least, for
-// its sums go through memory.
+// Into how many parts a workgroup's tiles are split.  The chip holds `slots` workgroups; few of
+// them leave it idle (one query of 16 sequences over 8192 keys, 128 workgroups: 263 us whole,
+// 101 us in 8 parts with the join).  Packed sequences of uneven length make as many as it holds
+// wait for the longest one's keys (11 sequences of 16384 tokens, 2048 workgroups of dK and dV:
+// 1360 us whole, 1180 us in 4 parts with the join; one sequence of 8192: 1570 and 1590).  A part
+// has four tiles at least, for its sums go through memory.
 int parts_of(Pass pass, const gefen_attention_task& t) {
     const int64_t slots = t.dtype == GEFEN_F32 ? 256 : 512, group = t.heads / t.kv_heads;
     const int64_t cols = pass == kKeysPass ? t.keys : t.queries * group;
     const int64_t tiles = pass == kKeysPass ? group * ((t.queries + BN - 1) / BN) : (t.keys + BN - 1) / BN;
     const int64_t wgs = t.batch * t.kv_heads * ((cols + kCols - 1) / kCols) * (pass == kKeysPass ? 2 : 1);
     if (wgs == 0 || tiles == 0) return 1;
-    const int64_t uneven = t.causal || t.offsets ? 2 : 1;
-    int64_t parts = (2 * slots * uneven / 2 + wgs - 1) / wgs;
+    int64_t parts = (2 * slots + wgs - 1) / wgs;
+    if (pass == kKeysPass && t.offsets && t.sequences > 1 && wgs < 8 * slots) parts = parts > 4 ? parts : 4;
     parts = parts < tiles / 4 ? parts : tiles / 4;
     return (int)(parts < 1 ? 1 : parts > 32 ? 32 : parts);
 }

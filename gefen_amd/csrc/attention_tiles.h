@@ -67,6 +67,28 @@ __device__ __forceinline__ f32x16 mma_rows(u32x4 a, u32x4 b, f32x16 c) {
     }
 }
 
+// acc[m, n] - x[m], x float32: a product over three bfloat16 parts of x, which hold 24 bits of
+// it.  A number of each row costs one read of a lane's chunk this way, where a lane's sixteen
+// float32 numbers are four.
+struct RowTerm {
+    typedef __attribute__((address_space(3))) u32x4 lds_chunk;
+    lds_chunk* p;  // a chunk a row: three parts and zeros
+    __device__ __forceinline__ static u32x4 split(float x) {
+        const __bf16 hi = (__bf16)x;
+        const float r1 = x - (float)hi;
+        const __bf16 mid = (__bf16)r1;
+        const __bf16 lo = (__bf16)(r1 - (float)mid);
+        return __builtin_bit_cast(u32x4, bf16x8{hi, mid, lo, (__bf16)0.0f, (__bf16)0.0f, (__bf16)0.0f, (__bf16)0.0f,
+                                                (__bf16)0.0f});
+    }
+    __device__ __forceinline__ f32x16 subtract(int r0, int lane, f32x16 acc) const {
+        const uint32_t one = lane < 32 ? 0xbf80bf80u : 0u;  // -1, -1, -1, 0 for k = 0 .. 3, zeros for the others
+        const u32x4 b = {one, one & 0xffffu, 0u, 0u};
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, p[r0 + (lane & 31)]),
+                                                       __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+    }
+};
+
 // Sixteen rows of p as the columns product takes them.
 template <typename T>
 struct PFrag {
