@@ -41,6 +41,8 @@ struct Shape {
     static constexpr int LANES = LANES_, CHUNKS = CHUNKS_;
     static constexpr int THREADS = LANES < 256 ? 256 : LANES, ROWS = THREADS / LANES;
     static constexpr int WIDTH = LANES * CHUNKS * 8;
+    // 16 waves on a CU leave 128 registers a lane: no row is loaded ahead and the weight is read again
+    static constexpr bool LEAN = LANES == 1024;
 };
 
 // The sum over the lanes of a row.  slot: LDS for a value of each wave.
@@ -106,34 +108,49 @@ __global__ void __launch_bounds__(S::THREADS) k_rms_forward(Params a) {
     const int width = (int)a.width;
     const uint64_t seed = a.drop.cut ? dropout_seed(a.drop) : 0;
     Eight<T> w[S::CHUNKS];
+    auto load_weight = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < S::CHUNKS; ++c) {
-        const int at = (c * S::LANES + lane) * 8;
-        if (at < width) w[c].load(static_cast<const T*>(a.weight) + at, width - at);
-    }
+        for (int c = 0; c < S::CHUNKS; ++c) {
+            const int at = (c * S::LANES + lane) * 8;
+            if (at < width) w[c].load(static_cast<const T*>(a.weight) + at, width - at);
+        }
+    };
+    if (!S::LEAN) load_weight();
     const int64_t step = (int64_t)gridDim.x * S::ROWS;
-    for (int64_t row = (int64_t)blockIdx.x * S::ROWS + threadIdx.x / S::LANES; row < a.rows; row += step) {
+    int64_t row = (int64_t)blockIdx.x * S::ROWS + threadIdx.x / S::LANES;
+    Eight<T> x[S::CHUNKS], r[S::CHUNKS];  // of the next row, on its way while this one is worked on
+    auto load = [&](int64_t at_row) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < S::CHUNKS; ++c) {
+            const int at = (c * S::LANES + lane) * 8, have = width - at;
+            if (have <= 0 || at_row >= a.rows) continue;
+            x[c].load(static_cast<const T*>(a.x) + at_row * a.x_stride + at, have);
+            if (a.residual) r[c].load(static_cast<const T*>(a.residual) + at_row * a.residual_stride + at, have);
+        }
+    };
+    if (!S::LEAN) load(row);
+    for (; row < a.rows; row += step) {
+        if (S::LEAN) load(row);
         float s[S::CHUNKS][8];
         double sq = 0.0;
 #pragma unroll
         for (int c = 0; c < S::CHUNKS; ++c) {
             const int at = (c * S::LANES + lane) * 8, have = width - at;
             if (have <= 0) continue;
-            Eight<T> x, r;
-            x.load(static_cast<const T*>(a.x) + row * a.x_stride + at, have);
-            if (a.residual) r.load(static_cast<const T*>(a.residual) + row * a.residual_stride + at, have);
             const uint32_t keep = a.drop.cut ? dropout_keep(a.drop, seed, row * a.width + at) : 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                float v = x[i];
+                float v = x[c][i];
                 if (a.drop.cut) v = dropped(v, keep, i, a.drop.scale);
-                if (a.residual) v += r[i];
+                if (a.residual) v += r[c][i];
                 s[c][i] = v;
                 sq = __builtin_fma((double)v, (double)v, sq);
-                x.set(i, v);
+                x[c].set(i, v);
             }
-            if (a.sum) x.store(static_cast<T*>(a.sum) + row * a.width + at, have);
+            if (a.sum) x[c].store(static_cast<T*>(a.sum) + row * a.width + at, have);
         }
+        if (S::LEAN) load_weight();
+        else load(row + step);
         sq = row_sum<S::LANES>(sq, slots);
         const float rstd = (float)(1.0 / sqrt(sq / (double)width + a.eps));
         if (a.rstd && lane == 0) a.rstd[row] = rstd;
@@ -193,20 +210,40 @@ __global__ void __launch_bounds__(S::THREADS) k_rms_backward(Params a) {
         for (int i = 0; i < 8; ++i) dw[c][i] = 0.0f;
     }
     const int64_t step = (int64_t)gridDim.x * S::ROWS;
-    for (int64_t row = (int64_t)blockIdx.x * S::ROWS + threadIdx.x / S::LANES; row < a.rows; row += step) {
-        const float rstd = a.rstd[row];
-        Eight<T> s[S::CHUNKS], dy[S::CHUNKS];
-        float dot = 0.0f;
+    int64_t row = (int64_t)blockIdx.x * S::ROWS + threadIdx.x / S::LANES;
+    struct Row {
+        Eight<T> s[S::CHUNKS], dy[S::CHUNKS], more[S::CHUNKS];
+        float rstd;
+    };
+    auto load = [&](Row& x, int64_t at_row) __attribute__((always_inline)) {
+        if (at_row >= a.rows) return;
+        x.rstd = a.rstd[at_row];
 #pragma unroll
         for (int c = 0; c < S::CHUNKS; ++c) {
             const int at = (c * S::LANES + lane) * 8, have = width - at;
             if (have <= 0) continue;
-            s[c].load(static_cast<const T*>(a.x) + row * a.x_stride + at, have);
-            dy[c].load(static_cast<const T*>(a.grad_y) + row * a.grad_y_stride + at, have);
+            x.s[c].load(static_cast<const T*>(a.x) + at_row * a.x_stride + at, have);
+            x.dy[c].load(static_cast<const T*>(a.grad_y) + at_row * a.grad_y_stride + at, have);
+            if (a.grad_sum) x.more[c].load(static_cast<const T*>(a.grad_sum) + at_row * a.grad_sum_stride + at, have);
+        }
+    };
+    Row x, next;
+    if (!S::LEAN) load(next, row);
+    for (; row < a.rows; row += step) {
+        if constexpr (S::LEAN) {
+            load(x, row);
+        } else {
+            x = next;
+            load(next, row + step);  // on its way while this one is worked on
+        }
+        float dot = 0.0f;
+#pragma unroll
+        for (int c = 0; c < S::CHUNKS; ++c) {
+            const int have = width - (c * S::LANES + lane) * 8;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if (i >= have) continue;
-                const float n = s[c][i] * rstd, t = dy[c][i] * n;
+                const float n = x.s[c][i] * x.rstd, t = x.dy[c][i] * n;
                 dot = __builtin_fmaf(t, w[c][i], dot);
                 dw[c][i] += t;
             }
@@ -217,13 +254,12 @@ __global__ void __launch_bounds__(S::THREADS) k_rms_backward(Params a) {
         for (int c = 0; c < S::CHUNKS; ++c) {
             const int at = (c * S::LANES + lane) * 8, have = width - at;
             if (have <= 0) continue;
-            Eight<T> more, dx;
-            if (a.grad_sum) more.load(static_cast<const T*>(a.grad_sum) + row * a.grad_sum_stride + at, have);
+            Eight<T> dx;
             float d[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                d[i] = rstd * (dy[c][i] * w[c][i] - s[c][i] * rstd * mean);
-                if (a.grad_sum) d[i] += more[i];
+                d[i] = x.rstd * (x.dy[c][i] * w[c][i] - x.s[c][i] * x.rstd * mean);
+                if (a.grad_sum) d[i] += x.more[c][i];
                 dx.set(i, d[i]);
             }
             if (a.grad_residual) dx.store(static_cast<T*>(a.grad_residual) + row * a.width + at, have);
@@ -265,31 +301,41 @@ __global__ void __launch_bounds__(S::THREADS) k_rms_backward(Params a) {
     }
 }
 
-// dw from the workgroups' sums: 32 columns a workgroup, its threads' 8 slices of the rows.
+// dw from the workgroups' sums: 32 columns a workgroup, the rows in kSlices of its threads.
+constexpr int kSlices = 32;
 template <typename T>
-__global__ void __launch_bounds__(256) k_rms_join(const float* partial, int blocks, int width, T* out) {
-    __shared__ float part[8][33];
-    const int col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+__global__ void __launch_bounds__(32 * kSlices) k_rms_join(const float* partial, int blocks, int width, T* out) {
+    __shared__ float part[kSlices][33];
+    const int lane = threadIdx.x & 31, col = blockIdx.x * 32 + lane, slice = threadIdx.x >> 5;
     float sum = 0.0f;
-    if (col < width)
-        for (int b = slice; b < blocks; b += 8) sum += partial[(int64_t)b * width + col];
-    part[slice][threadIdx.x & 31] = sum;
-    __syncthreads();
-    if (slice == 0 && col < width) {
-        for (int k = 1; k < 8; ++k) sum += part[k][threadIdx.x];
-        out[col] = from_f32<T>(sum);
+    if (col < width) {
+#pragma unroll 4
+        for (int b = slice; b < blocks; b += kSlices) sum += partial[(int64_t)b * width + col];
     }
+    part[slice][lane] = sum;
+    for (int half = kSlices / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (slice < half) part[slice][lane] += part[slice + half][lane];
+    }
+    if (slice == 0 && col < width) out[col] = from_f32<T>(part[0][lane]);
 }
 
-// Calls f with the shape that rows of `width` take.
-template <typename F>
+// Calls f with the shape that rows of `width` take: a wave a row as long as its elements fit
+// the lanes' registers, then as few lanes as do.
+constexpr int kWaveWidth = 2048;
+template <typename T, typename F>
 int with_shape(int64_t width, F f) {
     if (width <= 512) return f(Shape<64, 1>{});
     if (width <= 1024) return f(Shape<64, 2>{});
-    if (width <= 2048) return f(Shape<256, 1>{});
+    if (width <= kWaveWidth) return f(Shape<64, 4>{});
     if (width <= 4096) return f(Shape<256, 2>{});
-    if (width <= 8192) return f(Shape<256, 4>{});
-    if (width <= 16384) return f(Shape<1024, 2>{});
+    if constexpr (sizeof(T) == 4) {
+        if (width <= 8192) return f(Shape<512, 2>{});
+        if (width <= 16384) return f(Shape<1024, 2>{});
+    } else {
+        if (width <= 8192) return f(Shape<256, 4>{});
+        if (width <= 16384) return f(Shape<512, 4>{});
+    }
     return f(Shape<1024, 4>{});
 }
 template <typename F>
@@ -298,13 +344,9 @@ int with_type(int dtype, F f) {
     if (dtype == GEFEN_F16) return f(f16_t{});
     return f(bf16_t{});
 }
-template <typename S>
-int blocks_of(int64_t rows, int most) {
-    const int64_t want = (rows + S::ROWS - 1) / S::ROWS;
+int blocks_of(int64_t rows, int64_t width, int most) {
+    const int64_t each = width <= kWaveWidth ? 4 : 1, want = (rows + each - 1) / each;
     return (int)(want < most ? want : most);
-}
-int backward_blocks(int64_t rows, int64_t width) {
-    return with_shape(width, [&](auto s) { return blocks_of<decltype(s)>(rows, kBackwardBlocks); });
 }
 
 int check_task(const gefen_rms_norm_task* t) {
@@ -356,7 +398,7 @@ using namespace gefen;
 
 extern "C" size_t gefen_rms_norm_backward_workspace_size(const gefen_rms_norm_task* task) {
     if (check_task(task) != GEFEN_OK) return 0;
-    return (size_t)backward_blocks(task->rows, task->width) * task->width * 4 + 16;
+    return (size_t)blocks_of(task->rows, task->width, kBackwardBlocks) * task->width * 4 + 16;
 }
 
 extern "C" int gefen_rms_norm_forward(const gefen_rms_norm_task* task, gefen_stream_t stream) {
@@ -376,9 +418,10 @@ extern "C" int gefen_rms_norm_forward(const gefen_rms_norm_task* task, gefen_str
     const Params a = params_of(t);
     hipStream_t st = static_cast<hipStream_t>(stream);
     return with_type(t.dtype, [&](auto v) {
-        return with_shape(t.width, [&](auto s) {
+        using T = decltype(v);
+        return with_shape<T>(t.width, [&](auto s) {
             using S = decltype(s);
-            k_rms_forward<decltype(v), S><<<blocks_of<S>(t.rows, kForwardBlocks), S::THREADS, 0, st>>>(a);
+            k_rms_forward<T, S><<<blocks_of(t.rows, t.width, kForwardBlocks), S::THREADS, 0, st>>>(a);
             return launch_status("rms_norm");
         });
     });
@@ -404,9 +447,9 @@ extern "C" int gefen_rms_norm_backward(const gefen_rms_norm_task* task, void* wo
     hipStream_t st = static_cast<hipStream_t>(stream);
     return with_type(t.dtype, [&](auto v) {
         using T = decltype(v);
-        const int blocks = backward_blocks(t.rows, t.width);
+        const int blocks = blocks_of(t.rows, t.width, kBackwardBlocks);
         if (t.rows && (a.grad_x || a.grad_residual || a.partial)) {
-            const int rc = with_shape(t.width, [&](auto s) {
+            const int rc = with_shape<T>(t.width, [&](auto s) {
                 using S = decltype(s);
                 k_rms_backward<T, S><<<blocks, S::THREADS, 0, st>>>(a);
                 return launch_status("rms_norm");
@@ -414,7 +457,7 @@ extern "C" int gefen_rms_norm_backward(const gefen_rms_norm_task* task, void* wo
             if (rc) return rc;
         }
         if (a.partial) {
-            k_rms_join<T><<<(uint32_t)((t.width + 31) / 32), 256, 0, st>>>(a.partial, blocks, (int)t.width,
+            k_rms_join<T><<<(uint32_t)((t.width + 31) / 32), 32 * kSlices, 0, st>>>(a.partial, blocks, (int)t.width,
                                                                            static_cast<T*>(a.grad_weight));
             return launch_status("rms_norm");
         }
