@@ -375,7 +375,7 @@ template <typename T>
 constexpr float kBackwardShift = kHalf<T> ? 14.0f : 0.0f;
 
 template <typename T, int DP, bool ASYNC>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_forward(Params a) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) k_forward(Params a) {
     using TileT = Tile<T, BN, DP>;
     using PipeT = Pipe<T, DP, ASYNC>;
     constexpr int DT = DP / 32;
@@ -480,39 +480,42 @@ __global__ void __launch_bounds__(kThreads) k_join_forward(Params a) {
     const int64_t stat = ((int64_t)b * heads + h) * a.queries + i;
     float most = -INFINITY;
     for (int p = 0; p < a.parts; ++p) most = fmaxf(most, a.partial_lse[p * a.stats + stat]);
-    const int d = (threadIdx.x & 31) * 4;
+    const int d = (threadIdx.x & 31) * 4, have = a.width - d;
     float sum = 0.0f, out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
     for (int p = 0; p < a.parts; ++p) {
         const float lse = a.partial_lse[p * a.stats + stat];
+        u32x4 x = {0u, 0u, 0u, 0u};
+        if (have > 0) x = load_chunk(a.partial + p * a.partial_stride + row * a.width + d, have);
         if (lse == -INFINITY) continue;  // no keys
         const float w = __builtin_amdgcn_exp2f(lse - most);
         sum += w;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (d + k < a.width) out[k] = __builtin_fmaf(w, a.partial[p * a.partial_stride + row * a.width + d + k], out[k]);
+        for (int k = 0; k < 4; ++k) out[k] = __builtin_fmaf(w, __uint_as_float(x[k]), out[k]);
     }
     const bool empty = sum == 0.0f;
     // keys, but none of a finite score
     const float f = empty ? 1.0f : most == kAllInfinite ? __uint_as_float(0x7fc00000u) : 1.0f / sum;
-    if (d < a.width)
-        store4(static_cast<T*>(a.o.p) + row * a.width + d, out[0] * f, out[1] * f, out[2] * f, out[3] * f, a.width - d);
+    if (have > 0) store4(static_cast<T*>(a.o.p) + row * a.width + d, out[0] * f, out[1] * f, out[2] * f, out[3] * f, have);
     if (a.lse && d == 0) a.lse[stat] = empty ? 0.0f : (most + __builtin_amdgcn_logf(sum)) + (f != f ? f : 0.0f);
 }
 
-// The sum of the parts, in their order.
+// The sums of the parts, in their order: of dQ, or of dK and (blockIdx.y = 1) dV.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_join_sums(const float* partial, int parts, int64_t stride, int64_t numel,
-                                                        T* out) {
+                                                        T* first, T* second) {
     const int64_t e = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4;
     if (e >= numel) return;
     const int have = (int)min((int64_t)4, numel - e);
+    partial += blockIdx.y * parts * stride + e;
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
     for (int p = 0; p < parts; ++p) {
-        const u32x4 x = load_chunk(partial + p * stride + e, have);
+        const u32x4 x = load_chunk(partial + p * stride, have);
 #pragma unroll
         for (int k = 0; k < 4; ++k) sum[k] += __uint_as_float(x[k]);
     }
-    store4(out + e, sum[0], sum[1], sum[2], sum[3], have);
+    store4((blockIdx.y ? second : first) + e, sum[0], sum[1], sum[2], sum[3], have);
 }
 
 // The power of two that brings values of up to `most` into [-1, 1].
@@ -756,7 +759,7 @@ __device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile,
 // The workgroups of dK (the longer ones), then those of dV; of each the keys first that most
 // rows see.
 template <typename T, int DP, bool ASYNC>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_keys(Params a) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) k_backward_keys(Params a) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];  // Pipe::BYTES
     const int heads = a.batch * a.kv_heads, half = gridDim.x / 2;
     const bool values = blockIdx.x >= half;
@@ -785,11 +788,11 @@ int launch(Pass pass, const Params& a, hipStream_t st) {
         const int64_t rows = (int64_t)a.batch * a.queries * a.kv_heads * a.group;
         k_join_forward<T><<<(uint32_t)((rows + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st>>>(a);
     } else {
-        const View* const out[2] = {pass == kQueriesPass ? &a.gq : &a.gk, &a.gv};
-        for (int k = 0; k < (pass == kKeysPass ? 2 : 1); ++k)
-            k_join_sums<T><<<(uint32_t)((a.partial_stride / 4 + kThreads - 1) / kThreads + 1), kThreads, 0, st>>>(
-                a.partial + k * a.parts * a.partial_stride, a.parts, a.partial_stride, out[k]->batch * a.batch,
-                static_cast<T*>(out[k]->p));
+        const bool keys = pass == kKeysPass;
+        const View& out = keys ? a.gk : a.gq;
+        const int64_t numel = out.batch * a.batch;
+        k_join_sums<T><<<dim3((uint32_t)((numel + 4 * kThreads - 1) / (4 * kThreads)), keys ? 2 : 1), kThreads, 0, st>>>(
+            a.partial, a.parts, a.partial_stride, numel, static_cast<T*>(out.p), static_cast<T*>(a.gv.p));
     }
     return launch_status("attention");
 }
@@ -823,20 +826,24 @@ int64_t out_count(Pass pass, const gefen_attention_task& t) {
     return t.batch * t.width * (pass == kKeysPass ? t.keys * t.kv_heads : t.queries * t.heads);
 }
 
-// Into how many parts a workgroup's tiles are split.  The chip holds `slots` workgroups; few of
-// them leave it idle (one query of 16 sequences over 8192 keys, 128 workgroups: 263 us whole,
-// 101 us in 8 parts with the join).  Packed sequences of uneven length make as many as it holds
-// wait for the longest one's keys (11 sequences of 16384 tokens, 2048 workgroups of dK and dV:
-// 1360 us whole, 1180 us in 4 parts with the join; one sequence of 8192: 1570 and 1590).  A part
-// has four tiles at least, for its sums go through memory.
+// Into how many parts a workgroup's tiles are split.  The chip holds `slots` workgroups, and few
+// of them leave it idle: one query of 16 sequences over 8192 keys, 128 workgroups, took 263 us
+// whole, 100 us in 4 parts with the join and 107 in 8; 195 workgroups of 16 tiles took 31.5 us
+// whole and 32.2 in 2 parts, so there have to be three; those of dK and dV, which differ in
+// length, took 78 us whole and 61 in 2.  Packed sequences of uneven length make as many as the
+// chip holds wait for the longest one's keys (11 sequences of 16384 tokens, 2048 workgroups: 1360
+// us whole, 1115 us in 4 parts with the join; one sequence of 8192: 1570 and 1590).  A part has
+// four tiles at least, for its sums go through memory.
 int parts_of(Pass pass, const gefen_attention_task& t) {
+    const bool keys = pass == kKeysPass;
     const int64_t slots = t.dtype == GEFEN_F32 ? 256 : 512, group = t.heads / t.kv_heads;
-    const int64_t cols = pass == kKeysPass ? t.keys : t.queries * group;
-    const int64_t tiles = pass == kKeysPass ? group * ((t.queries + BN - 1) / BN) : (t.keys + BN - 1) / BN;
-    const int64_t wgs = t.batch * t.kv_heads * ((cols + kCols - 1) / kCols) * (pass == kKeysPass ? 2 : 1);
+    const int64_t cols = keys ? t.keys : t.queries * group;
+    const int64_t tiles = keys ? group * ((t.queries + BN - 1) / BN) : (t.keys + BN - 1) / BN;
+    const int64_t wgs = t.batch * t.kv_heads * ((cols + kCols - 1) / kCols) * (keys ? 2 : 1);
     if (wgs == 0 || tiles == 0) return 1;
-    int64_t parts = (2 * slots + wgs - 1) / wgs;
-    if (pass == kKeysPass && t.offsets && t.sequences > 1 && wgs < 8 * slots) parts = parts > 4 ? parts : 4;
+    int64_t parts = slots / wgs;
+    if (!keys && parts < 3) parts = 1;
+    if (keys && t.offsets && t.sequences > 1 && wgs < 8 * slots && parts < 4) parts = 4;
     parts = parts < tiles / 4 ? parts : tiles / 4;
     return (int)(parts < 1 ? 1 : parts > 32 ? 32 : parts);
 }
