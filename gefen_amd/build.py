@@ -36,7 +36,8 @@ LIBS = {
     "libgefen_hip.so": ["capi.cpp", "step.hip", "step_inst_bf16.hip", "step_inst_f16.hip", "step_inst_f32.hip",
                         "step_inst_bf16_f32.hip", "step_inst_f16_f32.hip", "codebook.hip", "period.hip", "ns_gemm.hip",
                         "newton_schulz.hip", "muon.hip", "gradient_norm.hip", "linear_cross_entropy.hip", "attention.hip",
-                        "rms_norm.hip", "dropout.hip"],
+                        "attention_inst_f32.hip", "attention_inst_f16.hip", "attention_inst_bf16.hip", "rms_norm.hip",
+                        "dropout.hip"],
     "libgefen_synth.so": ["capi.cpp", "synthetic.hip"],
 }
 
