@@ -161,8 +161,8 @@ struct Rows {
 
 // Fills two tiles, one behind the other, from rows r0 .. of two operands.  ASYNC: rows are
 // 16-byte aligned and a width of whole chunks (what lies behind the width is cleared once); issue() starts LOADS loads of a wave, for which the caller waits, each lane at
-// an offset of its own that stays the same from tile to tile.  What lies behind the last row
-// is left as it is: no step takes a row that it does not see.  Otherwise (ASYNC false) issue()
+// an offset of its own that stays the same from tile to tile, and zeros behind the last row
+// (what LDS held there would count as values that are not finite).  Otherwise (ASYNC false) issue()
 // takes the rows into registers, the last one again behind it, and land() writes them.
 template <typename T, int ROWS, int DP, bool ASYNC, int THREADS>
 struct Filler {
@@ -216,9 +216,12 @@ struct Filler {
             asm volatile("" : "+v"(t));  // rows are not kept in registers for the last tile's sake
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
-                bool have = off[i] != kBehind;
-                if (tail) have = have && r0 + row(i, t) < count;
-                if (have) load_to_lds(second(i) ? y : x, off[i], to + i * THREADS * 16);
+                const bool have = off[i] != kBehind, in = !tail || r0 + row(i, t) < count;
+                if (have && in) load_to_lds(second(i) ? y : x, off[i], to + i * THREADS * 16);
+                if (!in) {
+                    typedef __attribute__((address_space(3))) u32x4 lds_chunk;
+                    *(lds_chunk*)(uintptr_t)(to + (i * THREADS + t % 64) * 16) = u32x4{0u, 0u, 0u, 0u};
+                }
             }
         } else {
 #pragma unroll
@@ -800,14 +803,17 @@ int launch(Pass pass, const Params& a, hipStream_t st) {
     return launch_status("attention");
 }
 // Whether a tensor's rows are whole 16-byte chunks at distances that a tile's offsets hold.
-inline bool chunked(const Params& a, const View& v, int size) {
-    return aligned(v.p, 16) && a.width * size % 16 == 0 && v.batch * size % 16 == 0 && v.row * size % 16 == 0 &&
-           v.head * size % 16 == 0 && v.row < (int64_t)1 << 22;
+inline bool chunked(const Params& a, const View& v, int rows, int heads, int size) {
+    auto apart = [&](int64_t stride, int count) { return count <= 1 || stride * size % 16 == 0; };
+    return aligned(v.p, 16) && a.width * size % 16 == 0 && apart(v.batch, a.batch) && apart(v.row, rows) &&
+           apart(v.head, heads) && (rows <= 1 || v.row < (int64_t)1 << 22);
 }
 template <typename T, int DP>
 int launch_filler(Pass pass, const Params& a, hipStream_t st) {
     const bool keys = pass == kKeysPass;
-    const bool async = chunked(a, keys ? a.q : a.k, sizeof(T)) && chunked(a, keys ? a.go : a.v, sizeof(T));
+    const int rows = keys ? a.queries : a.keys, heads = keys ? a.kv_heads * a.group : a.kv_heads;
+    const bool async = chunked(a, keys ? a.q : a.k, rows, heads, sizeof(T)) &&
+                       chunked(a, keys ? a.go : a.v, rows, heads, sizeof(T));
     return async ? launch<T, DP, true>(pass, a, st) : launch<T, DP, false>(pass, a, st);
 }
 template <typename T>
