@@ -160,10 +160,12 @@ struct Rows {
 };
 
 // Fills two tiles, one behind the other, from rows r0 .. of two operands.  ASYNC: rows are
-// 16-byte aligned and a width of whole chunks (what lies behind the width is cleared once); issue() starts LOADS loads of a wave, for which the caller waits, each lane at
-// an offset of its own that stays the same from tile to tile, and zeros behind the last row
-// (what LDS held there would count as values that are not finite).  Otherwise (ASYNC false) issue()
-// takes the rows into registers, the last one again behind it, and land() writes them.
+// 16-byte aligned and a width of whole chunks (what lies behind the width is cleared once);
+// issue() starts LOADS loads of a wave, for which the caller waits, each lane at an offset of
+// its own that stays the same from tile to tile.  What lies behind the last row is left as it
+// is: no step takes a row that it does not see (zeros there cost heads of 128 8%).  Otherwise
+// (ASYNC false) issue() takes the rows into registers, the last one again behind it, and land()
+// writes them.
 template <typename T, int ROWS, int DP, bool ASYNC, int THREADS>
 struct Filler {
     using TileT = Tile<T, ROWS, DP>;
@@ -216,12 +218,9 @@ struct Filler {
             asm volatile("" : "+v"(t));  // rows are not kept in registers for the last tile's sake
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
-                const bool have = off[i] != kBehind, in = !tail || r0 + row(i, t) < count;
-                if (have && in) load_to_lds(second(i) ? y : x, off[i], to + i * THREADS * 16);
-                if (!in) {
-                    typedef __attribute__((address_space(3))) u32x4 lds_chunk;
-                    *(lds_chunk*)(uintptr_t)(to + (i * THREADS + t % 64) * 16) = u32x4{0u, 0u, 0u, 0u};
-                }
+                bool have = off[i] != kBehind;
+                if (tail) have = have && r0 + row(i, t) < count;
+                if (have) load_to_lds(second(i) ? y : x, off[i], to + i * THREADS * 16);
             }
         } else {
 #pragma unroll
@@ -328,6 +327,12 @@ struct Column {
             c[s] = at < width ? load_chunk(row + at, width - at) : u32x4{0u, 0u, 0u, 0u};
         }
     }
+    // The row has arrived: without a use before the tiles' loop the compiler waits for it within,
+    // each time, and so for the next tile's loads.
+    __device__ __forceinline__ void arrived() {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) asm volatile("" : "+v"(c[s]));
+    }
     // sum of this half's products with another row, float32
     __device__ __forceinline__ float dot(const Column& o) const {
         float sum = 0.0f;
@@ -367,6 +372,12 @@ __device__ __forceinline__ void store_column(T* row, const f32x16 (&acc)[DT], fl
         }
 }
 
+// LDS reads that are on their way before the matrix instruction of the first one, where stream()
+// orders them: the forward pass (11 packed sequences of 16384 tokens, heads of 64: 515 us, and
+// 535 as the compiler orders them) and dK and dV of wide heads (8192 tokens, heads of 128: 1477
+// and 1590 us; heads of 64: 1126 and 1026).  dQ took 768 and 770, 608 and 564 us.
+constexpr int kAhead = 4;
+
 // Half precision keeps 2^-14 .. 65504 at full precision, so what is rounded to it is brought
 // there by powers of two that are taken out again: probabilities by 2^14 in the backward pass
 // and 2^6 in the forward one (whose running maximum may lag by 2^8), and dO v - D by the
@@ -385,6 +396,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) 
     using TileT = Tile<T, BN, DP>;
     using PipeT = Pipe<T, DP, ASYNC>;
     constexpr int DT = DP / 32;
+    constexpr bool STREAM = sizeof(T) == 2;
     extern __shared__ __attribute__((aligned(1024))) char smem[];  // PipeT::BYTES
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     // the rows that see most keys first
@@ -402,6 +414,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) 
     PipeT pipe(a.k, a.v, keys.base, values.base, a.width, a.keys, smem);
     Column<T, DP> q;
     q.load(queries.at(a, uc), a.width, lane);
+    q.arrived();
     f32x16 acc[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
@@ -409,9 +422,15 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) 
 
     auto tile_step = [&](auto partial, int k0, const TileT& kt, const TileT& vt) __attribute__((always_inline)) {
         constexpr bool PARTIAL = decltype(partial)::value;
-        f32x16 s[2];
+        f32x16 s[2] = {};
+        if constexpr (STREAM && !PARTIAL) {
+            constexpr int STEPS = Column<T, DP>::STEPS;
+            stream<2 * STEPS, kAhead>([&](int i) { return kt.row_chunk(32 * (i / STEPS), i % STEPS, lane); },
+                                      [&](int i, u32x4 f) { s[i / STEPS] = mma_rows<T>(f, q.c[i % STEPS], s[i / STEPS]); });
+        } else {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) s[t] = rows_product(kt, 32 * t, q, lane);
+            for (int t = 0; t < 2; ++t) s[t] = rows_product(kt, 32 * t, q, lane);
+        }
         float most = -INFINITY;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -430,6 +449,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) 
             for (int dt = 0; dt < DT; ++dt) acc[dt] *= f;
         }
         const float shift = kForwardShift<T> - (top == -INFINITY ? 0.0f : top);
+        const RowRange rows = {span.lo - k0, span.hi - k0};
         uint32_t bad = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -440,13 +460,21 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) 
                 s[t][i] = p;
                 sum += p;
             }
+            if (STREAM && !PARTIAL) continue;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const PFrag<T> p = pack<T>(s[t], c);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
-                    acc[dt] = vt.template mma_columns<PARTIAL>(p, 32 * t + 16 * c, 32 * dt, lane, acc[dt], &bad);
+                    acc[dt] = vt.template mma_columns<PARTIAL>(p, 32 * t + 16 * c, 32 * dt, lane, acc[dt], rows, &bad);
             }
+        }
+        if constexpr (STREAM && !PARTIAL) {
+            PFrag<T> p[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) p[c] = pack<T>(s[c / 2], c % 2);
+            stream<4 * DT, kAhead>([&](int i) { return vt.column_chunk(16 * (i / DT), 32 * (i % DT), lane); },
+                                   [&](int i, u32x4 f) { acc[i % DT] = mma_chunk<T>(f, p[i / DT], acc[i % DT]); });
         }
         if (PARTIAL && __any((bad & kBadBits<T>) != 0)) vt.template add_nonfinite<false>(acc, BN, seen.lo - k0, seen.hi - k0, lane);
     };
@@ -602,6 +630,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
     delta += other_half(delta);
     if (lane < 32 && u < a.rows && part == 0) a.delta[stat_at(a, bh, u)] = delta;
     q.load(Rows<T, true>(a, a.q, b, hk).at(a, uc), a.width, lane);
+    q.arrived();
     const float shift = kBackwardShift<T> - a.lse[stat_at(a, bh, uc)];
     float unit = 1.0f;
     if constexpr (kHalf<T>) {
@@ -615,15 +644,16 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
 
     auto tile_step = [&](auto partial, int k0, const TileT& kt, const TileT& vt) __attribute__((always_inline)) {
         constexpr bool PARTIAL = decltype(partial)::value;
+        const RowRange rows = {span.lo - k0, span.hi - k0};
         uint32_t bad = 0;
 #pragma unroll 1
         for (int t = 0; t < 2; ++t) {
-            f32x16 s = rows_product(kt, 32 * t, q, lane);
-            f32x16 dp = {};
+            f32x16 s = {}, dp = {};
             if constexpr (DP <= 64) {  // wide heads took 7% longer this way
 #pragma unroll
                 for (int i = 0; i < 16; ++i) dp[i] = -delta;
             }
+            s = rows_product(kt, 32 * t, q, lane);
             dp = rows_product(vt, 32 * t, go, lane, dp);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -638,7 +668,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
                 const PFrag<T> ds = pack<T>(s, c);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
-                    acc[dt] = kt.template mma_columns<PARTIAL>(ds, 32 * t + 16 * c, 32 * dt, lane, acc[dt], &bad);
+                    acc[dt] = kt.template mma_columns<PARTIAL>(ds, 32 * t + 16 * c, 32 * dt, lane, acc[dt], rows, &bad);
             }
         }
         if (PARTIAL && __any((bad & kBadBits<T>) != 0)) kt.template add_nonfinite<true>(acc, BN, seen.lo - k0, seen.hi - k0, lane);
@@ -666,6 +696,7 @@ template <typename T, int DP, bool ASYNC, bool VALUES>
 __device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile, int part, char* smem) {
     using TileT = Tile<T, BN, DP>;
     constexpr int DT = DP / 32;
+    constexpr bool STREAM = sizeof(T) == 2 && DP > 64;
     // L / c and D of each buffer's rows, which the products subtract: as terms of their own, or
     // (float32) as numbers to start from
     constexpr bool TERMS = sizeof(T) == 2;
@@ -685,6 +716,8 @@ __device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile,
     Column<T, DP> k, v;
     k.load(Rows<T, false>(a, a.k, b, hk).at(a, jc), a.width, lane);
     if (!VALUES) v.load(Rows<T, false>(a, a.v, b, hk).at(a, jc), a.width, lane);
+    k.arrived();
+    if (!VALUES) v.arrived();
     // S - L / c is formed, and c applied after; with a c that is as good as zero, -L with a key of zeros
     float c = a.c, over = 1.0f / a.c;
     if (!(a.c > 5.4e-20f)) {
@@ -701,6 +734,7 @@ __device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile,
     auto tile_step = [&](auto partial, int i0, const TileT& qt, const TileT& gt, int buffer) __attribute__((always_inline)) {
         constexpr bool PARTIAL = decltype(partial)::value;
         const TileT& into = VALUES ? gt : qt;
+        const RowRange rows = {span.lo - i0, span.hi - i0};
         uint32_t bad = 0;
 #pragma unroll UNROLL
         for (int t = 0; t < BN / 32; ++t) {
@@ -715,8 +749,18 @@ __device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile,
                     if (!VALUES) dp[i] = row_starts[buffer][1][row_of(32 * t, i, lane)];
                 }
             }
-            s = rows_product(qt, 32 * t, k, lane, s);
-            if (!VALUES) dp = rows_product(gt, 32 * t, v, lane, dp);
+            if constexpr (STREAM && !PARTIAL) {
+                constexpr int STEPS = Column<T, DP>::STEPS;
+                stream<STEPS * (VALUES ? 1 : 2), kAhead>(
+                    [&](int i) { return (i < STEPS ? qt : gt).row_chunk(32 * t, i % STEPS, lane); },
+                    [&](int i, u32x4 f) {
+                        if (i < STEPS) s = mma_rows<T>(f, k.c[i], s);
+                        else dp = mma_rows<T>(f, v.c[i - STEPS], dp);
+                    });
+            } else {
+                s = rows_product(qt, 32 * t, k, lane, s);
+                if (!VALUES) dp = rows_product(gt, 32 * t, v, lane, dp);
+            }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int r = row_of(32 * t, i, lane);
@@ -724,12 +768,18 @@ __device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile,
                 if (!VALUES) p *= kHalf<T> ? dp[i] * unit : dp[i];
                 s[i] = PARTIAL && !within(i0 + r, seen) ? 0.0f : p;
             }
+            if constexpr (STREAM && !PARTIAL) {
+                const PFrag<T> p[2] = {pack<T>(s, 0), pack<T>(s, 1)};
+                stream<2 * DT, kAhead>([&](int i) { return into.column_chunk(32 * t + 16 * (i / DT), 32 * (i % DT), lane); },
+                                       [&](int i, u32x4 f) { acc[i % DT] = mma_chunk<T>(f, p[i / DT], acc[i % DT]); });
+                continue;
+            }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const PFrag<T> p = pack<T>(s, c);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
-                    acc[dt] = into.template mma_columns<PARTIAL>(p, 32 * t + 16 * c, 32 * dt, lane, acc[dt], &bad);
+                    acc[dt] = into.template mma_columns<PARTIAL>(p, 32 * t + 16 * c, 32 * dt, lane, acc[dt], rows, &bad);
             }
         }
         if (PARTIAL && __any((bad & kBadBits<T>) != 0))

@@ -118,6 +118,13 @@ __device__ __forceinline__ PFrag<T> pack(const f32x16& p, int chunk) {
     return out;
 }
 
+// A columns product's step of 16-bit elements: a tile's chunk and sixteen rows of p.
+template <typename T>
+__device__ __forceinline__ f32x16 mma_chunk(u32x4 a, const PFrag<T>& p, f32x16 acc) {
+    if constexpr (sizeof(T) == 2) acc = mma_rows<T>(a, p.v, acc);
+    return acc;
+}
+
 // Zeros in place of what is not finite; *bad gets bits of kBadBits where there was any.  The
 // largest exponent plus its lowest bit carries into the sign's place.
 template <typename T>
@@ -140,6 +147,12 @@ constexpr __device__ __forceinline__ int chunk_xor(int r, int chunks) {
                              : (r >> 2) & 3;
 }
 
+// Rows of a tile that a wave sees.
+struct RowRange {
+    int lo, hi;
+    __device__ __forceinline__ bool has(int r) const { return (uint32_t)(r - lo) < (uint32_t)(hi - lo); }
+};
+
 template <typename T, int BN, int DP>
 struct Tile {
     static constexpr int EPC = Elem<T>::EPC, LD = DP;
@@ -160,38 +173,42 @@ struct Tile {
     __device__ __forceinline__ u32x4 row_chunk(int r0, int c, int lane) const {
         return *(const lds_chunk*)(p + r0 * LD + place(lane & 31, (2 * c + (lane >> 5)) * EPC));
     }
-    // acc[d0 + .., n] += sum over rows r0 .. r0 + 15 (r0 a multiple of 16).  CHECK: what is not finite counts as
-    // zero, and *bad tells (kBadBits).
+    // The columns product's left side (16-bit elements): rows r0 .. r0 + 15 of columns d0 .. d0 + 31.
+    // In each group of 16 lanes, lane 4 j + q points at row j, elements 4 q .. 4 q + 3.
+    __device__ __forceinline__ u32x4 column_chunk(int r0, int d0, int lane) const {
+        typedef __attribute__((address_space(3))) bf16x4 lds_v4;
+        const int row = 4 * (lane >> 5) + ((lane & 15) >> 2);
+        const int col = d0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4*)(p + r0 * LD + place(row, col)));
+        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4*)(p + r0 * LD + place(row + 8, col)));
+        return __builtin_bit_cast(u32x4, bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+    }
+    // acc[d0 + .., n] += sum over rows r0 .. r0 + 15 (r0 a multiple of 16).  CHECK: rows
+    // outside `rows` count as zeros whatever LDS holds there; of the others, what is not finite
+    // does, and *bad tells (kBadBits).
     template <bool CHECK>
     __device__ __forceinline__ f32x16 mma_columns(const PFrag<T>& b, int r0, int d0, int lane, f32x16 acc,
-                                                  uint32_t* bad) const {
+                                                  RowRange rows, uint32_t* bad) const {
         const int h = lane >> 5;
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 uint32_t a = p[r0 * LD + place(8 * (i / 4) + 4 * h + i % 4, d0 + (lane & 31))];
-                if (CHECK) a = drop_nonfinite<T>(a, bad);
+                if (CHECK) a = drop_nonfinite<T>(rows.has(r0 + 8 * (i / 4) + 4 * h + i % 4) ? a : 0u, bad);
                 acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a), b.v[i], acc, 0, 0, 0);
             }
             return acc;
         } else {
-            // in each group of 16 lanes, lane 4 j + q points at row j, elements 4 q .. 4 q + 3
-            typedef __attribute__((address_space(3))) bf16x4 lds_v4;
-            const int row = 4 * h + ((lane & 15) >> 2);
-            const int col = d0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-            const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4*)(p + r0 * LD + place(row, col)));
-            const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_v4*)(p + r0 * LD + place(row + 8, col)));
-            u32x4 a = __builtin_bit_cast(u32x4, bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+            u32x4 a = column_chunk(r0, d0, lane);
             if (CHECK) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = drop_nonfinite<T>(a[i], bad);
+                for (int i = 0; i < 4; ++i) {
+                    const int r = r0 + 4 * h + 2 * (i & 1) + 8 * (i >> 1);
+                    a[i] &= (rows.has(r) ? 0x0000ffffu : 0u) | (rows.has(r + 1) ? 0xffff0000u : 0u);
+                    a[i] = drop_nonfinite<T>(a[i], bad);
+                }
             }
-            if constexpr (__is_same(T, f16_t))
-                return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b.v),
-                                                              acc, 0, 0, 0);
-            else
-                return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
-                                                               __builtin_bit_cast(bf16x8, b.v), acc, 0, 0, 0);
+            return mma_rows<T>(a, b.v, acc);
         }
     }
     // What the checked product has left out, for the rows in [lo, hi) that this lane's column
@@ -241,6 +258,22 @@ __device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, u
 // This wave's loads to LDS have landed and its LDS reads are done, then the barrier.
 __device__ __forceinline__ void wait_loads_and_sync() {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// use(i, read(i)) for i < N, the reads DEPTH ahead of their uses.  Left alone the compiler puts an
+// LDS read right before the matrix instruction that takes it and waits its latency out each time;
+// the barriers let nothing but vector and scalar arithmetic across.
+template <int N, int DEPTH, typename Read, typename Use>
+__device__ __forceinline__ void stream(Read read, Use use) {
+    u32x4 f[DEPTH];
+#pragma unroll
+    for (int i = 0; i < DEPTH && i < N; ++i) f[i] = read(i);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_barrier(0x6);
+        use(i, f[i % DEPTH]);
+        if (i + DEPTH < N) f[i % DEPTH] = read(i + DEPTH);
+    }
 }
 
 // EPC elements from p, of which the first `n` exist (n >= 1); zeros for the others.
