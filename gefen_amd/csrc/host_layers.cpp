@@ -4,8 +4,12 @@
 
 #include <cmath>
 #include <cstring>
+#include <functional>
+#include <initializer_list>
 #include <optional>
 #include <vector>
+
+#include <c10/hip/HIPGraphsC10Utils.h>
 
 #include "host_common.h"
 
@@ -66,6 +70,30 @@ void indices(const at::Tensor& t, const char* name, const at::Tensor& first) {
 }
 
 bool wants(const at::Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// Raises where a call under graph capture would join a graph of autograd that was recorded outside,
+// on the default stream: the backward pass waits for the stream of each node that it reaches, a
+// captured one cannot wait for that one, and torch's engine then ends the process.
+void no_eager_graph(std::initializer_list<std::reference_wrapper<const at::Tensor>> operands) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const at::Tensor& t : operands) {
+        if (!wants(t)) continue;
+        const auto node = t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
+        if (!node) continue;
+        const auto stream = node->stream();
+        if (stream && stream->id() == c10::hip::getDefaultHIPStream(t.device().index()).id())
+            throw std::runtime_error(
+                "Expected no autograd graph from outside the capture: drop what was computed from these tensors on the "
+                "default stream, or warm up on another one.");
+    }
+}
+
+// A tensor as a backward pass finds it, which hooks of saved tensors may have replaced.
+at::Tensor found(const at::Tensor& t, c10::IntArrayRef sizes, at::ScalarType type, const at::Tensor& first) {
+    TORCH_CHECK(t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == first.device(),
+                "Expected a saved tensor to come back with its shape, dtype and device.");
+    return t;
+}
 
 // What the last dimension holds, one after the other.
 at::Tensor rows_dense(const at::Tensor& t) {
@@ -154,7 +182,12 @@ class Attention : public torch::autograd::Function<Attention> {
         at::Tensor lse;
         at::Tensor out = attention_forward(query, key, value, lengths, offsets, causal, scale, &lse);
         ctx->save_for_backward({query, key, value, lengths, offsets, out, lse});
-        ctx->saved_data["options"] = std::vector<int64_t>{causal, bits_of(scale), need_q, need_kv};
+        ctx->saved_data["options"] =
+            std::vector<int64_t>{causal,         bits_of(scale), need_q,
+                                 need_kv,        key.size(-3),   key.size(-2),
+                                 lengths.defined() ? static_cast<int64_t>(lengths.scalar_type()) : 0,
+                                 offsets.defined() ? static_cast<int64_t>(offsets.scalar_type()) : 0,
+                                 offsets.defined() ? offsets.size(0) : 0};
         return out;
     }
 
@@ -164,10 +197,20 @@ class Attention : public torch::autograd::Function<Attention> {
         if (grads[0].defined()) {
             const std::vector<int64_t> o = ctx->saved_data["options"].toIntVector();
             const auto saved = ctx->get_saved_variables();
-            const at::Tensor &query = saved[0], &key = saved[1], &value = saved[2], &out = saved[5], &lse = saved[6];
+            const at::Tensor& go = grads[0];
+            const at::ScalarType type = go.scalar_type();
+            auto sizes = go.sizes().vec();
+            const at::Tensor query = found(saved[0], sizes, type, go), out = found(saved[5], sizes, type, go).contiguous();
+            const at::Tensor lse = found(saved[6], {query.numel() / query.size(-1)}, at::kFloat, go).contiguous();
+            sizes[sizes.size() - 3] = o[4];
+            sizes[sizes.size() - 2] = o[5];
+            const at::Tensor key = found(saved[1], sizes, type, go), value = found(saved[2], sizes, type, go);
+            at::Tensor lengths, offsets;
+            if (o[6]) lengths = found(saved[3], {query.size(0)}, static_cast<at::ScalarType>(o[6]), go).contiguous();
+            if (o[7]) offsets = found(saved[4], {o[8]}, static_cast<at::ScalarType>(o[7]), go).contiguous();
             c10::DeviceGuard guard(query.device());
-            AttentionCall c(query, key, value, saved[3], saved[4], o[0], double_of(o[1]));
-            c.go = rows_dense(grads[0]);
+            AttentionCall c(query, key, value, lengths, offsets, o[0], double_of(o[1]));
+            c.go = rows_dense(go);
             c.t.grad_out = c.go.data_ptr();
             AttentionCall::strides(c.go, c.t.grad_out_strides);
             c.t.out = out.data_ptr();
@@ -232,8 +275,10 @@ py::object attention(py::handle query_, py::handle key_, py::handle value_, py::
     const double scale = scale_.is_none() ? 1.0 / std::sqrt(static_cast<double>(query.size(-1))) : scale_.cast<double>();
     const bool grad = c10::GradMode::is_enabled();
     const bool need_q = grad && wants(query), need_kv = grad && (wants(key) || wants(value));
-    if (need_q || need_kv)
+    if (need_q || need_kv) {
+        no_eager_graph({query, key, value});
         return wrap(Attention::apply(query, key, value, maybe(lengths), maybe(offsets), causal, scale, need_q, need_kv));
+    }
     return wrap(attention_forward(query.detach(), key.detach(), value.detach(), lengths, offsets, causal, scale, nullptr));
 }
 
@@ -253,6 +298,7 @@ Seed seed_of(py::handle tensor, int64_t value, const at::Tensor& first) {
     plain_on(s.at, "seed", first);
     if (s.at.scalar_type() != at::kLong || s.at.numel() != 1)
         throw py::value_error("Expected seed to be an int or an int64 tensor of one element.");
+    if (s.at.dim()) s.at = s.at.reshape({});
     return s;
 }
 
@@ -319,7 +365,7 @@ class RmsNorm : public torch::autograd::Function<RmsNorm> {
         check(lib.rms_forward(&c.t, stream_of(x)));
         ctx->save_for_backward({s.defined() ? s : x, weight, rstd, seed});
         ctx->saved_data["options"] = std::vector<int64_t>{bits_of(eps), bits_of(dropout), seed_value, offset,
-                                                          need_x,       need_r,           need_w};
+                                                          need_x,       need_r,           need_w,     seed.defined()};
         if (s.defined()) return {y, s};
         return {y};
     }
@@ -332,7 +378,13 @@ class RmsNorm : public torch::autograd::Function<RmsNorm> {
             const std::vector<int64_t> o = ctx->saved_data["options"].toIntVector();
             const bool need_x = o[4], need_r = o[5], need_w = o[6];
             const auto saved = ctx->get_saved_variables();
-            const at::Tensor &s = saved[0], &weight = saved[1], &rstd = saved[2], &seed = saved[3];
+            const at::Tensor& first = grads[0].defined() ? grads[0] : grads[1];
+            const at::ScalarType type = first.scalar_type();
+            const at::Tensor s = found(saved[0], first.sizes(), type, first);
+            const at::Tensor weight = found(saved[1], {s.size(-1)}, type, first);
+            at::Tensor seed;
+            if (o[7]) seed = found(saved[3], {}, at::kLong, first);
+            const at::Tensor rstd = found(saved[2], {s.numel() / s.size(-1)}, at::kFloat, first).contiguous();
             c10::DeviceGuard guard(s.device());
             RmsCall c(s, weight, at::Tensor(), seed, {double_of(o[0]), double_of(o[1]), o[2], o[3]});
             const at::Tensor gy = as_rows(grads[0].defined() ? grads[0] : at::zeros(s.sizes(), s.options()));
@@ -396,8 +448,9 @@ py::object rms_norm(py::handle x_, py::handle weight_, py::handle residual_, dou
     const bool grad = c10::GradMode::is_enabled();
     const bool need_x = grad && wants(x), need_w = grad && wants(weight), need_r = grad && wants(residual);
     if (need_x || need_w || need_r) {
-        const variable_list out = RmsNorm::apply(x, weight, maybe(residual), maybe(seed.at), eps, dropout, seed.value, offset, need_x,
-                                                 need_r, need_w);
+        no_eager_graph({x, weight, residual});
+        const variable_list out = RmsNorm::apply(x, weight, maybe(residual), maybe(seed.at), eps, dropout, seed.value,
+                                                 offset, need_x, need_r, need_w);
         if (out.size() > 1) return py::make_tuple(wrap(out[0]), wrap(out[1]));
         return wrap(out[0]);
     }
@@ -460,7 +513,7 @@ class DropoutFunction : public torch::autograd::Function<DropoutFunction> {
         ctx->set_materialize_grads(false);
         const at::Tensor &residual = given(residual_), &seed = given(seed_);
         ctx->save_for_backward({seed});
-        ctx->saved_data["options"] = std::vector<int64_t>{bits_of(p), seed_value, offset, need_x, need_r};
+        ctx->saved_data["options"] = std::vector<int64_t>{bits_of(p), seed_value, offset, need_x, need_r, seed.defined()};
         return dropout_run(x, residual, p, seed, seed_value, offset);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -468,8 +521,11 @@ class DropoutFunction : public torch::autograd::Function<DropoutFunction> {
         variable_list out(8);
         if (grads[0].defined()) {
             const std::vector<int64_t> o = ctx->saved_data["options"].toIntVector();
-            if (o[3])
-                out[0] = dropout_run(grads[0], at::Tensor(), double_of(o[0]), ctx->get_saved_variables()[0], o[1], o[2]);
+            if (o[3]) {
+                at::Tensor seed;
+                if (o[5]) seed = found(ctx->get_saved_variables()[0], {}, at::kLong, grads[0]);
+                out[0] = dropout_run(grads[0], at::Tensor(), double_of(o[0]), seed, o[1], o[2]);
+            }
             if (o[4]) out[1] = grads[0];
         }
         return out;
@@ -490,8 +546,10 @@ py::object dropout(py::handle x_, py::handle residual_, double p, py::handle see
     const Seed seed = seed_of(seed_, seed_value, x);
     const bool grad = c10::GradMode::is_enabled();
     const bool need_x = grad && wants(x), need_r = grad && wants(residual);
-    if (need_x || need_r)
+    if (need_x || need_r) {
+        no_eager_graph({x, residual});
         return wrap(DropoutFunction::apply(x, maybe(residual), maybe(seed.at), p, seed.value, offset, need_x, need_r));
+    }
     return wrap(dropout_run(x.detach(), residual.defined() ? residual.detach() : residual, p, seed.at, seed.value, offset));
 }
 
