@@ -14,6 +14,15 @@
 // The heads that share a key head are rows of one problem: row u = query u / G of head
 // u % G of the group (G = heads / kv_heads), so a tile of keys and values is loaded once for
 // all of them, and a single new token still gives G rows.
+//
+// What bounds it: with many rows the matrix cores, and beside them the vector unit: a 32 x 32
+// block of S takes a wave some 480 cycles of exponentials, maxima and conversions, and its two
+// products of the forward pass 256 (heads of 64) or 512.  8192 causal tokens, 32 / 8 heads of
+// 128, bf16: forward 564 us, dQ 752, dK and dV 1390, which is 0.98, 1.10 and 0.99 PFLOP/s on the
+// 2, 3 and 5 products that they form (a large library product reaches 1.22; matrix cores busy
+// 51%, 60% and 58%, no bank conflicts, 1.9 to 2.0 GHz).  8 x 1024 tokens, 12 heads of 64,
+// float32: 151, 230 and 330 us, matrix cores busy 75%, 67% and 78%.  With one row a sequence,
+// HBM: one query in each of 16 sequences of up to 8192 keys, 392 MB of 8 heads of 128, takes 90 us.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -378,6 +387,17 @@ __device__ __forceinline__ void store_column(T* row, const f32x16 (&acc)[DT], fl
 // and 1590 us; heads of 64: 1126 and 1026).  dQ took 768 and 770, 608 and 564 us.
 constexpr int kAhead = 4;
 
+// How the forward pass takes a tile: all of it; what a wave's columns see of it (scores of -inf
+// for the rest, so c must not be zero); or that, with what is not finite kept from the columns
+// that do not see it (0 x inf is NaN), where the tile holds such elements at all, in rows that
+// the wave sees or in others.  Looking first cost less than keeping them out always: packed
+// sequences 530 us and 494.  Wider heads, whose registers it spills, gained 1%, dQ as much
+// (570 and 564), and dK and dV, whose code fills the instruction cache, lost (1013 and 1164):
+// they know the first and the last only.
+enum : int { kFull, kMasked, kChecked };
+template <int KIND>
+using Kind = std::integral_constant<int, KIND>;
+
 // Half precision keeps 2^-14 .. 65504 at full precision, so what is rounded to it is brought
 // there by powers of two that are taken out again: probabilities by 2^14 in the backward pass
 // and 2^6 in the forward one (whose running maximum may lag by 2^8), and dO v - D by the
@@ -420,10 +440,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) 
     for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x16{};
     float top = -INFINITY, sum = 0.0f;
 
-    auto tile_step = [&](auto partial, int k0, const TileT& kt, const TileT& vt) __attribute__((always_inline)) {
-        constexpr bool PARTIAL = decltype(partial)::value;
+    auto tile_step = [&](auto kind, int k0, const TileT& kt, const TileT& vt) __attribute__((always_inline)) {
+        constexpr bool PARTIAL = decltype(kind)::value != kFull, CHECK = decltype(kind)::value == kChecked;
         f32x16 s[2] = {};
-        if constexpr (STREAM && !PARTIAL) {
+        if constexpr (STREAM && !CHECK) {
             constexpr int STEPS = Column<T, DP>::STEPS;
             stream<2 * STEPS, kAhead>([&](int i) { return kt.row_chunk(32 * (i / STEPS), i % STEPS, lane); },
                                       [&](int i, u32x4 f) { s[i / STEPS] = mma_rows<T>(f, q.c[i % STEPS], s[i / STEPS]); });
@@ -456,33 +476,35 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) 
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.c, shift));
-                if (PARTIAL && !within(row_of(k0 + 32 * t, i, lane), seen)) p = 0.0f;
+                if (CHECK && !within(row_of(k0 + 32 * t, i, lane), seen)) p = 0.0f;
                 s[t][i] = p;
                 sum += p;
             }
-            if (STREAM && !PARTIAL) continue;
+            if (STREAM && !CHECK) continue;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const PFrag<T> p = pack<T>(s[t], c);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
-                    acc[dt] = vt.template mma_columns<PARTIAL>(p, 32 * t + 16 * c, 32 * dt, lane, acc[dt], rows, &bad);
+                    acc[dt] = vt.template mma_columns<CHECK>(p, 32 * t + 16 * c, 32 * dt, lane, acc[dt], rows, &bad);
             }
         }
-        if constexpr (STREAM && !PARTIAL) {
+        if constexpr (STREAM && !CHECK) {
             PFrag<T> p[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) p[c] = pack<T>(s[c / 2], c % 2);
             stream<4 * DT, kAhead>([&](int i) { return vt.column_chunk(16 * (i / DT), 32 * (i % DT), lane); },
                                    [&](int i, u32x4 f) { acc[i % DT] = mma_chunk<T>(f, p[i / DT], acc[i % DT]); });
         }
-        if (PARTIAL && __any((bad & kBadBits<T>) != 0)) vt.template add_nonfinite<false>(acc, BN, seen.lo - k0, seen.hi - k0, lane);
+        if (CHECK && __any((bad & kBadBits<T>) != 0)) vt.template add_nonfinite<false>(acc, BN, seen.lo - k0, seen.hi - k0, lane);
     };
 
     auto step = [&](int k0, const TileT& kt, const TileT& vt, int) __attribute__((always_inline)) {
         if (span.none(k0)) return;
-        if (span.full(k0)) tile_step(std::false_type{}, k0, kt, vt);
-        else tile_step(std::true_type{}, k0, kt, vt);
+        if (span.full(k0)) return tile_step(Kind<kFull>{}, k0, kt, vt);
+        if constexpr (sizeof(T) == 2 && DP <= (ASYNC ? 96 : 64))
+            if (a.c >= 1.2e-38f && vt.all_finite(lane)) return tile_step(Kind<kMasked>{}, k0, kt, vt);
+        tile_step(Kind<kChecked>{}, k0, kt, vt);
     };
     pipe.template run<false>(all, 1, 0, 0, part, a.parts, [](int, int, int) {}, [](int) {}, step);
     sum += other_half(sum);
@@ -690,8 +712,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
 
 // dK, or (VALUES) dV.  Together they would need 4 products instead of 5, but their
 // accumulators beside a lane's key and value leave no room for a second wave on a SIMD, and
-// that costs more: at 8192 causal tokens of 32 / 8 heads of 128 one kernel for both took 2022
-// us alone on its SIMDs and 1369 us as pairs of waves that hand P over through LDS.
+// that costs more: at 8192 causal tokens of 32 / 8 heads of 128 (bf16) one kernel for both took
+// 2022 us alone on its SIMDs and 1541 us as pairs of waves that hand P over through LDS, where
+// this one took 1530 (1390 with its LDS reads in order).
 template <typename T, int DP, bool ASYNC, bool VALUES>
 __device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile, int part, char* smem) {
     using TileT = Tile<T, BN, DP>;

@@ -173,6 +173,27 @@ struct Tile {
     __device__ __forceinline__ u32x4 row_chunk(int r0, int c, int lane) const {
         return *(const lds_chunk*)(p + r0 * LD + place(lane & 31, (2 * c + (lane >> 5)) * EPC));
     }
+    // Whether every element of the tile is finite: two operations a word, where keeping what is
+    // not out of the columns product takes five and a half.
+    __device__ __forceinline__ bool all_finite(int lane) const {
+        typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < BYTES / (16 * 64); ++i) {
+            const u32x4 w = ((const lds_chunk*)p)[64 * i + lane];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (sizeof(T) == 4)
+                    most = max(most, w[j] & 0x7fffffffu);
+                else
+                    most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most),
+                                                                                  __builtin_bit_cast(u16x2, w[j] & 0x7fff7fffu)));
+            }
+        }
+        if constexpr (sizeof(T) == 4) return !__any(most >= 0x7f800000u);
+        constexpr uint32_t inf = __is_same(T, f16_t) ? 0x7c00u : 0x7f80u;
+        return !__any((most & 0xffffu) >= inf || most >> 16 >= inf);
+    }
     // The columns product's left side (16-bit elements): rows r0 .. r0 + 15 of columns d0 .. d0 + 31.
     // In each group of 16 lanes, lane 4 j + q points at row j, elements 4 q .. 4 q + 3.
     __device__ __forceinline__ u32x4 column_chunk(int r0, int d0, int lane) const {

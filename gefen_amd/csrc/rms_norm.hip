@@ -5,7 +5,11 @@
 //   g = dy w,   ds += r (g - n mean(g n)),   dx = m ds / (1 - p),   dw = sum over rows of dy n
 //
 // Bound by HBM.  A row stays in the registers of the lanes that own it, so everything is read
-// once and written once: a wave owns a row of up to 1024 elements, a workgroup a longer one.
+// once and written once: a wave owns a row of up to 2048 elements (no wait for other waves), a
+// workgroup a longer one, and the next row is on its way while one is worked on.  8192 rows of
+// 4096, bf16, with a residual: forward 51 us (5.3 TB/s), backward 46 (5.9) and the join of dw 4;
+// 16384 rows of 2048 into 8 bits 51 us (4.6); a copy of 2 GiB moves 4.9.  Fewer rows do not fill
+// the chip: 1531 of 1001 halves take 9 + 12 + 4.5 us, where 24 MB would take 5.
 // The squares are summed in float64, where no 16-bit or float32 value over- or underflows.
 // dw: a workgroup takes rows in strides of the grid and sums its columns in registers, the
 // workgroups' sums are added in a second launch, always in the same order.
@@ -321,7 +325,8 @@ __global__ void __launch_bounds__(32 * kSlices) k_rms_join(const float* partial,
 }
 
 // Calls f with the shape that rows of `width` take: a wave a row as long as its elements fit
-// the lanes' registers, then as few lanes as do.
+// the lanes' registers (16384 rows of 2048: 63 us by a workgroup each and not ahead, 51 so), then
+// as few lanes as do.
 constexpr int kWaveWidth = 2048;
 template <typename T, typename F>
 int with_shape(int64_t width, F f) {
