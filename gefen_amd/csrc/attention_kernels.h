@@ -7,9 +7,9 @@
 //
 // Neither S nor P is stored: the forward pass keeps a running maximum and sum per row, and
 // the backward pass forms P again from L.  It takes two kernels, one that owns queries (dQ,
-// and D on its way) and one that owns keys (dK, dV): S and dO v are formed in both, seven
-// products in place of five, and in return every sum has one owner and one order, with no
-// atomics.
+// and D on its way) and one that owns keys (dK, dV, in workgroups of their own): S and dO v are
+// formed again, eight products in place of five, and in return every sum has one owner and one
+// order, with no atomics.
 //
 // The heads that share a key head are rows of one problem: row u = query u / G of head
 // u % G of the group (G = heads / kv_heads), so a tile of keys and values is loaded once for
