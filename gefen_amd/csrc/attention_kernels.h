@@ -589,7 +589,8 @@ __device__ __forceinline__ float largest_norm(const Params& a, int which, int bh
     return m;
 }
 
-// Largest norms of the rows of v that take part, and of go, for half precision; 16 lanes a row.
+// Largest norms of the rows of v and of go that take part (what the others hold must not reach
+// the scale either), for half precision; 16 lanes a row.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_range(Params a) {
     const int heads = a.batch * a.kv_heads, which = blockIdx.y, part = blockIdx.x % kRangeParts,
@@ -597,11 +598,18 @@ __global__ void __launch_bounds__(kThreads) k_range(Params a) {
     const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
     const Rows<T, true> grads(a, a.go, b, hk);
     const Rows<T, false> values(a, a.v, b, hk);
-    int rows = which ? a.rows : a.keys;
-    if (!which && a.key_lengths) rows = clamped(a.key_lengths, a.lengths64, b, a.keys);
+    Interval in = {0, which ? a.queries : a.keys};
+    if (a.offsets) {
+        in = {clamped(a.offsets, a.offsets64, 0, a.queries), clamped(a.offsets, a.offsets64, a.sequences, a.queries)};
+    } else {
+        const int seen = a.key_lengths ? clamped(a.key_lengths, a.lengths64, b, a.keys) : a.keys;
+        if (!which || seen == 0) in.hi = min(in.hi, seen);
+        if (which && a.causal) in.lo = max(0, a.queries - a.keys);
+    }
+    const int lo = in.lo * (which ? a.group : 1), rows = in.hi * (which ? a.group : 1);
     const int c = (threadIdx.x & 15) * Elem<T>::EPC;
     float most = 0.0f;
-    for (int r = part * (kThreads / 16) + (threadIdx.x >> 4); r < rows; r += kRangeParts * (kThreads / 16)) {
+    for (int r = lo + part * (kThreads / 16) + (threadIdx.x >> 4); r < rows; r += kRangeParts * (kThreads / 16)) {
         const T* row = which ? grads.at(a, r) : values.at(a, r);
         float sq = 0.0f;
         if (c < a.width) {
@@ -879,7 +887,7 @@ int launch(Pass pass, const Params& a, hipStream_t st) {
 inline bool chunked(const Params& a, const View& v, int rows, int heads, int size) {
     auto apart = [&](int64_t stride, int count) { return count <= 1 || stride * size % 16 == 0; };
     return aligned(v.p, 16) && a.width * size % 16 == 0 && apart(v.batch, a.batch) && apart(v.row, rows) &&
-           apart(v.head, heads) && (rows <= 1 || v.row < (int64_t)1 << 22);
+           apart(v.head, heads) && (rows <= 1 || (v.row >= 0 && v.row < (int64_t)1 << 22));
 }
 template <typename T, int DP>
 int launch_filler(Pass pass, const Params& a, hipStream_t st) {
