@@ -392,8 +392,8 @@ constexpr int kAhead = 4;
 // that do not see it (0 x inf is NaN), where the tile holds such elements at all, in rows that
 // the wave sees or in others.  Looking first cost less than keeping them out always: packed
 // sequences 530 us and 494.  Wider heads, whose registers it spills, gained 1%, dQ as much
-// (570 and 564), and dK and dV, whose code fills the instruction cache, lost (1013 and 1164):
-// they know the first and the last only.
+// (570 and 564), and dK and dV, whose third wave on a SIMD has no registers to spare, lost (1013
+// and 1164): they know the first and the last only.
 enum : int { kFull, kMasked, kChecked };
 template <int KIND>
 using Kind = std::integral_constant<int, KIND>;
@@ -411,8 +411,15 @@ constexpr float kForwardShift = kHalf<T> ? 6.0f : 0.0f;
 template <typename T>
 constexpr float kBackwardShift = kHalf<T> ? 14.0f : 0.0f;
 
+// Waves on a SIMD: the third one of narrow heads hides more than the few registers that it
+// spills cost (packed sequences, heads of 64: 511 us with two, 444 with three).
+template <typename T>
+constexpr int forward_waves(int dp) {
+    return sizeof(T) == 2 ? (dp <= 64 ? 3 : 2) : dp <= 64 ? 2 : 1;
+}
+
 template <typename T, int DP, bool ASYNC>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) k_forward(Params a) {
+__global__ void __launch_bounds__(kThreads, forward_waves<T>(DP)) k_forward(Params a) {
     using TileT = Tile<T, BN, DP>;
     using PipeT = Pipe<T, DP, ASYNC>;
     constexpr int DT = DP / 32;
