@@ -252,21 +252,13 @@ struct Tile {
     }
 };
 
-// BYTES from each active lane's address (or base, wave-uniform, + offset bytes) to its place
-// after lds (wave-uniform): lane * BYTES.
+// 16 bytes from each active lane's address, base (wave-uniform) + offset bytes, to its place
+// after lds (wave-uniform): lane * 16.
 // Written as assembly because the compiler otherwise holds every transposing LDS read back
 // until all such loads in flight have landed; it has no register result, and
 // wait_loads_and_sync waits for it.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: the compiler sets it before each use of its own
-template <int BYTES>
-__device__ __forceinline__ void load_to_lds(const void* at, uint32_t lds) {
-    static_assert(BYTES == 4 || BYTES == 16, "");
-    lds = __builtin_amdgcn_readfirstlane((int)lds);
-    if constexpr (BYTES == 16)
-        asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(at) : "m0");
-    else asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(at) : "m0");
-}
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t lds) {
     const uint64_t b = reinterpret_cast<uint64_t>(base);
     const uint64_t s = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32 |
