@@ -256,14 +256,17 @@ struct Tile {
 // after lds (wave-uniform): lane * 16.
 // Written as assembly because the compiler otherwise holds every transposing LDS read back
 // until all such loads in flight have landed; it has no register result, and
-// wait_loads_and_sync waits for it.
+// wait_loads_and_sync waits for it.  The compiler counts no wait states into or inside the block,
+// so it brings those that the load needs: one behind the write of m0, and five behind a vector
+// instruction that wrote its base (which may be the last one before the block), the write of m0
+// and s_nop 3 together.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: the compiler sets it before each use of its own
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t lds) {
     const uint64_t b = reinterpret_cast<uint64_t>(base);
     const uint64_t s = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32 |
                        (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)),
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)),
                  "v"(offset), "s"(s)
                  : "m0");
 }
