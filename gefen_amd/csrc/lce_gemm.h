@@ -98,15 +98,22 @@ typedef __attribute__((address_space(3))) uint16_t lds_u16;
 // 64 lanes' 16 bytes at base + voff to the 1024 LDS bytes at lds.  Written as assembly
 // because the compiler otherwise holds every transposing LDS read back until all such
 // loads in flight have landed; it has no register result, and wait_loads_and_sync
-// waits for it.
+// waits for it.  The compiler counts no wait states into or inside the block, so it brings
+// those that the load needs: one behind the write of m0, and five behind a vector
+// instruction that wrote a word of its resource (which may be the last one before the
+// block), the write of m0 and s_nop 3 together.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: the compiler sets it before each use of its own
 template <bool STREAM>
 __device__ __forceinline__ void load_to_lds(i32x4 rsrc, int voff, uint32_t lds) {
     if constexpr (STREAM)
-        asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(lds), "v"(voff), "s"(rsrc)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(lds), "v"(voff),
+                     "s"(rsrc)
                      : "m0");
-    else asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "m0");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff),
+                     "s"(rsrc)
+                     : "m0");
 }
 #pragma clang diagnostic pop
 

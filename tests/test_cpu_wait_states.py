@@ -4,7 +4,7 @@ gfx950 has the programmer (the compiler, outside of inline assembly) put at leas
 
 * one wait state between a write of m0 and a load to LDS, which takes its place in LDS from it;
 * five between a vector instruction that writes a scalar register and a memory instruction that
-  reads it, here a load's base.
+  reads it, here a load's base or resource.
 
 An instruction is a wait state, s_nop n is n + 1.  A load brings all of them with the write of its
 m0, so that what the compiler puts in front does not matter."""
@@ -66,6 +66,13 @@ def counted(listings, mnemonic):
 
 def test_attention_waits_before_its_loads(listings):
     found = list(counted(listings, "global_load"))
+    assert found
+    assert min(m0 for m0, _ in found) >= M0
+    assert min(base for _, base in found) >= ADDRESS
+
+
+def test_linear_cross_entropy_waits_before_its_loads(listings):
+    found = list(counted(listings, "buffer_load"))
     assert found
     assert min(m0 for m0, _ in found) >= M0
     assert min(base for _, base in found) >= ADDRESS
