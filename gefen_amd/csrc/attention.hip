@@ -58,6 +58,10 @@ void set_parts(Pass pass, const gefen_attention_task& t, float* memory, Params* 
     a->stats = round16(stat_count(t));
 }
 
+// Workgroups along x that every pass can launch: HIP takes fewer than 2^32 work items there.
+// Split work (parts_of) has a few thousand, and what doubles or multiplies a grid is along y and z.
+constexpr int64_t kMostBlocks = (((int64_t)1 << 32) - 1) / kThreads;
+
 // Checks what does not depend on the direction.
 int check_task(const gefen_attention_task* t) {
     if (!t) return fail_inval("attention: no task");
@@ -71,10 +75,11 @@ int check_task(const gefen_attention_task* t) {
     if (t->batch > most || t->queries > most || t->keys > most || t->heads > 65536)
         return fail_inval("attention: sizes out of range");
     const int64_t group = t->heads / t->kv_heads, pairs = t->batch * t->kv_heads;
-    const int64_t most_blocks = 0x7fffffff / 64;
-    if (t->queries * group > most || pairs > most || pairs * ((t->queries * group + kCols - 1) / kCols) > most_blocks ||
-        pairs * ((t->keys + kCols - 1) / kCols) > most_blocks)
-        return fail_inval("attention: sizes out of range");
+    if (t->queries * group > most || pairs > most || pairs * ((t->queries * group + kCols - 1) / kCols) > kMostBlocks ||
+        pairs * ((t->keys + kCols - 1) / kCols) > kMostBlocks)
+        return fail_inval("attention: sizes out of range: batch * kv_heads times the blocks of %d keys, or of "
+                          "queries * heads / kv_heads, must stay below 2^24",
+                          kCols);
     if (!(t->scale >= 0.0) || !isfinite(t->scale)) return fail_inval("attention: scale must be finite and not negative");
     if (t->offsets && (t->batch != 1 || t->queries != t->keys || t->sequences < 0 || t->sequences > most))
         return fail_inval("attention: packed sequences are one batch of as many queries as keys");

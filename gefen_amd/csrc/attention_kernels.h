@@ -600,8 +600,7 @@ __device__ __forceinline__ float largest_norm(const Params& a, int which, int bh
 // the scale either), for half precision; 16 lanes a row.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) k_range(Params a) {
-    const int heads = a.batch * a.kv_heads, which = blockIdx.y, part = blockIdx.x % kRangeParts,
-              bh = blockIdx.x / kRangeParts;
+    const int heads = a.batch * a.kv_heads, bh = blockIdx.x, part = blockIdx.y, which = blockIdx.z;
     const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
     const Rows<T, true> grads(a, a.go, b, hk);
     const Rows<T, false> values(a, a.v, b, hk);
@@ -855,11 +854,9 @@ __device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile,
 template <typename T, int DP, bool ASYNC>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 || DP <= 64 ? 2 : 1) k_backward_keys(Params a) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];  // Pipe::BYTES
-    const int heads = a.batch * a.kv_heads, half = gridDim.x / 2;
-    const bool values = blockIdx.x >= half;
-    const int block = values ? blockIdx.x - half : blockIdx.x;
+    const int heads = a.batch * a.kv_heads, block = blockIdx.x;
     const int bh = block % heads, part = block / heads % a.parts, tile = block / heads / a.parts;
-    if (values) backward_keys<T, DP, ASYNC, true>(a, bh, tile, part, smem);
+    if (blockIdx.y) backward_keys<T, DP, ASYNC, true>(a, bh, tile, part, smem);
     else backward_keys<T, DP, ASYNC, false>(a, bh, tile, part, smem);
 }
 
@@ -875,7 +872,7 @@ int launch(Pass pass, const Params& a, hipStream_t st) {
     constexpr int lds = Pipe<T, DP, ASYNC>::BYTES;
     if (pass == kForwardPass) k_forward<T, DP, ASYNC><<<grid, kThreads, lds, st>>>(a);
     else if (pass == kQueriesPass) k_backward_queries<T, DP, ASYNC><<<grid, kThreads, lds, st>>>(a);
-    else k_backward_keys<T, DP, ASYNC><<<2 * grid, kThreads, lds, st>>>(a);
+    else k_backward_keys<T, DP, ASYNC><<<dim3(grid, 2), kThreads, lds, st>>>(a);
     if (int rc = launch_status("attention")) return rc;
     if (a.parts == 1) return GEFEN_OK;
     if (pass == kForwardPass) {
@@ -914,7 +911,7 @@ int launch_width(Pass pass, const Params& a, hipStream_t st) {
 // The norms that half precision's backward passes scale by.
 template <typename T>
 int launch_range(const Params& a, hipStream_t st) {
-    k_range<T><<<dim3((uint32_t)(a.batch * a.kv_heads * kRangeParts), 2), kThreads, 0, st>>>(a);
+    k_range<T><<<dim3((uint32_t)a.batch * (uint32_t)a.kv_heads, kRangeParts, 2), kThreads, 0, st>>>(a);
     return launch_status("attention");
 }
 

@@ -537,7 +537,9 @@ int gefen_scale_from_f32(const float* a, void* a_out, int64_t a_numel, const flo
  * their way into the second products (float16: scaled into its range, P down to 2^-28 (backward),
  * dS down to 2^-28 of the bound that the norms of the rows of value and grad_out give, one bound
  * a query in grad_query, one a key head in grad_key).  What a query does not see does not reach
- * it, whatever it holds, nor the other way round.  Every sum has a fixed order. */
+ * it, whatever it holds, nor the other way round.  Every sum has a fixed order.  batch * kv_heads
+ * times the blocks of 128 keys, and of 128 of queries * heads / kv_heads, must stay below 2^24 (what
+ * a launch holds); what is larger is refused in both directions. */
 enum { GEFEN_ATTENTION_MAX_WIDTH = 128 };
 typedef struct gefen_attention_task {
     const void* query;
