@@ -79,8 +79,14 @@ __device__ __forceinline__ float row_max(float v, float* slot) {
     return v;
 }
 
-// Eight values times inv as 8-bit floating point, the largest ones clamped.
-__device__ __forceinline__ uint64_t eight_bits(const float* v, float inv, bool e5m2) {
+// Eight values over scale as 8-bit floating point, the largest ones clamped.  What is rounded is
+// the float32 quotient: a product with inv = 1 / scale crosses a middle between two values of the
+// format now and then.  NEAR (scale is finite, and not so small that what follows underflows): that
+// product, and what it is off by, exact or nearly so in one fused operation, times inv once more;
+// it differs from the quotient where that lies within 2^-22 steps of float32 of a middle between
+// two of those.  16384 rows of 2048: 53 us, 57 with a division, 51 with the product alone.
+template <bool NEAR>
+__device__ __forceinline__ uint64_t eight_bits(const float* v, float scale, float inv, bool e5m2) {
     const float most = e5m2 ? 57344.0f : 448.0f;
     uint32_t out[2];
 #pragma unroll
@@ -88,7 +94,13 @@ __device__ __forceinline__ uint64_t eight_bits(const float* v, float inv, bool e
         float t[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float a = v[4 * h + i] * inv;
+            float a = v[4 * h + i];
+            if constexpr (NEAR) {
+                const float q = a * inv;
+                a = __builtin_fmaf(__builtin_fmaf(-q, scale, a), inv, q);
+            } else {
+                a /= scale;
+            }
             t[i] = a != a ? a : fminf(fmaxf(a, -most), most);
         }
         int w = 0;
@@ -175,16 +187,17 @@ __global__ void __launch_bounds__(S::THREADS) k_rms_forward(Params a) {
         if (!a.out8) continue;
         most = row_max<S::LANES>(most, slots_max);
         const bool e5m2 = a.out8 == GEFEN_RMS_E5M2;
-        // a scale below float32's normal range has no reciprocal there
+        // a scale below float32's normal range would have few bits
         float scale = most / (e5m2 ? 57344.0f : 448.0f);
         if (most > 0.0f) scale = fmaxf(scale, 1.17549435e-38f);
-        const float inv = most == 0.0f ? 0.0f : 1.0f / scale;
         if (lane == 0) a.scales[row] = scale;
+        const float by = most == 0.0f ? 1.0f : scale, inv = 1.0f / by;
+        const bool near = by >= 0x1p-100f && by < INFINITY;
 #pragma unroll
         for (int c = 0; c < S::CHUNKS; ++c) {
             const int at = (c * S::LANES + lane) * 8, have = width - at;
             if (have <= 0) continue;
-            const uint64_t q = eight_bits(s[c], inv, e5m2);
+            const uint64_t q = near ? eight_bits<true>(s[c], by, inv, e5m2) : eight_bits<false>(s[c], by, inv, e5m2);
             uint8_t* out = static_cast<uint8_t*>(a.y) + row * a.width + at;
             if (have >= 8) {
                 typedef uint64_t __attribute__((aligned(1))) any_t;
