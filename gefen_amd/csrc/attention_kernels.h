@@ -411,15 +411,19 @@ constexpr float kForwardShift = kHalf<T> ? 6.0f : 0.0f;
 template <typename T>
 constexpr float kBackwardShift = kHalf<T> ? 14.0f : 0.0f;
 
-// Waves on a SIMD: the third one of narrow heads hides more than the few registers that it
-// spills cost (packed sequences, heads of 64: 511 us with two, 444 with three).
+// Waves on a SIMD.  The third one of heads of up to 64 hides more than the registers that it spills
+// cost (43 words; packed sequences, heads of 64: 511 us with two, 444 with three; 8192 causal tokens,
+// 32 heads of 32: 265 and 227).  Tiles that come through registers leave fewer: none is spilled up to
+// 32 (heads of 17: 374 us with two, 288 with three), 89 words above (12 heads of 63 of 8 x 1024
+// tokens 107 us with two, 142 with three; 11 packed sequences, 32 heads of 64 off alignment, 260 and
+// 403; only 8192 tokens of 32 heads of 63 lost with two, 1146 and 978).
 template <typename T>
-constexpr int forward_waves(int dp) {
-    return sizeof(T) == 2 ? (dp <= 64 ? 3 : 2) : dp <= 64 ? 2 : 1;
+constexpr int forward_waves(int dp, bool async) {
+    return sizeof(T) == 2 ? (dp <= (async ? 64 : 32) ? 3 : 2) : dp <= 64 ? 2 : 1;
 }
 
 template <typename T, int DP, bool ASYNC>
-__global__ void __launch_bounds__(kThreads, forward_waves<T>(DP)) k_forward(Params a) {
+__global__ void __launch_bounds__(kThreads, forward_waves<T>(DP, ASYNC)) k_forward(Params a) {
     using TileT = Tile<T, BN, DP>;
     using PipeT = Pipe<T, DP, ASYNC>;
     constexpr int DT = DP / 32;
