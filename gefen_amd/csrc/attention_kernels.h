@@ -29,6 +29,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "attention_tiles.h"
@@ -411,19 +412,22 @@ constexpr float kForwardShift = kHalf<T> ? 6.0f : 0.0f;
 template <typename T>
 constexpr float kBackwardShift = kHalf<T> ? 14.0f : 0.0f;
 
-// Waves on a SIMD.  The third one of heads of up to 64 hides more than the registers that it spills
-// cost (43 words; packed sequences, heads of 64: 511 us with two, 444 with three; 8192 causal tokens,
-// 32 heads of 32: 265 and 227).  Tiles that come through registers leave fewer: none is spilled up to
-// 32 (heads of 17: 374 us with two, 288 with three), 89 words above (12 heads of 63 of 8 x 1024
-// tokens 107 us with two, 142 with three; 11 packed sequences, 32 heads of 64 off alignment, 260 and
-// 403; only 8192 tokens of 32 heads of 63 lost with two, 1146 and 978).
+// Waves on a SIMD of the forward pass.  The third one of heads of up to 64 hides more than the
+// registers that it spills cost (43 words; packed sequences, heads of 64: 511 us with two, 444 with
+// three; 8192 causal tokens, 32 heads of 32: 265 and 227), if there are workgroups for it: up to
+// kTwoEach it only spills (one query of 16 sequences, 32 / 8 heads of 64: 52 us with two, 58 with
+// three; 777 queries over 1003 keys: 21.8 and 23.8).  Tiles that come through registers leave fewer:
+// none is spilled up to 32 (heads of 17: 374 us with two, 288 with three), 89 words above (12 heads
+// of 63 of 8 x 1024 tokens 107 us with two, 142 with three; 11 packed sequences, 32 heads of 64 off
+// alignment, 260 and 403; only 8192 tokens of 32 heads of 63 lost with two, 1146 and 978).
 template <typename T>
 constexpr int forward_waves(int dp, bool async) {
     return sizeof(T) == 2 ? (dp <= (async ? 64 : 32) ? 3 : 2) : dp <= 64 ? 2 : 1;
 }
+constexpr int kTwoEach = 512;  // workgroups of four waves, two waves a SIMD
 
-template <typename T, int DP, bool ASYNC>
-__global__ void __launch_bounds__(kThreads, forward_waves<T>(DP, ASYNC)) k_forward(Params a) {
+template <typename T, int DP, bool ASYNC, int WAVES>
+__global__ void __launch_bounds__(kThreads, WAVES) k_forward(Params a) {
     using TileT = Tile<T, BN, DP>;
     using PipeT = Pipe<T, DP, ASYNC>;
     constexpr int DT = DP / 32;
@@ -874,7 +878,9 @@ int launch(Pass pass, const Params& a, hipStream_t st) {
     const int64_t tiles = ((pass == kKeysPass ? a.keys : a.rows) + kCols - 1) / kCols;
     const uint32_t grid = (uint32_t)(heads * tiles * a.parts);
     constexpr int lds = Pipe<T, DP, ASYNC>::BYTES;
-    if (pass == kForwardPass) k_forward<T, DP, ASYNC><<<grid, kThreads, lds, st>>>(a);
+    constexpr int waves = forward_waves<T>(DP, ASYNC), few = DP > 32 ? std::min(waves, 2) : waves;
+    constexpr auto forward = k_forward<T, DP, ASYNC, waves>, forward_few = k_forward<T, DP, ASYNC, few>;
+    if (pass == kForwardPass) (grid <= kTwoEach ? forward_few : forward)<<<grid, kThreads, lds, st>>>(a);
     else if (pass == kQueriesPass) k_backward_queries<T, DP, ASYNC><<<grid, kThreads, lds, st>>>(a);
     else k_backward_keys<T, DP, ASYNC><<<dim3(grid, 2), kThreads, lds, st>>>(a);
     if (int rc = launch_status("attention")) return rc;
