@@ -22,14 +22,18 @@ int64_t out_count(Pass pass, const gefen_attention_task& t) {
     return t.batch * t.width * (pass == kKeysPass ? t.keys * t.kv_heads : t.queries * t.heads);
 }
 
-// Into how many parts a workgroup's tiles are split.  The chip holds `slots` workgroups, and few
-// of them leave it idle: one query of 16 sequences over 8192 keys, 128 workgroups, took 263 us
-// whole, 100 us in 4 parts with the join and 107 in 8; 195 workgroups of 16 tiles took 31.5 us
-// whole and 32.2 in 2 parts, so there have to be three; those of dK and dV, which differ in
-// length, took 78 us whole and 61 in 2.  Packed sequences of uneven length make as many as the
-// chip holds wait for the longest one's keys (11 sequences of 16384 tokens, 2048 workgroups: 1360
-// us whole, 1115 us in 4 parts with the join; one sequence of 8192: 1570 and 1590).  A part has
-// four tiles at least, for its sums go through memory.
+// Into how many parts a workgroup's tiles are split.  Few workgroups leave the chip idle: one
+// query of 16 sequences over 8192 keys, 128 of them, took 263 us whole, 100 us in 4 parts with the
+// join and 107 in 8; 195 workgroups of 16 tiles took 31.5 us whole and 32.2 in 2 parts, so there
+// have to be three; those of dK and dV, which differ in length, took 78 us whole and 61 in 2.
+// `slots` is what the chip holds of heads above 64, a workgroup a CU in float32 and two in 16 bits;
+// narrower heads, of which it holds up to twice as many, are split for the same number.
+// Packed sequences of uneven length make as many as the chip holds wait for the longest one's keys
+// (11 sequences of 16384 tokens, 2048 workgroups: 1360 us whole, 1115 us in 4 parts with the join;
+// one sequence of 8192: 1570 and 1590).  A part has four tiles at least, for its sums go through
+// memory: of the whole axis, and where sequences are split for their lengths of their mean one (64
+// sequences of 128 tokens, 8 heads of 128: dK and dV 46 us whole, 184 in 4 parts with the join; one
+// of 8192 beside 1024 of 8, 32 / 8 heads: 1530 us whole and 1620).
 int parts_of(Pass pass, const gefen_attention_task& t) {
     const bool keys = pass == kKeysPass;
     const int64_t slots = t.dtype == GEFEN_F32 ? 256 : 512, group = t.heads / t.kv_heads;
@@ -39,7 +43,10 @@ int parts_of(Pass pass, const gefen_attention_task& t) {
     if (wgs == 0 || tiles == 0) return 1;
     int64_t parts = slots / wgs;
     if (!keys && parts < 3) parts = 1;
-    if (keys && t.offsets && t.sequences > 1 && wgs < 8 * slots && parts < 4) parts = 4;
+    if (keys && t.offsets && t.sequences > 1 && wgs < 8 * slots && parts < 4) {
+        const int64_t mean = (t.queries + t.sequences - 1) / t.sequences;
+        parts = std::max(parts, std::min((int64_t)4, group * ((mean + BN - 1) / BN) / 4));
+    }
     parts = parts < tiles / 4 ? parts : tiles / 4;
     return (int)(parts < 1 ? 1 : parts > 32 ? 32 : parts);
 }
