@@ -15,14 +15,20 @@
 // u % G of the group (G = heads / kv_heads), so a tile of keys and values is loaded once for
 // all of them, and a single new token still gives G rows.
 //
+// P and dS are rounded to the operands' 16 bits on their way into the second products, whose matrix
+// instructions take no more, and D is formed of the rounded output; float32 rounds neither.  So dQ
+// and dK of bfloat16 are off by 2.6e-3 (float16 3.1e-4) where their own rounding is 1.7e-3 (2.1e-4);
+// 2.4e-3 of it are the rounding of dS and of the result.
+//
 // What bounds it: with many rows the matrix cores, and beside them the vector unit: a 32 x 32
 // block of S takes a wave some 480 cycles of exponentials, maxima and conversions, and its two
 // products of the forward pass 256 (heads of 64) or 512.  8192 causal tokens, 32 / 8 heads of
-// 128, bf16: forward 564 us, dQ 752, dK and dV 1390, which is 0.98, 1.10 and 0.99 PFLOP/s on the
-// 2, 3 and 5 products that they form (a large library product reaches 1.22; matrix cores busy
-// 51%, 60% and 58%, no bank conflicts, 1.9 to 2.0 GHz).  8 x 1024 tokens, 12 heads of 64,
-// float32: 151, 230 and 330 us, matrix cores busy 75%, 67% and 78%.  With one row a sequence,
-// HBM: one query in each of 16 sequences of up to 8192 keys, 392 MB of 8 heads of 128, takes 90 us.
+// 128, bf16: forward 547 us, dQ 725, dK and dV 1320, which is 1.00, 1.14 and 1.04 PFLOP/s on the
+// 2, 3 and 5 products that they form (a large library product reaches 1.24 on that card; matrix
+// cores busy 49%, 59% and 58%, no bank conflicts, 1.95 to 2.1 GHz; 600, 800 and 1440 us on one whose
+// product reaches 1.18).  8 x 1024 tokens, 12 heads of 64, float32: 142, 219 and 310 us, matrix cores
+// busy 74%, 66% and 78%.  With one row a sequence, HBM: one query in each of 16 sequences of up to
+// 8192 keys, 392 MB of 8 heads of 128, takes 90 us with the join.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -732,11 +738,14 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) k_backward_q
     else store_column(static_cast<T*>(a.gq.p) + at, acc, f, a.width, lane);
 }
 
-// dK, or (VALUES) dV.  Together they would need 4 products instead of 5, but their
-// accumulators beside a lane's key and value leave no room for a second wave on a SIMD, and
-// that costs more: at 8192 causal tokens of 32 / 8 heads of 128 (bf16) one kernel for both took
-// 2022 us alone on its SIMDs and 1541 us as pairs of waves that hand P over through LDS, where
-// this one took 1530 (1390 with its LDS reads in order).
+// dK, or (VALUES) dV.  Together they would need 4 products instead of 5, but their accumulators
+// beside a lane's key and value leave no room for a second wave on a SIMD: one kernel for both took
+// 2022 us at 8192 causal tokens of 32 / 8 heads of 128 (bf16), where this one takes 1320 to 1440.  As
+// pairs of waves that share 32 keys, one of which hands P over through LDS (rounded, so that dK's dS
+// had a rounding more), both took 1369 us when this one took 1636.  Since then this one takes the rows
+// from the last one on (1423) and orders its LDS reads (1530 to 1394 on another card); pairs without
+// that order took 1541 beside the 1530, and 296 us beside 330 for float32 heads of 64.  With both they
+// have not been measured.
 template <typename T, int DP, bool ASYNC, bool VALUES>
 __device__ __forceinline__ void backward_keys(const Params& a, int bh, int tile, int part, char* smem) {
     using TileT = Tile<T, BN, DP>;

@@ -8,7 +8,7 @@
 // once and written once: a wave owns a row of up to 2048 elements (no wait for other waves), a
 // workgroup a longer one, and the next row is on its way while one is worked on.  8192 rows of
 // 4096, bf16, with a residual: forward 51 us (5.3 TB/s), backward 46 (5.9) and the join of dw 4;
-// 16384 rows of 2048 into 8 bits 51 us (4.6); a copy of 2 GiB moves 4.9.  Fewer rows do not fill
+// 16384 rows of 2048 into 8 bits 54 us (4.3); a copy of 2 GiB moves 4.9.  Fewer rows do not fill
 // the chip: 1531 of 1001 halves take 9 + 12 + 4.5 us, where 24 MB would take 5.
 // The squares are summed in float64, where no 16-bit or float32 value over- or underflows.
 // dw: a workgroup takes rows in strides of the grid and sums its columns in registers, the
@@ -84,7 +84,7 @@ __device__ __forceinline__ float row_max(float v, float* slot) {
 // format now and then.  NEAR (scale is finite, and not so small that what follows underflows): that
 // product, and what it is off by, exact or nearly so in one fused operation, times inv once more;
 // it differs from the quotient where that lies within 2^-22 steps of float32 of a middle between
-// two of those.  16384 rows of 2048: 53 us, 57 with a division, 51 with the product alone.
+// two of those.  16384 rows of 2048: 53 to 54 us, 57 with a division, 51 with the product alone.
 template <bool NEAR>
 __device__ __forceinline__ uint64_t eight_bits(const float* v, float scale, float inv, bool e5m2) {
     const float most = e5m2 ? 57344.0f : 448.0f;

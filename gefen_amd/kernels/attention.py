@@ -29,14 +29,16 @@ def attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, ca
     ``h // (heads // kv_heads)``.  ``scale`` (1 / sqrt(width) by default) is not negative.
 
     Query i sees key j where ``j < key_lengths[b]`` (int32 or int64 [batch] on the device) and,
-    with ``causal``, where ``j <= i + keys - queries``: the last query at the last key.  With
+    with ``causal``, where ``j <= i + keys - queries``: the last query at the last key (of the
+    tensor, not of ``key_lengths``).  With
     ``offsets`` (int32 or int64 [sequences + 1] on the device, ascending) the tensors are packed
     sequences [tokens, heads, width], sequence s holding the tokens from ``offsets[s]`` to
     ``offsets[s + 1]``, and a token sees its own sequence only.
 
     A query that sees no key gives zeros and has no gradient, and so does a key that no query
     sees; what is not seen does not reach a result, whatever it holds.  The result can be
-    differentiated once."""
+    differentiated once.  ``batch * kv_heads`` times the blocks of 128 keys, or of 128 of
+    ``queries * heads / kv_heads``, is below 2^24."""
     if scale is not None:
         scale = float(scale)
         if not 0.0 <= scale < float("inf"):

@@ -54,7 +54,8 @@ def rms_norm_quantized(x: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e
                        dtype: torch.dtype = torch.float8_e4m3fn) -> Tuple[torch.Tensor, ...]:
     """``rms_norm`` with y in 8 bits: (q, scales), or (q, scales, s) with a residual.  q has the
     dtype ``float8_e4m3fn`` or ``float8_e5m2`` and x's shape, scales [...] are float32, and
-    ``q * scales[..., None]`` is y with each row's largest value at the largest of the dtype.
+    ``q * scales[..., None]`` is y with each row's largest value at the largest of the dtype; q is
+    the nearest to the float32 quotient of y and the scale.
     For evaluation: an 8-bit tensor carries no gradient, so it is refused where one is wanted."""
     eps = _eps(eps)
     if dtype not in (torch.float8_e4m3fn, torch.float8_e5m2):

@@ -573,7 +573,7 @@ int gefen_attention_backward(const gefen_attention_task* task, void* workspace, 
  * and its gradient (see gefen_dropout for the mask; element e = row * width + column).  Forward
  * works on s before its rounding to dtype, backward on the stored s and the stored r.  With
  * GEFEN_RMS_E4M3 or _E5M2, y is 8-bit floating point: y = q * scales[row], the row's largest
- * value at the largest of the format (448, 57344). */
+ * value at the largest of the format (448, 57344) and q the nearest of it to the float32 quotient. */
 enum { GEFEN_RMS_SAME = 0, GEFEN_RMS_E4M3 = 1, GEFEN_RMS_E5M2 = 2 };
 enum { GEFEN_RMS_MAX_WIDTH = 32768 };
 typedef struct gefen_rms_norm_task {
