@@ -266,7 +266,8 @@ __device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, u
     const uint64_t b = reinterpret_cast<uint64_t>(base);
     const uint64_t s = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32 |
                        (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)),
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(
+                     __builtin_amdgcn_readfirstlane((int)lds)),
                  "v"(offset), "s"(s)
                  : "m0");
 }

@@ -11,6 +11,9 @@
 // 16384 rows of 2048 into 8 bits 54 us (4.3); a copy of 2 GiB moves 4.9.  Fewer rows do not fill
 // the chip: 1531 of 1001 halves take 9 + 12 + 4.5 us, where 24 MB would take 5.
 // The squares are summed in float64, where no 16-bit or float32 value over- or underflows.
+// The backward pass reads s as it was rounded for its caller: dw of 16 bits is off by 2.5e-3 (bfloat16)
+// where its own rounding is 1.7e-3.  s in float32, or x and the residual in its place, would be a
+// tensor more to keep from the forward pass and to read, a quarter of the backward pass's bytes.
 // dw: a workgroup takes rows in strides of the grid and sums its columns in registers, the
 // workgroups' sums are added in a second launch, always in the same order.
 #include <hip/hip_runtime.h>
@@ -97,7 +100,7 @@ __device__ __forceinline__ uint64_t eight_bits(const float* v, float scale, floa
             float a = v[4 * h + i];
             if constexpr (NEAR) {
                 const float q = a * inv;
-                a = __builtin_fmaf(__builtin_fmaf(-q, scale, a), inv, q);
+                a = __builtin_fmaf(-__builtin_fmaf(q, scale, -a), inv, q);  // this way round -0 stays
             } else {
                 a /= scale;
             }

@@ -44,3 +44,15 @@ def test_values_are_the_quotients(name, width, largest):
         assert bool((scales.cpu() == float(scale)).all())
         want = nearest(w / scale, fmt) * x
         assert torch.equal(q.float().cpu(), want), int((q.float().cpu() != want).sum())
+
+
+@pytest.mark.parametrize("name", ["float8_e4m3fn", "float8_e5m2"])
+@pytest.mark.parametrize("largest", [2.0, 1e-36])
+def test_zeros_keep_their_sign(name, largest):
+    """-0 over a positive scale is -0, beside values that underflow to it."""
+    from gefen_amd import rms_norm_quantized
+
+    x = torch.tensor([1.0, -1.0, 0.0, -0.0, 1e-30, -1e-30, 0.0, -0.0, 0.5] * 30, device="cuda")
+    w = torch.full_like(x, largest)
+    q, _ = rms_norm_quantized(x, w, eps=0.0, dtype=getattr(torch, name))
+    assert torch.equal(torch.signbit(q.float()), torch.signbit(x))
